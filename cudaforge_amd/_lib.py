@@ -101,7 +101,7 @@ class KVPageCopyC(ctypes.Structure):
 
 
 # The ABI these signatures describe (CFA_ABI_VERSION of include/cudaforge_amd.h).
-ABI_VERSION = 200
+ABI_VERSION = 201
 
 # name -> (restype, argtypes); every symbol the header declares.
 SIGNATURES: dict[str, tuple] = {
@@ -155,6 +155,11 @@ SIGNATURES: dict[str, tuple] = {
         _i, [_p, _i, _p, _i, _i, _i, _i, _i, _f, _p, _p, _p, _i, _i, _i, _p, _i, _p, _p]),
     "cfa_rope_kv_strided": (
         _i, [_p, _p, _i, _i, _i, _i, _i, _f, _p, _p, _i64p, _p, _i64p, _p, _p]),
+    "cfa_qk_norm_rope_kv": (
+        _i,
+        [_p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _i, _p, _i, _i, _p, _i, _i, _i, _i, _p,
+         _f, _i, _p, _p, _i, _f, _p, _p, _p, _i, _i, _i, _i, _p, _i, _p, _p],
+    ),
     "cfa_silu_mul": (_i, [_p, _p, _i, _i, _p]),
     "cfa_gemm_bf16_skinny_workspace_size": (_sz, [_i, _i, _i, _i]),
     "cfa_gemm_bf16_skinny": (_i, [_p, _p, _p, _i, _i, _i, _i, _p, _sz, _p]),

@@ -57,8 +57,9 @@ const char *cfa_last_error(void);
  * library built from this header.  Major 2 changed two contracts of major 1:
  * cfa_tree_verify takes (workspace, workspace_bytes) before its stream, and
  * python-mode cfa_chain_verify reads uniforms [B, K+2] (row stride K+2), not
- * [B, K+1].  Binding code checks the major before its first call. */
-#define CFA_ABI_VERSION 200
+ * [B, K+1].  Minor 1 of it adds cfa_qk_norm_rope_kv.
+ * Binding code checks the major before its first call. */
+#define CFA_ABI_VERSION 201
 int cfa_version(void);
 
 /* ---------------------------------------------------------------------------
@@ -407,6 +408,42 @@ int cfa_rope_kv_strided(const void *qkv, const int32_t *positions, int B, int n,
                         void *v_cache, const int64_t *v_strides, const int32_t *slots,
                         void *stream);
 int cfa_silu_mul(const void *gu, void *out, int M, int F, void *stream);
+
+/* ---------------------------------------------------------------------------
+ * RMSNorm of every q and k head, rotary positions of either layout and the
+ * write of k and v into the paged cache, in one pass over a QKV projection
+ * (the reference's rope_kernel, csrc/include/cudaforge/kernels/rope.cuh:35-66,
+ * has the half layout over whole heads alone).
+ *
+ *   q [T, n_q_heads, head_dim], k, v [T, n_kv_heads, head_dim]: bf16, or fp16
+ *     (fp16 = 1); element strides of tokens and heads are the caller's,
+ *     head_dim (a multiple of 8, at most 256) is contiguous; 16-byte aligned
+ *     heads take wide accesses
+ *   y = x * rsqrt(mean(x^2) + eps) * w for q and k heads with q_norm / k_norm
+ *     [head_dim] (NULL: y = x), of the element type or fp32 (norm_f32 = 1)
+ *   the pairs of the first rotary_dim elements, (i, i + rotary_dim / 2) or with
+ *     interleaved = 1 (2i, 2i + 1), turn by positions[t] * turns[i], turns
+ *     [rotary_dim / 2] being 64-bit fractions of a turn per position: (a, b) ->
+ *     factor * (a cos - b sin, b cos + a sin); rotary_dim 0: no rotation
+ *   q_out [T, n_q_heads, head_dim] contiguous, not overlapping q, k or v
+ *   k and v of token j of sequence b go to slot base_lens[b] + j of `layer` in
+ *     the pools (layout and block_tables [B, max_blocks_per_seq] as for
+ *     cfa_tree_attention; any block_size).  cu_seqlens [B + 1] (rising): token
+ *     t is j = t - cu_seqlens[b] of the sequence that holds it; NULL: T / B
+ *     tokens a sequence
+ * fp32 arithmetic, rounded once; v is copied.  Tokens of no sequence leave
+ * every output untouched; so do k and v of a token whose page is not mapped
+ * (block id outside the pool, slot outside the table).  T = 0 and B = 0 are
+ * allowed and launch nothing. */
+int cfa_qk_norm_rope_kv(const void *q, int64_t q_stride_t, int64_t q_stride_h, const void *k,
+                        int64_t k_stride_t, int64_t k_stride_h, const void *v, int64_t v_stride_t,
+                        int64_t v_stride_h, int fp16, const int32_t *positions, int T, int B,
+                        const int32_t *cu_seqlens, int n_q_heads, int n_kv_heads, int head_dim,
+                        int rotary_dim, const uint64_t *turns, float factor, int interleaved,
+                        const void *q_norm, const void *k_norm, int norm_f32, float eps,
+                        void *q_out, void *k_pool, void *v_pool, int num_blocks, int num_layers,
+                        int layer, int block_size, const int32_t *block_tables,
+                        int max_blocks_per_seq, const int32_t *base_lens, void *stream);
 
 /* Few-row bf16 GEMM: c [M, N] = a [M, K] x w [K, N], all row-major bf16, fp32
  * accumulation on MFMA, 1 <= M <= 128, N % 64 == 0, K % 128 == 0, pointers
