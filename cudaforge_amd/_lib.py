@@ -127,6 +127,18 @@ SIGNATURES: dict[str, tuple] = {
         [_p, _p, _p, _p, _i, _p, _i, _i, _i, _i, _p, _i64, _i, _i, _i, _i, _i, _i, _f, _i, _i,
          _p, _p, _sz, _p],
     ),
+    "cfa_tree_attention_scored_workspace_size": (_sz, [_i, _i, _i, _i, _i, _i, _i, _i]),
+    "cfa_tree_attention_scored": (
+        _i,
+        [_p, _p, _p, _i, _p, _i, _p, _i, _i, _i, _i, _p, _i64, _i, _i, _i, _i, _i, _i, _f, _f, _p,
+         _i, _i, _i, _p, _p, _sz, _p],
+    ),
+    "cfa_prompt_attention_workspace_size": (_sz, [_i, _i, _i, _i, _i, _i, _i, _i, _i]),
+    "cfa_prompt_attention": (
+        _i,
+        [_p, _p, _p, _i, _p, _i, _p, _i, _i, _i, _i, _p, _i, _i, _i, _i, _i, _f, _f, _p, _i, _i, _i,
+         _i, _p, _p, _sz, _p],
+    ),
     "cfa_tree_verify_workspace_size": (_sz, [_i]),
     "cfa_tree_verify": (
         _i,

@@ -1,0 +1,235 @@
+// scored_attention.hip -- the entry points of scored_attention.hpp: argument
+// checks, the plan of blocks and splits, and the workspace.
+#include "scored_attention.hpp"
+
+#include <algorithm>
+#include <cmath>
+
+namespace cfa {
+namespace scored {
+
+extern template int launch<64, BF16>(const Args &, bool, unsigned, hipStream_t);
+extern template int launch<128, BF16>(const Args &, bool, unsigned, hipStream_t);
+extern template int launch<64, FP16>(const Args &, bool, unsigned, hipStream_t);
+extern template int launch<128, FP16>(const Args &, bool, unsigned, hipStream_t);
+
+static size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
+
+struct Plan {
+  int TQ, splits;
+  long long blocks;  // blocks to launch
+  bool one;          // one 16-row query tile a wave
+  size_t part_bytes(long long tokens, int Hq, int D) const {
+    return align256((size_t)splits * tokens * Hq * D * 4);
+  }
+  size_t bytes(long long tokens, int Hq, int D) const {
+    return splits == 1 ? 0
+                       : part_bytes(tokens, Hq, D) +
+                             align256((size_t)splits * tokens * Hq * sizeof(float2));
+  }
+};
+
+// Tokens per block, and the splits of the keys: about one work-group per CU
+// (each holds most of a CU's LDS), of at least five tiles where there are more
+// than four (a split begins with the latency of its first transfers).
+// `longest` bounds a sequence's queries; tokens is the number of all.
+static Plan plan(long long tokens, long long longest, int B, int G, int Hkv, int max_keys,
+                 int window, int num_splits, bool tree) {
+  Plan p;
+  p.one = longest * G <= kRowsOneTile;
+  p.TQ = (int)std::max(1LL, std::min(longest, (long long)(p.one ? kRowsOneTile : kMaxRows) / G));
+  p.blocks = tree ? (long long)B * ((longest + p.TQ - 1) / p.TQ) : tokens / p.TQ + B;
+  const long long busy =  // blocks that have queries, at least
+      tree ? p.blocks : std::max<long long>((tokens + p.TQ - 1) / p.TQ, std::min<long long>(B, tokens));
+  int tiles = std::max(1, (max_keys + kKT - 1) / kKT);
+  if (window > 0)
+    tiles = (int)std::min<long long>(
+        tiles, ((long long)window + (tree ? 64 : p.TQ) + kKT - 2) / kKT + 1);
+  int s;
+  if (num_splits > 0) {
+    s = num_splits;
+  } else {
+    const long long items = std::max(1LL, busy * Hkv);
+    const int cus = abi::device_cu_count();
+    s = (int)std::max(1LL, (cus + items - 1) / items);
+    s = std::min(s, std::max(4, tiles / 5));
+    if (s == 2 && tiles <= 8) s = 1;
+  }
+  p.splits = std::min(s, tiles);
+  return p;
+}
+
+static int check_scores(float sm_scale, float soft_cap, int window) {
+  using namespace cfa::abi;
+  if (!std::isfinite(sm_scale)) return fail_arg("sm_scale must be finite");
+  if (!(soft_cap == 0.0f || (soft_cap >= 1e-6f && std::isfinite(soft_cap))))
+    return fail_arg("soft_cap must be 0 (no cap) or finite and at least 1e-6");
+  if (window < 0) return fail_arg("window must not be negative (0: none)");
+  return CFA_OK;
+}
+
+static int check_heads(int Hq, int Hkv, int D) {
+  using namespace cfa::abi;
+  if (D != 64 && D != 128) return fail_arg("head_dim must be 64 or 128");
+  if (Hkv <= 0 || Hq <= 0 || Hq % Hkv)
+    return fail_arg("n_q_heads must be a positive multiple of n_kv_heads");
+  if (Hq / Hkv > kMaxRows) return fail_arg("n_q_heads / n_kv_heads must be at most 256");
+  return CFA_OK;
+}
+
+static int check_pool(int num_blocks, int num_layers, int layer, int block_size, int max_blocks) {
+  using namespace cfa::abi;
+  if (block_size <= 0 || block_size % 16) return fail_arg("block_size must be a multiple of 16");
+  if (num_blocks <= 0 || num_layers <= 0 || layer < 0 || layer >= num_layers)
+    return fail_arg("bad pool geometry (num_blocks, num_layers, layer)");
+  if (max_blocks <= 0) return fail_arg("max_blocks_per_seq must be positive");
+  if ((long long)max_blocks * block_size > 0x7fffff00LL)
+    return fail_arg("a block table must cover less than 2^31 - 256 positions");
+  return CFA_OK;
+}
+
+static int run(Args &a, const Plan &p, int D, int fp16, float sm_scale, float soft_cap,
+               void *workspace, size_t workspace_bytes, void *stream) {
+  using namespace cfa::abi;
+  a.TQ = p.TQ;
+  a.splits = p.splits;
+  a.blocks = (int)p.blocks;
+  a.cap = soft_cap;
+  a.scale = soft_cap > 0.0f ? sm_scale / soft_cap : sm_scale;
+  const long long grid = (long long)p.splits * a.Hkv * p.blocks;
+  if (grid * kNT >= (1LL << 32)) return fail_arg("too many queries for one call");
+  if (p.splits > 1) {
+    if (!workspace || workspace_bytes < p.bytes(a.T, a.Hq, D))
+      return fail_arg("workspace too small (see the entry point's _workspace_size)");
+    if (((uintptr_t)workspace & 15) != 0) return fail_arg("workspace must be 16-byte aligned");
+    a.part_o = (float *)workspace;
+    a.part_ml = (float2 *)((char *)workspace + p.part_bytes(a.T, a.Hq, D));
+  }
+  hipStream_t st = (hipStream_t)stream;
+  if (D == 128)
+    return fp16 ? launch<128, FP16>(a, p.one, (unsigned)grid, st)
+                : launch<128, BF16>(a, p.one, (unsigned)grid, st);
+  return fp16 ? launch<64, FP16>(a, p.one, (unsigned)grid, st)
+              : launch<64, BF16>(a, p.one, (unsigned)grid, st);
+}
+
+}  // namespace scored
+}  // namespace cfa
+
+using namespace cfa::scored;
+
+extern "C" size_t cfa_tree_attention_scored_workspace_size(int B, int N, int n_q_heads,
+                                                           int n_kv_heads, int head_dim,
+                                                           int max_keys, int window,
+                                                           int num_splits) {
+  cfa::abi::clear_error();
+  if (B <= 0 || N <= 0 || window < 0 || check_heads(n_q_heads, n_kv_heads, head_dim) != CFA_OK)
+    return 0;
+  const Plan p = plan((long long)B * N, N, B, n_q_heads / n_kv_heads, n_kv_heads, max_keys, window,
+                      num_splits, true);
+  return p.bytes((long long)B * N, n_q_heads, head_dim);
+}
+
+extern "C" int cfa_tree_attention_scored(
+    const void *q, const void *k_pool, const void *v_pool, int fp16, const int32_t *block_tables,
+    int max_blocks_per_seq, const int32_t *ctx_lens, int num_blocks, int num_layers, int layer,
+    int block_size, const uint64_t *tree_mask, int64_t tree_mask_stride_b, int B, int N,
+    int first_node, int n_q_heads, int n_kv_heads, int head_dim, float sm_scale, float soft_cap,
+    const float *alibi_slopes, int window, int max_keys, int num_splits, void *out,
+    void *workspace, size_t workspace_bytes, void *stream) {
+  using namespace cfa::abi;
+  clear_error();
+  if (!q || !k_pool || !v_pool || !block_tables || !ctx_lens || !tree_mask || !out)
+    return fail_arg("null pointer argument");
+  if (B <= 0 || N <= 0 || N > 64) return fail_arg("need B > 0 and 0 < N <= 64 tree nodes");
+  if (first_node < 0 || first_node >= N) return fail_arg("need 0 <= first_node < N");
+  if (int rc = check_heads(n_q_heads, n_kv_heads, head_dim)) return rc;
+  if (int rc = check_pool(num_blocks, num_layers, layer, block_size, max_blocks_per_seq)) return rc;
+  if (int rc = check_scores(sm_scale, soft_cap, window)) return rc;
+  if (max_keys < N) return fail_arg("max_keys must be at least N (context + tree tokens)");
+  if ((long long)max_blocks_per_seq * block_size < max_keys)
+    return fail_arg("max_blocks_per_seq * block_size must cover max_keys");
+  if (num_splits < 0) return fail_arg("num_splits must not be negative");
+  Args a{};
+  a.q = (const uint16_t *)q;
+  a.kpool = (const uint16_t *)k_pool;
+  a.vpool = (const uint16_t *)v_pool;
+  a.bt = block_tables;
+  a.ctx = ctx_lens;
+  a.mask = tree_mask;
+  a.mask_sb = tree_mask_stride_b;
+  a.slopes = alibi_slopes;
+  a.out = (uint16_t *)out;
+  a.Nq = N - first_node;
+  if ((long long)B * a.Nq >= (1LL << 31)) return fail_arg("too many queries for one call");
+  a.T = B * a.Nq;
+  a.B = B;
+  a.N = N;
+  a.q0 = first_node;
+  a.Hq = n_q_heads;
+  a.Hkv = n_kv_heads;
+  a.G = n_q_heads / n_kv_heads;
+  a.max_blocks = max_blocks_per_seq;
+  a.num_blocks = num_blocks;
+  a.num_layers = num_layers;
+  a.layer = layer;
+  a.bs = block_size;
+  a.window = window;
+  const Plan p = plan(a.T, a.Nq, B, a.G, n_kv_heads, max_keys, window, num_splits, true);
+  return run(a, p, head_dim, fp16, sm_scale, soft_cap, workspace, workspace_bytes, stream);
+}
+
+extern "C" size_t cfa_prompt_attention_workspace_size(int T, int B, int n_q_heads, int n_kv_heads,
+                                                      int head_dim, int max_query, int max_keys,
+                                                      int window, int num_splits) {
+  cfa::abi::clear_error();
+  if (B <= 0 || T <= 0 || max_query <= 0 || window < 0 ||
+      check_heads(n_q_heads, n_kv_heads, head_dim) != CFA_OK)
+    return 0;
+  const Plan p = plan(T, std::min(max_query, T), B, n_q_heads / n_kv_heads, n_kv_heads, max_keys,
+                      window, num_splits, false);
+  return p.bytes(T, n_q_heads, head_dim);
+}
+
+extern "C" int cfa_prompt_attention(
+    const void *q, const void *k_pool, const void *v_pool, int fp16, const int32_t *block_tables,
+    int max_blocks_per_seq, const int32_t *ctx_lens, int num_blocks, int num_layers, int layer,
+    int block_size, const int32_t *cu_seqlens, int T, int B, int n_q_heads, int n_kv_heads,
+    int head_dim, float sm_scale, float soft_cap, const float *alibi_slopes, int window,
+    int max_query, int max_keys, int num_splits, void *out, void *workspace,
+    size_t workspace_bytes, void *stream) {
+  using namespace cfa::abi;
+  clear_error();
+  if (T < 0 || B < 0) return fail_arg("need T, B >= 0");
+  if (int rc = check_heads(n_q_heads, n_kv_heads, head_dim)) return rc;
+  if (int rc = check_pool(num_blocks, num_layers, layer, block_size, max_blocks_per_seq)) return rc;
+  if (int rc = check_scores(sm_scale, soft_cap, window)) return rc;
+  if (max_query <= 0 || max_keys <= 0) return fail_arg("max_query and max_keys must be positive");
+  if (num_splits < 0) return fail_arg("num_splits must not be negative");
+  if (T == 0 || B == 0) return CFA_OK;
+  if (!q || !k_pool || !v_pool || !block_tables || !ctx_lens || !cu_seqlens || !out)
+    return fail_arg("null pointer argument");
+  Args a{};
+  a.q = (const uint16_t *)q;
+  a.kpool = (const uint16_t *)k_pool;
+  a.vpool = (const uint16_t *)v_pool;
+  a.bt = block_tables;
+  a.ctx = ctx_lens;
+  a.cu = cu_seqlens;
+  a.slopes = alibi_slopes;
+  a.out = (uint16_t *)out;
+  a.T = T;
+  a.B = B;
+  a.Hq = n_q_heads;
+  a.Hkv = n_kv_heads;
+  a.G = n_q_heads / n_kv_heads;
+  a.max_blocks = max_blocks_per_seq;
+  a.num_blocks = num_blocks;
+  a.num_layers = num_layers;
+  a.layer = layer;
+  a.bs = block_size;
+  a.window = window;
+  const Plan p = plan(T, std::min(max_query, T), B, a.G, n_kv_heads, max_keys, window, num_splits,
+                      false);
+  return run(a, p, head_dim, fp16, sm_scale, soft_cap, workspace, workspace_bytes, stream);
+}

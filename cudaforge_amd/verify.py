@@ -11,6 +11,8 @@ Reference semantics (paths inside Bahaa-Labs/CUDAForge):
   chain_verify, mode="python"  cudaforge/speculative.py:152-195
   tree_attention               paged layout of csrc/src/memory/paged_kv_cache.cpp:
                                13-21, 409-421; descriptor of paged_kv_cache.h:81-94
+  prompt_attention             dense causal attention of csrc/kernels/cuda/
+                               flash_attn_v2.cu:45-195, over the paged layout
   kv_commit                    device half of append_tokens, paged_kv_cache.cpp:255-286
   tree_verify                  speculative.cpp:50-150 generalised to a draft tree
 """
@@ -163,9 +165,51 @@ def chain_verify(target: torch.Tensor, draft: Optional[torch.Tensor],
 
 
 def tree_attention_workspace_bytes(B: int, N: int, n_q_heads: int, n_kv_heads: int,
-                                   head_dim: int, max_keys: int, num_splits: int = 0) -> int:
+                                   head_dim: int, max_keys: int, num_splits: int = 0, *,
+                                   scored: bool = False, window: int = 0) -> int:
+    """Workspace of ``tree_attention`` for N query nodes; `scored`: with a cap,
+    a bias, a window or fp16 tensors."""
+    if scored or window:
+        return int(_lib.load().cfa_tree_attention_scored_workspace_size(
+            B, N, n_q_heads, n_kv_heads, head_dim, max_keys, window, num_splits))
     return int(_lib.load().cfa_tree_attention_workspace_size(B, N, n_q_heads, n_kv_heads,
                                                               head_dim, max_keys, num_splits))
+
+
+def _half_dtype(q) -> torch.dtype:
+    """bfloat16, or float16 where q is."""
+    is_half = isinstance(q, torch.Tensor) and q.dtype == torch.float16
+    return torch.float16 if is_half else torch.bfloat16
+
+
+def _check_pools(k_pool: torch.Tensor, v_pool: torch.Tensor, dtype: torch.dtype, dev, Hq: int,
+                 D: int):
+    for name, pool in (("k_pool", k_pool), ("v_pool", v_pool)):
+        _require_cuda(name, pool, dtype, dev)
+        if pool.dim() != 5 or not pool.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous [blocks, layers, Hkv, block_size, D] tensor")
+    if k_pool.shape != v_pool.shape:
+        raise ValueError("k_pool and v_pool must have the same shape")
+    if k_pool.shape[4] != D:
+        raise ValueError("head_dim of q and of the pools differ")
+
+
+def _check_slopes(alibi_slopes: Optional[torch.Tensor], Hq: int, dev) -> Optional[torch.Tensor]:
+    if alibi_slopes is None:
+        return None
+    _require_cuda("alibi_slopes", alibi_slopes, torch.float32, dev)
+    if tuple(alibi_slopes.shape) != (Hq,):
+        raise ValueError(f"alibi_slopes must be [Hq] = [{Hq}]")
+    return alibi_slopes.contiguous()
+
+
+def _check_out(out: Optional[torch.Tensor], q: torch.Tensor) -> torch.Tensor:
+    if out is None:
+        return torch.empty_like(q)
+    _require_cuda("out", out, q.dtype, q.device)
+    if out.shape != q.shape or not out.is_contiguous():
+        raise ValueError("out must be a contiguous tensor of q's shape")
+    return out
 
 
 def tree_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
@@ -173,7 +217,9 @@ def tree_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
                    tree_mask: torch.Tensor, *, layer: int = 0,
                    sm_scale: Optional[float] = None, max_keys: Optional[int] = None,
                    num_splits: int = 0, out: Optional[torch.Tensor] = None,
-                   workspace: Optional[torch.Tensor] = None, first_node: int = 0) -> torch.Tensor:
+                   workspace: Optional[torch.Tensor] = None, first_node: int = 0,
+                   soft_cap: float = 0.0, alibi_slopes: Optional[torch.Tensor] = None,
+                   window: int = 0) -> torch.Tensor:
     """Tree-masked attention of draft-tree nodes over a paged KV cache.
 
     q [B, Nq, Hq, D] bf16 (D = 128 or 64): the queries of tree nodes
@@ -184,8 +230,19 @@ def tree_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
     ctx_len + i, i < N); tree_mask int64 [N] or [B, N] holding each node's
     64-bit ancestor-or-self mask.  max_keys bounds ctx_len + N on the host
     (computed with one sync when omitted).  Returns [B, Nq, Hq, D] bf16.
+
+    A tree of one node (tree_mask [1] holding 1) is plain decode.
+
+    Scores of other decoders (``cfa_tree_attention_scored``): soft_cap > 0
+    takes cap * tanh(s / cap) of each scaled score; alibi_slopes [Hq] fp32
+    subtracts slope * distance, where a node stands at ctx_len + its depth (the
+    bits of its mask less one); window > 0 hides keys at a distance of window
+    and more.  q and the pools may then be fp16, and Hq / Hkv * Nq may exceed
+    256; fp16 tensors take this path by themselves.  A query that sees no key
+    gets zeros.
     """
-    _require_cuda("q", q, torch.bfloat16)
+    dtype = _half_dtype(q)
+    _require_cuda("q", q, dtype)
     dev = q.device
     if q.dim() != 4:
         raise ValueError("q must be [B, Nq, Hq, D]")
@@ -194,15 +251,8 @@ def tree_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
         raise ValueError("first_node must be >= 0")
     N = first_node + Nq
     q = q.contiguous()
-    for name, pool in (("k_pool", k_pool), ("v_pool", v_pool)):
-        _require_cuda(name, pool, torch.bfloat16, dev)
-        if pool.dim() != 5 or not pool.is_contiguous():
-            raise ValueError(f"{name} must be a contiguous [blocks, layers, Hkv, block_size, D] tensor")
-    if k_pool.shape != v_pool.shape:
-        raise ValueError("k_pool and v_pool must have the same shape")
-    nblk, nlayers, Hkv, bs, Dp = k_pool.shape
-    if Dp != D:
-        raise ValueError("head_dim of q and of the pools differ")
+    _check_pools(k_pool, v_pool, dtype, dev, Hq, D)
+    nblk, nlayers, Hkv, bs, _ = k_pool.shape
     _require_cuda("block_tables", block_tables, torch.int32, dev)
     if block_tables.dim() != 2 or block_tables.shape[0] != B:
         raise ValueError("block_tables must be [B, max_blocks]")
@@ -223,20 +273,113 @@ def tree_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
         sm_scale = D ** -0.5
     if max_keys is None:
         max_keys = int(ctx_lens.max().item()) + N
-    if out is None:
+    scored = (soft_cap != 0.0 or alibi_slopes is not None or window != 0
+              or dtype == torch.float16)
+    if scored:
+        alibi_slopes = _check_slopes(alibi_slopes, Hq, dev)
+        out = _check_out(out, q)
+    elif out is None:
         out = torch.empty_like(q)
     lib = _lib.load()
-    need = int(lib.cfa_tree_attention_workspace_size(B, Nq, Hq, Hkv, D, max_keys, num_splits))
-    if workspace is None or workspace.numel() < need:
-        workspace = torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
     with torch.cuda.device(dev):
-        rc = lib.cfa_tree_attention(
-            q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), block_tables.data_ptr(),
-            block_tables.shape[1], ctx_lens.data_ptr(), nblk, nlayers, int(layer), bs,
-            tree_mask.data_ptr(), mstride, B, N, int(first_node), Hq, Hkv, D, ctypes.c_float(sm_scale),
-            int(max_keys), int(num_splits), out.data_ptr(), workspace.data_ptr(),
-            workspace.numel(), _stream_ptr(dev))
-    _lib.check(rc, "cfa_tree_attention")
+        if scored:
+            need = int(lib.cfa_tree_attention_scored_workspace_size(
+                B, Nq, Hq, Hkv, D, max_keys, window, num_splits))
+        else:
+            need = int(lib.cfa_tree_attention_workspace_size(B, Nq, Hq, Hkv, D, max_keys,
+                                                             num_splits))
+        if workspace is None or workspace.numel() < need:
+            workspace = torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
+        if scored:
+            rc = lib.cfa_tree_attention_scored(
+                q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), int(dtype == torch.float16),
+                block_tables.data_ptr(), block_tables.shape[1], ctx_lens.data_ptr(), nblk, nlayers,
+                int(layer), bs, tree_mask.data_ptr(), mstride, B, N, int(first_node), Hq, Hkv, D,
+                sm_scale, soft_cap, _ptr(alibi_slopes), int(window), int(max_keys),
+                int(num_splits), out.data_ptr(), workspace.data_ptr(), workspace.numel(),
+                _stream_ptr(dev))
+        else:
+            rc = lib.cfa_tree_attention(
+                q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), block_tables.data_ptr(),
+                block_tables.shape[1], ctx_lens.data_ptr(), nblk, nlayers, int(layer), bs,
+                tree_mask.data_ptr(), mstride, B, N, int(first_node), Hq, Hkv, D,
+                ctypes.c_float(sm_scale), int(max_keys), int(num_splits), out.data_ptr(),
+                workspace.data_ptr(), workspace.numel(), _stream_ptr(dev))
+    _lib.check(rc, "cfa_tree_attention_scored" if scored else "cfa_tree_attention")
+    return out
+
+
+def prompt_attention_workspace_bytes(T: int, B: int, n_q_heads: int, n_kv_heads: int,
+                                     head_dim: int, max_query: int, max_keys: int,
+                                     window: int = 0, num_splits: int = 0) -> int:
+    return int(_lib.load().cfa_prompt_attention_workspace_size(
+        T, B, n_q_heads, n_kv_heads, head_dim, max_query, max_keys, window, num_splits))
+
+
+def prompt_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
+                     block_tables: torch.Tensor, ctx_lens: torch.Tensor,
+                     cu_seqlens: torch.Tensor, *, layer: int = 0,
+                     sm_scale: Optional[float] = None, max_query: Optional[int] = None,
+                     max_keys: Optional[int] = None, soft_cap: float = 0.0,
+                     alibi_slopes: Optional[torch.Tensor] = None, window: int = 0,
+                     num_splits: int = 0, out: Optional[torch.Tensor] = None,
+                     workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Causal attention of prompt chunks over a paged KV cache
+    (``cfa_prompt_attention``).
+
+    q [T, Hq, D] (bf16 or fp16, D = 128 or 64) holds B sequences' new tokens one
+    after another: cu_seqlens int32 [B + 1] says where each begins.  ctx_lens
+    [B] int32 are the tokens in front of each chunk (0 for a first one); the
+    chunk's own K and V are in the pages already (``rotary.qk_norm_rope_kv``),
+    and token i of it sees the slots up to ctx_len + i.  Pools, block_tables,
+    soft_cap, alibi_slopes and window are those of ``tree_attention``.
+    max_query and max_keys are guesses of the longest chunk and of the largest
+    ctx_len + chunk (default T and the tables' capacity): they plan the call,
+    and any positive values are right.  Rows of q behind the last sequence get
+    no output: `out` keeps what it had there.  Returns out [T, Hq, D].
+    """
+    dtype = _half_dtype(q)
+    _require_cuda("q", q, dtype)
+    dev = q.device
+    if q.dim() != 3:
+        raise ValueError("q must be [T, Hq, D]")
+    T, Hq, D = q.shape
+    q = q.contiguous()
+    _check_pools(k_pool, v_pool, dtype, dev, Hq, D)
+    nblk, nlayers, Hkv, bs, _ = k_pool.shape
+    _require_cuda("ctx_lens", ctx_lens, torch.int32, dev)
+    if ctx_lens.dim() != 1:
+        raise ValueError("ctx_lens must be [B]")
+    B = ctx_lens.shape[0]
+    _require_cuda("block_tables", block_tables, torch.int32, dev)
+    if block_tables.dim() != 2 or block_tables.shape[0] != B:
+        raise ValueError("block_tables must be [B, max_blocks]")
+    _require_cuda("cu_seqlens", cu_seqlens, torch.int32, dev)
+    if tuple(cu_seqlens.shape) != (B + 1,):
+        raise ValueError("cu_seqlens must be [B + 1]")
+    block_tables, ctx_lens, cu_seqlens = (t.contiguous() for t in
+                                          (block_tables, ctx_lens, cu_seqlens))
+    alibi_slopes = _check_slopes(alibi_slopes, Hq, dev)
+    out = _check_out(out, q)
+    if sm_scale is None:
+        sm_scale = D ** -0.5
+    if max_query is None:
+        max_query = max(T, 1)
+    if max_keys is None:
+        max_keys = max(block_tables.shape[1] * bs, 1)
+    lib = _lib.load()
+    with torch.cuda.device(dev):
+        need = int(lib.cfa_prompt_attention_workspace_size(T, B, Hq, Hkv, D, max_query, max_keys,
+                                                           window, num_splits))
+        if workspace is None or workspace.numel() < need:
+            workspace = torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
+        rc = lib.cfa_prompt_attention(
+            q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), int(dtype == torch.float16),
+            block_tables.data_ptr(), block_tables.shape[1], ctx_lens.data_ptr(), nblk, nlayers,
+            int(layer), bs, cu_seqlens.data_ptr(), T, B, Hq, Hkv, D, sm_scale, soft_cap,
+            _ptr(alibi_slopes), int(window), int(max_query), int(max_keys), int(num_splits),
+            out.data_ptr(), workspace.data_ptr(), workspace.numel(), _stream_ptr(dev))
+    _lib.check(rc, "cfa_prompt_attention")
     return out
 
 

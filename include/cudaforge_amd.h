@@ -57,7 +57,8 @@ const char *cfa_last_error(void);
  * library built from this header.  Major 2 changed two contracts of major 1:
  * cfa_tree_verify takes (workspace, workspace_bytes) before its stream, and
  * python-mode cfa_chain_verify reads uniforms [B, K+2] (row stride K+2), not
- * [B, K+1].  Minor 1 of it adds cfa_qk_norm_rope_kv.
+ * [B, K+1].  Minor 1 of it adds cfa_qk_norm_rope_kv,
+ * cfa_tree_attention_scored and cfa_prompt_attention.
  * Binding code checks the major before its first call. */
 #define CFA_ABI_VERSION 201
 int cfa_version(void);
@@ -213,6 +214,66 @@ int cfa_tree_attention(const void *q, const void *k_pool, const void *v_pool,
                        int B, int N, int first_node, int n_q_heads, int n_kv_heads,
                        int head_dim, float sm_scale, int max_keys, int num_splits, void *out,
                        void *workspace, size_t workspace_bytes, void *stream);
+
+/* ---------------------------------------------------------------------------
+ * The same with capped scores, a distance bias or a sliding window (no
+ * counterpart in the reference), and for fp16: draft trees, and plain decode
+ * as trees of one node (tree_mask {1}).
+ *
+ *   fp16       0: q, pools and out are bf16; 1: fp16
+ *   soft_cap   s = soft_cap * tanh(s / soft_cap) for the scaled score s (0: none)
+ *   alibi_slopes [n_q_heads] fp32 (NULL: none): s -= slope * (query's position -
+ *              key's position), after the cap.  A tree node stands at ctx_len +
+ *              its depth, the number of bits of its tree_mask less one
+ *   window     a key is visible only while (query's position - key's position)
+ *              < window (0: no window).  Pages that lie wholly in front of every
+ *              query's window are not read and may be unmapped or reused
+ * Everything else is cfa_tree_attention's, except: n_q_heads / n_kv_heads times
+ * the query nodes may exceed 256; max_keys only plans the splits (a longer
+ * context is still attended to in full); partials are fp32.  A query that sees
+ * no key gets zeros.  Keys that no query of its block sees do not reach the
+ * output; a NaN or infinity in the V of a key that some of them see reaches all
+ * of that sequence's queries in the block.
+ * soft_cap is 0 or at least 1e-6.  The workspace size takes the query nodes (N
+ * - first_node) for N; 0: none is needed. */
+size_t cfa_tree_attention_scored_workspace_size(int B, int N, int n_q_heads, int n_kv_heads,
+                                                int head_dim, int max_keys, int window,
+                                                int num_splits);
+int cfa_tree_attention_scored(const void *q, const void *k_pool, const void *v_pool, int fp16,
+                              const int32_t *block_tables, int max_blocks_per_seq,
+                              const int32_t *ctx_lens, int num_blocks, int num_layers, int layer,
+                              int block_size, const uint64_t *tree_mask,
+                              int64_t tree_mask_stride_b, int B, int N, int first_node,
+                              int n_q_heads, int n_kv_heads, int head_dim, float sm_scale,
+                              float soft_cap, const float *alibi_slopes, int window, int max_keys,
+                              int num_splits, void *out, void *workspace, size_t workspace_bytes,
+                              void *stream);
+
+/* Chunks of prompts: causal attention of B sequences' new tokens, packed, over
+ * the paged cache, with the same scores (the reference has dense causal
+ * attention of whole prompts, csrc/kernels/cuda/flash_attn_v2.cu:45-195).
+ *
+ *   q, out     [T, n_q_heads, head_dim]; tokens cu_seqlens[b] .. cu_seqlens[b +
+ *              1] - 1 (int32 [B + 1], rising) are sequence b's
+ *   ctx_lens   [B] tokens of the sequence in front of the chunk (a first chunk:
+ *              0); the chunk's own K and V sit at slots ctx_len + i already, and
+ *              token i sees every slot up to ctx_len + i
+ *   max_query, max_keys  host-side guesses of the longest chunk and of the
+ *              largest ctx_len + chunk; they plan blocks and splits, results are
+ *              right for any positive values
+ * Rows of tokens that belong to no sequence are left as they were.  T = 0 and
+ * B = 0 are allowed.  No key behind a block's last token is read. */
+size_t cfa_prompt_attention_workspace_size(int T, int B, int n_q_heads, int n_kv_heads,
+                                           int head_dim, int max_query, int max_keys, int window,
+                                           int num_splits);
+int cfa_prompt_attention(const void *q, const void *k_pool, const void *v_pool, int fp16,
+                         const int32_t *block_tables, int max_blocks_per_seq,
+                         const int32_t *ctx_lens, int num_blocks, int num_layers, int layer,
+                         int block_size, const int32_t *cu_seqlens, int T, int B, int n_q_heads,
+                         int n_kv_heads, int head_dim, float sm_scale, float soft_cap,
+                         const float *alibi_slopes, int window, int max_query, int max_keys,
+                         int num_splits, void *out, void *workspace, size_t workspace_bytes,
+                         void *stream);
 
 /* ---------------------------------------------------------------------------
  * Tree verification: multi-candidate rejection sampling down a draft tree,
