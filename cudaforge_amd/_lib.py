@@ -121,6 +121,9 @@ SIGNATURES: dict[str, tuple] = {
     "cfa_sample_workspace_size": (_sz, [_i, _i, _i, _i]),
     "cfa_sample": (
         _i, [_p, _i64, _i, _i, _i, _i, _f, _i, _f, _i, _p, _p, _p, _p, _sz, _p]),
+    "cfa_sample_rows_workspace_size": (_sz, [_i, _i]),
+    "cfa_sample_rows": (
+        _i, [_p, _i64, _i, _i, _i, _i, _p, _f, _p, _i, _p, _f, _p, _f, _p, _p, _p, _p, _sz, _p]),
     "cfa_tree_attention_workspace_size": (_sz, [_i, _i, _i, _i, _i, _i, _i]),
     "cfa_tree_attention": (
         _i,

@@ -20,6 +20,10 @@ filtered (top-p keep rule of ``cudaforge/speculative.py:67-81`` plus top-k,
 renormalised), or greedy top-k; several independent draws per row.
 ``expand_tree_level`` uses it to draw the children of draft-tree nodes.
 
+``sample_rows`` (``cfa_sample_rows``) serves batches whose requests have their
+own temperature, top-k, top-p and min-p; ``filtered_probs`` gives the same
+rows' probabilities alone, for verification (``input_kind="probs"``).
+
 Every call runs on the HIP library; there is no CPU fallback.
 """
 from __future__ import annotations
@@ -39,6 +43,9 @@ __all__ = [
     "fused_sampling_triton",
     "launch_fused_sampling",
     "expand_tree_level",
+    "sample_rows",
+    "sample_rows_workspace_bytes",
+    "filtered_probs",
 ]
 
 _SMODES = {"multinomial": _lib.CFA_SAMPLE_MULTINOMIAL, "filtered": _lib.CFA_SAMPLE_FILTERED,
@@ -187,6 +194,97 @@ def expand_tree_level(draft_rows: torch.Tensor, *, children: int = 2, mode: str 
         out = sample(draft_rows, mode="greedy", draws=children)
         return (out, None) if return_probs else out
     raise ValueError("mode must be 'sample' or 'greedy'")
+
+
+_ROW_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def sample_rows_workspace_bytes(R: int, V: int) -> int:
+    return int(_lib.load().cfa_sample_rows_workspace_size(R, V))
+
+
+def _setting(name: str, value, R: int, dtype: torch.dtype, dev, ok, says: str):
+    """(device pointer or None, scalar, what to keep alive) of a row setting."""
+    if isinstance(value, torch.Tensor):
+        _require_cuda(name, value, dtype, dev)
+        if tuple(value.shape) != (R,):
+            raise ValueError(f"{name} must be a number or [R] = [{R}]")
+        value = value.contiguous()
+        return value.data_ptr(), 0, value
+    if not ok(value):
+        raise ValueError(f"{name} must be {says}")
+    return None, value, None
+
+
+def sample_rows(rows: torch.Tensor, uniforms: Optional[torch.Tensor] = None, *,
+                temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, draws: Optional[int] = None,
+                generator: Optional[torch.Generator] = None, return_probs: bool = False,
+                workspace: Optional[torch.Tensor] = None):
+    """Draw from rows [R, V] of logits (fp32, bf16 or fp16), each row with its
+    own settings: temperature, top_p, min_p (fp32 [R] tensors) and top_k (int32
+    [R]), or numbers for all rows.
+
+    A row keeps its first tokens in the order of falling logits (equal ones:
+    lower index first): rank < top_k (<= 0: off), softmax mass in front < top_p
+    (1: off), probability >= min_p times the largest (0: off); temperature 0
+    keeps the largest alone.  uniforms fp32 [R, draws] in [0, 1) pick the first
+    kept index whose kept mass exceeds u of the whole; without them they come
+    from `generator` (`draws` a row, default 1).  -inf masks a token; a row of
+    masked tokens alone gives -1.  Returns int32 [R, draws], and with
+    return_probs the renormalised probabilities [R, V] fp32 the draws used.
+    """
+    if not isinstance(rows, torch.Tensor) or rows.device.type != "cuda":
+        raise ValueError("rows must be a HIP device tensor")
+    if rows.dtype not in _ROW_TYPES:
+        raise ValueError("rows must be float32, bfloat16 or float16")
+    if rows.dim() != 2 or rows.shape[1] == 0:
+        raise ValueError("rows must be [R, V] with V > 0")
+    R, V = rows.shape
+    dev = rows.device
+    if rows.stride(1) != 1 or (R > 1 and rows.stride(0) < V):
+        rows = rows.contiguous()
+    if uniforms is not None:
+        _require_cuda("uniforms", uniforms, torch.float32, dev)
+        if uniforms.dim() != 2 or uniforms.shape[0] != R or draws not in (None, uniforms.shape[1]):
+            raise ValueError("uniforms must be [R, draws]")
+        uniforms = uniforms.contiguous()
+        draws = uniforms.shape[1]
+    else:
+        draws = 1 if draws is None else int(draws)
+        if draws < 0:
+            raise ValueError("draws must not be negative")
+        uniforms = torch.rand(R, draws, device=dev, generator=generator, dtype=torch.float32)
+    settings = [
+        _setting("temperature", temperature, R, torch.float32, dev,
+                 lambda v: 0.0 <= v < float("inf"), "finite and not negative"),
+        _setting("top_k", top_k, R, torch.int32, dev, lambda v: v == int(v), "an integer"),
+        _setting("top_p", top_p, R, torch.float32, dev, lambda v: 0.0 < v <= 1.0, "in (0, 1]"),
+        _setting("min_p", min_p, R, torch.float32, dev, lambda v: 0.0 <= v <= 1.0, "in [0, 1]")]
+    (t, t0, _), (k, k0, _), (p, p0, _), (m, m0, _) = settings
+    k0 = min(max(int(k0), 0), 2 ** 31 - 1)
+    tokens = torch.empty(R, draws, dtype=torch.int32, device=dev)
+    probs = torch.empty(R, V, dtype=torch.float32, device=dev) if return_probs else None
+    lib = _lib.load()
+    need = int(lib.cfa_sample_rows_workspace_size(R, V))
+    if workspace is None or workspace.numel() < need:
+        workspace = torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
+    with torch.cuda.device(dev):
+        rc = lib.cfa_sample_rows(
+            rows.data_ptr(), rows.stride(0), _ROW_TYPES[rows.dtype], R, V, draws, t, t0, k, k0, p,
+            p0, m, m0, uniforms.data_ptr(), tokens.data_ptr(),
+            probs.data_ptr() if return_probs else None, workspace.data_ptr(), workspace.numel(),
+            _stream_ptr(dev))
+    _lib.check(rc, "cfa_sample_rows")
+    return (tokens, probs) if return_probs else tokens
+
+
+def filtered_probs(rows: torch.Tensor, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
+                   workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The probabilities [R, V] fp32 that sample_rows draws from: what
+    ``verify.chain_verify`` and ``verify.tree_verify`` take as
+    ``input_kind="probs"`` of filtered distributions."""
+    return sample_rows(rows, draws=0, temperature=temperature, top_k=top_k, top_p=top_p,
+                       min_p=min_p, return_probs=True, workspace=workspace)[1]
 
 
 class _Null:

@@ -58,7 +58,7 @@ const char *cfa_last_error(void);
  * cfa_tree_verify takes (workspace, workspace_bytes) before its stream, and
  * python-mode cfa_chain_verify reads uniforms [B, K+2] (row stride K+2), not
  * [B, K+1].  Minor 1 of it adds cfa_qk_norm_rope_kv,
- * cfa_tree_attention_scored and cfa_prompt_attention.
+ * cfa_tree_attention_scored, cfa_prompt_attention and cfa_sample_rows.
  * Binding code checks the major before its first call. */
 #define CFA_ABI_VERSION 201
 int cfa_version(void);
@@ -172,6 +172,36 @@ int cfa_sample(const float *rows, int64_t row_stride, int input_kind, int R, int
                float temperature, int top_k, float top_p, int mode, const float *uniforms,
                int32_t *out_tokens, float *out_probs, void *workspace, size_t workspace_bytes,
                void *stream);
+
+/* Draws from rows that have settings of their own (the reference's sampler
+ * takes one top_k / top_p for all and applies neither, sampling.h:18-28).
+ *
+ *   rows        [R, V] of elem_type 0 fp32, 1 bf16 or 2 fp16, row r at rows + r *
+ *               row_stride elements; V <= 2^20.  -inf masks a token, NaN counts
+ *               as -inf, +inf as the largest finite value
+ *   temperature, top_k, top_p, min_p   [R] device arrays, or NULL: the scalar
+ *               behind each holds for all rows
+ *   uniforms    [R, draws] fp32 in [0, 1); draws <= 64, independent draws
+ * With w_i = exp((x_i - max) / T) and Z their sum, in the order of falling x
+ * (equal values: lower index first) a row keeps its first tokens, those with
+ * rank < top_k (<= 0: all), mass in front of them < top_p Z (>= 1: all) and w >=
+ * min_p (<= 0: all), at least one.  A draw takes the first kept index, in the
+ * order of indices, whose kept mass up to and with itself exceeds u times the
+ * kept mass.  T <= 0 (and NaN) keeps the largest alone.  Unlike
+ * CFA_SAMPLE_FILTERED, equal values at a border are not kept together.
+ *   out_tokens  [R, draws] int32; -1 in a row whose every token is masked
+ *   out_probs   [R, V] fp32 contiguous, or NULL: the kept tokens' weights over
+ *               their sum, zeros elsewhere.  With draws = 0 only these
+ * Weights are formed in fp64 and summed exactly (41 fractional bits of the
+ * largest weight of 8192 tokens): results do not depend on the run.
+ * workspace: cfa_sample_rows_workspace_size bytes, 16-byte aligned; calls that
+ * share one must not overlap.  R = 0 is allowed. */
+size_t cfa_sample_rows_workspace_size(int R, int V);
+int cfa_sample_rows(const void *rows, int64_t row_stride, int elem_type, int R, int V, int draws,
+                    const float *temperature, float temperature_all, const int32_t *top_k,
+                    int top_k_all, const float *top_p, float top_p_all, const float *min_p,
+                    float min_p_all, const float *uniforms, int32_t *out_tokens, float *out_probs,
+                    void *workspace, size_t workspace_bytes, void *stream);
 
 /* ---------------------------------------------------------------------------
  * Tree-masked verification attention over a paged KV cache (bf16, MFMA).
