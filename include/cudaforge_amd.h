@@ -192,8 +192,8 @@ int cfa_sample(const float *rows, int64_t row_stride, int input_kind, int R, int
  *   out_tokens  [R, draws] int32; -1 in a row whose every token is masked
  *   out_probs   [R, V] fp32 contiguous, or NULL: the kept tokens' weights over
  *               their sum, zeros elsewhere.  With draws = 0 only these
- * Weights are formed in fp64 and summed exactly (41 fractional bits of the
- * largest weight of 8192 tokens): results do not depend on the run.
+ * Weights are formed in fp64 and summed exactly as fractions of 36 bits of the
+ * largest weight of 8192 tokens: results do not depend on the run.
  * workspace: cfa_sample_rows_workspace_size bytes, 16-byte aligned; calls that
  * share one must not overlap.  R = 0 is allowed. */
 size_t cfa_sample_rows_workspace_size(int R, int V);

@@ -36,13 +36,13 @@ def test_nothing_to_draw_launches_nothing():
 
 
 def test_workspace_size():
-    # per 8192 tokens: the maximum, 512 counts and 512 masses; per row its cut
+    # per 8192 tokens: the maximum and 512 bins; per row its cut
     def up(x):
         return -(-x // 256) * 256
 
     for R, V in ((1, 1), (3, 8192), (64, 128256), (2, 2 ** 20)):
         n = R * -(-V // 8192)
-        assert sample_rows_workspace_bytes(R, V) == up(4 * n) + up(n * 2048) + up(n * 4096) + up(32 * R)
+        assert sample_rows_workspace_bytes(R, V) == up(4 * n) + up(n * 4096) + up(32 * R)
     assert sample_rows_workspace_bytes(0, 10) == 0
     assert sample_rows_workspace_bytes(1, 2 ** 20 + 1) == 0
 

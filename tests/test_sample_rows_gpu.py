@@ -1,11 +1,13 @@
 """GPU tier: cfa_sample_rows against its definition in 64 bits, on the host.
 
-Tokens are whole numbers and must be equal.  Both sides sum about V weights
-with errors below 2^-41 of the largest each, so a draw whose uniform (or a
-top-p border) lies within 1e-9 of a step of the sums could differ; `_want` finds
-such draws (about one in 10^4 here) and the tests exclude them by that rule.
-Probabilities: the kept weight over the kept mass, rounded once to fp32 (2^-24)
-on top of fp64 and 2^-41 sums: 2^-23 of the value."""
+Tokens are whole numbers and must be equal.  The kernel's weights are off by
+2^-37 of the largest at most, to either side: a sum of V = 128256 by sqrt(V) 2^-37
+0.58 = 1.5e-9 of the largest weight (one standard deviation), less of the whole.
+A draw whose uniform (or a top-p border) lies within 1e-9 of a step of the sums
+could therefore differ; `_want` finds such draws (about one in 10^4 here) and the
+tests exclude them by that rule.  Probabilities: the kept weight over the kept
+mass, rounded once to fp32 (2^-24) on top of sums off by 2^-29: 2^-23 of the
+value."""
 import numpy as np
 import pytest
 import torch
