@@ -96,6 +96,21 @@ static int run(Args &a, const Plan &p, int D, int fp16, float sm_scale, float so
   a.blocks = (int)p.blocks;
   a.cap = soft_cap;
   a.scale = soft_cap > 0.0f ? sm_scale / soft_cap : sm_scale;
+  if (soft_cap > 0.0f) {
+    const double t = (double)sm_scale / soft_cap, unit = soft_cap * 1.4426950408889634 * t;
+    a.k0 = (float)(unit * kT0);
+    a.k1 = (float)(unit * kT1 * t * t);
+    a.k2 = (float)(unit * kT2 * t * t * t * t);
+    a.k3 = (float)(unit * kT3 * t * t * t * t * t * t);
+    // a coefficient that fp32 does not hold (scores far below the cap) is left
+    // out, and the polynomial kept to where its term is below 5e-7
+    double far = kTanhSmall;
+    if (std::fabs(a.k3) < 1e-37f) a.k3 = 0.0f, far = 0.14;
+    if (std::fabs(a.k2) < 1e-37f) a.k2 = 0.0f, far = 0.04;
+    if (std::fabs(a.k1) < 1e-37f) a.k1 = 0.0f, far = 0.001;
+    const double small = t != 0.0 ? far / std::fabs(t) : 1e18;
+    a.small = (float)std::min(small, 1e18);  // (x^2 stays in fp32's range)
+  }
   const long long grid = (long long)p.splits * a.Hkv * p.blocks;
   if (grid * kNT >= (1LL << 32)) return fail_arg("too many queries for one call");
   if (p.splits > 1) {

@@ -18,12 +18,12 @@
 // stream through LDS, and each lane owns one query column.  What differs:
 //  * Q stays as it is and the scale is applied to the products in fp32 (one
 //    fma a score, with the base): a pre-scaled Q would be rounded once more.
-//  * tanh.  While every |s / cap| of a wave's tile is below 3/4, tanh(t) / t is
-//    a polynomial of degree 4 in t^2 (least maximum relative error on that
-//    range, 5.7e-7): it keeps small scores exact under a large cap, where 1 -
-//    2 / (1 + e^2t) cancels, and is six fp32 operations against two
-//    transcendental ones (16 cycles each) and three others.  Tiles beyond that
-//    take the exponential form.
+//  * tanh.  While every |s / cap| of a wave's tile is below 1/2, tanh(t) / t is
+//    a polynomial of degree 3 in t^2 (least maximum relative error on that
+//    range, 5.4e-7): it keeps small scores exact under a large cap, where 1 -
+//    2 / (1 + e^2t) cancels, and with its coefficients in the products' units it
+//    is five fp32 operations, against two transcendental ones (16 cycles each)
+//    and three others.  Tiles beyond that take the exponential form.
 //  * Capped scores without a bias lie in [-cap, cap], so bf16 probabilities
 //    need no running maximum while 2^(cap log2 e) times a sum of values stays
 //    in fp32's range (kFixedCap): P = exp2(s), no maxima, no rescaling.  Others
@@ -48,13 +48,14 @@ namespace scored {
 
 using namespace cfa::tree;
 
-// tanh(t) / t = kT0 + kT1 t^2 + ... + kT4 t^8 for |t| <= kTanhSmall
-constexpr float kTanhSmall = 0.75f;
-constexpr float kT0 = 0.9999994349232844f, kT1 = -0.3332825152895064f, kT2 = 0.13258983189591972f,
-                kT3 = -0.05005630179239906f, kT4 = 0.012929631620462257f;
+// tanh(t) / t = kT0 + kT1 t^2 + kT2 t^4 + kT3 t^6 for |t| <= kTanhSmall
+constexpr float kTanhSmall = 0.5f;
+constexpr float kT0 = 0.9999994557706551f, kT1 = -0.3332631793391637f, kT2 = 0.13190296581701041f,
+                kT3 = -0.04440222555554884f;
 // cap log2(e) up to which exp2 needs no base: sums of 2^24 keys times values
 // of 2^20 stay below 2^127, and 2^-80 is a normal bf16
 constexpr float kFixedCap = 80.0f;
+constexpr int kPeekSteps = 4;  // tiles of a split from which the last one is seen first
 
 struct Args {
   const uint16_t *q;      // [rows of tokens, Hq, D]
@@ -75,6 +76,9 @@ struct Args {
   int max_blocks, num_blocks, num_layers, layer, bs;
   int splits, window;
   float scale, cap;       // scale as given, or with a cap scale / cap
+  // with a cap: its score in log2 units is x (k0 + k1 x^2 + k2 x^4 + k3 x^6) for
+  // a product |x| <= small
+  float k0, k1, k2, k3, small;
 };
 
 // The block of query tokens of a work-group.
@@ -125,23 +129,21 @@ __device__ __forceinline__ bool find_block(const Args &a, int id, int lane, Bloc
   return false;
 }
 
-// What a lane knows of its query column besides Q.
-struct Column {
-  uint64_t anc;  // trees: visible nodes (ancestors inside the window)
-  int pos;       // position
-  int first;     // first visible position (window), else 0
-  float slope2;  // slope * log2(e)
+// What a query row's scores need besides its Q, in LDS: registers held across
+// the MFMA phase are what its operand reads are scheduled ahead with (four more,
+// and the compiler drops that schedule: 692 against 519 us for the plain prompt).
+struct Row {
+  uint64_t anc;   // trees: visible nodes (ancestors inside the window)
+  int pos;        // position
+  int first;      // first visible position (window), else 0
+  float slope2;   // distance bias: slope * log2(e)
 };
 
-// Scores of one tile in log2 units less the base (S in: raw products), masked,
-// to probabilities; the lazy maximum where kFixed does not hold.
 template <int D, int QT, class T, bool CAP, bool BIAS, bool FIXED>
-__device__ __forceinline__ void score_phase(const Lane<D, QT, T> &ln, const Column (&cl)[QT],
-                                            const Args &a, float k0, float cap2, int kbase, int ctx,
-                                            int least, int most_first, const int *sdepth,
-                                            Scores<QT> &S, Softmax<QT> &sm,
-                                            f32x4 (&o)[QT][D / 16], f32x4 (&lacc)[QT],
-                                            Probs<QT, T> &P) {
+__device__ __forceinline__ void raw_scores(const Lane<D, QT, T> &ln, const float (&base_of)[QT],
+                                           const Args &a, float k0, float cap2, int kbase, int ctx,
+                                           int least, int most_first, const Row *rows,
+                                           const float *move, Scores<QT> &S) {
   const bool tree = a.mask != nullptr;
   // tanh: the polynomial while the whole wave's tile is small
   bool small = true;
@@ -155,70 +157,75 @@ __device__ __forceinline__ void score_phase(const Lane<D, QT, T> &ln, const Colu
         for (int t = 0; t < 2; ++t)
 #pragma unroll
           for (int i = 0; i < 4; ++i) m = fmaxf(m, fabsf(S.s[qt][blk][t][i]));
-    // a.scale = sm_scale / cap; NaN (lost by fmaxf) stays NaN in either form
-    small = __ballot(m * fabsf(a.scale) > kTanhSmall) == 0;
+    // (NaN, lost by fmaxf, stays NaN in either form)
+    small = __ballot(m > a.small) == 0;
   }
-  const bool tree_keys = tree && kbase + kKT > ctx;
+  // f(score, what to add to it): every score of the tile.  (The choice of form
+  // stays outside: as a condition inside the loops it became a branch a score,
+  // 964 us instead of the present time for the capped prompt of 8192.)
+  auto every = [&](auto f) {
 #pragma unroll
-  for (int qt = 0; qt < QT; ++qt) {
-    float base = FIXED ? 0.0f : -sm.b[qt];
-    const float slope = BIAS ? cl[qt].slope2 : 0.0f;
-    if constexpr (BIAS)  // of the lane's first key; exact until rounded once
-      base += slope * (float)(kbase + 8 * ln.g - cl[qt].pos);
+    for (int qt = 0; qt < QT; ++qt) {
+      float base = FIXED ? 0.0f : -base_of[qt], slope = 0.0f;
+      if constexpr (BIAS) {  // of the lane's first key; exact until rounded once
+        slope = rows[qt * 16].slope2;
+        base += slope * (float)(kbase + 8 * ln.g - rows[qt * 16].pos);
+      }
+#pragma unroll
+      for (int blk = 0; blk < 2; ++blk)
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            S.s[qt][blk][t][i] =
+                f(S.s[qt][blk][t][i],
+                  BIAS ? fmaf(slope, (float)(blk * 32 + 4 * t + i), base) : base);
+    }
+  };
+  if constexpr (!CAP) {
+    every([&](float x, float add) { return fmaf(x, k0, add); });
+  } else if (small) {
+    every([&](float x, float add) {
+      const float w = x * x;
+      float p = fmaf(w, a.k3, a.k2);
+      p = fmaf(w, p, a.k1);
+      p = fmaf(w, p, a.k0);
+      return FIXED ? x * p : fmaf(x, p, add);
+    });
+  } else {
+    every([&](float x, float add) {
+      const float r = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * k0));
+      return fmaf(r, -2.0f * cap2, FIXED ? cap2 : cap2 + add);
+    });
+  }
+  if (BIAS && tree && kbase + kKT > ctx) {
+    // a tree key stands at ctx + its depth, not at its slot
+    const float *mv = move + (kbase + 8 * ln.g - ctx);
 #pragma unroll
     for (int blk = 0; blk < 2; ++blk)
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int off = blk * 32 + 4 * t + i;
-          float add = BIAS ? fmaf(slope, (float)off, base) : base;
-          const float x = S.s[qt][blk][t][i];
-          if constexpr (CAP) {
-            if (small) {
-              const float u = x * a.scale, w = u * u;
-              float p = fmaf(w, kT4, kT3);
-              p = fmaf(w, p, kT2);
-              p = fmaf(w, p, kT1);
-              p = fmaf(w, p, kT0);
-              S.s[qt][blk][t][i] = fmaf(u * cap2, p, add);
-            } else {
-              const float r = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * k0));
-              S.s[qt][blk][t][i] = fmaf(r, -2.0f * cap2, cap2 + add);
-            }
-          } else {
-            S.s[qt][blk][t][i] = fmaf(x, k0, add);
-          }
+          const float by = mv[blk * 32 + 4 * t + i];
+#pragma unroll
+          for (int qt = 0; qt < QT; ++qt)
+            S.s[qt][blk][t][i] = fmaf(rows[qt * 16].slope2, by, S.s[qt][blk][t][i]);
         }
-    if constexpr (BIAS) {
-      if (tree_keys) {
-        // a tree key's distance is the difference of the depths
-#pragma unroll
-        for (int blk = 0; blk < 2; ++blk)
-#pragma unroll
-          for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int slot = kbase + 8 * ln.g + blk * 32 + 4 * t + i;
-              const int j = min(max(slot - ctx, 0), 63);
-              const int moved = slot >= ctx ? ctx + sdepth[j] - slot : 0;
-              S.s[qt][blk][t][i] = fmaf(slope, (float)moved, S.s[qt][blk][t][i]);
-            }
-      }
-    }
   }
   if (kbase + kKT > least || kbase < most_first) {
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
       // bit k: tile key k is visible to this column
+      const Row r = rows[qt * 16];
       uint64_t vis;
       if (tree) {
-        vis = tile_visibility(kbase, ctx, cl[qt].anc);
+        vis = tile_visibility(kbase, ctx, r.anc);
       } else {
-        const int n = cl[qt].pos + 1 - kbase;
+        const int n = r.pos + 1 - kbase;
         vis = n >= 64 ? ~0ull : (n <= 0 ? 0ull : ((1ull << n) - 1));
       }
-      const int cut = min(cl[qt].first, tree ? ctx : cl[qt].first) - kbase;  // keys in front
+      const int cut = min(r.first, tree ? ctx : r.first) - kbase;  // keys in front
       if (cut > 0) vis = cut >= 64 ? 0ull : vis >> cut << cut;
       vis >>= 8 * ln.g;
 #pragma unroll
@@ -231,38 +238,48 @@ __device__ __forceinline__ void score_phase(const Lane<D, QT, T> &ln, const Colu
                 ((vis >> (blk * 32 + 4 * t + i)) & 1ull) ? S.s[qt][blk][t][i] : -INFINITY;
     }
   }
+}
+
+template <int QT>
+__device__ __forceinline__ float score_max(const Scores<QT> &S, int qt) {
+  float v = -INFINITY;
+#pragma unroll
+  for (int blk = 0; blk < 2; ++blk)
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v = fmaxf(v, S.s[qt][blk][t][i]);
+  return column_max(v);
+}
+
+// Scores of one tile to probabilities; the columns' lazy bases b (log2 units; 0:
+// none yet, where the sum is 0 too) where FIXED does not hold.
+template <int D, int QT, class T, bool FIXED>
+__device__ __forceinline__ void score_phase(Scores<QT> &S, float (&b)[QT], f32x4 (&o)[QT][D / 16],
+                                            f32x4 (&lacc)[QT], Probs<QT, T> &P) {
   if constexpr (!FIXED) {
     float mx[QT];
-    bool resc[QT];
     bool any = false;
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
-      float v = -INFINITY;
-#pragma unroll
-      for (int blk = 0; blk < 2; ++blk)
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) v = fmaxf(v, S.s[qt][blk][t][i]);
-      mx[qt] = column_max(v);
-      resc[qt] = mx[qt] > -INFINITY && (!sm.valid[qt] || mx[qt] > kRescaleSlack);
-      any |= resc[qt];
+      mx[qt] = score_max(S, qt);
+      const bool unset = b[qt] == 0.0f && lacc[qt][0] == 0.0f && mx[qt] > -INFINITY;
+      mx[qt] = mx[qt] > kRescaleSlack || unset ? mx[qt] : 0.0f;  // what the base moves by
+      any |= mx[qt] != 0.0f;
     }
     if (__ballot(any) != 0) {
 #pragma unroll
       for (int qt = 0; qt < QT; ++qt) {
-        const float d = resc[qt] ? mx[qt] : 0.0f;
-        const float alpha =
-            resc[qt] ? (sm.valid[qt] ? __builtin_amdgcn_exp2f(-d) : 0.0f) : 1.0f;
-        sm.b[qt] += d;
-        sm.valid[qt] = sm.valid[qt] || resc[qt];
+        // (a base falls only while the sums are still 0)
+        const float alpha = __builtin_amdgcn_exp2f(-fmaxf(mx[qt], 0.0f));
+        b[qt] += mx[qt];
         lacc[qt] *= alpha;
 #pragma unroll
         for (int dt = 0; dt < D / 16; ++dt) o[qt][dt] *= alpha;
 #pragma unroll
         for (int blk = 0; blk < 2; ++blk)
 #pragma unroll
-          for (int t = 0; t < 2; ++t) S.s[qt][blk][t] -= d;
+          for (int t = 0; t < 2; ++t) S.s[qt][blk][t] -= mx[qt];
       }
     }
   }
@@ -291,7 +308,10 @@ __global__ __launch_bounds__(kNT) void scored_attn_kernel(Args a) {
   // row offsets of the split's 16-key groups; a ring of kMaxGroups, refilled
   // half a ring at a time in longer splits
   __shared__ long long gtab[kMaxGroups];
-  __shared__ int sdepth[64];
+  __shared__ long long gpeek[kKT / 16];
+  // trees: how far node j's position lies from its slot, at 64 + j; 0 around them
+  __shared__ float smove[192];
+  __shared__ Row srow[kMaxRows];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, g = lane >> 4;
@@ -316,7 +336,8 @@ __global__ __launch_bounds__(kNT) void scored_attn_kernel(Args a) {
   const int nkeys = min(ctx + last, cap_keys);
 
   Lane<D, QT, T> ln;
-  Column cl[QT];
+  float base[QT];  // exponent bases
+  Row row[QT];
   bool qvalid[QT];
   ln.g = g;
   int low;  // the first query's position (trees: the shallowest's)
@@ -324,7 +345,10 @@ __global__ __launch_bounds__(kNT) void scored_attn_kernel(Args a) {
     const uint64_t nodes = a.N >= 64 ? ~0ull : ((1ull << a.N) - 1);
     const uint64_t mine = lane < a.N ? a.mask[(long long)b * a.mask_sb + lane] & nodes : 0ull;
     const int depth = max((int)__popcll(mine) - 1, 0);
-    if (wave == 0) sdepth[lane] = depth;
+    if (BIAS && wave < 3) {
+      const int node = lane + 64 * (wave - 1);  // wave 1 holds the nodes
+      smove[64 + node] = node >= 0 && node < a.N ? (float)(depth - node) : 0.0f;
+    }
     const int j = a.q0 + blk.i0;
     int d = lane >= j && lane < j + blk.nt ? depth : 64;
 #pragma unroll
@@ -337,11 +361,11 @@ __global__ __launch_bounds__(kNT) void scored_attn_kernel(Args a) {
       const int node = j + (qvalid[qt] ? r / a.G : 0);
       uint64_t anc = __shfl((unsigned long long)mine, node, 64);
       const int dq = __shfl(depth, node, 64);
-      cl[qt].pos = ctx + dq;
+      row[qt].pos = ctx + dq;
       if (a.window > 0)  // nodes that lie `window` and more above are out of it
         for (int m = 0; m < a.N; ++m)
           if (dq - __shfl(depth, m, 64) >= a.window) anc &= ~(1ull << m);
-      cl[qt].anc = qvalid[qt] ? anc : 0ull;
+      row[qt].anc = qvalid[qt] ? anc : 0ull;
     }
   } else {
     low = ctx + blk.i0;
@@ -349,8 +373,8 @@ __global__ __launch_bounds__(kNT) void scored_attn_kernel(Args a) {
     for (int qt = 0; qt < QT; ++qt) {
       const int r = (wave * QT + qt) * 16 + col;
       qvalid[qt] = r < rows;
-      cl[qt].pos = low + (qvalid[qt] ? r / a.G : 0);
-      cl[qt].anc = 0;
+      row[qt].pos = low + (qvalid[qt] ? r / a.G : 0);
+      row[qt].anc = 0;
     }
   }
   const int high = tree ? ctx + 63 : low + blk.nt - 1;  // no query stands behind it
@@ -361,7 +385,7 @@ __global__ __launch_bounds__(kNT) void scored_attn_kernel(Args a) {
   const int tlo = from / kKT, thi = (nkeys + kKT - 1) / kKT;
   const int tps = (thi - tlo + a.splits - 1) / a.splits;
   const int t0 = tlo + split * tps, t1 = min(thi, t0 + tps);
-  const int g0 = t0 * (kKT / 16);
+  const int steps = t1 - t0;
   constexpr float kLog2e = 1.4426950408889634f;
   const float cap2 = a.cap * kLog2e;
   // without a cap: score in log2 units = product * k0; with one: e^(2 s / cap)
@@ -373,8 +397,10 @@ __global__ __launch_bounds__(kNT) void scored_attn_kernel(Args a) {
     const int r = (wave * QT + qt) * 16 + col;
     const int nl = qvalid[qt] ? r / a.G : 0, hg = qvalid[qt] ? r % a.G : 0;
     const int head = h * a.G + hg;
-    cl[qt].first = a.window > 0 ? max(cl[qt].pos - a.window + 1, 0) : 0;
-    cl[qt].slope2 = BIAS ? a.slopes[head] * kLog2e : 0.0f;
+    row[qt].first = a.window > 0 ? max(row[qt].pos - a.window + 1, 0) : 0;
+    row[qt].slope2 = BIAS ? a.slopes[head] * kLog2e : 0.0f;
+    if (g == 0) srow[r] = row[qt];
+    base[qt] = 0.0f;
     const uint16_t *qp = a.q + (((long long)blk.t0 + nl) * a.Hq + head) * D;
 #pragma unroll
     for (int kk = 0; kk < D / 32; ++kk) {
@@ -392,79 +418,112 @@ __global__ __launch_bounds__(kNT) void scored_attn_kernel(Args a) {
   }
 
   const DmaOffs<D> doff = dma_offsets<D>(wave, lane);
-  auto issue = [&](int u, uint8_t *kdst, uint8_t *vdst) {
-    const int kbase = u * kKT, gi = kbase / 16 - g0;
-    const long long *kt = gtab + (gi + 2 * (wave >> 2) + (wave & 1)) % kMaxGroups;
-    const long long *vt = gtab + (gi + (wave >> 1)) % kMaxGroups;
+  auto issue_from = [&](const long long *tab, int u, uint8_t *kdst, uint8_t *vdst) {
+    const int kbase = (t0 + u) * kKT;
+    const long long *kt = tab + 2 * (wave >> 2) + (wave & 1);
+    const long long *vt = tab + (wave >> 1);
     if (kbase + kKT <= nkeys && kbase >= from)
       issue_tile_full<D>(a, kt, vt, doff, kdst, vdst, wave);
     else
       issue_tile<D, true>(a, kt, vt, kbase, nkeys, kdst, vdst, wave, lane, from);
   };
+  auto issue = [&](int u, uint8_t *kdst, uint8_t *vdst) {
+    issue_from(gtab + u * (kKT / 16) % kMaxGroups, u, kdst, vdst);
+  };
   const int32_t *btb = a.bt + (long long)b * a.max_blocks;
-  const int ng = (t1 - t0) * (kKT / 16);
+  constexpr int kPerTile = kKT / 16;
+  const int ng = steps * kPerTile;
   auto look_up = [&](int first, int n) {
-    for (int i = first + tid; i < min(first + n, ng); i += kNT)
-      gtab[i % kMaxGroups] = group_row_offset<D, true>(a, btb, g0 + i, nkeys, h, from);
+    for (int i = first + tid; i < min(first + n, ng); i += kNT) {
+      gtab[i % kMaxGroups] =
+          group_row_offset<D, true>(a, btb, t0 * kPerTile + i, nkeys, h, from);
+    }
   };
   look_up(0, kMaxGroups);
+  // Under a distance bias the last tile's keys, the nearest, set the exponent
+  // bases before the first tile: from far to near, steep slopes would rescale
+  // the outputs at every tile (the biased prompt of 8192 693 us).
+  const bool peek = BIAS && steps >= kPeekSteps;
+  if (BIAS && tid < kPerTile)
+    gpeek[tid] = group_row_offset<D, true>(a, btb, (t1 - 1) * kPerTile + tid, nkeys, h, from);
   wait_vmcnt<0>();
   __syncthreads();
 
   f32x4 o[QT][D / 16];
   f32x4 lacc[QT];
-  Softmax<QT> sm;
+  const Row *const rows_at = srow + wave * QT * 16 + col;
   float zero[QT];
 #pragma unroll
   for (int qt = 0; qt < QT; ++qt) {
     zero[qt] = 0.0f;
-    sm.b[qt] = 0.0f;
-    sm.valid[qt] = FIXED;
     lacc[qt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int dt = 0; dt < D / 16; ++dt) o[qt][dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   }
 
-  if (t0 < t1) {
+  if (steps > 0) {
     // the phases and barriers of tree_attention.hip's loop
-    for (int u = t0; u < min(t0 + 3, t1); ++u)
-      issue(u, kring + ((u - t0) % kKStages) * kTileBytes,
-            vring + ((u - t0) % kVStages) * kTileBytes);
-    const int later = min(t0 + 3, t1) - 1 - t0;
+    // (the last K stage and V stage are free until the loop)
+    if (peek)
+      issue_from(gpeek, steps - 1, kring + (kKStages - 1) * kTileBytes,
+                 vring + (kVStages - 1) * kTileBytes);
+    for (int u = 0; u < min(3, steps); ++u)
+      issue(u, kring + (u % kKStages) * kTileBytes, vring + (u % kVStages) * kTileBytes);
+    Scores<QT> S;
+    const bool busy = wave * QT * 16 < rows;  // wave-uniform
+    if constexpr (BIAS) {
+      if (peek) {
+        wait_vmcnt<3 * kLoadsPerTile>();
+        block_barrier();
+        if (busy) {
+          qk_tile(ln, kring + (kKStages - 1) * kTileBytes, zero, S);
+          raw_scores<D, QT, T, CAP, BIAS, FIXED>(ln, base, a, k0, cap2, (t1 - 1) * kKT, ctx, least,
+                                                 most_first, rows_at, smove + 64, S);
+#pragma unroll
+          for (int qt = 0; qt < QT; ++qt) {
+            const float m = score_max(S, qt);
+            base[qt] = m > -INFINITY ? m : 0.0f;
+          }
+        }
+        block_barrier();
+      }
+    }
+    const int later = min(3, steps) - 1;
     if (later >= 2) wait_vmcnt<2 * kLoadsPerTile>();
     else if (later == 1) wait_vmcnt<kLoadsPerTile>();
     else wait_vmcnt<0>();
     block_barrier();
     const bool lag = wave >= kWaves / 2;
     if (lag) block_barrier();
-    Scores<QT> S;
     Probs<QT, T> P;
-    const bool busy = wave * QT * 16 < rows;  // wave-uniform
     if (busy) qk_tile(ln, kring, zero, S);
-    for (int t = t0; t < t1; ++t) {
-      const int kbase = t * kKT;
-      const int u = t + 3 - t0;
+    for (int u = 0; u < steps; ++u) {
+      const int kbase = (t0 + u) * kKT;
+      const int ahead = u + 3;
       // (both halves' groups were in use until now: the one in front of this
-      // tile has no readers left, and its new entries have them 125 tiles on)
-      if (t > t0 && (t - t0) % (kMaxTilesPerSplit / 2) == 0) {
-        look_up((t - t0) * (kKT / 16) + kMaxGroups / 2, kMaxGroups / 2);
+      // step has no readers left, and its new entries have them 125 steps on)
+      if (u > 0 && u % (kMaxTilesPerSplit / 2) == 0) {
+        look_up(u * kPerTile + kMaxGroups / 2, kMaxGroups / 2);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       }
       if (!lag) {
         block_barrier();
       } else {
-        if (t + 2 < t1) wait_vmcnt<kLoadsPerTile>();
+        if (u + 2 < steps) wait_vmcnt<kLoadsPerTile>();
         else wait_vmcnt<0>();
         block_barrier();
       }
-      if (t + 3 < t1)
-        issue(t + 3, kring + (u % kKStages) * kTileBytes, vring + (u % kVStages) * kTileBytes);
-      if (busy)
-        score_phase<D, QT, T, CAP, BIAS, FIXED>(ln, cl, a, k0, cap2, kbase, ctx, least, most_first,
-                                                sdepth, S, sm, o, lacc, P);
+      if (ahead < steps)
+        issue(ahead, kring + (ahead % kKStages) * kTileBytes,
+              vring + (ahead % kVStages) * kTileBytes);
+      if (busy) {
+        raw_scores<D, QT, T, CAP, BIAS, FIXED>(ln, base, a, k0, cap2, kbase, ctx, least, most_first,
+                                               rows_at, smove + 64, S);
+        score_phase<D, QT, T, FIXED>(S, base, o, lacc, P);
+      }
       if (!lag) {
-        if (t + 3 < t1) wait_vmcnt<2 * kLoadsPerTile>();
-        else if (t + 2 < t1) wait_vmcnt<kLoadsPerTile>();
+        if (ahead < steps) wait_vmcnt<2 * kLoadsPerTile>();
+        else if (u + 2 < steps) wait_vmcnt<kLoadsPerTile>();
         else wait_vmcnt<0>();
         block_barrier();
       } else {
@@ -472,8 +531,8 @@ __global__ __launch_bounds__(kNT) void scored_attn_kernel(Args a) {
       }
       __builtin_amdgcn_s_setprio(1);
       if (busy)
-        mfma_phase(ln, kring + ((t + 1 - t0) % kKStages) * kTileBytes,
-                   vring + ((t - t0) % kVStages) * kTileBytes, zero, P, S, o, lacc);
+        mfma_phase(ln, kring + ((u + 1) % kKStages) * kTileBytes,
+                   vring + (u % kVStages) * kTileBytes, zero, P, S, o, lacc);
       __builtin_amdgcn_s_setprio(0);
     }
     if (!lag) block_barrier();
@@ -484,9 +543,9 @@ __global__ __launch_bounds__(kNT) void scored_attn_kernel(Args a) {
     const float ls = lacc[qt][0];
     if (!qvalid[qt]) continue;
     const int r = (wave * QT + qt) * 16 + col;
-    const long long row = ((long long)blk.t0 + r / a.G) * a.Hq + (long long)h * a.G + r % a.G;
+    const long long orow = ((long long)blk.t0 + r / a.G) * a.Hq + (long long)h * a.G + r % a.G;
     if (a.splits == 1) {
-      uint16_t *op = a.out + row * D;
+      uint16_t *op = a.out + orow * D;
       const float inv = ls != 0.0f ? 1.0f / ls : 0.0f;
 #pragma unroll
       for (int dt = 0; dt < D / 16; ++dt) {
@@ -496,12 +555,12 @@ __global__ __launch_bounds__(kNT) void scored_attn_kernel(Args a) {
         *reinterpret_cast<uint2 *>(op + dt * 16 + 4 * g) = w;
       }
     } else {
-      const long long prow = (long long)split * a.T * a.Hq + row;
+      const long long prow = (long long)split * a.T * a.Hq + orow;
       float *pp = a.part_o + prow * D;
 #pragma unroll
       for (int dt = 0; dt < D / 16; ++dt)
         *reinterpret_cast<f32x4 *>(pp + dt * 16 + 4 * g) = o[qt][dt];
-      if (g == 0) a.part_ml[prow] = make_float2(sm.valid[qt] ? sm.b[qt] : -INFINITY, ls);
+      if (g == 0) a.part_ml[prow] = make_float2(ls != 0.0f ? base[qt] : -INFINITY, ls);
     }
   }
 }
