@@ -86,12 +86,24 @@ struct Block {
   int b, t0, nt, i0;  // sequence, first token (global), tokens, the first's index in it
 };
 
-// Trees: block = sequence * ceil(Nq / TQ) + part.  Prompts: the blocks of all
+// Trees: block = sequence * ceil(Nq / TQ) + part, with the sequences in the order
+// of falling length where one wave can rank them: the work-groups that start
+// last are then the short ones (64 single tokens over 1024 to 4096 keys, 172 us
+// in the batch's order).  Prompts: the blocks of all
 // sequences are numbered through, each sequence's last (longest) one first.
 __device__ __forceinline__ bool find_block(const Args &a, int id, int lane, Block &k) {
   if (a.mask) {
     const int per = (a.Nq + a.TQ - 1) / a.TQ;
     k.b = id / per;
+    if (a.B > 1 && a.B <= 64) {
+      const int mine = lane < a.B ? a.ctx[lane] : 0;
+      int rank = 0;
+      for (int j = 0; j < a.B; ++j) {
+        const int c = __builtin_amdgcn_readlane(mine, j);
+        rank += c > mine || (c == mine && j < lane);
+      }
+      k.b = __ffsll((unsigned long long)__ballot(lane < a.B && rank == k.b)) - 1;
+    }
     k.i0 = (id % per) * a.TQ;
     k.t0 = k.b * a.Nq + k.i0;
     k.nt = min(a.TQ, a.Nq - k.i0);
@@ -305,13 +317,15 @@ __global__ __launch_bounds__(kNT) void scored_attn_kernel(Args a) {
   constexpr int kLoadsPerTile = Gm::kLoadsPerTile;
   __shared__ __align__(16) uint8_t kring[kKStages * kTileBytes];
   __shared__ __align__(16) uint8_t vring[kVStages * kTileBytes];
-  // row offsets of the split's 16-key groups; a ring of kMaxGroups, refilled
-  // half a ring at a time in longer splits
-  __shared__ long long gtab[kMaxGroups];
+  // row offsets of the split's 16-key groups; a ring, refilled half a ring at a
+  // time in longer splits (its size, and the rows', let two work-groups of one
+  // query tile and head_dim 64 share a CU's LDS)
+  constexpr int kRing = D == 64 ? 512 : 1024;
+  __shared__ long long gtab[kRing];
   __shared__ long long gpeek[kKT / 16];
   // trees: how far node j's position lies from its slot, at 64 + j; 0 around them
   __shared__ float smove[192];
-  __shared__ Row srow[kMaxRows];
+  __shared__ Row srow[QT == 1 ? kMaxRows / 2 : kMaxRows];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, g = lane >> 4;
@@ -428,18 +442,18 @@ __global__ __launch_bounds__(kNT) void scored_attn_kernel(Args a) {
       issue_tile<D, true>(a, kt, vt, kbase, nkeys, kdst, vdst, wave, lane, from);
   };
   auto issue = [&](int u, uint8_t *kdst, uint8_t *vdst) {
-    issue_from(gtab + u * (kKT / 16) % kMaxGroups, u, kdst, vdst);
+    issue_from(gtab + u * (kKT / 16) % kRing, u, kdst, vdst);
   };
   const int32_t *btb = a.bt + (long long)b * a.max_blocks;
   constexpr int kPerTile = kKT / 16;
   const int ng = steps * kPerTile;
   auto look_up = [&](int first, int n) {
     for (int i = first + tid; i < min(first + n, ng); i += kNT) {
-      gtab[i % kMaxGroups] =
+      gtab[i % kRing] =
           group_row_offset<D, true>(a, btb, t0 * kPerTile + i, nkeys, h, from);
     }
   };
-  look_up(0, kMaxGroups);
+  look_up(0, kRing);
   // Under a distance bias the last tile's keys, the nearest, set the exponent
   // bases before the first tile: from far to near, steep slopes would rescale
   // the outputs at every tile (the biased prompt of 8192 693 us).
@@ -500,10 +514,10 @@ __global__ __launch_bounds__(kNT) void scored_attn_kernel(Args a) {
     for (int u = 0; u < steps; ++u) {
       const int kbase = (t0 + u) * kKT;
       const int ahead = u + 3;
-      // (both halves' groups were in use until now: the one in front of this
-      // step has no readers left, and its new entries have them 125 steps on)
-      if (u > 0 && u % (kMaxTilesPerSplit / 2) == 0) {
-        look_up(u * kPerTile + kMaxGroups / 2, kMaxGroups / 2);
+      // (both halves' groups were in use until now: the one in front of this step
+      // has no readers left, and its new entries have them half a ring on)
+      if (u > 0 && u % (kRing / kPerTile / 2) == 0) {
+        look_up(u * kPerTile + kRing / 2, kRing / 2);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       }
       if (!lag) {
@@ -531,7 +545,8 @@ __global__ __launch_bounds__(kNT) void scored_attn_kernel(Args a) {
       }
       __builtin_amdgcn_s_setprio(1);
       if (busy)
-        mfma_phase(ln, kring + ((u + 1) % kKStages) * kTileBytes,
+        // (one query tile has half the products per operand read)
+        mfma_phase<D, QT, T, QT == 1 ? 4 : 2>(ln, kring + ((u + 1) % kKStages) * kTileBytes,
                    vring + (u % kVStages) * kTileBytes, zero, P, S, o, lacc);
       __builtin_amdgcn_s_setprio(0);
     }

@@ -295,7 +295,7 @@ struct Softmax {
 // issued right behind its predecessor stalls the matrix pipe.  Lane (g, col)
 // reads V rows blk*32 + 8g + 0..7 at d = dt*16 + col through two transposed
 // 4x16 reads.
-template <int D, int QT, class E = BF16>
+template <int D, int QT, class E = BF16, int READS = 2>
 __device__ __forceinline__ void mfma_phase(const Lane<D, QT, E> &ln, const uint8_t *Knext, const uint8_t *Vs,
                                            const float *b, const Probs<QT, E> &P, Scores<QT> &S,
                                            f32x4 (&o)[QT][D / 16], f32x4 (&lacc)[QT]) {
@@ -340,13 +340,13 @@ __device__ __forceinline__ void mfma_phase(const Lane<D, QT, E> &ln, const uint8
               Mfma<E>::run(kf, ln.qf[qt][kk], kk == 0 ? negb[qt] : S.s[qt][blk][T]);
       }
 #if CFA_TA_SGB
-  // software pipeline of the operand reads: four fragments ahead, then two
+  // software pipeline of the operand reads: four fragments ahead, then READS
   // reads after every pair of MFMAs
   __builtin_amdgcn_sched_group_barrier(0x0100, 8, 0);
 #pragma unroll
   for (int j = 0; j < Geo<D, QT>::kMfma / 2; ++j) {
     __builtin_amdgcn_sched_group_barrier(0x0008, 2, 0);
-    __builtin_amdgcn_sched_group_barrier(0x0100, 2, 0);
+    __builtin_amdgcn_sched_group_barrier(0x0100, READS, 0);
   }
 #endif
 }
