@@ -32,7 +32,10 @@ __device__ __forceinline__ uint16_t pack1(float f) {
 }
 template <class T>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-  return (uint32_t)pack1<T>(lo) | ((uint32_t)pack1<T>(hi) << 16);
+  typedef typename T::elem pair __attribute__((ext_vector_type(2)));
+  typedef float floats __attribute__((ext_vector_type(2)));
+  // one instruction for bf16
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((floats{lo, hi}), pair));
 }
 
 }  // namespace cfa

@@ -28,6 +28,7 @@
 namespace cfa {
 namespace rotary {
 
+constexpr int kIter = 4;   // rows of a lane group whose loads are in flight at once
 constexpr int kWaves = 4;  // waves per work-group, each with its own (token, heads)
 enum Layout { kHalf = 0, kHalfAny = 1, kNeighbours = 2 };
 
@@ -46,7 +47,7 @@ struct Args {
   int num_blocks, max_blocks, bs;
   const int32_t *block_tables, *base;
   long long blk_stride, layer_off, head_stride;
-  int chunks;  // head chunks per token
+  int chunks, rounds;  // waves a token; rounds of rows a wave
 };
 
 // Sum over the LPR lanes of a head, every lane gets it.
@@ -96,29 +97,52 @@ __device__ __forceinline__ void unpack8(const uint4 &v, float (&x)[8]) {
   unpack2<T>(v.w, x[6], x[7]);
 }
 
-// Weights e .. e + 7 of a norm (1 where there is none).
-template <class T>
+// Weights e .. e + 7 of a norm (1 where there is none); PAR: 16-byte loads.
+template <class T, bool PAR>
 __device__ __forceinline__ void weights8(const void *w, int f32, int e, float (&x)[8]) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) x[i] = 1.0f;
   if (!w) return;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    if (f32) {
-      x[i] = reinterpret_cast<const float *>(w)[e + i];
+  if (f32) {
+    const float *p = reinterpret_cast<const float *>(w) + e;
+    if constexpr (PAR) {
+      const float4 a = reinterpret_cast<const float4 *>(p)[0];
+      const float4 b = reinterpret_cast<const float4 *>(p)[1];
+      x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w;
+      x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
     } else {
-      float hi;
-      unpack2<T>(reinterpret_cast<const uint16_t *>(w)[e + i], x[i], hi);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = p[i];
+    }
+  } else {
+    unpack8<T>(load8<PAR>(reinterpret_cast<const uint16_t *>(w) + e), x);
+  }
+}
+
+// N frequencies from number i on.
+template <int N, bool PAR>
+__device__ __forceinline__ void turns_at(const Args &a, int i, uint64_t (&t)[N]) {
+#pragma unroll
+  for (int k = 0; k < N; k += 2) {
+    if constexpr (PAR) {
+      const ulonglong2 v = *reinterpret_cast<const ulonglong2 *>(a.turns + i + k);
+      t[k] = v.x;
+      t[k + 1] = v.y;
+    } else {
+      t[k] = a.turns[i + k];
+      t[k + 1] = a.turns[i + k + 1];
     }
   }
 }
 
-// factor * (cos, sin) of position p on pair i.
-__device__ __forceinline__ void angle(const Args &a, int p, int i, float &cs, float &sn) {
-  const uint64_t turn = a.turns[i] * (uint64_t)(int64_t)p;
+// factor * (cos, sin) of position p on a pair's frequency.  The instructions take turns; over
+// [-1/2, 1/2] they are off by at most 2^-22.9 (six million values measured),
+// where the library's cospi and sinpi take some 30 instructions each.
+__device__ __forceinline__ void angle(const Args &a, int p, uint64_t turns, float &cs, float &sn) {
+  const uint64_t turn = turns * (uint64_t)(int64_t)p;
   const float f = (float)(int32_t)(turn >> 32) * 0x1p-32f;  // [-1/2, 1/2] turns
-  cs = a.factor * cospif(2.0f * f);
-  sn = a.factor * sinpif(2.0f * f);
+  cs = a.factor * __builtin_amdgcn_cosf(f);
+  sn = a.factor * __builtin_amdgcn_sinf(f);
 }
 
 // The sequence b and the place j in it of token t; false where t belongs to
@@ -139,8 +163,8 @@ __device__ __forceinline__ bool place(const Args &a, int t, int lane, int &b, in
   return j >= 0;
 }
 
-// One wave = one token and ITER * 64 / LPR consecutive rows of its Hq q heads,
-// Hkv k heads and Hkv v heads.
+// One wave = one token and `rounds` times ITER * 64 / LPR consecutive rows of its
+// Hq q heads, Hkv k heads and Hkv v heads.
 template <class T, int LPR, int LAYOUT, bool VEC, int ITER>
 __global__ __launch_bounds__(kWaves * 64) void qk_norm_rope_kv_kernel(Args a) {
   constexpr int RPW = 64 / LPR;
@@ -148,25 +172,28 @@ __global__ __launch_bounds__(kWaves * 64) void qk_norm_rope_kv_kernel(Args a) {
   const long long item = (long long)blockIdx.x * kWaves + (threadIdx.x >> 6);
   const int t = (int)(item / a.chunks), chunk = (int)(item % a.chunks);
   if (t >= a.T) return;
-  int b, j;
-  if (!place(a, t, lane, b, j)) return;
   const int e = 8 * l, H = a.Hq + 2 * a.Hkv;
   const bool mine = e < a.D;
-  const int row0 = chunk * ITER * RPW + lane / LPR;
+  const int row0 = chunk * a.rounds * ITER * RPW + lane / LPR;
 
   uint4 raw[ITER];
+  auto load = [&](int round) {
 #pragma unroll
-  for (int it = 0; it < ITER; ++it) {
-    const int row = row0 + it * RPW;
-    raw[it] = make_uint4(0, 0, 0, 0);
-    if (row < H && mine) {
-      const uint16_t *src =
-          row < a.Hq ? a.q + t * a.q_st + row * a.q_sh
-                     : row < a.Hq + a.Hkv ? a.k + t * a.k_st + (row - a.Hq) * a.k_sh
-                                          : a.v + t * a.v_st + (row - a.Hq - a.Hkv) * a.v_sh;
-      raw[it] = load8<VEC>(src + e);
+    for (int it = 0; it < ITER; ++it) {
+      const int row = row0 + (round * ITER + it) * RPW;
+      raw[it] = make_uint4(0, 0, 0, 0);
+      if (row < H && mine) {
+        const uint16_t *src =
+            row < a.Hq ? a.q + t * a.q_st + row * a.q_sh
+                       : row < a.Hq + a.Hkv ? a.k + t * a.k_st + (row - a.Hq) * a.k_sh
+                                            : a.v + t * a.v_st + (row - a.Hq - a.Hkv) * a.v_sh;
+        raw[it] = load8<VEC>(src + e);
+      }
     }
-  }
+  };
+  load(0);
+  int b, j;
+  if (!place(a, t, lane, b, j)) return;
   // this lane's cosines and sines: c[i], s[i] of element e + i, the sine with
   // the sign that its partner's value takes
   float c[8], s[8], wq[8], wk[8];
@@ -178,12 +205,30 @@ __global__ __launch_bounds__(kWaves * 64) void qk_norm_rope_kv_kernel(Args a) {
     s[i] = 0.0f;
   }
   if constexpr (LAYOUT == kNeighbours) {
+    if (e + 8 <= a.R) {
+      uint64_t f[4];
+      turns_at<4, VEC>(a, e / 2, f);
+#pragma unroll
+      for (int i = 0; i < 8; i += 2) angle(a, p, f[i / 2], c[i], s[i + 1]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; i += 2)
+        if (e + i < a.R) angle(a, p, a.turns[(e + i) / 2], c[i], s[i + 1]);
+    }
 #pragma unroll
     for (int i = 0; i < 8; i += 2) {
-      if (e + i < a.R) {
-        angle(a, p, (e + i) / 2, c[i], s[i + 1]);
-        c[i + 1] = c[i];
-        s[i] = -s[i + 1];
+      c[i + 1] = c[i];
+      s[i] = -s[i + 1];
+    }
+  } else if constexpr (LAYOUT == kHalf) {
+    if (e < a.R) {  // a lane's eight lie in one half
+      const bool first = e < half;
+      uint64_t f[8];
+      turns_at<8, VEC>(a, first ? e : e - half, f);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        angle(a, p, f[i], c[i], s[i]);
+        s[i] = first ? -s[i] : s[i];
       }
     }
   } else {
@@ -191,14 +236,14 @@ __global__ __launch_bounds__(kWaves * 64) void qk_norm_rope_kv_kernel(Args a) {
     for (int i = 0; i < 8; ++i) {
       if (e + i < a.R) {
         const bool first = e + i < half;
-        angle(a, p, first ? e + i : e + i - half, c[i], s[i]);
+        angle(a, p, a.turns[first ? e + i : e + i - half], c[i], s[i]);
         if (first) s[i] = -s[i];
       }
     }
   }
   if (mine) {
-    weights8<T>(a.q_w, a.w_f32, e, wq);
-    weights8<T>(a.k_w, a.w_f32, e, wk);
+    weights8<T, VEC>(a.q_w, a.w_f32, e, wq);
+    weights8<T, VEC>(a.k_w, a.w_f32, e, wk);
   }
   // the page of this token's slot
   const long long slot = (long long)a.base[b] + j;
@@ -208,64 +253,66 @@ __global__ __launch_bounds__(kWaves * 64) void qk_norm_rope_kv_kernel(Args a) {
   const bool mapped = blk >= 0 && blk < a.num_blocks;
   const long long at = blk * a.blk_stride + a.layer_off + (slot - page * a.bs) * a.D;
 
+  for (int round = 0; round < a.rounds; ++round) {
 #pragma unroll
-  for (int it = 0; it < ITER; ++it) {
-    const int row = row0 + it * RPW;
-    const bool is_q = row < a.Hq, is_v = row >= a.Hq + a.Hkv;
-    float x[8], y[8];
-    unpack8<T>(raw[it], x);
-    float ss = 0.0f;
+    for (int it = 0; it < ITER; ++it) {
+      const int row = row0 + (round * ITER + it) * RPW;
+      const bool is_q = row < a.Hq, is_v = row >= a.Hq + a.Hkv;
+      float x[8], y[8];
+      unpack8<T>(raw[it], x);
+      float ss = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) ss += x[i] * x[i];
-    ss = group_sum<LPR>(ss);
-    const bool norm = (is_q ? a.q_w : a.k_w) != nullptr;
-    const float inv = norm ? rsqrtf(ss / (float)a.D + a.eps) : 1.0f;
+      for (int i = 0; i < 8; ++i) ss += x[i] * x[i];
+      ss = group_sum<LPR>(ss);
+      const bool norm = (is_q ? a.q_w : a.k_w) != nullptr;
+      const float inv = norm ? rsqrtf(ss / (float)a.D + a.eps) : 1.0f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] *= inv * (is_q ? wq[i] : wk[i]);
-    if constexpr (LAYOUT == kHalf) {
-      // R / 2 is a multiple of 8: the partner's elements are one lane's
-      const int to = e < half ? lane + half / 8 : (e < a.R ? lane - half / 8 : lane);
+      for (int i = 0; i < 8; ++i) x[i] *= inv * (is_q ? wq[i] : wk[i]);
+      if constexpr (LAYOUT == kHalf) {
+        // R / 2 is a multiple of 8: the partner's elements are one lane's
+        const int to = e < half ? lane + half / 8 : (e < a.R ? lane - half / 8 : lane);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] = __shfl(x[i], to, 64);
-    } else if constexpr (LAYOUT == kHalfAny) {
-      // element by element: partner e + i +- R / 2, in lane (e + i +- R / 2) / 8
+        for (int i = 0; i < 8; ++i) y[i] = __shfl(x[i], to, 64);
+      } else if constexpr (LAYOUT == kHalfAny) {
+        // element by element: partner e + i +- R / 2, in lane (e + i +- R / 2) / 8
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int el = e + i;
-        const int pe = el < half ? el + half : (el < a.R ? el - half : el);
-        const int from = lane - l + pe / 8;
-        float v = 0.0f;
+        for (int i = 0; i < 8; ++i) {
+          const int el = e + i;
+          const int pe = el < half ? el + half : (el < a.R ? el - half : el);
+          const int from = lane - l + pe / 8;
+          float v = 0.0f;
 #pragma unroll
-        for (int m = 0; m < 8; ++m) {
-          const float got = __shfl(x[m], from, 64);
-          if (pe % 8 == m) v = got;
+          for (int m = 0; m < 8; ++m) {
+            const float got = __shfl(x[m], from, 64);
+            if (pe % 8 == m) v = got;
+          }
+          y[i] = v;
         }
-        y[i] = v;
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = x[i ^ 1];
       }
-    } else {
+      if (row >= H || !mine) continue;
+      // (elements behind the rotated ones are selected, not turned by 0: they
+      // may be infinite)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] = x[i ^ 1];
+      for (int i = 0; i < 8; ++i) x[i] = e + i < a.R ? x[i] * c[i] + y[i] * s[i] : x[i];
+      uint32_t w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = pack2<T>(x[2 * i], x[2 * i + 1]);
+      if (is_v) {  // as it is
+        w[0] = raw[it].x;
+        w[1] = raw[it].y;
+        w[2] = raw[it].z;
+        w[3] = raw[it].w;
+      }
+      if (is_q)
+        store8<VEC>(a.q_out + ((long long)t * a.Hq + row) * a.D + e, w);
+      else if (mapped)
+        store8<VEC>((is_v ? a.vc + (row - a.Hq - a.Hkv) * a.head_stride
+                          : a.kc + (row - a.Hq) * a.head_stride) + at + e, w);
     }
-    if (row >= H || !mine) continue;
-    // (elements behind the rotated ones are selected, not turned by 0: they
-    // may be infinite)
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      x[i] = e + i < a.R ? x[i] * c[i] + y[i] * s[i] : x[i];
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = pack2<T>(x[2 * i], x[2 * i + 1]);
-    if (is_v) {  // as it is
-      w[0] = raw[it].x;
-      w[1] = raw[it].y;
-      w[2] = raw[it].z;
-      w[3] = raw[it].w;
-    }
-    if (is_q)
-      store8<VEC>(a.q_out + ((long long)t * a.Hq + row) * a.D + e, w);
-    else if (mapped)
-      store8<VEC>((is_v ? a.vc + (row - a.Hq - a.Hkv) * a.head_stride
-                        : a.kc + (row - a.Hq) * a.head_stride) + at + e, w);
+    if (round + 1 < a.rounds) load(round + 1);
   }
 }
 
@@ -274,17 +321,28 @@ int launch(Args a, hipStream_t st) {
   constexpr int RPW = 64 / LPR;
   const int H = a.Hq + 2 * a.Hkv;
   const long long few = (long long)a.T * ((H + RPW - 1) / RPW);
-  auto grid = [&](int iter) {
-    a.chunks = (H + iter * RPW - 1) / (iter * RPW);
+  auto grid = [&](int iter, int rounds) {
+    a.rounds = rounds;
+    a.chunks = (H + iter * rounds * RPW - 1) / (iter * rounds * RPW);
     return dim3((unsigned)(((long long)a.T * a.chunks + kWaves - 1) / kWaves));
   };
-  // four rows a lane group where that leaves enough waves to fill the device
-  if (few >= 4 * 2048)
-    CFA_LAUNCH("qk_norm_rope_kv", (qk_norm_rope_kv_kernel<T, LPR, LAYOUT, VEC, 4>), grid(4),
+  // `few`: waves of one row a lane group.  A token's heads all in one wave where
+  // that leaves 8192 waves of kIter rows' work (angles and weights are then formed
+  // once a token), else kIter rows a group where that leaves 2048 waves, else one.
+  // us, 48 heads of 128, one row a group / kIter rows / all heads in a wave: 504
+  // tokens 10.1 / 10.6 / 14, 2000 tokens 22 / 19.6 / 20.5, 3200 tokens 36 / 27 / 24, 8149
+  // tokens 104 / 73 / 58.  With 2 / 6 / 8 / 12 rows in flight: 59.5 / 59.2 / 62 / 69.
+  if (few >= 8192 * kIter) {
+    const int all = (H + kIter * RPW - 1) / (kIter * RPW);
+    CFA_LAUNCH("qk_norm_rope_kv", (qk_norm_rope_kv_kernel<T, LPR, LAYOUT, VEC, kIter>),
+               grid(kIter, all), dim3(kWaves * 64), 0, st, a);
+  } else if (few >= 8192) {
+    CFA_LAUNCH("qk_norm_rope_kv", (qk_norm_rope_kv_kernel<T, LPR, LAYOUT, VEC, kIter>),
+               grid(kIter, 1), dim3(kWaves * 64), 0, st, a);
+  } else {
+    CFA_LAUNCH("qk_norm_rope_kv", (qk_norm_rope_kv_kernel<T, LPR, LAYOUT, VEC, 1>), grid(1, 1),
                dim3(kWaves * 64), 0, st, a);
-  else
-    CFA_LAUNCH("qk_norm_rope_kv", (qk_norm_rope_kv_kernel<T, LPR, LAYOUT, VEC, 1>), grid(1),
-               dim3(kWaves * 64), 0, st, a);
+  }
   return CFA_OK;
 }
 
@@ -375,7 +433,8 @@ extern "C" int cfa_qk_norm_rope_kv(
   a.blk_stride = (long long)num_layers * n_kv_heads * a.head_stride;
   a.layer_off = (long long)layer * n_kv_heads * a.head_stride;
   const bool vec = (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)q_out |
-                     (uintptr_t)k_pool | (uintptr_t)v_pool) & 15) == 0 &&
+                     (uintptr_t)k_pool | (uintptr_t)v_pool | (uintptr_t)turns |
+                     (uintptr_t)q_norm | (uintptr_t)k_norm) & 15) == 0 &&
                    ((q_stride_t | q_stride_h | k_stride_t | k_stride_h | v_stride_t | v_stride_h) &
                     7) == 0;
   const int layout = interleaved ? kNeighbours : (rotary_dim % 16 == 0 ? kHalf : kHalfAny);

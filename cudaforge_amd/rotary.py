@@ -10,7 +10,6 @@ and the usual scalings for contexts longer than the trained one.
 """
 from __future__ import annotations
 
-import ctypes
 import math
 from typing import Optional
 
@@ -18,7 +17,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from .verify import _ptr, _require_cuda, _stream_ptr
+from .verify import _on, _ptr, _require_cuda, _stream_ptr
 
 __all__ = ["Rotary", "qk_norm_rope_kv"]
 
@@ -234,34 +233,27 @@ def qk_norm_rope_kv(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions
         _require_cuda("q_out", q_out, dt, dev)
         if tuple(q_out.shape) != (T, Hq, D) or not q_out.is_contiguous():
             raise ValueError("q_out must be a contiguous [T, Hq, D]")
+        lo = q_out.data_ptr()
+        hi = lo + 2 * T * Hq * D
         for name, x in (("q", q), ("k", k), ("v", v)):
-            if _overlap(q_out, x):
+            (t, h, _), (st, sh, _), at = x.shape, x.stride(), x.data_ptr()
+            if hi > at and at + 2 * ((t - 1) * st + (h - 1) * sh + D) > lo and T:
                 raise ValueError(f"q_out must not overlap {name}")
-    positions, block_tables, base_lens = (t.contiguous() for t in
-                                          (positions, block_tables, base_lens))
-    with torch.cuda.device(dev):
+    positions = positions.contiguous()
+    block_tables = block_tables.contiguous()
+    base_lens = base_lens.contiguous()
+    with _on(dev):
         rc = _lib.load().cfa_qk_norm_rope_kv(
             q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
             v.data_ptr(), v.stride(0), v.stride(1), int(dt == torch.float16),
             positions.data_ptr(), T, B, _ptr(cu_seqlens), Hq, Hkv, D, rot,
             rotary.turns.data_ptr() if rot else None,
-            ctypes.c_float(rotary.factor if rot else 1.0),
+            rotary.factor if rot else 1.0,
             int(rot > 0 and rotary.layout == "interleaved"), _ptr(q_norm), _ptr(k_norm),
-            int(norm is not None and norm.dtype == torch.float32), ctypes.c_float(eps),
+            int(norm is not None and norm.dtype == torch.float32), eps,
             q_out.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), nblk, nlayers, int(layer), bs,
             block_tables.data_ptr(), block_tables.shape[1], base_lens.data_ptr(),
             _stream_ptr(dev))
     _lib.check(rc, "cfa_qk_norm_rope_kv")
     return q_out
 
-
-def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """Whether the address ranges that a and b span meet."""
-    def span(x):
-        n = 1 + sum((s - 1) * st for s, st in zip(x.shape, x.stride()))
-        return x.data_ptr(), x.data_ptr() + n * x.element_size()
-
-    if a.numel() == 0 or b.numel() == 0:
-        return False
-    (a0, a1), (b0, b1) = span(a), span(b)
-    return a0 < b1 and b0 < a1

@@ -34,7 +34,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from .verify import _KINDS, _require_cuda, _stream_ptr
+from .verify import _KINDS, _on, _require_cuda, _stream_ptr
 
 __all__ = [
     "SamplingParams",
@@ -268,7 +268,7 @@ def sample_rows(rows: torch.Tensor, uniforms: Optional[torch.Tensor] = None, *,
     need = int(lib.cfa_sample_rows_workspace_size(R, V))
     if workspace is None or workspace.numel() < need:
         workspace = torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
-    with torch.cuda.device(dev):
+    with _on(dev):
         rc = lib.cfa_sample_rows(
             rows.data_ptr(), rows.stride(0), _ROW_TYPES[rows.dtype], R, V, draws, t, t0, k, k0, p,
             p0, m, m0, uniforms.data_ptr(), tokens.data_ptr(),
