@@ -91,6 +91,8 @@ static int check_pool(int num_blocks, int num_layers, int layer, int block_size,
 static int run(Args &a, const Plan &p, int D, int fp16, float sm_scale, float soft_cap,
                void *workspace, size_t workspace_bytes, void *stream) {
   using namespace cfa::abi;
+  if ((((uintptr_t)a.q | (uintptr_t)a.kpool | (uintptr_t)a.vpool | (uintptr_t)a.out) & 15) != 0)
+    return fail_arg("q, the pools and out must be 16-byte aligned");
   a.TQ = p.TQ;
   a.splits = p.splits;
   a.blocks = (int)p.blocks;
@@ -114,6 +116,8 @@ static int run(Args &a, const Plan &p, int D, int fp16, float sm_scale, float so
   const long long grid = (long long)p.splits * a.Hkv * p.blocks;
   if (grid * kNT >= (1LL << 32)) return fail_arg("too many queries for one call");
   if (p.splits > 1) {
+    if ((long long)a.T * a.Hq * (D / 4) >= (1LL << 32))  // the merge's threads
+      return fail_arg("too many queries for one call");
     if (!workspace || workspace_bytes < p.bytes(a.T, a.Hq, D))
       return fail_arg("workspace too small (see the entry point's _workspace_size)");
     if (((uintptr_t)workspace & 15) != 0) return fail_arg("workspace must be 16-byte aligned");

@@ -347,7 +347,7 @@ __global__ __launch_bounds__(kNT) void scored_attn_kernel(Args a) {
   const int cap_keys = a.max_blocks * a.bs;
   const int last = tree ? a.N : blk.i0 + blk.nt;  // keys behind the context
   const int ctx = min(max(a.ctx[b], 0), max(cap_keys - last, 0));
-  const int nkeys = min(ctx + last, cap_keys);
+  int nkeys = min(ctx + last, cap_keys);  // trees: cut behind the last visible node
 
   Lane<D, QT, T> ln;
   float base[QT];  // exponent bases
@@ -357,28 +357,32 @@ __global__ __launch_bounds__(kNT) void scored_attn_kernel(Args a) {
   int low;  // the first query's position (trees: the shallowest's)
   if (tree) {
     const uint64_t nodes = a.N >= 64 ? ~0ull : ((1ull << a.N) - 1);
-    const uint64_t mine = lane < a.N ? a.mask[(long long)b * a.mask_sb + lane] & nodes : 0ull;
+    uint64_t mine = lane < a.N ? a.mask[(long long)b * a.mask_sb + lane] & nodes : 0ull;
     const int depth = max((int)__popcll(mine) - 1, 0);
     if (BIAS && wave < 3) {
       const int node = lane + 64 * (wave - 1);  // wave 1 holds the nodes
       smove[64 + node] = node >= 0 && node < a.N ? (float)(depth - node) : 0.0f;
     }
     const int j = a.q0 + blk.i0;
-    int d = lane >= j && lane < j + blk.nt ? depth : 64;
+    if (a.window > 0)  // nodes that lie `window` and more above are out of it
+      for (int m = 0; m < a.N; ++m)
+        if (depth - __builtin_amdgcn_readlane(depth, m) >= a.window) mine &= ~(1ull << m);
+    const bool asks = lane >= j && lane < j + blk.nt;
+    int d = asks ? depth : 64, behind = asks && mine ? 64 - __clzll((long long)mine) : 0;
 #pragma unroll
-    for (int s = 32; s >= 1; s >>= 1) d = min(d, __shfl_xor(d, s, 64));
+    for (int s = 32; s >= 1; s >>= 1) {
+      d = min(d, __shfl_xor(d, s, 64));
+      behind = max(behind, __shfl_xor(behind, s, 64));
+    }
     low = ctx + __builtin_amdgcn_readfirstlane(d);
+    nkeys = ctx + __builtin_amdgcn_readfirstlane(behind);
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
       const int r = (wave * QT + qt) * 16 + col;
       qvalid[qt] = r < rows;
       const int node = j + (qvalid[qt] ? r / a.G : 0);
-      uint64_t anc = __shfl((unsigned long long)mine, node, 64);
-      const int dq = __shfl(depth, node, 64);
-      row[qt].pos = ctx + dq;
-      if (a.window > 0)  // nodes that lie `window` and more above are out of it
-        for (int m = 0; m < a.N; ++m)
-          if (dq - __shfl(depth, m, 64) >= a.window) anc &= ~(1ull << m);
+      const uint64_t anc = __shfl((unsigned long long)mine, node, 64);
+      row[qt].pos = ctx + __shfl(depth, node, 64);
       row[qt].anc = qvalid[qt] ? anc : 0ull;
     }
   } else {
@@ -399,7 +403,7 @@ __global__ __launch_bounds__(kNT) void scored_attn_kernel(Args a) {
   const int tlo = from / kKT, thi = (nkeys + kKT - 1) / kKT;
   const int tps = (thi - tlo + a.splits - 1) / a.splits;
   const int t0 = tlo + split * tps, t1 = min(thi, t0 + tps);
-  const int steps = t1 - t0;
+  const int steps = from < nkeys ? t1 - t0 : 0;
   constexpr float kLog2e = 1.4426950408889634f;
   const float cap2 = a.cap * kLog2e;
   // without a cap: score in log2 units = product * k0; with one: e^(2 s / cap)

@@ -222,12 +222,19 @@ def _check_slopes(alibi_slopes: Optional[torch.Tensor], Hq: int, dev) -> Optiona
     return alibi_slopes.contiguous()
 
 
+def _aligned(q: torch.Tensor) -> torch.Tensor:
+    """q, or a copy of it where it does not begin on 16 bytes."""
+    return q if q.data_ptr() % 16 == 0 else q.clone()
+
+
 def _check_out(out: Optional[torch.Tensor], q: torch.Tensor) -> torch.Tensor:
     if out is None:
         return torch.empty_like(q)
     _require_cuda("out", out, q.dtype, q.device)
     if out.shape != q.shape or not out.is_contiguous():
         raise ValueError("out must be a contiguous tensor of q's shape")
+    if out.data_ptr() % 16:
+        raise ValueError("out must be 16-byte aligned")
     return out
 
 
@@ -296,6 +303,7 @@ def tree_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
               or dtype == torch.float16)
     if scored:
         alibi_slopes = _check_slopes(alibi_slopes, Hq, dev)
+        q = _aligned(q)
         out = _check_out(out, q)
     elif out is None:
         out = torch.empty_like(q)
@@ -379,6 +387,7 @@ def prompt_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor
     block_tables, ctx_lens, cu_seqlens = (t.contiguous() for t in
                                           (block_tables, ctx_lens, cu_seqlens))
     alibi_slopes = _check_slopes(alibi_slopes, Hq, dev)
+    q = _aligned(q)
     out = _check_out(out, q)
     if sm_scale is None:
         sm_scale = D ** -0.5

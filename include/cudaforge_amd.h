@@ -261,9 +261,10 @@ int cfa_tree_attention(const void *q, const void *k_pool, const void *v_pool,
  * Everything else is cfa_tree_attention's, except: n_q_heads / n_kv_heads times
  * the query nodes may exceed 256; max_keys only plans the splits (a longer
  * context is still attended to in full); partials are fp32.  A query that sees
- * no key gets zeros.  Keys that no query of its block sees do not reach the
- * output; a NaN or infinity in the V of a key that some of them see reaches all
- * of that sequence's queries in the block.
+ * no key gets zeros.  Keys in front of the first and behind the last that a
+ * sequence's queries see are not read; a NaN or infinity in the V of one between
+ * them may reach all of that sequence's queries.  q, the pools and out must be
+ * 16-byte aligned.
  * soft_cap is 0 or at least 1e-6.  The workspace size takes the query nodes (N
  * - first_node) for N; 0: none is needed. */
 size_t cfa_tree_attention_scored_workspace_size(int B, int N, int n_q_heads, int n_kv_heads,

@@ -31,7 +31,8 @@ COMMON = [(dict(Hq=0), "n_q_heads"), (dict(Hkv=3), "multiple"), (dict(Hq=514), "
 
 
 @pytest.mark.parametrize("change,msg", COMMON + [
-    (dict(q=None), "null"), (dict(out=None), "null"), (dict(B=0), "B > 0"), (dict(N=65), "64"),
+    (dict(q=None), "null"), (dict(out=None), "null"), (dict(q=264), "aligned"),
+    (dict(out=258), "aligned"), (dict(B=0), "B > 0"), (dict(N=65), "64"),
     (dict(N=0), "64"), (dict(first=15), "first_node"), (dict(first=-1), "first_node"),
     (dict(keys=14), "max_keys"), (dict(keys=129), "cover"), (dict(splits=2, keys=128), "workspace")])
 def test_tree_refusals(change, msg):
@@ -51,7 +52,8 @@ def _prompt(**change):
 
 
 @pytest.mark.parametrize("change,msg", COMMON + [
-    (dict(q=None), "null"), (dict(out=None), "null"), (dict(T=-1), "T, B"), (dict(B=-1), "T, B"),
+    (dict(q=None), "null"), (dict(out=None), "null"), (dict(q=264), "aligned"),
+    (dict(out=258), "aligned"), (dict(T=-1), "T, B"), (dict(B=-1), "T, B"),
     (dict(mq=0), "max_query"), (dict(keys=0), "max_keys"), (dict(splits=2, keys=128), "workspace"),
     (dict(T=2 ** 30), "too many")])
 def test_prompt_refusals(change, msg):

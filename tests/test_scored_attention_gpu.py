@@ -181,6 +181,69 @@ def test_slots_behind_the_sequence_are_not_read(device):
         _tree(device, [100], 3, 8, 2, 128, name, spoil=spoil)
 
 
+def test_nodes_behind_the_last_visible_are_not_read(device):
+    """A padded batch: nodes 5 .. 8 of the first tree do not exist, their slots
+    hold NaN; their queries see the context alone."""
+    chain = [int(m) for m in T.ancestor_masks(T.chain_parents(9))]
+    masks = [chain[:5] + [0] * 4, chain]
+
+    def spoil(kp, vp, bt):
+        for pos in range(70 + 5, 70 + 9):
+            kp[int(bt[0, pos // 16]), :, :, pos % 16] = float("nan")
+            vp[int(bt[0, pos // 16]), :, :, pos % 16] = float("inf")
+
+    for name in ("c50", "b", "w9", "c+b+w3"):
+        for splits in (1, 2):
+            _tree(device, [70, 20], 9, 8, 2, 64, name, masks=masks, spoil=spoil, num_splits=splits)
+
+
+def test_nothing_visible_reads_nothing(device):
+    def spoil(kp, vp, bt):
+        kp[:] = float("nan")
+        vp[:] = float("nan")
+
+    for ctx, name in ((0, "c50"), (0, "b"), (37, "w1"), (64, "b+w1")):
+        got = _tree(device, [ctx], 3, 8, 2, 64, name, masks=[0, 0, 0], spoil=spoil)
+        assert (got == 0).all()
+
+
+def test_alignment(device):
+    """q is copied where it does not begin on 16 bytes; out and pools are refused."""
+    q, kp, vp, bt = R.tree_case([50], 3, 8, 2, 64, BF)
+    masks = [1, 3, 5]
+    want, tol = R.tree_want(q, kp, vp, bt, [50], masks, window=20)
+    off = torch.zeros(q.numel() + 1, dtype=BF, device=device)
+    view = off[1:].view(q.shape)
+    view.copy_(q)
+    a = [kp.to(device), vp.to(device), bt.to(device), torch.tensor([50], dtype=torch.int32,
+                                                                  device=device)]
+    m = _mask_tensor(masks, device)
+    got = tree_attention(view, *a, m, window=20)
+    assert ((got.cpu().double() - want).abs() <= tol).all()
+    with pytest.raises(ValueError, match="aligned"):
+        tree_attention(view, *a, m, window=20, out=view)
+    with pytest.raises(ValueError, match="aligned"):
+        pool = torch.zeros(kp.numel() + 1, dtype=BF, device=device)[1:].view(kp.shape)
+        tree_attention(view, pool, *a[1:], m, window=20)
+    cu = torch.tensor([0, 3], dtype=torch.int32, device=device)
+    got = prompt_attention(view[0], *a, cu, window=20)
+    # (as the chain of three nodes)
+    want, tol = R.prompt_want(q[0], kp, vp, bt, [50], [3], window=20)
+    assert ((got.cpu().double() - want).abs() <= tol).all()
+
+
+def test_out_may_be_q(device):
+    """Every row is read before it is written, by the same work-group."""
+    q, kp, vp, bt = (x.to(device) for x in R.tree_case([300, 40], 15, 8, 2, 64, BF))
+    lens = torch.tensor([300, 40], dtype=torch.int32, device=device)
+    m = _mask_tensor([int(x) for x in T.ancestor_masks(T.binary_tree_parents(15))], device)
+    for splits in (1, 3):
+        want = tree_attention(q, kp, vp, bt, lens, m, soft_cap=30.0, num_splits=splits)
+        got = q.clone()
+        tree_attention(got, kp, vp, bt, lens, m, soft_cap=30.0, num_splits=splits, out=got)
+        assert torch.equal(got, want)
+
+
 def test_corrupt_tables_and_lengths_stay_in_the_pool(device):
     """Block ids and lengths outside what there is are clamped."""
     q, kp, vp, bt = R.tree_case([100, 30], 3, 8, 2, 64, BF)
