@@ -139,13 +139,16 @@ class Rotary:
         return r
 
 
-def _heads3(name: str, x: torch.Tensor, T: int, D: int, dtype, dev) -> torch.Tensor:
+def _heads3(name: str, x: torch.Tensor, T: int, D: int, dtype, dev):
+    """(heads, stride of tokens, stride of heads) of x [T, heads, D]."""
     _require_cuda(name, x, dtype, dev)
-    if x.dim() != 3 or x.shape[0] != T or x.shape[2] != D:
+    shape = x.shape
+    if len(shape) != 3 or shape[0] != T or shape[2] != D:
         raise ValueError(f"{name} must be [T, heads, D] with T = {T}, D = {D}")
-    if x.numel() and x.stride(2) != 1:
+    st, sh, se = x.stride()
+    if se != 1 and x.numel():
         raise ValueError(f"{name}'s last dimension must be contiguous")
-    return x
+    return shape[1], st, sh
 
 
 def qk_norm_rope_kv(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor,
@@ -179,11 +182,10 @@ def qk_norm_rope_kv(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions
     if q.dim() != 3:
         raise ValueError("q must be [T, Hq, D]")
     T, Hq, D = q.shape
-    _heads3("q", q, T, D, dt, dev)
-    _heads3("k", k, T, D, dt, dev)
-    _heads3("v", v, T, D, dt, dev)
-    Hkv = k.shape[1]
-    if v.shape[1] != Hkv:
+    _, q_st, q_sh = _heads3("q", q, T, D, dt, dev)
+    Hkv, k_st, k_sh = _heads3("k", k, T, D, dt, dev)
+    v_heads, v_st, v_sh = _heads3("v", v, T, D, dt, dev)
+    if v_heads != Hkv:
         raise ValueError("k and v must have the same number of heads")
     _require_cuda("positions", positions, torch.int32, dev)
     if tuple(positions.shape) != (T,):
@@ -244,8 +246,7 @@ def qk_norm_rope_kv(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions
     base_lens = base_lens.contiguous()
     with _on(dev):
         rc = _lib.load().cfa_qk_norm_rope_kv(
-            q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
-            v.data_ptr(), v.stride(0), v.stride(1), int(dt == torch.float16),
+            q.data_ptr(), q_st, q_sh, k.data_ptr(), k_st, k_sh, v.data_ptr(), v_st, v_sh, int(dt == torch.float16),
             positions.data_ptr(), T, B, _ptr(cu_seqlens), Hq, Hkv, D, rot,
             rotary.turns.data_ptr() if rot else None,
             rotary.factor if rot else 1.0,
