@@ -29,11 +29,16 @@ struct Plan {
   }
 };
 
-// Tokens per block, and the splits of the keys: about one work-group per CU
-// (each holds most of a CU's LDS), of at least five tiles where there are more
-// than four (a split begins with the latency of its first transfers).
+// Tokens per block, and the splits of the keys.  A work-group holds most of a
+// CU's LDS, so they run in rounds of one a CU (two of one query tile and head_dim
+// 64); in units of one tile's time (1.1 to
+// 1.6 us) it spends about 5 on its first transfers and its output, and splits
+// cost 4 for the merge's launch and their partials' bytes, written and read.  us,
+// head_dim 128, without splits / with the fewest that fill the device: 512 new
+// tokens 24.5 / 28.4, 1024 tokens 37.2 / 40.6, 64 tokens behind 8000 208 / 32, 16 trees
+// of 63 nodes behind 4096 146 / 107, 40 single tokens behind 4000 160 / 139.
 // `longest` bounds a sequence's queries; tokens is the number of all.
-static Plan plan(long long tokens, long long longest, int B, int G, int Hkv, int max_keys,
+static Plan plan(long long tokens, long long longest, int B, int G, int Hkv, int D, int max_keys,
                  int window, int num_splits, bool tree) {
   Plan p;
   p.one = longest * G <= kRowsOneTile;
@@ -45,17 +50,22 @@ static Plan plan(long long tokens, long long longest, int B, int G, int Hkv, int
   if (window > 0)
     tiles = (int)std::min<long long>(
         tiles, ((long long)window + (tree ? 64 : p.TQ) + kKT - 2) / kKT + 1);
-  int s;
+  long long s = 1;
   if (num_splits > 0) {
     s = num_splits;
   } else {
     const long long items = std::max(1LL, busy * Hkv);
-    const int cus = abi::device_cu_count();
-    s = (int)std::max(1LL, (cus + items - 1) / items);
-    s = std::min(s, std::max(4, tiles / 5));
-    if (s == 2 && tiles <= 8) s = 1;
+    const long long cus = abi::device_cu_count() * (p.one && D == 64 ? 2 : 1);
+    const double part = (double)tokens * Hkv * G * D * 8 / 6.4e6;  // bytes of a tile's time
+    double least = 0.0;
+    for (long long n = 1; n <= std::min<long long>(tiles, std::max(1LL, 4 * cus / items)); ++n) {
+      const double rounds = (double)((items * n + cus - 1) / cus);
+      const double time = rounds * (5.0 + (double)((tiles + n - 1) / n)) +
+                          (n > 1 ? 4.0 + (double)n * part : 0.0);
+      if (n == 1 || time < least) s = n, least = time;
+    }
   }
-  p.splits = std::min(s, tiles);
+  p.splits = (int)std::min<long long>(s, tiles);
   return p;
 }
 
@@ -144,8 +154,8 @@ extern "C" size_t cfa_tree_attention_scored_workspace_size(int B, int N, int n_q
   cfa::abi::clear_error();
   if (B <= 0 || N <= 0 || window < 0 || check_heads(n_q_heads, n_kv_heads, head_dim) != CFA_OK)
     return 0;
-  const Plan p = plan((long long)B * N, N, B, n_q_heads / n_kv_heads, n_kv_heads, max_keys, window,
-                      num_splits, true);
+  const Plan p = plan((long long)B * N, N, B, n_q_heads / n_kv_heads, n_kv_heads, head_dim, max_keys,
+                      window, num_splits, true);
   return p.bytes((long long)B * N, n_q_heads, head_dim);
 }
 
@@ -194,7 +204,8 @@ extern "C" int cfa_tree_attention_scored(
   a.layer = layer;
   a.bs = block_size;
   a.window = window;
-  const Plan p = plan(a.T, a.Nq, B, a.G, n_kv_heads, max_keys, window, num_splits, true);
+  const Plan p = plan(a.T, a.Nq, B, a.G, n_kv_heads, head_dim, max_keys, window, num_splits,
+                      true);
   return run(a, p, head_dim, fp16, sm_scale, soft_cap, workspace, workspace_bytes, stream);
 }
 
@@ -205,8 +216,8 @@ extern "C" size_t cfa_prompt_attention_workspace_size(int T, int B, int n_q_head
   if (B <= 0 || T <= 0 || max_query <= 0 || window < 0 ||
       check_heads(n_q_heads, n_kv_heads, head_dim) != CFA_OK)
     return 0;
-  const Plan p = plan(T, std::min(max_query, T), B, n_q_heads / n_kv_heads, n_kv_heads, max_keys,
-                      window, num_splits, false);
+  const Plan p = plan(T, std::min(max_query, T), B, n_q_heads / n_kv_heads, n_kv_heads, head_dim,
+                      max_keys, window, num_splits, false);
   return p.bytes(T, n_q_heads, head_dim);
 }
 
@@ -248,7 +259,7 @@ extern "C" int cfa_prompt_attention(
   a.layer = layer;
   a.bs = block_size;
   a.window = window;
-  const Plan p = plan(T, std::min(max_query, T), B, a.G, n_kv_heads, max_keys, window, num_splits,
-                      false);
+  const Plan p = plan(T, std::min(max_query, T), B, a.G, n_kv_heads, head_dim, max_keys, window,
+                      num_splits, false);
   return run(a, p, head_dim, fp16, sm_scale, soft_cap, workspace, workspace_bytes, stream);
 }
