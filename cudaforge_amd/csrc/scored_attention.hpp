@@ -34,6 +34,14 @@
 //    gone or reused), and whole tiles in front of it are skipped.
 //  * Splits are cut on the device, from each block's own first and last tile,
 //    and leave fp32 sums for a log-sum-exp merge.
+//
+// Bound: prompts by the matrix products and the scores' vector work beside them
+// (8192 tokens, 32 heads of 128 over 8: 521 us, 1055 TFLOP/s; capped at 50 573,
+// biased 543, both 731; the matrix units busy 45% of the capped one); single
+// tokens by HBM (64 sequences to 4096 keys, capped: 126 us, 5.4 TB/s); trees by both
+// (16 of 63 nodes behind 4096, capped: 102 us with the merge, 660 TFLOP/s, 2.8
+// TB/s); small calls by latency (about 5 us in front of the first tile, 1.2 to 1.7
+// a tile, 2 for the output, 4 for a merge).
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -88,8 +96,8 @@ struct Block {
 
 // Trees: block = sequence * ceil(Nq / TQ) + part, with the sequences in the order
 // of falling length where one wave can rank them: the work-groups that start
-// last are then the short ones (64 single tokens over 1024 to 4096 keys, 172 us
-// in the batch's order).  Prompts: the blocks of all
+// last are then the short ones (64 single tokens over 1024 to 4096 keys, 126 us
+// against 172 in the batch's order).  Prompts: the blocks of all
 // sequences are numbered through, each sequence's last (longest) one first.
 __device__ __forceinline__ bool find_block(const Args &a, int id, int lane, Block &k) {
   if (a.mask) {
@@ -174,7 +182,7 @@ __device__ __forceinline__ void raw_scores(const Lane<D, QT, T> &ln, const float
   }
   // f(score, what to add to it): every score of the tile.  (The choice of form
   // stays outside: as a condition inside the loops it became a branch a score,
-  // 964 us instead of the present time for the capped prompt of 8192.)
+  // 964 us against 573 for the capped prompt of 8192.)
   auto every = [&](auto f) {
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
@@ -460,7 +468,7 @@ __global__ __launch_bounds__(kNT) void scored_attn_kernel(Args a) {
   look_up(0, kRing);
   // Under a distance bias the last tile's keys, the nearest, set the exponent
   // bases before the first tile: from far to near, steep slopes would rescale
-  // the outputs at every tile (the biased prompt of 8192 693 us).
+  // the outputs at every tile (the biased prompt of 8192 693 us against 543).
   const bool peek = BIAS && steps >= kPeekSteps;
   if (BIAS && tid < kPerTile)
     gpeek[tid] = group_row_offset<D, true>(a, btb, (t1 - 1) * kPerTile + tid, nkeys, h, from);
