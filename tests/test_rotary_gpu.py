@@ -244,3 +244,56 @@ def test_refusals_on_the_device(device):
     empty = qk_norm_rope_kv(**{**ok, "q": d[:0, :4], "k": d[:0, 4:6], "v": d[:0, 6:],
                                "positions": pd[:0]})
     assert empty.shape == (0, 4, 64)
+
+
+@pytest.mark.parametrize("D,rot,layout,norm", [
+    (128, 128, "half", True), (128, 128, "interleaved", False), (128, 100, "half", True),
+    (64, 32, "half", False), (256, 256, "half", True)])
+@pytest.mark.parametrize("T", [700, 2800, 9001])
+def test_large_batches_are_small_ones(device, D, rot, layout, norm, T):
+    """A row is the same bits whatever its batch (which sets how many rows a wave
+    takes): one call against calls of 100 tokens."""
+    Hq, Hkv, bs = 16, 2, 16
+    g = torch.Generator(device=device).manual_seed(21)
+    qkv = torch.randn(T, Hq + 2 * Hkv, D, device=device, generator=g).to(BF)
+    w = (1 + 0.1 * torch.randn(D, device=device, generator=g)).to(BF) if norm else None
+    pos = torch.randint(0, 100000, (T,), device=device, generator=g, dtype=torch.int32)
+    rotary = Rotary(rot, layout=layout, device=device)
+    pages = (T + bs - 1) // bs
+    pools = [torch.full((pages, 1, Hkv, bs, D), 3.0, dtype=BF, device=device) for _ in range(4)]
+    bt = torch.randperm(pages, device=device, generator=g).int().view(1, pages)
+    q, k, v = qkv.split([Hq, Hkv, Hkv], 1)
+    zero = torch.zeros(1, dtype=torch.int32, device=device)
+    got = qk_norm_rope_kv(q, k, v, pos, rotary, *pools[:2], bt, zero, q_norm=w, k_norm=w)
+    want = torch.cat([
+        qk_norm_rope_kv(q[t: t + 100], k[t: t + 100], v[t: t + 100], pos[t: t + 100], rotary,
+                        *pools[2:], bt, zero + t, q_norm=w, k_norm=w) for t in range(0, T, 100)])
+    assert torch.equal(got, want)
+    assert torch.equal(pools[0], pools[2]) and torch.equal(pools[1], pools[3])
+
+
+def test_offsets_past_32_bits(device):
+    """Pages behind 2^31 elements of the pools, and q's tokens so far apart."""
+    Hq, Hkv, D, bs, blocks = 4, 8, 128, 16, 140000
+    g = torch.Generator(device=device).manual_seed(22)
+    big = [torch.empty(blocks, 1, Hkv, bs, D, dtype=BF, device=device) for _ in range(2)]
+    small = [torch.empty(3, 1, Hkv, bs, D, dtype=BF, device=device) for _ in range(2)]
+    far = torch.empty((1 << 31) + 4096, dtype=BF, device=device)
+    q = far.as_strided((3, Hq, D), ((1 << 30) + 128, D, 1))
+    q.copy_(torch.randn(3, Hq, D, device=device, generator=g))
+    k, v = (torch.randn(3, Hkv, D, device=device, generator=g).to(BF) for _ in range(2))
+    pos = torch.tensor([5, 6, 70000], dtype=torch.int32, device=device)
+    rotary = Rotary(D, device=device)
+    base = torch.tensor([15], dtype=torch.int32, device=device)
+    pages = [139998, 131073, 7]
+    out = []
+    for pools, table in ((big, pages), (small, [0, 1, 2])):
+        bt = torch.tensor([table], dtype=torch.int32, device=device)
+        out.append(qk_norm_rope_kv(q, k, v, pos, rotary, *pools, bt, base))
+    assert torch.equal(*out)
+    for b, s in zip(big, small):
+        assert torch.equal(b[139998, :, :, 15], s[0, :, :, 15])
+        assert torch.equal(b[131073, :, :, :2], s[1, :, :, :2])
+    want = qk_norm_rope_kv(q.contiguous(), k, v, pos, rotary, *small,
+                           torch.tensor([[0, 1, 2]], dtype=torch.int32, device=device), base)
+    assert torch.equal(out[0], want)

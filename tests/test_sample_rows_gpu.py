@@ -291,3 +291,13 @@ def test_refusals_on_the_device(device):
         with pytest.raises(ValueError):
             sample_rows(**{**dict(rows=rd, uniforms=ud), **bad})
     assert sample_rows(rd[:0], ud[:0]).shape == (0, 3)
+
+
+def test_offsets_past_32_bits(device):
+    rows, u = _rows(3, 9000, seed=41)
+    far = torch.empty((1 << 31) + 20000, device=device)
+    view = far.as_strided((3, 9000), ((1 << 30) + 4, 1))
+    view.copy_(rows)
+    want = sample_rows(rows.to(device), u.to(device), top_p=0.9, return_probs=True)
+    got = sample_rows(view, u.to(device), top_p=0.9, return_probs=True)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])

@@ -461,3 +461,52 @@ def test_refusals_on_the_device(device):
             prompt_attention(**{**okp, **bad})
     none = prompt_attention(**{**okp, "q": qd[0, :0]})
     assert none.shape == (0, 8, 64)
+
+
+def test_offsets_past_32_bits(device):
+    """Pages behind 2^31 elements of the pools: as from small pools."""
+    Hq, Hkv, D, bs, blocks = 32, 8, 128, 16, 140000
+    big = [torch.empty(blocks, 1, Hkv, bs, D, dtype=BF, device=device) for _ in range(2)]
+    g = torch.Generator(device=device).manual_seed(31)
+    small = [torch.randn(20, 1, Hkv, bs, D, device=device, generator=g).to(BF) for _ in range(2)]
+    pages = torch.cat([torch.arange(139985, 140000), torch.arange(131071, 131076)])
+    for b, s in zip(big, small):
+        b[pages.to(device)] = s
+    few = torch.arange(20, dtype=torch.int32, device=device).view(1, 20)
+    many = pages.to(torch.int32).to(device).view(1, 20)
+    q = torch.randn(1, 15, Hq, D, device=device, generator=g).to(BF)
+    lens = torch.tensor([300], dtype=torch.int32, device=device)
+    m = _mask_tensor([int(x) for x in T.ancestor_masks(T.binary_tree_parents(15))], device)
+    cu = torch.tensor([0, 15], dtype=torch.int32, device=device)
+    for kw in (dict(soft_cap=50.0), dict(window=70)):
+        assert torch.equal(tree_attention(q, *big, many, lens, m, **kw),
+                           tree_attention(q, *small, few, lens, m, **kw))
+        assert torch.equal(prompt_attention(q[0], *big, many, lens, cu, **kw),
+                           prompt_attention(q[0], *small, few, lens, cu, **kw))
+
+
+def test_a_spoilt_query_spoils_its_own_row(device):
+    q, kp, vp, bt = (x.to(device) for x in R.tree_case([200], 9, 8, 2, 64, BF))
+    lens = torch.tensor([200], dtype=torch.int32, device=device)
+    cu = torch.tensor([0, 9], dtype=torch.int32, device=device)
+    m = _mask_tensor([int(x) for x in T.ancestor_masks(T.chain_parents(9))], device)
+    bad = q.clone()
+    bad[0, 4, 3] = float("nan")
+    for kw in (dict(), dict(soft_cap=30.0), dict(alibi_slopes=_slopes(8).to(device)),
+               dict(soft_cap=30.0, alibi_slopes=_slopes(8).to(device))):
+        a, b = (prompt_attention(x[0], kp, vp, bt, lens, cu, **kw) for x in (q, bad))
+        assert b[4, 3].isnan().all()
+        b[4, 3] = a[4, 3]
+        assert torch.equal(a, b)
+        if kw:
+            a, b = (tree_attention(x, kp, vp, bt, lens, m, **kw) for x in (q, bad))
+            b[0, 4, 3] = a[0, 4, 3]
+            assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("B", [65, 130])
+def test_many_sequences(device, B):
+    """More than the 64 that a wave ranks by their length."""
+    rng = np.random.default_rng(B)
+    _tree(device, rng.integers(0, 150, B).tolist(), 3, 4, 2, 64, "c50")
+    _tree(device, rng.integers(0, 150, B).tolist(), 1, 4, 2, 128, "b+w30")
