@@ -176,37 +176,37 @@ def qk_norm_rope_kv(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions
     """
     if not isinstance(q, torch.Tensor) or q.dtype not in (torch.bfloat16, torch.float16):
         raise ValueError("q must be a bfloat16 or float16 tensor")
-    dt = q.dtype
-    _require_cuda("q", q, dt)
-    dev = q.device
-    if q.dim() != 3:
+    dt, dev, shape = q.dtype, q.device, q.shape
+    if len(shape) != 3:
         raise ValueError("q must be [T, Hq, D]")
-    T, Hq, D = q.shape
-    _, q_st, q_sh = _heads3("q", q, T, D, dt, dev)
+    T, Hq, D = shape
+    _, q_st, q_sh = _heads3("q", q, T, D, dt, None)
     Hkv, k_st, k_sh = _heads3("k", k, T, D, dt, dev)
     v_heads, v_st, v_sh = _heads3("v", v, T, D, dt, dev)
     if v_heads != Hkv:
         raise ValueError("k and v must have the same number of heads")
     _require_cuda("positions", positions, torch.int32, dev)
-    if tuple(positions.shape) != (T,):
+    if positions.shape != (T,):
         raise ValueError(f"positions must be [T] = [{T}]")
     for name, pool in (("k_pool", k_pool), ("v_pool", v_pool)):
         _require_cuda(name, pool, dt, dev)
-        if pool.dim() != 5 or not pool.is_contiguous():
+        pools = pool.shape
+        if len(pools) != 5 or not pool.is_contiguous():
             raise ValueError(f"{name} must be a contiguous [blocks, layers, Hkv, block_size, D] tensor")
-    if k_pool.shape != v_pool.shape:
+    if k_pool.shape != pools:
         raise ValueError("k_pool and v_pool must have the same shape")
-    nblk, nlayers, ph, bs, pd = k_pool.shape
-    if (ph, pd) != (Hkv, D):
+    nblk, nlayers, ph, bs, pd = pools
+    if ph != Hkv or pd != D:
         raise ValueError("the pools' heads and head_dim must be k's")
     _require_cuda("block_tables", block_tables, torch.int32, dev)
     _require_cuda("base_lens", base_lens, torch.int32, dev)
-    B = base_lens.shape[0] if base_lens.dim() == 1 else -1
-    if B < 0 or block_tables.dim() != 2 or block_tables.shape[0] != B:
+    tables, lens = block_tables.shape, base_lens.shape
+    if len(lens) != 1 or len(tables) != 2 or tables[0] != lens[0]:
         raise ValueError("base_lens must be [B] and block_tables [B, max_blocks]")
+    B = lens[0]
     if cu_seqlens is not None:
         _require_cuda("cu_seqlens", cu_seqlens, torch.int32, dev)
-        if tuple(cu_seqlens.shape) != (B + 1,):
+        if cu_seqlens.shape != (B + 1,):
             raise ValueError("cu_seqlens must be [B + 1]")
         cu_seqlens = cu_seqlens.contiguous()
     elif T and (B == 0 or T % B):
@@ -217,7 +217,7 @@ def qk_norm_rope_kv(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions
         if not isinstance(w, torch.Tensor) or w.dtype not in (dt, torch.float32):
             raise ValueError(f"{name} must be {dt} or float32")
         _require_cuda(name, w, w.dtype, dev)
-        if tuple(w.shape) != (D,) or not w.is_contiguous():
+        if w.shape != (D,) or not w.is_contiguous():
             raise ValueError(f"{name} must be a contiguous [D] = [{D}]")
     if q_norm is not None and k_norm is not None and q_norm.dtype != k_norm.dtype:
         raise ValueError("q_norm and k_norm must have the same dtype")
@@ -227,34 +227,35 @@ def qk_norm_rope_kv(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions
     rot = 0 if rotary is None else rotary.rotary_dim
     if rot > D:
         raise ValueError("rotary_dim exceeds the head's size")
+    turns = None
     if rot:
-        _require_cuda("rotary.turns", rotary.turns, torch.int64, dev)
+        turns = rotary.turns
+        _require_cuda("rotary.turns", turns, torch.int64, dev)
     if q_out is None:
         q_out = torch.empty(T, Hq, D, dtype=dt, device=dev)
     else:
         _require_cuda("q_out", q_out, dt, dev)
-        if tuple(q_out.shape) != (T, Hq, D) or not q_out.is_contiguous():
+        if q_out.shape != shape or not q_out.is_contiguous():
             raise ValueError("q_out must be a contiguous [T, Hq, D]")
         lo = q_out.data_ptr()
         hi = lo + 2 * T * Hq * D
-        for name, x in (("q", q), ("k", k), ("v", v)):
-            (t, h, _), (st, sh, _), at = x.shape, x.stride(), x.data_ptr()
-            if hi > at and at + 2 * ((t - 1) * st + (h - 1) * sh + D) > lo and T:
+        for name, x, h, st, sh in (("q", q, Hq, q_st, q_sh), ("k", k, Hkv, k_st, k_sh),
+                                   ("v", v, Hkv, v_st, v_sh)):
+            at = x.data_ptr()
+            if hi > at and at + 2 * ((T - 1) * st + (h - 1) * sh + D) > lo and T:
                 raise ValueError(f"q_out must not overlap {name}")
     positions = positions.contiguous()
     block_tables = block_tables.contiguous()
     base_lens = base_lens.contiguous()
     with _on(dev):
         rc = _lib.load().cfa_qk_norm_rope_kv(
-            q.data_ptr(), q_st, q_sh, k.data_ptr(), k_st, k_sh, v.data_ptr(), v_st, v_sh, int(dt == torch.float16),
-            positions.data_ptr(), T, B, _ptr(cu_seqlens), Hq, Hkv, D, rot,
-            rotary.turns.data_ptr() if rot else None,
-            rotary.factor if rot else 1.0,
-            int(rot > 0 and rotary.layout == "interleaved"), _ptr(q_norm), _ptr(k_norm),
-            int(norm is not None and norm.dtype == torch.float32), eps,
-            q_out.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), nblk, nlayers, int(layer), bs,
-            block_tables.data_ptr(), block_tables.shape[1], base_lens.data_ptr(),
-            _stream_ptr(dev))
+            q.data_ptr(), q_st, q_sh, k.data_ptr(), k_st, k_sh, v.data_ptr(), v_st, v_sh,
+            dt == torch.float16, positions.data_ptr(), T, B, _ptr(cu_seqlens), Hq, Hkv, D, rot,
+            _ptr(turns), rotary.factor if rot else 1.0,
+            rot > 0 and rotary.layout == "interleaved", _ptr(q_norm), _ptr(k_norm),
+            norm is not None and norm.dtype == torch.float32, eps, q_out.data_ptr(),
+            k_pool.data_ptr(), v_pool.data_ptr(), nblk, nlayers, int(layer), bs,
+            block_tables.data_ptr(), tables[1], base_lens.data_ptr(), _stream_ptr(dev))
     _lib.check(rc, "cfa_qk_norm_rope_kv")
     return q_out
 
