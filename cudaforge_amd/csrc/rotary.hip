@@ -20,8 +20,8 @@
 // (16 bytes a lane): its sum of squares stays in the group, and a half-layout
 // pair is one exchange between two of its lanes.  A wave keeps one token, so
 // that its angles and the norms' weights are formed once for its heads.  8149
-// tokens of 48 heads of 128: 54.7 us, 3.7 TB/s (pages scattered, 256 bytes a row); 504
-// tokens 7.4 us, 8 tokens 5.
+// tokens of 48 heads of 128: 51 us, 3.9 TB/s (pages scattered, 256 bytes a row); 504
+// tokens 7 us, 8 tokens 5.
 #include <hip/hip_runtime.h>
 
 #include "abi_internal.hpp"
@@ -81,7 +81,10 @@ __device__ __forceinline__ uint4 load8(const uint16_t *p) {
 template <bool VEC>
 __device__ __forceinline__ void store8(uint16_t *p, const uint32_t (&w)[4]) {
   if constexpr (VEC) {
-    *reinterpret_cast<uint4 *>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    // past the caches: 8149 tokens 57 -> 52.4 us, and with the attention that reads
+    // them next 31.6 -> 29.7 (4 chunks of 256), 556 -> 558 (one of 8192)
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+    __builtin_nontemporal_store(u32x4{w[0], w[1], w[2], w[3]}, reinterpret_cast<u32x4 *>(p));
   } else {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
