@@ -945,8 +945,9 @@ __global__ __launch_bounds__(kNT) void probs_kernel(Args a) {
   }
   float *out = a.probs + (long long)r * a.V + i0;
   if (a.V % 4 == 0 && i0 + kPer <= a.V) {
-    reinterpret_cast<float4 *>(out)[0] = make_float4(p[0], p[1], p[2], p[3]);
-    reinterpret_cast<float4 *>(out)[1] = make_float4(p[4], p[5], p[6], p[7]);
+    typedef float f32x4 __attribute__((ext_vector_type(4)));
+    __builtin_nontemporal_store(f32x4{p[0], p[1], p[2], p[3]}, reinterpret_cast<f32x4 *>(out));
+    __builtin_nontemporal_store(f32x4{p[4], p[5], p[6], p[7]}, reinterpret_cast<f32x4 *>(out) + 1);
   } else {
 #pragma unroll
     for (int j = 0; j < kPer; ++j)

@@ -56,6 +56,8 @@ namespace scored {
 
 using namespace cfa::tree;
 
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
 // tanh(t) / t = kT0 + kT1 t^2 + kT2 t^4 + kT3 t^6 for |t| <= kTanhSmall
 constexpr float kTanhSmall = 0.5f;
 constexpr float kT0 = 0.9999994557706551f, kT1 = -0.3332631793391637f, kT2 = 0.13190296581701041f,
@@ -83,6 +85,7 @@ struct Args {
   int blocks;             // blocks launched (trees: B * ceil(Nq / TQ))
   int max_blocks, num_blocks, num_layers, layer, bs;
   int splits, window;
+  int past;               // results are stored past the caches
   float scale, cap;       // scale as given, or with a cap scale / cap
   // with a cap: its score in log2 units is x (k0 + k1 x^2 + k2 x^4 + k3 x^6) for
   // a product |x| <= small
@@ -565,6 +568,20 @@ __global__ __launch_bounds__(kNT) void scored_attn_kernel(Args a) {
     if (!lag) block_barrier();
   }
 
+  // Up to 24 MB of results pass the caches, since what they hold dirty at a kernel's
+  // end delays the next (one tree of 63 nodes, 16 MB of partials 30.4 against 27.3
+  // us; four prompts of 512, 17 MB 26.3 against 24.4); more fills them either way
+  // (16 trees, 33 MB 109.2 against 110.1; a prompt of 8192, 67 MB 588 against 599).
+  auto put = [&](auto *at, auto v) {
+    // (the empty asm keep the compiler from joining the two into a plain store)
+    if (a.past) {
+      asm volatile("");
+      __builtin_nontemporal_store(v, at);
+    } else {
+      *at = v;
+      asm volatile("");
+    }
+  };
 #pragma unroll
   for (int qt = 0; qt < QT; ++qt) {
     const float ls = lacc[qt][0];
@@ -579,14 +596,14 @@ __global__ __launch_bounds__(kNT) void scored_attn_kernel(Args a) {
         uint2 w;
         w.x = pack2<T>(o[qt][dt][0] * inv, o[qt][dt][1] * inv);
         w.y = pack2<T>(o[qt][dt][2] * inv, o[qt][dt][3] * inv);
-        *reinterpret_cast<uint2 *>(op + dt * 16 + 4 * g) = w;
+        put(reinterpret_cast<u32x2 *>(op + dt * 16 + 4 * g), u32x2{w.x, w.y});
       }
     } else {
       const long long prow = (long long)split * a.T * a.Hq + orow;
       float *pp = a.part_o + prow * D;
 #pragma unroll
       for (int dt = 0; dt < D / 16; ++dt)
-        *reinterpret_cast<f32x4 *>(pp + dt * 16 + 4 * g) = o[qt][dt];
+        put(reinterpret_cast<f32x4 *>(pp + dt * 16 + 4 * g), o[qt][dt]);
       if (g == 0) a.part_ml[prow] = make_float2(ls != 0.0f ? base[qt] : -INFINITY, ls);
     }
   }
@@ -594,7 +611,9 @@ __global__ __launch_bounds__(kNT) void scored_attn_kernel(Args a) {
 
 // Log-sum-exp merge of the splits: out = sum_s w_s o_s / sum_s w_s l_s with
 // w_s = 2^(b_s - max b); four values a thread, D / 4 threads a row.  Rows of
-// tokens that belong to no prompt are left alone.
+// tokens that belong to no prompt are left alone.  Every value is touched once, so
+// loads and stores pass the caches (16 trees of 63 nodes, two splits: the whole call
+// 109 -> 104 us).
 constexpr int kMergeRegs = 8;  // splits whose loads are issued in one round
 template <int D, class T>
 __global__ __launch_bounds__(256) void scored_merge_kernel(Args a) {
@@ -617,7 +636,7 @@ __global__ __launch_bounds__(256) void scored_merge_kernel(Args a) {
       if (s0 + s < a.splits) {
         const long long p = (long long)(s0 + s) * rows + row;
         ml[s] = a.part_ml[p];
-        v[s] = *reinterpret_cast<const f32x4 *>(a.part_o + p * D + e);
+        v[s] = __builtin_nontemporal_load(reinterpret_cast<const f32x4 *>(a.part_o + p * D + e));
       }
     }
     float m = M;
@@ -641,7 +660,7 @@ __global__ __launch_bounds__(256) void scored_merge_kernel(Args a) {
   uint2 w;
   w.x = pack2<T>(acc[0] * inv, acc[1] * inv);
   w.y = pack2<T>(acc[2] * inv, acc[3] * inv);
-  *reinterpret_cast<uint2 *>(a.out + row * D + e) = w;
+  __builtin_nontemporal_store(u32x2{w.x, w.y}, reinterpret_cast<u32x2 *>(a.out + row * D + e));
 }
 
 template <int D, int QT, class T>
