@@ -29,43 +29,82 @@ struct Plan {
   }
 };
 
-// Tokens per block, and the splits of the keys.  A work-group holds most of a
-// CU's LDS, so they run in rounds of one a CU (two of one query tile and head_dim
-// 64); in units of one tile's time (1.1 to
-// 1.6 us) it spends about 5 on its first transfers and its output, and splits
-// cost 4 for the merge's launch and their partials' bytes, written and read.  us,
-// head_dim 128, without splits / with the fewest that fill the device: 512 new
-// tokens 24.5 / 28.4, 1024 tokens 37.2 / 40.6, 64 tokens behind 8000 208 / 32, 16 trees
-// of 63 nodes behind 4096 146 / 107, 40 single tokens behind 4000 160 / 139.
+// Query rows of a block (256 in two tiles a wave, or 128 or 64 in one) and splits of
+// the keys, by the time that they would take.  In us, as measured over prompts of 128
+// to 4096 tokens and trees of 31 and 63 nodes: a work-group's first transfers and
+// output, and each of its tiles,
+//    rows           256         128         64
+//    head_dim 128   6.8 + 1.6   4.3 + 1.1   3.5 + 1.0
+//    head_dim 64    4.5 + 1.4   3.0 + 1.0   2.5 + 0.84
+// one work-group a CU (of one tile and head_dim 64, two with 1.4 to 2 times the
+// throughput); a merge's launch 6, and the partials' bytes, written and read.  A call
+// takes at least its longest work-group, the sum of all over the CUs (a prompt's
+// have half the tiles of its last on average; trees' and tokens' come in whole
+// rounds), and the tiles' bytes at 6 TB/s, from whichever cache.
+// Fewer rows must gain 5%: they read keys and values more often.  us with 256 / 128 /
+// 64 rows, head_dim 128: a prompt of 512 24.0 / 17.5 / 15.5, of 1024 36.5 / 26.2 / 29.7,
+// of 2048 62 / 56 / 88, four of 512 24.4 / 29.9 / 40; one tree of 63 nodes behind 4096
+// 26.9 / 21.8 / 21.4, 24 of them 159 / 193 / 223.  Splits, of a prompt's 64 tokens behind
+// 8000: 208 without, 28 with 16.
 // `longest` bounds a sequence's queries; tokens is the number of all.
 static Plan plan(long long tokens, long long longest, int B, int G, int Hkv, int D, int max_keys,
                  int window, int num_splits, bool tree) {
-  Plan p;
-  p.one = longest * G <= kRowsOneTile;
-  p.TQ = (int)std::max(1LL, std::min(longest, (long long)(p.one ? kRowsOneTile : kMaxRows) / G));
-  p.blocks = tree ? (long long)B * ((longest + p.TQ - 1) / p.TQ) : tokens / p.TQ + B;
-  const long long busy =  // blocks that have queries, at least
-      tree ? p.blocks : std::max<long long>((tokens + p.TQ - 1) / p.TQ, std::min<long long>(B, tokens));
-  int tiles = std::max(1, (max_keys + kKT - 1) / kKT);
-  if (window > 0)
-    tiles = (int)std::min<long long>(
-        tiles, ((long long)window + (tree ? 64 : p.TQ) + kKT - 2) / kKT + 1);
-  long long s = 1;
-  if (num_splits > 0) {
-    s = num_splits;
-  } else {
-    const long long items = std::max(1LL, busy * Hkv);
-    const long long cus = abi::device_cu_count() * (p.one && D == 64 ? 2 : 1);
-    const double part = (double)tokens * Hkv * G * D * 8 / 6.4e6;  // bytes of a tile's time
-    double least = 0.0;
-    for (long long n = 1; n <= std::min<long long>(tiles, std::max(1LL, 4 * cus / items)); ++n) {
-      const double rounds = (double)((items * n + cus - 1) / cus);
-      const double time = rounds * (5.0 + (double)((tiles + n - 1) / n)) +
-                          (n > 1 ? 4.0 + (double)n * part : 0.0);
-      if (n == 1 || time < least) s = n, least = time;
+  struct Rows {
+    int rows;
+    double first, tile, share;
+  };
+  static constexpr Rows kRows[2][3] = {
+      {{kMaxRows, 6.8, 1.6, 1.0}, {kMaxRows / 2, 4.3, 1.1, 1.0}, {kRowsOneTile, 3.5, 1.0, 1.0}},
+      {{kMaxRows, 4.5, 1.4, 1.0}, {kMaxRows / 2, 3.0, 1.0, 1.4}, {kRowsOneTile, 2.5, 0.84, 2.0}}};
+  const double merged = (double)tokens * Hkv * G * D * 8 / 5.2e6;  // a split's bytes
+  Plan p{};
+  double least = 0.0;
+  for (int i = 0; i < 3; ++i) {
+    const Rows &c = kRows[D == 64][i];
+    // (the fewest rows that hold a sequence's, or else a token's heads, are the last)
+    const bool enough = i < 2 && std::max<long long>(longest, 1) * G <= kRows[D == 64][i + 1].rows;
+    if (enough || (i > 0 && G > c.rows)) continue;
+    const int TQ = (int)std::max(1LL, std::min(longest, (long long)c.rows / G));
+    const long long blocks =
+        tree ? (long long)B * ((longest + TQ - 1) / TQ) : tokens / TQ + B;
+    const long long busy =  // blocks that have queries, about
+        tree ? blocks
+             : std::max(tokens / TQ + std::min<long long>(B, tokens) / 2,
+                        std::max<long long>(1, std::min<long long>(B, tokens)));
+    int tiles = std::max(1, (max_keys + kKT - 1) / kKT);
+    double mean = tiles;
+    if (window > 0)
+      mean = tiles = (int)std::min<long long>(
+          tiles, ((long long)window + (tree ? 64 : TQ) + kKT - 2) / kKT + 1);
+    else if (!tree)
+      mean = std::max(1.0, tiles - 0.5 * (double)std::min<long long>(longest, max_keys) / kKT);
+    const double cus = abi::device_cu_count(), items = (double)std::max(1LL, busy * Hkv);
+    const double bytes = items * mean * kKT * D * 4 / 6e6;
+    long long n = num_splits > 0 ? std::min(num_splits, tiles) : 1;
+    while (true) {
+      const long long per = (tiles + n - 1) / n;
+      const double longest_of = c.first + c.tile * (double)per;
+      const double a_cu = items * (double)n / cus;
+      double time = std::max(longest_of, bytes);
+      if (tree)
+        time = std::max(time, std::ceil(a_cu) / c.share * longest_of);
+      else
+        time = std::max(time, a_cu / c.share * (std::max(c.first, 6.0) +
+                                                c.tile * std::max(1.0, mean / (double)n)));
+      if (n > 1) time += 6.0 + (double)n * merged;
+      if (p.splits == 0 || time < least * (p.TQ == TQ ? 1.0 : 0.95)) {
+        p.TQ = TQ;
+        p.blocks = blocks;
+        p.one = i > 0;
+        p.splits = (int)n;
+        least = time;
+      }
+      // (the next number of splits that makes them shorter, up to 4 rounds)
+      if (num_splits > 0 || per == 1) break;
+      n = (tiles + per - 2) / (per - 1);
+      if (items * (double)n > 4.0 * c.share * cus) break;
     }
   }
-  p.splits = (int)std::min<long long>(s, tiles);
   return p;
 }
 
