@@ -57,6 +57,7 @@ namespace scored {
 using namespace cfa::tree;
 
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 // tanh(t) / t = kT0 + kT1 t^2 + kT2 t^4 + kT3 t^6 for |t| <= kTanhSmall
 constexpr float kTanhSmall = 0.5f;
@@ -95,7 +96,21 @@ struct Args {
 // The block of query tokens of a work-group.
 struct Block {
   int b, t0, nt, i0;  // sequence, first token (global), tokens, the first's index in it
+  int ctx;            // as given
 };
+
+// Inclusive sum over the wave's lanes, within the vector registers.
+__device__ __forceinline__ int lane_scan(int v) {
+#define CFA_SCAN_STEP(ctrl, rows) v += __builtin_amdgcn_update_dpp(0, v, ctrl, rows, 0xf, false);
+  CFA_SCAN_STEP(0x111, 0xf)  // from 1, 2, 4 and 8 lanes in front, in rows of 16
+  CFA_SCAN_STEP(0x112, 0xf)
+  CFA_SCAN_STEP(0x114, 0xf)
+  CFA_SCAN_STEP(0x118, 0xf)
+  CFA_SCAN_STEP(0x142, 0xa)  // lane 15 to the next row
+  CFA_SCAN_STEP(0x143, 0xc)  // lane 31 to the upper half
+#undef CFA_SCAN_STEP
+  return v;
+}
 
 // Trees: block = sequence * ceil(Nq / TQ) + part, with the sequences in the order
 // of falling length where one wave can rank them: the work-groups that start
@@ -114,6 +129,9 @@ __device__ __forceinline__ bool find_block(const Args &a, int id, int lane, Bloc
         rank += c > mine || (c == mine && j < lane);
       }
       k.b = __ffsll((unsigned long long)__ballot(lane < a.B && rank == k.b)) - 1;
+      k.ctx = __builtin_amdgcn_readlane(mine, k.b);
+    } else {
+      k.ctx = a.ctx[k.b];
     }
     k.i0 = (id % per) * a.TQ;
     k.t0 = k.b * a.Nq + k.i0;
@@ -123,31 +141,28 @@ __device__ __forceinline__ bool find_block(const Args &a, int id, int lane, Bloc
   int before = 0;  // blocks of the sequences in front of this round's
   for (int b0 = 0; b0 < a.B; b0 += 64) {
     const int b = b0 + lane;
-    int len = 0, at = 0;
+    int len = 0, at = 0, ctx = 0;
     if (b < a.B) {
       at = a.cu[b];
+      ctx = a.ctx[b];
       // (an end behind the tokens there are, or in front of the start, is cut)
       len = at < 0 ? 0 : max(min(a.cu[b + 1], a.T) - at, 0);
     }
     const int n = (len + a.TQ - 1) / a.TQ;
-    int upto = n;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int v = __shfl_up(upto, o, 64);
-      if (lane >= o) upto += v;
-    }
+    const int upto = lane_scan(n);
     const uint64_t hit = __ballot(before + upto > id);
     if (hit) {
       const int w = __ffsll((unsigned long long)hit) - 1;
-      const int r = id - before - __shfl(upto - n, w, 64);  // place among its blocks
-      const int wl = __shfl(len, w, 64), nb = __shfl(n, w, 64);
+      const int nb = __builtin_amdgcn_readlane(n, w);
+      const int r = id - before - __builtin_amdgcn_readlane(upto, w) + nb;  // among its blocks
       k.b = b0 + w;
       k.i0 = (nb - 1 - r) * a.TQ;
-      k.t0 = __shfl(at, w, 64) + k.i0;
-      k.nt = min(a.TQ, wl - k.i0);
+      k.t0 = __builtin_amdgcn_readlane(at, w) + k.i0;
+      k.nt = min(a.TQ, __builtin_amdgcn_readlane(len, w) - k.i0);
+      k.ctx = __builtin_amdgcn_readlane(ctx, w);
       return true;
     }
-    before += __shfl(upto, 63, 64);
+    before += __builtin_amdgcn_readlane(upto, 63);
   }
   return false;
 }
@@ -350,6 +365,7 @@ __global__ __launch_bounds__(kNT) void scored_attn_kernel(Args a) {
   blk.t0 = __builtin_amdgcn_readfirstlane(blk.t0);
   blk.nt = __builtin_amdgcn_readfirstlane(blk.nt);
   blk.i0 = __builtin_amdgcn_readfirstlane(blk.i0);
+  blk.ctx = __builtin_amdgcn_readfirstlane(blk.ctx);
   const int b = blk.b, rows = blk.nt * a.G;
   const bool tree = a.mask != nullptr;
 
@@ -357,7 +373,7 @@ __global__ __launch_bounds__(kNT) void scored_attn_kernel(Args a) {
   // capacity are clamped rather than trusted)
   const int cap_keys = a.max_blocks * a.bs;
   const int last = tree ? a.N : blk.i0 + blk.nt;  // keys behind the context
-  const int ctx = min(max(a.ctx[b], 0), max(cap_keys - last, 0));
+  const int ctx = min(max(blk.ctx, 0), max(cap_keys - last, 0));
   int nkeys = min(ctx + last, cap_keys);  // trees: cut behind the last visible node
 
   Lane<D, QT, T> ln;
@@ -582,30 +598,47 @@ __global__ __launch_bounds__(kNT) void scored_attn_kernel(Args a) {
       asm volatile("");
     }
   };
+  if (a.splits == 1) {
+    // through LDS (the K ring's, once every wave is done with it), so that whole rows
+    // are stored, 16 bytes a lane; 16-byte chunk c of row r lies at c ^ r % (D / 8)
+    constexpr int kChunks = D / 8;
+    __syncthreads();
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+      const int r0 = (wave * QT + qt) * 16;
+      uint8_t *const tile = kring + r0 * D * 2;
+      const float ls = lacc[qt][0], inv = ls != 0.0f ? 1.0f / ls : 0.0f;
+#pragma unroll
+      for (int dt = 0; dt < D / 16; ++dt) {
+        uint2 w;
+        w.x = pack2<T>(o[qt][dt][0] * inv, o[qt][dt][1] * inv);
+        w.y = pack2<T>(o[qt][dt][2] * inv, o[qt][dt][3] * inv);
+        const int c = (dt * 2 + (g >> 1)) ^ (col % kChunks);
+        *reinterpret_cast<uint2 *>(tile + col * D * 2 + c * 16 + (g & 1) * 8) = w;
+      }
+#pragma unroll
+      for (int i = 0; i < kChunks / 4; ++i) {
+        const int x = i * 64 + lane, rr = x / kChunks, c = x % kChunks, r = r0 + rr;
+        const u32x4 v = *reinterpret_cast<const u32x4 *>(
+            tile + rr * D * 2 + ((c ^ (rr % kChunks)) << 4));
+        const long long orow = ((long long)blk.t0 + r / a.G) * a.Hq + (long long)h * a.G + r % a.G;
+        if (r < rows) put(reinterpret_cast<u32x4 *>(a.out + orow * D + c * 8), v);
+      }
+    }
+    return;
+  }
 #pragma unroll
   for (int qt = 0; qt < QT; ++qt) {
     const float ls = lacc[qt][0];
     if (!qvalid[qt]) continue;
     const int r = (wave * QT + qt) * 16 + col;
     const long long orow = ((long long)blk.t0 + r / a.G) * a.Hq + (long long)h * a.G + r % a.G;
-    if (a.splits == 1) {
-      uint16_t *op = a.out + orow * D;
-      const float inv = ls != 0.0f ? 1.0f / ls : 0.0f;
+    const long long prow = (long long)split * a.T * a.Hq + orow;
+    float *pp = a.part_o + prow * D;
 #pragma unroll
-      for (int dt = 0; dt < D / 16; ++dt) {
-        uint2 w;
-        w.x = pack2<T>(o[qt][dt][0] * inv, o[qt][dt][1] * inv);
-        w.y = pack2<T>(o[qt][dt][2] * inv, o[qt][dt][3] * inv);
-        put(reinterpret_cast<u32x2 *>(op + dt * 16 + 4 * g), u32x2{w.x, w.y});
-      }
-    } else {
-      const long long prow = (long long)split * a.T * a.Hq + orow;
-      float *pp = a.part_o + prow * D;
-#pragma unroll
-      for (int dt = 0; dt < D / 16; ++dt)
-        put(reinterpret_cast<f32x4 *>(pp + dt * 16 + 4 * g), o[qt][dt]);
-      if (g == 0) a.part_ml[prow] = make_float2(ls != 0.0f ? base[qt] : -INFINITY, ls);
-    }
+    for (int dt = 0; dt < D / 16; ++dt)
+      put(reinterpret_cast<f32x4 *>(pp + dt * 16 + 4 * g), o[qt][dt]);
+    if (g == 0) a.part_ml[prow] = make_float2(ls != 0.0f ? base[qt] : -INFINITY, ls);
   }
 }
 
