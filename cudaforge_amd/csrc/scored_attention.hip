@@ -173,7 +173,7 @@ static int run(Args &a, const Plan &p, int D, int fp16, float sm_scale, float so
     a.part_o = (float *)workspace;
     a.part_ml = (float2 *)((char *)workspace + p.part_bytes(a.T, a.Hq, D));
   }
-  a.past = (long long)p.splits * a.T * a.Hq * D * (p.splits > 1 ? 4 : 2) <= 24LL << 20;
+  a.past = (long long)p.splits * a.T * a.Hq * D * 4 <= 24LL << 20;
   hipStream_t st = (hipStream_t)stream;
   if (D == 128)
     return fp16 ? launch<128, FP16>(a, p.one, (unsigned)grid, st)

@@ -86,7 +86,7 @@ struct Args {
   int blocks;             // blocks launched (trees: B * ceil(Nq / TQ))
   int max_blocks, num_blocks, num_layers, layer, bs;
   int splits, window;
-  int past;               // results are stored past the caches
+  int past;               // partials are stored past the caches
   float scale, cap;       // scale as given, or with a cap scale / cap
   // with a cap: its score in log2 units is x (k0 + k1 x^2 + k2 x^4 + k3 x^6) for
   // a product |x| <= small
@@ -584,20 +584,10 @@ __global__ __launch_bounds__(kNT) void scored_attn_kernel(Args a) {
     if (!lag) block_barrier();
   }
 
-  // Up to 24 MB of results pass the caches, since what they hold dirty at a kernel's
-  // end delays the next (one tree of 63 nodes, 16 MB of partials 30.4 against 27.3
-  // us; four prompts of 512, 17 MB 26.3 against 24.4); more fills them either way
-  // (16 trees, 33 MB 109.2 against 110.1; a prompt of 8192, 67 MB 588 against 599).
-  auto put = [&](auto *at, auto v) {
-    // (the empty asm keep the compiler from joining the two into a plain store)
-    if (a.past) {
-      asm volatile("");
-      __builtin_nontemporal_store(v, at);
-    } else {
-      *at = v;
-      asm volatile("");
-    }
-  };
+  // Results pass the caches, since what these hold dirty at a kernel's end delays the
+  // next (32 prompts of 256 tokens 72.0 -> 64.5 us, one of 8192 494 -> 492); partials
+  // only up to 24 MB (one tree of 63 nodes, 16 MB: 30.4 -> 27.3), since the merge finds
+  // part of more in them (256 tokens behind 8000, 34 MB: 50.8 -> 52.6).
   if (a.splits == 1) {
     // through LDS (the K ring's, once every wave is done with it), so that whole rows
     // are stored, 16 bytes a lane; 16-byte chunk c of row r lies at c ^ r % (D / 8)
@@ -622,11 +612,22 @@ __global__ __launch_bounds__(kNT) void scored_attn_kernel(Args a) {
         const u32x4 v = *reinterpret_cast<const u32x4 *>(
             tile + rr * D * 2 + ((c ^ (rr % kChunks)) << 4));
         const long long orow = ((long long)blk.t0 + r / a.G) * a.Hq + (long long)h * a.G + r % a.G;
-        if (r < rows) put(reinterpret_cast<u32x4 *>(a.out + orow * D + c * 8), v);
+        if (r < rows)
+          __builtin_nontemporal_store(v, reinterpret_cast<u32x4 *>(a.out + orow * D + c * 8));
       }
     }
     return;
   }
+  auto put = [&](f32x4 *at, f32x4 v) {
+    // (the empty asm keep the compiler from joining the two into a plain store)
+    if (a.past) {
+      asm volatile("");
+      __builtin_nontemporal_store(v, at);
+    } else {
+      *at = v;
+      asm volatile("");
+    }
+  };
 #pragma unroll
   for (int qt = 0; qt < QT; ++qt) {
     const float ls = lacc[qt][0];
