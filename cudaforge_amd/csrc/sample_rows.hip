@@ -548,9 +548,11 @@ __global__ __launch_bounds__(kNT) void row_kernel(Args a) {
   fill_table(table);
   if (tid < a.slices) {
     const double sq = floor((double)mine * q.c);
-    // (a slice of masked tokens alone has no histogram: shift -1)
-    sshift[tid] = mine == -INFINITY ? -1 : (int)fmin(qtop - sq, (double)kBins);
-    soct[tid] = mine == -INFINITY ? 0 : (int)fmin((top - octave(sq)) / kSub, 4000.0);
+    // (a slice of masked tokens alone has no histogram: shift -1.  Kept in range
+    // whatever the workspace holds: calls that share one at once, which they must
+    // not, get wrong tokens but read nothing outside of it.)
+    sshift[tid] = mine == -INFINITY ? -1 : (int)fmin(fmax(qtop - sq, 0.0), (double)kBins);
+    soct[tid] = mine == -INFINITY ? 0 : (int)fmin(fmax((top - octave(sq)) / kSub, 0.0), 4000.0);
     skept[tid] = 0;
   }
   if (tid == 0) {
@@ -705,12 +707,12 @@ __global__ __launch_bounds__(kNT) void row_kernel(Args a) {
           const uint32_t kj = j0 + lane < list_n[p] ? list_key[j] : 0;
           const bool in = j0 + lane < list_n[p] && kj >= lo && kj <= hi;
           const uint64_t b = __ballot(in);
-          if (in) {
-            const int to = got + __popcll(b & ((1ull << lane) - 1));
+          const int to = got + (int)__popcll(b & ((1ull << lane) - 1));
+          if (in && to < kFew) {
             dcnt[to] = kj;
             dcnt[kFew + to] = list_idx[j];
           }
-          got += __popcll(b);
+          got = min(got + (int)__popcll(b), kFew);
         }
       }
       const bool live = lane < got;
@@ -884,6 +886,7 @@ __global__ __launch_bounds__(kNT) void row_kernel(Args a) {
         const uint64_t some = __ballot(own[k] > 0.0);
         if (some) at = k * 64 + 63 - __clzll((long long)some);
       }
+      at = max(at, 0);
     }
     float x[kPer];
     const int i0 = at * kSlice + tid * kPer;
