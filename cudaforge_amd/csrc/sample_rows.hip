@@ -30,7 +30,7 @@
 // Bound: the first launch by fp64 arithmetic and LDS atomics (64 bf16 rows of 128256:
 // 15.5 us, 1.1 TB/s; 72 fp32 rows 18.6 us, 2 TB/s), the second by one CU's reading of
 // its row (40 to 85 GB/s) and its dependent phases (31 and 36 us; one row of 32000
-// 15.6), the probabilities by HBM (72 rows 16.8 us, 4.4 TB/s).
+// 15.6), the probabilities by HBM (72 rows 12.8 us, 5.8 TB/s).
 #include <hip/hip_runtime.h>
 
 #include <cfloat>
@@ -59,7 +59,7 @@ enum Type { kF32 = 0, kBF16 = 1, kFP16 = 2 };
 struct Args {
   const void *rows;
   long long stride;
-  int type, R, V, draws, slices, vec;
+  int type, R, V, draws, slices;
   const float *temp, *top_p, *min_p;  // [R] or null: the scalar
   const int32_t *top_k;
   float temp0, top_p0, min_p0;
@@ -119,16 +119,22 @@ __device__ __forceinline__ float load1(const Args &a, long long row, int i) {
   }
 }
 
-// Tokens i .. i + 7 of a row as they are, by 16-byte loads (a.vec, all of them
-// in the row).
+// Tokens i .. i + 7 of a row as they are (all of them in the row), by 16-byte loads
+// at any element: rows of an odd length begin anywhere (50257 fp32 tokens by single
+// loads 41 us in the second launch, against 20 now).
 template <int TYPE>
 struct Raw {
+  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+  typedef u32x4 at_element __attribute__((aligned(2)));
   uint4 v[TYPE == kF32 ? 2 : 1];
   __device__ __forceinline__ void load(const Args &a, long long row, int i) {
     const char *p = reinterpret_cast<const char *>(a.rows) +
                     (row * a.stride + i) * (TYPE == kF32 ? 4 : 2);
 #pragma unroll
-    for (int k = 0; k < (TYPE == kF32 ? 2 : 1); ++k) v[k] = reinterpret_cast<const uint4 *>(p)[k];
+    for (int k = 0; k < (TYPE == kF32 ? 2 : 1); ++k) {
+      const u32x4 w = reinterpret_cast<const at_element *>(p)[k];
+      v[k] = make_uint4(w.x, w.y, w.z, w.w);
+    }
   }
   // A value's bits where most() has a word's upper ones.
   static __device__ __forceinline__ int word(float x) {
@@ -160,7 +166,7 @@ struct Raw {
 // Tokens i .. i + 7 of a row (-inf behind its end).
 template <int TYPE>
 __device__ __forceinline__ void load8(const Args &a, long long row, int i, float (&x)[kPer]) {
-  if (a.vec && i + kPer <= a.V) {
+  if (i + kPer <= a.V) {
     Raw<TYPE> v;
     v.load(a, row, i);
     v.get(x);
@@ -439,28 +445,20 @@ __device__ __forceinline__ uint32_t each_in_row(const Args &a, long long r, uint
   const int t0 = threadIdx.x * kPer;
   for (int b = 0; b < a.V; b += kRounds * kSlice) {
     uint64_t mask = 0;
-    if (a.vec) {
-      Raw<TYPE> v[kRounds];
+    Raw<TYPE> v[kRounds];
 #pragma unroll
-      for (int k = 0; k < kRounds; ++k)
-        if (b + k * kSlice + t0 + kPer <= a.V) v[k].load(a, r, b + k * kSlice + t0);
+    for (int k = 0; k < kRounds; ++k)
+      if (b + k * kSlice + t0 + kPer <= a.V) v[k].load(a, r, b + k * kSlice + t0);
 #pragma unroll
-      for (int k = 0; k < kRounds; ++k) {
-        const int i = b + k * kSlice + t0;
-        float x[kPer];
-        if (i + kPer <= a.V) {
-          if (positive && __ballot(v[k].most() >= border) == 0) continue;
-          v[k].get(x);
-          mask |= (uint64_t)marks(x) << (8 * k);
-        } else if (i < a.V) {
-          load8<TYPE>(a, r, i, x);
-          mask |= (uint64_t)marks(x) << (8 * k);
-        }
-      }
-    } else {
-      for (int k = 0; k < kRounds; ++k) {
-        float x[kPer];
-        load8<TYPE>(a, r, min(b + k * kSlice + t0, a.V), x);
+    for (int k = 0; k < kRounds; ++k) {
+      const int i = b + k * kSlice + t0;
+      float x[kPer];
+      if (i + kPer <= a.V) {
+        if (positive && __ballot(v[k].most() >= border) == 0) continue;
+        v[k].get(x);
+        mask |= (uint64_t)marks(x) << (8 * k);
+      } else if (i < a.V) {
+        load8<TYPE>(a, r, i, x);
         mask |= (uint64_t)marks(x) << (8 * k);
       }
     }
@@ -947,10 +945,12 @@ __global__ __launch_bounds__(kNT) void probs_kernel(Args a) {
     p[j] = kept ? (float)(weight(x[j], k.c, k.top, table) * k.scale) : 0.0f;
   }
   float *out = a.probs + (long long)r * a.V + i0;
-  if (a.V % 4 == 0 && i0 + kPer <= a.V) {
+  if (i0 + kPer <= a.V) {  // (rows of an odd length begin anywhere)
     typedef float f32x4 __attribute__((ext_vector_type(4)));
-    __builtin_nontemporal_store(f32x4{p[0], p[1], p[2], p[3]}, reinterpret_cast<f32x4 *>(out));
-    __builtin_nontemporal_store(f32x4{p[4], p[5], p[6], p[7]}, reinterpret_cast<f32x4 *>(out) + 1);
+    typedef f32x4 at_element __attribute__((aligned(4)));
+    __builtin_nontemporal_store(f32x4{p[0], p[1], p[2], p[3]}, reinterpret_cast<at_element *>(out));
+    __builtin_nontemporal_store(f32x4{p[4], p[5], p[6], p[7]},
+                                reinterpret_cast<at_element *>(out) + 1);
   } else {
 #pragma unroll
     for (int j = 0; j < kPer; ++j)
@@ -1022,8 +1022,7 @@ extern "C" int cfa_sample_rows(const void *rows, int64_t row_stride, int elem_ty
   a.draws = draws;
   a.slices = (V + kSlice - 1) / kSlice;
   if (((long long)R + 7) / 8 * 8 * a.slices * kNT >= (1LL << 32)) return fail_arg("too many rows for one call");
-  const int size = elem_type == kF32 ? 4 : 2;
-  a.vec = (uintptr_t)rows % 16 == 0 && row_stride * size % 16 == 0;
+  if ((uintptr_t)rows % (elem_type == kF32 ? 4 : 2)) return fail_arg("rows must be aligned to its elements");
   a.temp = temperature;
   a.temp0 = temperature_all;
   a.top_k = top_k;

@@ -13,8 +13,8 @@
 //
 // The tiles, rings, transposed products and phases are those of
 // tree_attention.hip (tree_tiles.hpp): one work-group takes up to 256 query
-// rows (the G = Hq / Hkv heads of a KV head times 256 / G tokens) over a split
-// of the keys; its waves keep Q^T in registers while 64-key tiles of K and V
+// rows (the G = Hq / Hkv heads of a KV head times 256 / G tokens; 128 or 64 rows
+// where those would leave CUs idle) over a split of the keys; its waves keep Q^T in registers while 64-key tiles of K and V
 // stream through LDS, and each lane owns one query column.  What differs:
 //  * Q stays as it is and the scale is applied to the products in fp32 (one
 //    fma a score, with the base): a pre-scaled Q would be rounded once more.
@@ -36,12 +36,12 @@
 //    and leave fp32 sums for a log-sum-exp merge.
 //
 // Bound: prompts by the matrix products and the scores' vector work beside them
-// (8192 tokens, 32 heads of 128 over 8: 521 us, 1055 TFLOP/s; capped at 50 573,
-// biased 543, both 731; the matrix units busy 45% of the capped one); single
-// tokens by HBM (64 sequences to 4096 keys, capped: 126 us, 5.4 TB/s); trees by both
-// (16 of 63 nodes behind 4096, capped: 102 us with the merge, 660 TFLOP/s, 2.8
-// TB/s); small calls by latency (about 5 us in front of the first tile, 1.2 to 1.7
-// a tile, 2 for the output, 4 for a merge).
+// (8192 tokens, 32 heads of 128 over 8: 494 us, 1113 TFLOP/s; capped at 50 567,
+// biased 546, both 714, a window of 1024 156; the matrix units busy 45% of the capped
+// one); single tokens by HBM (64 sequences to 4096 keys, capped: 125 us, 5.4 TB/s);
+// trees by both (16 of 63 nodes behind 4096, capped: 102 us with the merge, 660
+// TFLOP/s, 2.8 TB/s); small calls by latency (about 4.5 us in front of the first tile,
+// 0.8 to 1.6 a tile, 1.5 for the output, 4 for a merge).
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -200,7 +200,7 @@ __device__ __forceinline__ void raw_scores(const Lane<D, QT, T> &ln, const float
   }
   // f(score, what to add to it): every score of the tile.  (The choice of form
   // stays outside: as a condition inside the loops it became a branch a score,
-  // 964 us against 573 for the capped prompt of 8192.)
+  // 964 us against 567 for the capped prompt of 8192.)
   auto every = [&](auto f) {
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
@@ -487,7 +487,7 @@ __global__ __launch_bounds__(kNT) void scored_attn_kernel(Args a) {
   look_up(0, kRing);
   // Under a distance bias the last tile's keys, the nearest, set the exponent
   // bases before the first tile: from far to near, steep slopes would rescale
-  // the outputs at every tile (the biased prompt of 8192 693 us against 543).
+  // the outputs at every tile (the biased prompt of 8192 693 us against 546).
   const bool peek = BIAS && steps >= kPeekSteps;
   if (BIAS && tid < kPerTile)
     gpeek[tid] = group_row_offset<D, true>(a, btb, (t1 - 1) * kPerTile + tid, nkeys, h, from);
