@@ -66,32 +66,18 @@ __device__ __forceinline__ float group_sum(float v) {
   return v;
 }
 
-// Eight elements at p: one 16-byte load, or (VEC = false) eight of 2 bytes.
-template <bool VEC>
-__device__ __forceinline__ uint4 load8(const uint16_t *p) {
-  if constexpr (VEC) {
-    return *reinterpret_cast<const uint4 *>(p);
-  } else {
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = (uint32_t)p[2 * i] | ((uint32_t)p[2 * i + 1] << 16);
-    return make_uint4(w[0], w[1], w[2], w[3]);
-  }
+// Sixteen bytes at any element: views of a projection may begin anywhere, and an
+// access that an address splits costs little (eight of 2 bytes: four times as many).
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef u32x4 at_element __attribute__((aligned(2)));
+__device__ __forceinline__ uint4 load8(const void *p) {
+  const u32x4 w = *reinterpret_cast<const at_element *>(p);
+  return make_uint4(w.x, w.y, w.z, w.w);
 }
-template <bool VEC>
+// Past the caches: 8149 tokens 57 -> 52.4 us, and with the attention that reads them
+// next 31.6 -> 29.7 (4 chunks of 256), 556 -> 558 (one of 8192).
 __device__ __forceinline__ void store8(uint16_t *p, const uint32_t (&w)[4]) {
-  if constexpr (VEC) {
-    // past the caches: 8149 tokens 57 -> 52.4 us, and with the attention that reads
-    // them next 31.6 -> 29.7 (4 chunks of 256), 556 -> 558 (one of 8192)
-    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-    __builtin_nontemporal_store(u32x4{w[0], w[1], w[2], w[3]}, reinterpret_cast<u32x4 *>(p));
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      p[2 * i] = (uint16_t)w[i];
-      p[2 * i + 1] = (uint16_t)(w[i] >> 16);
-    }
-  }
+  __builtin_nontemporal_store(u32x4{w[0], w[1], w[2], w[3]}, reinterpret_cast<at_element *>(p));
 }
 
 template <class T>
@@ -102,41 +88,31 @@ __device__ __forceinline__ void unpack8(const uint4 &v, float (&x)[8]) {
   unpack2<T>(v.w, x[6], x[7]);
 }
 
-// Weights e .. e + 7 of a norm (1 where there is none); PAR: 16-byte loads.
-template <class T, bool PAR>
+// Weights e .. e + 7 of a norm (1 where there is none).
+template <class T>
 __device__ __forceinline__ void weights8(const void *w, int f32, int e, float (&x)[8]) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) x[i] = 1.0f;
   if (!w) return;
   if (f32) {
     const float *p = reinterpret_cast<const float *>(w) + e;
-    if constexpr (PAR) {
-      const float4 a = reinterpret_cast<const float4 *>(p)[0];
-      const float4 b = reinterpret_cast<const float4 *>(p)[1];
-      x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w;
-      x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-    } else {
+    const uint4 a = load8(p), b = load8(p + 4);
+    const uint32_t u[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = p[i];
-    }
+    for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(u[i]);
   } else {
-    unpack8<T>(load8<PAR>(reinterpret_cast<const uint16_t *>(w) + e), x);
+    unpack8<T>(load8(reinterpret_cast<const uint16_t *>(w) + e), x);
   }
 }
 
 // N frequencies from number i on.
-template <int N, bool PAR>
+template <int N>
 __device__ __forceinline__ void turns_at(const Args &a, int i, uint64_t (&t)[N]) {
 #pragma unroll
   for (int k = 0; k < N; k += 2) {
-    if constexpr (PAR) {
-      const ulonglong2 v = *reinterpret_cast<const ulonglong2 *>(a.turns + i + k);
-      t[k] = v.x;
-      t[k + 1] = v.y;
-    } else {
-      t[k] = a.turns[i + k];
-      t[k + 1] = a.turns[i + k + 1];
-    }
+    const uint4 v = load8(a.turns + i + k);
+    t[k] = ((uint64_t)v.y << 32) | v.x;
+    t[k + 1] = ((uint64_t)v.w << 32) | v.z;
   }
 }
 
@@ -170,7 +146,7 @@ __device__ __forceinline__ bool place(const Args &a, int t, int lane, int &b, in
 
 // One wave = one token and `rounds` times ITER * 64 / LPR consecutive rows of its
 // Hq q heads, Hkv k heads and Hkv v heads.
-template <class T, int LPR, int LAYOUT, bool VEC, int ITER>
+template <class T, int LPR, int LAYOUT, int ITER>
 __global__ __launch_bounds__(kWaves * 64) void qk_norm_rope_kv_kernel(Args a) {
   constexpr int RPW = 64 / LPR;
   const int lane = threadIdx.x & 63, l = lane % LPR;
@@ -192,7 +168,7 @@ __global__ __launch_bounds__(kWaves * 64) void qk_norm_rope_kv_kernel(Args a) {
             row < a.Hq ? a.q + t * a.q_st + row * a.q_sh
                        : row < a.Hq + a.Hkv ? a.k + t * a.k_st + (row - a.Hq) * a.k_sh
                                             : a.v + t * a.v_st + (row - a.Hq - a.Hkv) * a.v_sh;
-        raw[it] = load8<VEC>(src + e);
+        raw[it] = load8(src + e);
       }
     }
   };
@@ -212,7 +188,7 @@ __global__ __launch_bounds__(kWaves * 64) void qk_norm_rope_kv_kernel(Args a) {
   if constexpr (LAYOUT == kNeighbours) {
     if (e + 8 <= a.R) {
       uint64_t f[4];
-      turns_at<4, VEC>(a, e / 2, f);
+      turns_at<4>(a, e / 2, f);
 #pragma unroll
       for (int i = 0; i < 8; i += 2) angle(a, p, f[i / 2], c[i], s[i + 1]);
     } else {
@@ -229,7 +205,7 @@ __global__ __launch_bounds__(kWaves * 64) void qk_norm_rope_kv_kernel(Args a) {
     if (e < a.R) {  // a lane's eight lie in one half
       const bool first = e < half;
       uint64_t f[8];
-      turns_at<8, VEC>(a, first ? e : e - half, f);
+      turns_at<8>(a, first ? e : e - half, f);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         angle(a, p, f[i], c[i], s[i]);
@@ -247,8 +223,8 @@ __global__ __launch_bounds__(kWaves * 64) void qk_norm_rope_kv_kernel(Args a) {
     }
   }
   if (mine) {
-    weights8<T, VEC>(a.q_w, a.w_f32, e, wq);
-    weights8<T, VEC>(a.k_w, a.w_f32, e, wk);
+    weights8<T>(a.q_w, a.w_f32, e, wq);
+    weights8<T>(a.k_w, a.w_f32, e, wk);
   }
   // the page of this token's slot
   const long long slot = (long long)a.base[b] + j;
@@ -312,16 +288,16 @@ __global__ __launch_bounds__(kWaves * 64) void qk_norm_rope_kv_kernel(Args a) {
         w[3] = raw[it].w;
       }
       if (is_q)
-        store8<VEC>(a.q_out + ((long long)t * a.Hq + row) * a.D + e, w);
+        store8(a.q_out + ((long long)t * a.Hq + row) * a.D + e, w);
       else if (mapped)
-        store8<VEC>((is_v ? a.vc + (row - a.Hq - a.Hkv) * a.head_stride
+        store8((is_v ? a.vc + (row - a.Hq - a.Hkv) * a.head_stride
                           : a.kc + (row - a.Hq) * a.head_stride) + at + e, w);
     }
     if (round + 1 < a.rounds) load(round + 1);
   }
 }
 
-template <class T, int LPR, int LAYOUT, bool VEC>
+template <class T, int LPR, int LAYOUT>
 int launch(Args a, hipStream_t st) {
   constexpr int RPW = 64 / LPR;
   const int H = a.Hq + 2 * a.Hkv;
@@ -339,36 +315,33 @@ int launch(Args a, hipStream_t st) {
   // tokens 104 / 73 / 58.  With 2 / 6 / 8 / 12 rows in flight: 59.5 / 59.2 / 62 / 69.
   if (few >= 8192 * kIter) {
     const int all = (H + kIter * RPW - 1) / (kIter * RPW);
-    CFA_LAUNCH("qk_norm_rope_kv", (qk_norm_rope_kv_kernel<T, LPR, LAYOUT, VEC, kIter>),
+    CFA_LAUNCH("qk_norm_rope_kv", (qk_norm_rope_kv_kernel<T, LPR, LAYOUT, kIter>),
                grid(kIter, all), dim3(kWaves * 64), 0, st, a);
   } else if (few >= 8192) {
-    CFA_LAUNCH("qk_norm_rope_kv", (qk_norm_rope_kv_kernel<T, LPR, LAYOUT, VEC, kIter>),
+    CFA_LAUNCH("qk_norm_rope_kv", (qk_norm_rope_kv_kernel<T, LPR, LAYOUT, kIter>),
                grid(kIter, 1), dim3(kWaves * 64), 0, st, a);
   } else {
-    CFA_LAUNCH("qk_norm_rope_kv", (qk_norm_rope_kv_kernel<T, LPR, LAYOUT, VEC, 1>), grid(1, 1),
+    CFA_LAUNCH("qk_norm_rope_kv", (qk_norm_rope_kv_kernel<T, LPR, LAYOUT, 1>), grid(1, 1),
                dim3(kWaves * 64), 0, st, a);
   }
   return CFA_OK;
 }
 
 template <class T, int LPR>
-int launch_layout(const Args &a, int layout, bool vec, hipStream_t st) {
-  switch (layout * 2 + (vec ? 1 : 0)) {
-    case 0: return launch<T, LPR, kHalf, false>(a, st);
-    case 1: return launch<T, LPR, kHalf, true>(a, st);
-    case 2: return launch<T, LPR, kHalfAny, false>(a, st);
-    case 3: return launch<T, LPR, kHalfAny, true>(a, st);
-    case 4: return launch<T, LPR, kNeighbours, false>(a, st);
-    default: return launch<T, LPR, kNeighbours, true>(a, st);
+int launch_layout(const Args &a, int layout, hipStream_t st) {
+  switch (layout) {
+    case kHalf: return launch<T, LPR, kHalf>(a, st);
+    case kHalfAny: return launch<T, LPR, kHalfAny>(a, st);
+    default: return launch<T, LPR, kNeighbours>(a, st);
   }
 }
 
 template <class T>
-int launch_type(const Args &a, int layout, bool vec, hipStream_t st) {
-  if (a.D <= 32) return launch_layout<T, 4>(a, layout, vec, st);
-  if (a.D <= 64) return launch_layout<T, 8>(a, layout, vec, st);
-  if (a.D <= 128) return launch_layout<T, 16>(a, layout, vec, st);
-  return launch_layout<T, 32>(a, layout, vec, st);
+int launch_type(const Args &a, int layout, hipStream_t st) {
+  if (a.D <= 32) return launch_layout<T, 4>(a, layout, st);
+  if (a.D <= 64) return launch_layout<T, 8>(a, layout, st);
+  if (a.D <= 128) return launch_layout<T, 16>(a, layout, st);
+  return launch_layout<T, 32>(a, layout, st);
 }
 
 }  // namespace rotary
@@ -437,13 +410,8 @@ extern "C" int cfa_qk_norm_rope_kv(
   a.head_stride = (long long)block_size * head_dim;
   a.blk_stride = (long long)num_layers * n_kv_heads * a.head_stride;
   a.layer_off = (long long)layer * n_kv_heads * a.head_stride;
-  const bool vec = (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)q_out |
-                     (uintptr_t)k_pool | (uintptr_t)v_pool | (uintptr_t)turns |
-                     (uintptr_t)q_norm | (uintptr_t)k_norm) & 15) == 0 &&
-                   ((q_stride_t | q_stride_h | k_stride_t | k_stride_h | v_stride_t | v_stride_h) &
-                    7) == 0;
   const int layout = interleaved ? kNeighbours : (rotary_dim % 16 == 0 ? kHalf : kHalfAny);
   hipStream_t st = (hipStream_t)stream;
-  return fp16 ? launch_type<cfa::FP16>(a, layout, vec, st)
-              : launch_type<cfa::BF16>(a, layout, vec, st);
+  return fp16 ? launch_type<cfa::FP16>(a, layout, st)
+              : launch_type<cfa::BF16>(a, layout, st);
 }
