@@ -39,8 +39,8 @@
 // (8192 tokens, 32 heads of 128 over 8: 494 us, 1113 TFLOP/s; capped at 50 567,
 // biased 546, both 714, a window of 1024 156; the matrix units busy 45% of the capped
 // one); single tokens by HBM (64 sequences to 4096 keys, capped: 125 us, 5.4 TB/s);
-// trees by both (16 of 63 nodes behind 4096, capped: 102 us with the merge, 660
-// TFLOP/s, 2.8 TB/s); small calls by latency (about 4.5 us in front of the first tile,
+// trees by both (16 of 63 nodes behind 4096, capped: 98 us with the merge, 690
+// TFLOP/s, 3 TB/s); small calls by latency (about 4.5 us in front of the first tile,
 // 0.8 to 1.6 a tile, 1.5 for the output, 4 for a merge).
 #pragma once
 
@@ -647,9 +647,11 @@ __global__ __launch_bounds__(kNT) void scored_attn_kernel(Args a) {
 // w_s = 2^(b_s - max b); four values a thread, D / 4 threads a row.  Rows of
 // tokens that belong to no prompt are left alone.  Every value is touched once, so
 // loads and stores pass the caches (16 trees of 63 nodes, two splits: the whole call
-// 109 -> 104 us).
-constexpr int kMergeRegs = 8;  // splits whose loads are issued in one round
-template <int D, class T>
+// 102 -> 97 us).
+// REGS: splits whose loads are issued in one round, 4 for up to 4 splits, else 8 (16
+// trees of 63 nodes, two splits: 10.2 us with 2 or 4, 12.3 with 8, 17 with 16; one
+// token behind 8000, 32 splits: 14.3, 11.0, 9.6, 9.6).
+template <int D, class T, int REGS>
 __global__ __launch_bounds__(256) void scored_merge_kernel(Args a) {
   constexpr int kTPR = D / 4;
   const long long row = (long long)blockIdx.x * (256 / kTPR) + threadIdx.x / kTPR;
@@ -662,11 +664,11 @@ __global__ __launch_bounds__(256) void scored_merge_kernel(Args a) {
   }
   float M = -INFINITY, L = 0.0f;
   f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int s0 = 0; s0 < a.splits; s0 += kMergeRegs) {
-    float2 ml[kMergeRegs];
-    f32x4 v[kMergeRegs];
+  for (int s0 = 0; s0 < a.splits; s0 += REGS) {
+    float2 ml[REGS];
+    f32x4 v[REGS];
 #pragma unroll
-    for (int s = 0; s < kMergeRegs; ++s) {
+    for (int s = 0; s < REGS; ++s) {
       if (s0 + s < a.splits) {
         const long long p = (long long)(s0 + s) * rows + row;
         ml[s] = a.part_ml[p];
@@ -675,14 +677,14 @@ __global__ __launch_bounds__(256) void scored_merge_kernel(Args a) {
     }
     float m = M;
 #pragma unroll
-    for (int s = 0; s < kMergeRegs; ++s)
+    for (int s = 0; s < REGS; ++s)
       if (s0 + s < a.splits) m = fmaxf(m, ml[s].x);
     const float base = m == -INFINITY ? 0.0f : m;
     const float w0 = __builtin_amdgcn_exp2f(M - base);
     L *= w0;
     acc *= w0;
 #pragma unroll
-    for (int s = 0; s < kMergeRegs; ++s)
+    for (int s = 0; s < REGS; ++s)
       if (s0 + s < a.splits) {
         const float w = __builtin_amdgcn_exp2f(ml[s].x - base);
         L += w * ml[s].y;
@@ -721,8 +723,11 @@ int launch(const Args &a, bool one, unsigned grid, hipStream_t st) {
   if (rc != CFA_OK || a.splits == 1) return rc;
   const long long rows = (long long)a.T * a.Hq;
   const int per = 256 / (D / 4);
-  CFA_LAUNCH("scored_merge", (scored_merge_kernel<D, T>), dim3((unsigned)((rows + per - 1) / per)),
-             dim3(256), 0, st, a);
+  const dim3 merges((unsigned)((rows + per - 1) / per));
+  if (a.splits <= 4)
+    CFA_LAUNCH("scored_merge", (scored_merge_kernel<D, T, 4>), merges, dim3(256), 0, st, a);
+  else
+    CFA_LAUNCH("scored_merge", (scored_merge_kernel<D, T, 8>), merges, dim3(256), 0, st, a);
   return CFA_OK;
 }
 
