@@ -17,7 +17,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from .verify import _on, _ptr, _require_cuda, _stream_ptr
+from .verify import _on, _ptr, _require_all, _require_cuda, _stream_ptr
 
 __all__ = ["Rotary", "qk_norm_rope_kv"]
 
@@ -139,9 +139,8 @@ class Rotary:
         return r
 
 
-def _heads3(name: str, x: torch.Tensor, T: int, D: int, dtype, dev):
+def _heads3(name: str, x: torch.Tensor, T: int, D: int):
     """(heads, stride of tokens, stride of heads) of x [T, heads, D]."""
-    _require_cuda(name, x, dtype, dev)
     shape = x.shape
     if len(shape) != 3 or shape[0] != T or shape[2] != D:
         raise ValueError(f"{name} must be [T, heads, D] with T = {T}, D = {D}")
@@ -180,16 +179,18 @@ def qk_norm_rope_kv(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions
     if len(shape) != 3:
         raise ValueError("q must be [T, Hq, D]")
     T, Hq, D = shape
-    _, q_st, q_sh = _heads3("q", q, T, D, dt, None)
-    Hkv, k_st, k_sh = _heads3("k", k, T, D, dt, dev)
-    v_heads, v_st, v_sh = _heads3("v", v, T, D, dt, dev)
+    _require_all(dev, (("q", q, dt), ("k", k, dt), ("v", v, dt),
+                       ("positions", positions, torch.int32), ("k_pool", k_pool, dt),
+                       ("v_pool", v_pool, dt), ("block_tables", block_tables, torch.int32),
+                       ("base_lens", base_lens, torch.int32)))
+    _, q_st, q_sh = _heads3("q", q, T, D)
+    Hkv, k_st, k_sh = _heads3("k", k, T, D)
+    v_heads, v_st, v_sh = _heads3("v", v, T, D)
     if v_heads != Hkv:
         raise ValueError("k and v must have the same number of heads")
-    _require_cuda("positions", positions, torch.int32, dev)
     if positions.shape != (T,):
         raise ValueError(f"positions must be [T] = [{T}]")
     for name, pool in (("k_pool", k_pool), ("v_pool", v_pool)):
-        _require_cuda(name, pool, dt, dev)
         pools = pool.shape
         if len(pools) != 5 or not pool.is_contiguous():
             raise ValueError(f"{name} must be a contiguous [blocks, layers, Hkv, block_size, D] tensor")
@@ -198,8 +199,6 @@ def qk_norm_rope_kv(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions
     nblk, nlayers, ph, bs, pd = pools
     if ph != Hkv or pd != D:
         raise ValueError("the pools' heads and head_dim must be k's")
-    _require_cuda("block_tables", block_tables, torch.int32, dev)
-    _require_cuda("base_lens", base_lens, torch.int32, dev)
     tables, lens = block_tables.shape, base_lens.shape
     if len(lens) != 1 or len(tables) != 2 or tables[0] != lens[0]:
         raise ValueError("base_lens must be [B] and block_tables [B, max_blocks]")

@@ -73,6 +73,23 @@ def _require_cuda(name: str, t: torch.Tensor, dtype: torch.dtype, device=None) -
         raise ValueError(f"{name} must be {dtype} (got {t.dtype})")
 
 
+def _require_all(device: torch.device, named) -> None:
+    """_require_cuda of each (name, tensor, dtype) on `device`, in half its time
+    where all is well."""
+    index = device.index
+    try:
+        for _, t, dtype in named:
+            if t.dtype is not dtype or t.get_device() != index:
+                break
+        else:
+            if index is not None and device.type == "cuda":
+                return
+    except AttributeError:
+        pass
+    for name, t, dtype in named:
+        _require_cuda(name, t, dtype, device)
+
+
 @dataclass
 class ChainVerifyOutput:
     """Per-sequence results of one chain verification (all int32 device tensors).
@@ -204,10 +221,8 @@ def _half_dtype(q) -> torch.dtype:
     return torch.float16 if is_half else torch.bfloat16
 
 
-def _check_pools(k_pool: torch.Tensor, v_pool: torch.Tensor, dtype: torch.dtype, dev, Hq: int,
-                 D: int):
+def _check_pools(k_pool: torch.Tensor, v_pool: torch.Tensor, D: int):
     for name, pool in (("k_pool", k_pool), ("v_pool", v_pool)):
-        _require_cuda(name, pool, dtype, dev)
         if pool.dim() != 5 or not pool.is_contiguous():
             raise ValueError(f"{name} must be a contiguous [blocks, layers, Hkv, block_size, D] tensor")
     if k_pool.shape != v_pool.shape:
@@ -280,17 +295,17 @@ def tree_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
         raise ValueError("first_node must be >= 0")
     N = first_node + Nq
     q = q.contiguous()
-    _check_pools(k_pool, v_pool, dtype, dev, Hq, D)
+    _require_all(dev, (("k_pool", k_pool, dtype), ("v_pool", v_pool, dtype),
+                       ("block_tables", block_tables, torch.int32),
+                       ("ctx_lens", ctx_lens, torch.int32), ("tree_mask", tree_mask, torch.int64)))
+    _check_pools(k_pool, v_pool, D)
     nblk, nlayers, Hkv, bs, _ = k_pool.shape
-    _require_cuda("block_tables", block_tables, torch.int32, dev)
     if block_tables.dim() != 2 or block_tables.shape[0] != B:
         raise ValueError("block_tables must be [B, max_blocks]")
     block_tables = block_tables.contiguous()
-    _require_cuda("ctx_lens", ctx_lens, torch.int32, dev)
     if tuple(ctx_lens.shape) != (B,):
         raise ValueError("ctx_lens must be [B]")
     ctx_lens = ctx_lens.contiguous()
-    _require_cuda("tree_mask", tree_mask, torch.int64, dev)
     if tree_mask.dim() == 1 and tree_mask.shape[0] == N:
         mstride = 0
     elif tree_mask.dim() == 2 and tuple(tree_mask.shape) == (B, N):
@@ -375,16 +390,17 @@ def prompt_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor
         raise ValueError("q must be [T, Hq, D]")
     T, Hq, D = q.shape
     q = q.contiguous()
-    _check_pools(k_pool, v_pool, dtype, dev, Hq, D)
+    _require_all(dev, (("k_pool", k_pool, dtype), ("v_pool", v_pool, dtype),
+                       ("ctx_lens", ctx_lens, torch.int32),
+                       ("block_tables", block_tables, torch.int32),
+                       ("cu_seqlens", cu_seqlens, torch.int32)))
+    _check_pools(k_pool, v_pool, D)
     nblk, nlayers, Hkv, bs, _ = k_pool.shape
-    _require_cuda("ctx_lens", ctx_lens, torch.int32, dev)
     if ctx_lens.dim() != 1:
         raise ValueError("ctx_lens must be [B]")
     B = ctx_lens.shape[0]
-    _require_cuda("block_tables", block_tables, torch.int32, dev)
     if block_tables.dim() != 2 or block_tables.shape[0] != B:
         raise ValueError("block_tables must be [B, max_blocks]")
-    _require_cuda("cu_seqlens", cu_seqlens, torch.int32, dev)
     if tuple(cu_seqlens.shape) != (B + 1,):
         raise ValueError("cu_seqlens must be [B + 1]")
     block_tables, ctx_lens, cu_seqlens = (t.contiguous() for t in
