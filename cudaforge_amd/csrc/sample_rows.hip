@@ -27,7 +27,7 @@
 //     row, from cache) and selects among them by radix, to the exact token;
 //     then each draw's slice from the slices' kept masses, and the token by a
 //     scan of that slice.
-// Bound: the first launch by fp64 arithmetic and LDS atomics (64 bf16 rows of 128256:
+// Bound: the first launch by fp64 arithmetic (64 bf16 rows of 128256:
 // 15.5 us, 1.1 TB/s; 72 fp32 rows 18.6 us, 2 TB/s), the second by one CU's reading of
 // its row (40 to 85 GB/s) and its dependent phases (31 and 36 us; one row of 32000
 // 15.6), the probabilities by HBM (72 rows 12.8 us, 5.8 TB/s).
