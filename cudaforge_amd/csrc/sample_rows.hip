@@ -33,10 +33,9 @@
 // 15.6), the probabilities by HBM (72 rows 12.8 us, 5.8 TB/s).
 #include <hip/hip_runtime.h>
 
-#include <cfloat>
-
 #include "abi_internal.hpp"
 #include "half_types.hpp"
+#include "row_codes.hpp"
 
 namespace cfa {
 namespace rows {
@@ -53,8 +52,6 @@ constexpr int kWaveList = kList / (kNT / 64);
 constexpr int kFew = 64;             // tokens that one wave ranks by itself
 constexpr int kFrac = 36;            // fraction bits of a weight (below 2)
 constexpr int kSumBits = 50;         // 8192 weights; a bin's count lies above their sum
-
-enum Type { kF32 = 0, kBF16 = 1, kFP16 = 2 };
 
 struct Args {
   const void *rows;
@@ -78,32 +75,6 @@ struct Kept {
   double c, top, scale;  // bins per unit of x; bin of 2^0; 1 / kept mass
   uint32_t key;          // kept: a larger code, or this one up to index `last`
   int last;
-};
-
-// The values of a type as codes, whole numbers in their order: the bits of the
-// fp32 value, turned over where it is negative, less the low ones that the type
-// does not have (16 in bf16, 13 in fp16), so that equal values are neighbours'
-// distance of one apart from the next.
-template <int TYPE>
-struct Code {
-  static constexpr int kDrop = TYPE == kF32 ? 0 : (TYPE == kBF16 ? 16 : 13);
-  static constexpr float kMost =
-      TYPE == kF32 ? FLT_MAX : (TYPE == kBF16 ? 3.38953138925153547590e38f : 65504.0f);
-  static __device__ __forceinline__ uint32_t of(float x) {
-    const uint32_t b = __float_as_uint(x);
-    return ((b & 0x80000000u) ? ~b : b | 0x80000000u) >> kDrop;
-  }
-  static __device__ __forceinline__ float value(uint32_t c) {
-    c <<= kDrop;
-    return __uint_as_float((c & 0x80000000u) ? c & 0x7fffffffu
-                                             : ~(c | ((1u << kDrop) - 1)));
-  }
-  static __device__ __forceinline__ uint32_t lowest() { return of(-kMost); }
-  static __device__ __forceinline__ uint32_t most() { return of(kMost); }
-  // A logit as the rules take it: NaN as -inf, +inf as the largest finite, -0 as 0.
-  static __device__ __forceinline__ float clean(float x) {
-    return x != x ? -INFINITY : fminf(x, kMost) + 0.0f;
-  }
 };
 
 template <int TYPE>
@@ -410,21 +381,20 @@ __device__ __forceinline__ double log2_of(double m, const double *table) {
 // positive border are passed over by their largest word alone (as whole numbers,
 // whose order is that of positive floats); the others are marked in a mask, and
 // each lane then visits its own (a branch a token for whole waves, with its
-// visits one by one, took 15 us against 6 where a hundredth are hits).  Values
-// compare as fp32 (in the codes' order; NaN nowhere, +inf with the largest).
+// visits one by one, took 15 us against 6 where a hundredth are hits).
 template <int TYPE, int kRounds, class F>
 __device__ __forceinline__ uint32_t each_in_row(const Args &a, long long r, uint32_t klo,
                                                 uint32_t khi, F f) {
   using C = Code<TYPE>;
   uint32_t got = 0;
-  if (klo > khi) return got;
-  const float flo = C::value(klo), fhi = khi >= C::most() ? INFINITY : C::value(khi);
-  const bool positive = flo > 0.0f;
-  const int border = Raw<TYPE>::word(flo);
+  const Span<TYPE> in(klo, khi);
+  if (in.none) return got;
+  const bool positive = in.least > 0.0f;
+  const int border = Raw<TYPE>::word(in.least);
   auto marks = [&](const float (&x)[kPer]) {
     uint32_t m = 0;
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) m |= x[j] >= flo && x[j] <= fhi ? 1u << j : 0u;
+    for (int j = 0; j < kPer; ++j) m |= in.holds(x[j]) ? 1u << j : 0u;
     return m;
   };
   // the marked tokens of a round of eights that begin at base + k kSlice

@@ -301,3 +301,22 @@ def test_offsets_past_32_bits(device):
     want = sample_rows(rows.to(device), u.to(device), top_p=0.9, return_probs=True)
     got = sample_rows(view, u.to(device), top_p=0.9, return_probs=True)
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("dtype,top,zeros,each,top_k", [
+    (torch.float32, 101.5, 10000, 3333, 15000), (torch.float32, 101.5, 10000, 3333, 10001),
+    (torch.bfloat16, 54.0, 3000, 3000, 5000), (torch.bfloat16, 54.0, 9000, 3000, 9500),
+    (torch.float16, 54.0, 3000, 3000, 5000)])
+def test_zeros_beside_negative_subnormals(device, dtype, top, zeros, each, top_k):
+    """The last bin holds zeros and more than a list's 8192 of the least negative
+    values; the selection's borders fall between them, where -0 has a code that no
+    token has.  Kept: the first top_k by value, then index."""
+    least = {torch.float32: 2.0 ** -149, torch.bfloat16: 2.0 ** -133, torch.float16: 2.0 ** -24}[dtype]
+    x = torch.cat([torch.tensor([top]), torch.zeros(zeros // 2), torch.zeros(zeros - zeros // 2) * -1.0]
+                  + [torch.full((each,), -k * least, dtype=torch.float64).float() for k in (1, 2, 3)])
+    rows = torch.stack([x[torch.randperm(len(x), generator=torch.Generator().manual_seed(s))]
+                        for s in (1, 2)]).to(dtype)
+    assert (rows < 0).sum() == 6 * each and (rows == 0).sum() == 2 * zeros
+    u = torch.tensor([[0.0, 0.5, 0.99]] * 2)
+    for k in (top_k, top_k + 1, zeros, zeros + 1, zeros + 2, zeros + 1 + each, zeros + each + 2):
+        assert _check(device, rows, u, top_k=k) == 0
