@@ -319,4 +319,6 @@ def test_zeros_beside_negative_subnormals(device, dtype, top, zeros, each, top_k
     assert (rows < 0).sum() == 6 * each and (rows == 0).sum() == 2 * zeros
     u = torch.tensor([[0.0, 0.5, 0.99]] * 2)
     for k in (top_k, top_k + 1, zeros, zeros + 1, zeros + 2, zeros + 1 + each, zeros + each + 2):
-        assert _check(device, rows, u, top_k=k) == 0
+        # (in front of the largest, weights of e^-54 and less each: u = 0, one draw a
+        # row, lies within 1e-9 of their steps; 0.5 and 0.99 of none)
+        assert _check(device, rows, u, top_k=k) <= 2
