@@ -171,7 +171,8 @@ __device__ __forceinline__ bool find_block(const Args &a, int id, int lane, Bloc
 // the MFMA phase are what its operand reads are scheduled ahead with (four more,
 // and the compiler drops that schedule: 692 against 519 us for the plain prompt).
 struct Row {
-  uint64_t anc;   // trees: visible nodes (ancestors inside the window)
+  uint64_t anc;   // trees: visible nodes (ancestors inside the window); prompts:
+                  // the keys up to the row's own, of those that the table covers
   int pos;        // position
   int first;      // first visible position (window), else 0
   float slope2;   // distance bias: slope * log2(e)
@@ -260,7 +261,7 @@ __device__ __forceinline__ void raw_scores(const Lane<D, QT, T> &ln, const float
       if (tree) {
         vis = tile_visibility(kbase, ctx, r.anc);
       } else {
-        const int n = r.pos + 1 - kbase;
+        const int n = (int)r.anc - kbase;
         vis = n >= 64 ? ~0ull : (n <= 0 ? 0ull : ((1ull << n) - 1));
       }
       const int cut = min(r.first, tree ? ctx : r.first) - kbase;  // keys in front
@@ -369,11 +370,11 @@ __global__ __launch_bounds__(kNT) void scored_attn_kernel(Args a) {
   const int b = blk.b, rows = blk.nt * a.G;
   const bool tree = a.mask != nullptr;
 
-  // positions past the block table are never read (lengths beyond the table's
-  // capacity are clamped rather than trusted)
+  // positions past the block table are never read: a tree's context is cut to
+  // leave room for its nodes, a prompt's keys end with the table
   const int cap_keys = a.max_blocks * a.bs;
   const int last = tree ? a.N : blk.i0 + blk.nt;  // keys behind the context
-  const int ctx = min(max(blk.ctx, 0), max(cap_keys - last, 0));
+  const int ctx = min(max(blk.ctx, 0), tree ? max(cap_keys - last, 0) : 0x7fffffff - last);
   int nkeys = min(ctx + last, cap_keys);  // trees: cut behind the last visible node
 
   Lane<D, QT, T> ln;
@@ -419,14 +420,15 @@ __global__ __launch_bounds__(kNT) void scored_attn_kernel(Args a) {
       const int r = (wave * QT + qt) * 16 + col;
       qvalid[qt] = r < rows;
       row[qt].pos = low + (qvalid[qt] ? r / a.G : 0);
-      row[qt].anc = 0;
+      row[qt].anc = min(row[qt].pos + 1, nkeys);
     }
   }
   const int high = tree ? ctx + 63 : low + blk.nt - 1;  // no query stands behind it
   // the first position that any row sees, and the last first one
   const int from = a.window > 0 ? min(max(low - a.window + 1, 0), tree ? ctx : nkeys - 1) : 0;
   const int most_first = a.window > 0 ? max(high - a.window + 1, 0) : 0;
-  const int least = tree ? ctx : low + 1;  // keys below it are visible to all (but the window)
+  // keys below it are visible to all (but the window)
+  const int least = tree ? ctx : min(low + 1, nkeys);
   const int tlo = from / kKT, thi = (nkeys + kKT - 1) / kKT;
   const int tps = (thi - tlo + a.splits - 1) / a.splits;
   const int t0 = tlo + split * tps, t1 = min(thi, t0 + tps);

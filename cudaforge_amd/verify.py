@@ -381,7 +381,8 @@ def prompt_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor
     max_query and max_keys are guesses of the longest chunk and of the largest
     ctx_len + chunk (default T and the tables' capacity): they plan the call,
     and any positive values are right.  Rows of q behind the last sequence get
-    no output: `out` keeps what it had there.  Returns out [T, Hq, D].
+    no output: `out` keeps what it had there.  Tokens behind a table's last page
+    see what the table covers.  Returns out [T, Hq, D].
     """
     dtype = _half_dtype(q)
     _require_cuda("q", q, dtype)

@@ -293,7 +293,9 @@ int cfa_tree_attention_scored(const void *q, const void *k_pool, const void *v_p
  *              largest ctx_len + chunk; they plan blocks and splits, results are
  *              right for any positive values
  * Rows of tokens that belong to no sequence are left as they were.  T = 0 and
- * B = 0 are allowed.  No key behind a block's last token is read. */
+ * B = 0 are allowed.  No key behind a block's last token is read, nor any behind
+ * the block table: a chunk that runs past it sees the slots that the table covers,
+ * each token at its own position. */
 size_t cfa_prompt_attention_workspace_size(int T, int B, int n_q_heads, int n_kv_heads,
                                            int head_dim, int max_query, int max_keys, int window,
                                            int num_splits);

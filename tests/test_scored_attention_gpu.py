@@ -510,3 +510,39 @@ def test_many_sequences(device, B):
     rng = np.random.default_rng(B)
     _tree(device, rng.integers(0, 150, B).tolist(), 3, 4, 2, 64, "c50")
     _tree(device, rng.integers(0, 150, B).tolist(), 1, 4, 2, 128, "b+w30")
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("name", ["", "c50", "b", "c+b", "w20", "b+w45"])
+def test_prompt_longer_than_its_table(device, name, D):
+    """Tables of 48 slots: chunks and contexts that run past them see the 48, each
+    token at its own position (a window that has passed them leaves nothing); a
+    sequence beside them is as it would be alone."""
+    cap, ctx, lens = 48, [0, 20, 300, 5], [70, 100, 9, 33]
+    _, kp, vp, bt = R.tree_case([cap] * 4, 0, 8, 2, D, BF)
+    assert bt.shape == (4, 3)
+    q = (2.0 * torch.randn(sum(lens), 8, D, generator=torch.Generator().manual_seed(6))).to(BF)
+    kw = _score(name, 8)
+    at = np.concatenate([[0], np.cumsum(lens)]).tolist()
+    want, tol = zip(*[R.attend(q[t: t + n], R.gather(kp, bt[b], cap, 0), R.gather(vp, bt[b], cap, 0),
+                               torch.arange(c, c + n), torch.arange(cap),
+                               torch.arange(c, c + n)[:, None] >= torch.arange(cap), D ** -0.5, **kw)
+                      for b, (c, n, t) in enumerate(zip(ctx, lens, at))])
+    for splits in (1, 2):
+        got = prompt_attention(q.to(device), kp.to(device), vp.to(device), bt.to(device),
+                               torch.tensor(ctx, dtype=torch.int32, device=device),
+                               torch.tensor(at, dtype=torch.int32, device=device),
+                               num_splits=splits, **_args(kw, device)).cpu().double()
+        err = (got - torch.cat(want)).abs()
+        assert (err <= torch.cat(tol)).all(), (err / torch.cat(tol)).max()
+
+
+def test_prompt_lengths_out_of_range_stay_in_the_pool(device):
+    q, kp, vp, bt = R.tree_case([100, 30], 20, 8, 2, 64, BF)
+    qd, kd, vd, bd = (x.to(device) for x in (q, kp, vp, bt))
+    for lens in ([-5, 10 ** 6], [2 ** 31 - 1, -2 ** 31], [2 ** 31 - 20, 120]):
+        for kw in (dict(soft_cap=50.0), dict(window=20), dict(alibi_slopes=_slopes(8).to(device))):
+            out = prompt_attention(qd.view(40, 8, 64), kd, vd, bd,
+                                   torch.tensor(lens, dtype=torch.int32, device=device),
+                                   torch.tensor([0, 20, 40], dtype=torch.int32, device=device), **kw)
+            assert torch.isfinite(out).all()
