@@ -1,5 +1,5 @@
-// row_codes.hpp -- logits as whole numbers in their order, and ranges of these as
-// fp32 comparisons (sample_rows.hip).
+// row_codes.hpp -- logits as whole numbers in their order, ranges of these as fp32
+// comparisons, and the logarithm behind min-p's border (sample_rows.hip).
 #pragma once
 
 #include <float.h>
@@ -52,6 +52,21 @@ struct Span {
   }
   CFA_HD bool holds(float x) const { return x >= least && x <= most; }
 };
+
+constexpr int kSub = 16;  // bins per octave of weight
+
+// log2(f) for f in [1, 2), from an approximation l of it (off by 2^-19 at most): l
+// and what it misses, from f 2^-l - 1 by two terms of its series (the third is below
+// 2^-57).  2^-l is table[j] = 2^((j + 1/2) / 16) times a power series of which eight
+// terms leave 2^-69.  Off by 2^-50 at most, all roundings counted.
+CFA_HD double log2_from(double f, float l, const double *table) {
+  const double z = -(double)l * kSub, q = floor(z);
+  const double x = (z - q - 0.5) * (0.69314718055994530942 / kSub);
+  double p = 1.0;
+  for (int k = 8; k >= 1; --k) p = fma(p, x * (1.0 / k), 1.0);
+  const double d = fma(f, ldexp(table[(int)q & (kSub - 1)] * p, (int)q >> 4), -1.0);
+  return l + (d - 0.5 * d * d) * 1.4426950408889634074;
+}
 
 }  // namespace rows
 }  // namespace cfa

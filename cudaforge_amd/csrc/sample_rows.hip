@@ -44,7 +44,6 @@ constexpr int kNT = 1024;
 constexpr int kPer = 8;              // consecutive tokens of a thread
 constexpr int kSlice = kNT * kPer;   // tokens of a slice
 constexpr int kMaxSlices = 128;      // V <= 2^20
-constexpr int kSub = 16;             // bins per octave of weight
 constexpr int kBins = 512;           // 32 octaves, the last bin takes the rest
 constexpr int kDigits = 1024;        // radix of the selection inside a bin
 constexpr int kList = 8192;          // tokens of a bin that fit LDS
@@ -362,16 +361,12 @@ __device__ __forceinline__ uint32_t first_code(double q, double c) {
   return k;
 }
 
-// log2(m) for 0 < m <= 1, to about 2^-50: the fp32 logarithm, then what it
-// misses from m 2^-l - 1 (of the order of 1e-6, so two terms of its series).
+// log2(m) for 0 < m <= 1 (of 1: 0, without any rounding).
 __device__ __forceinline__ double log2_of(double m, const double *table) {
+  if (m == 1.0) return 0.0;
   const int e = ilogb(m);
   const double f = ldexp(m, -e);  // [1, 2)
-  const double l = (double)__builtin_amdgcn_logf((float)f);
-  const double z = -l * kSub, q = floor(z);
-  const double back = ldexp(table[(int)q & (kSub - 1)] * exp2_sub(z - q), (int)q >> 4);  // 2^-l
-  const double d = fma(f, back, -1.0);
-  return e + l + (d - 0.5 * d * d) * 1.4426950408889634074;
+  return e + log2_from(f, __builtin_amdgcn_logf((float)f), table);
 }
 
 // f(code, index, at) for the tokens of a row with codes klo .. khi, `at`

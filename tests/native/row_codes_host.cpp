@@ -35,3 +35,10 @@ extern "C" uint32_t codes_of(int type, float x) {
 extern "C" float codes_value(int type, uint32_t c) {
   return of_type(type, [&](auto t) { return decltype(t)::value(c); });
 }
+
+// log2_from with an approximation that is `off` from the fp32 logarithm.
+extern "C" double codes_log2(double f, float off) {
+  double table[kSub];
+  for (int j = 0; j < kSub; ++j) table[j] = exp2((j + 0.5) / kSub);
+  return log2_from(f, log2f((float)f) + off, table);
+}

@@ -1,7 +1,8 @@
 """CPU tier: the codes and ranges of csrc/row_codes.hpp (compiled with g++), by
 which the sampler's second launch selects: a token outside the range that it asked
-for would be counted outside its tables."""
+for would be counted outside its tables; and the logarithm of min-p's border."""
 import ctypes
+import decimal
 import os
 import subprocess
 
@@ -26,6 +27,8 @@ def codes():
     lib.codes_of.argtypes = [ctypes.c_int, ctypes.c_float]
     lib.codes_value.restype = ctypes.c_float
     lib.codes_value.argtypes = [ctypes.c_int, ctypes.c_uint32]
+    lib.codes_log2.restype = ctypes.c_double
+    lib.codes_log2.argtypes = [ctypes.c_double, ctypes.c_float]
     lib.codes_wrong.argtypes = [ctypes.c_int, ctypes.c_uint32, ctypes.c_uint32, ctypes.c_void_p,
                                 ctypes.c_int]
     return lib
@@ -86,3 +89,22 @@ def test_the_range_of_minus_zero_alone_is_empty(codes, kind):
     zero = np.array([0.0, -0.0], dtype=np.float32)
     c = codes.codes_of(kind, -0.0)
     assert codes.codes_wrong(kind, c, c, zero.ctypes.data, 2) == 0
+
+
+def test_logarithm_of_a_fraction(codes):
+    """Against 40 digits.  Roundings: the table's entry and the series' last sum 2^-53
+    of 2^-l each, their product 2^-53, the fma 2^-54, times log2(e): below 2^-50.6; the
+    sum with l 2^-54.  The third term of the series of log2(1 + d), |d| < 2^-18.5: 2^-56."""
+    ctx = decimal.Context(prec=40)
+    ln2 = ctx.ln(decimal.Decimal(2))
+    rng = np.random.default_rng(1)
+    worst = 0.0
+    fs = np.concatenate([1.0 + rng.random(300), 1.0 + 2.0 ** -rng.integers(1, 24, 40).astype(float),
+                         2.0 - 2.0 ** -rng.integers(1, 24, 40).astype(float), [1.0]])
+    for f in fs.astype(np.float32).astype(np.float64):
+        if f >= 2.0:
+            continue
+        want = ctx.ln(decimal.Decimal(float(f))) / ln2
+        for off in (0.0, 2.0 ** -20, -2.0 ** -20):
+            worst = max(worst, abs(float(decimal.Decimal(codes.codes_log2(float(f), off)) - want)))
+    assert worst <= 2.0 ** -50

@@ -322,3 +322,36 @@ def test_zeros_beside_negative_subnormals(device, dtype, top, zeros, each, top_k
         # (in front of the largest, weights of e^-54 and less each: u = 0, one draw a
         # row, lies within 1e-9 of their steps; 0.5 and 0.99 of none)
         assert _check(device, rows, u, top_k=k) <= 2
+
+
+@pytest.mark.parametrize("t", [1.0, 30.0, 0.01])
+def test_min_p_of_one_keeps_the_largest_alone(device, t):
+    """exp((x - max) / T) >= 1 for equal values only, however near the others are."""
+    near = torch.tensor([0.0, -1e-12, -1e-13, -1e-14, -1e-17, -1e-30, -2.0 ** -149, 0.0])
+    for scale in (1.0, t):
+        rows = (near * scale)[torch.randperm(8, generator=torch.Generator().manual_seed(3))].view(1, 8)
+        p = filtered_probs(rows.to(device), temperature=t, min_p=1.0).cpu()
+        assert torch.equal(p, (rows == 0).float() / (rows == 0).sum())
+
+
+@pytest.mark.parametrize("t", [1.0, 8.0])
+@pytest.mark.parametrize("m", [0.5, 0.25, 0.1, 0.9, 0.75])
+def test_min_p_border(device, t, m):
+    """Values next to max + T ln(min_p), where fp32 resolves far below T: the border is
+    T ln 2 2^-50 (the logarithm) and 2^-51 (sums in fp64, of at most 19) off at most,
+    so values 2e-14 T from it fall on their side."""
+    import decimal
+
+    m = float(np.float32(m))
+    drop = decimal.Decimal(t) * decimal.Context(prec=40).ln(decimal.Decimal(m))
+    top = float(np.float32(float(-drop)))
+    border = decimal.Decimal(top) + drop                # |border| < 2^-24 T: steps of 2^-48 T
+    off = [s * d * t for d in (2e-14, 1e-13, 1e-12, 1e-9) for s in (1, -1)]
+    vals = np.array([top] + [float(border) + o for o in off], dtype=np.float32)
+    dist = [abs(decimal.Decimal(float(v)) - border) for v in vals[1:]]
+    assert min(dist) > decimal.Decimal(1e-14 * t)
+    want = np.array([decimal.Decimal(float(v)) >= border for v in vals])
+    assert want.sum() == 5
+    rows = torch.from_numpy(vals).view(1, -1)
+    p = filtered_probs(rows.to(device), temperature=t, min_p=m).cpu().numpy()[0]
+    assert np.array_equal(p > 0, want)
