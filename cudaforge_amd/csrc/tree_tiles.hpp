@@ -113,7 +113,7 @@ __device__ __forceinline__ long long group_row_offset(const A &a, const int32_t 
   const int gstart = clamp_pos<kFrom>(gi * 16, from, nkeys);
   const int page = min(gstart / a.bs, a.max_blocks - 1);
   const int blk = min(max(btb[page], 0), a.num_blocks - 1);
-  return (((long long)blk * a.num_layers + a.layer) * a.Hkv + h) * (long long)(a.bs * D) +
+  return (((long long)blk * a.num_layers + a.layer) * a.Hkv + h) * ((long long)a.bs * D) +
          (long long)(gstart - page * a.bs) * D;
 }
 

@@ -546,3 +546,28 @@ def test_prompt_lengths_out_of_range_stay_in_the_pool(device):
                                    torch.tensor(lens, dtype=torch.int32, device=device),
                                    torch.tensor([0, 20, 40], dtype=torch.int32, device=device), **kw)
             assert torch.isfinite(out).all()
+
+
+@pytest.mark.parametrize("scored", [False, True])
+def test_pages_of_2_to_the_31_elements(device, scored):
+    """One page holds a whole sequence, and more elements than 32 bits count: the
+    second layer's begin behind it."""
+    Hq, D, bs = 4, 128, 1 << 24
+    big = [torch.empty(1, 2, 1, bs, D, dtype=BF, device=device) for _ in range(2)]
+    g = torch.Generator(device=device).manual_seed(17)
+    small = [torch.randn(1, 2, 1, 112, D, device=device, generator=g).to(BF) for _ in range(2)]
+    for b, s in zip(big, small):
+        b[:, :, :, :112] = s
+    table = torch.zeros(1, 1, dtype=torch.int32, device=device)
+    q = torch.randn(1, 9, Hq, D, device=device, generator=g).to(BF)
+    lens = torch.tensor([100], dtype=torch.int32, device=device)
+    m = _mask_tensor([int(x) for x in T.ancestor_masks(T.binary_tree_parents(9))], device)
+    cu = torch.tensor([0, 9], dtype=torch.int32, device=device)
+    kw = dict(soft_cap=50.0) if scored else {}
+    for layer in (0, 1):
+        a, b = (tree_attention(q, *p, table, lens, m, layer=layer, max_keys=109, **kw)
+                for p in (big, small))
+        assert torch.equal(a, b)
+        a, b = (prompt_attention(q[0], *p, table, lens, cu, layer=layer, max_keys=109, **kw)
+                for p in (big, small))
+        assert torch.equal(a, b)
