@@ -34,7 +34,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from .verify import _KINDS, _on, _require_cuda, _stream_ptr
+from .verify import _KINDS, _on, _require_cuda, _stream_ptr, _workspace
 
 __all__ = [
     "SamplingParams",
@@ -266,8 +266,7 @@ def sample_rows(rows: torch.Tensor, uniforms: Optional[torch.Tensor] = None, *,
     probs = torch.empty(R, V, dtype=torch.float32, device=dev) if return_probs else None
     lib = _lib.load()
     need = int(lib.cfa_sample_rows_workspace_size(R, V))
-    if workspace is None or workspace.numel() < need:
-        workspace = torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
+    workspace = _workspace(workspace, need, dev)
     with _on(dev):
         rc = lib.cfa_sample_rows(
             rows.data_ptr(), rows.stride(0), _ROW_TYPES[rows.dtype], R, V, draws, t, t0, k, k0, p,

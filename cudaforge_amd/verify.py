@@ -90,6 +90,18 @@ def _require_all(device: torch.device, named) -> None:
         _require_cuda(name, t, dtype, device)
 
 
+def _workspace(workspace: Optional[torch.Tensor], need: int, device: torch.device) -> torch.Tensor:
+    """The caller's workspace where it holds `need` bytes, else a new one; one that
+    lies elsewhere is refused (its address would be written to as if on `device`)."""
+    if workspace is not None:
+        _require_cuda("workspace", workspace, getattr(workspace, "dtype", None), device)
+        if not workspace.is_contiguous():
+            raise ValueError("workspace must be contiguous")
+        if workspace.numel() >= need:
+            return workspace
+    return torch.empty(max(need, 1), dtype=torch.uint8, device=device)
+
+
 @dataclass
 class ChainVerifyOutput:
     """Per-sequence results of one chain verification (all int32 device tensors).
@@ -333,8 +345,7 @@ def tree_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
         else:
             need = int(lib.cfa_tree_attention_workspace_size(B, Nq, Hq, Hkv, D, max_keys,
                                                              num_splits))
-        if workspace is None or workspace.numel() < need:
-            workspace = torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
+        workspace = _workspace(workspace, need, dev)
         if scored:
             rc = lib.cfa_tree_attention_scored(
                 q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), int(dtype == torch.float16),
@@ -419,8 +430,7 @@ def prompt_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor
     with _on(dev):
         need = int(lib.cfa_prompt_attention_workspace_size(T, B, Hq, Hkv, D, max_query, max_keys,
                                                            window, num_splits))
-        if workspace is None or workspace.numel() < need:
-            workspace = torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
+        workspace = _workspace(workspace, need, dev)
         rc = lib.cfa_prompt_attention(
             q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), int(dtype == torch.float16),
             block_tables.data_ptr(), block_tables.shape[1], ctx_lens.data_ptr(), nblk, nlayers,

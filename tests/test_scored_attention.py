@@ -94,3 +94,15 @@ def test_host_tensors_are_refused():
         tree_attention(q, pool, pool, i.view(1, 1), i, torch.ones(3, dtype=torch.int64), soft_cap=50.0)
     with pytest.raises(ValueError, match="device tensor"):
         prompt_attention(q[0], pool, pool, i.view(1, 1), i, torch.zeros(2, dtype=torch.int32))
+
+
+def test_workspace_elsewhere_is_refused():
+    """Before a device is reached: its address is the host's."""
+    from cudaforge_amd.verify import _workspace
+
+    there = torch.device("cuda", 0)
+    for n in (4, 4096):
+        with pytest.raises(ValueError, match="workspace"):
+            _workspace(torch.empty(n, dtype=torch.uint8), 64, there)
+    with pytest.raises(TypeError, match="workspace"):
+        _workspace([0] * 64, 64, there)

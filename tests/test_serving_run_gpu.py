@@ -170,3 +170,22 @@ def test_prompt_tree_and_decode(device, dtype, D, score):
     slots([len(s) for s in seqs])
     # layer 0 was never written
     assert kp[:, 0].isnan().all() and vp[:, 0].isnan().all()
+
+
+def test_workspaces_of_the_host_are_refused(device):
+    """Its address would be written to as the device's; nothing is launched."""
+    q, kp, vp, bt = (x.to(device) for x in R.tree_case([500], 3, 8, 2, 64, torch.bfloat16))
+    lens, cu = (torch.tensor(x, dtype=torch.int32, device=device) for x in ([500], [0, 3]))
+    masks = torch.tensor([1, 3, 5], device=device)
+    rows = torch.randn(2, 300, device=device)
+    host = torch.empty(1 << 20, dtype=torch.uint8)
+    strided = torch.empty(1, dtype=torch.uint8, device=device).expand(1 << 20)
+    for ws in (host, strided):
+        for call in (lambda: tree_attention(q, kp, vp, bt, lens, masks, max_keys=503, workspace=ws),
+                     lambda: tree_attention(q, kp, vp, bt, lens, masks, soft_cap=50.0, max_keys=503,
+                                            num_splits=2, workspace=ws),
+                     lambda: prompt_attention(q[0], kp, vp, bt, lens, cu, num_splits=2, workspace=ws),
+                     lambda: sample_rows(rows, workspace=ws),
+                     lambda: filtered_probs(rows, top_k=3, workspace=ws)):
+            with pytest.raises(ValueError, match="workspace"):
+                call()
