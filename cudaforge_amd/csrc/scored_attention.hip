@@ -113,6 +113,9 @@ static int check_scores(float sm_scale, float soft_cap, int window) {
   if (!std::isfinite(sm_scale)) return fail_arg("sm_scale must be finite");
   if (!(soft_cap == 0.0f || (soft_cap >= 1e-6f && std::isfinite(soft_cap))))
     return fail_arg("soft_cap must be 0 (no cap) or finite and at least 1e-6");
+  // (the factor of a product in log2 units: infinite, it would make NaN of a 0)
+  if (!std::isfinite((soft_cap > 0.0f ? 2.0f * (sm_scale / soft_cap) : sm_scale) * 1.4426951f))
+    return fail_arg("sm_scale is out of fp32's range (of soft_cap, where there is one)");
   if (window < 0) return fail_arg("window must not be negative (0: none)");
   return CFA_OK;
 }
@@ -161,6 +164,8 @@ static int run(Args &a, const Plan &p, int D, int fp16, float sm_scale, float so
     if (std::fabs(a.k1) < 1e-37f) a.k1 = 0.0f, far = 0.001;
     const double small = t != 0.0 ? far / std::fabs(t) : 1e18;
     a.small = (float)std::min(small, 1e18);  // (x^2 stays in fp32's range)
+    // a coefficient past fp32's range (scores far above the cap): no polynomial
+    if (!std::isfinite(a.k1) || !std::isfinite(a.k2) || !std::isfinite(a.k3)) a.small = -1.0f;
   }
   const long long grid = (long long)p.splits * a.Hkv * p.blocks;
   if (grid * kNT >= (1LL << 32)) return fail_arg("too many queries for one call");

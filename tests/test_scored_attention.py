@@ -106,3 +106,13 @@ def test_workspace_elsewhere_is_refused():
             _workspace(torch.empty(n, dtype=torch.uint8), 64, there)
     with pytest.raises(TypeError, match="workspace"):
         _workspace([0] * 64, 64, there)
+
+
+def test_scales_past_fp32_are_refused():
+    for call in (_tree, _prompt):
+        for change in (dict(scale=3e38), dict(scale=-3e38), dict(scale=1e33, cap=1e-6),
+                       dict(scale=1.2e38, cap=1.0)):
+            assert call(**change) == _lib.CFA_ERR_ARG
+            assert "sm_scale" in _lib.last_error()
+        # (refused for something else, behind the scale's check)
+        assert call(scale=2e38, keys=0) == _lib.CFA_ERR_ARG and "max_keys" in _lib.last_error()

@@ -571,3 +571,31 @@ def test_pages_of_2_to_the_31_elements(device, scored):
         a, b = (prompt_attention(q[0], *p, table, lens, cu, layer=layer, max_keys=109, **kw)
                 for p in (big, small))
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("scale,cap", [(1e3, 1e-4), (1e4, 1e-6), (1e6, 1.0), (2e30, 50.0)])
+@pytest.mark.parametrize("bias", [False, True])
+def test_scales_far_above_the_cap(device, scale, cap, bias):
+    """tanh is a step there; products of exactly 0 stay 0 (the polynomial's
+    coefficients would be infinite)."""
+    q, kp, vp, bt = R.tree_case([70], 3, 8, 2, 64, BF)
+    q[0, 1] = 0.0
+    q[0, 0, 1] = 0.0
+    kw = dict(cap=cap, **(dict(slopes=_slopes(8)) if bias else {}))
+    # (a product's fp32 sum may have the other sign only where |q.k| < 72 2^-24 sum |q k|)
+    want, tol = R.tree_want(q, kp, vp, bt, [70], [1, 3, 5], scale=scale, **kw)
+    k64 = R.gather(kp, bt[0], 73, 0)
+    prod = torch.stack([q[0, :, h].double() @ k64[h // 4].t() for h in range(8)], 1)
+    mag = torch.stack([q[0, :, h].double().abs() @ k64[h // 4].abs().t() for h in range(8)], 1)
+    assert ((prod.abs() > 72 * 2.0 ** -24 * mag) | (mag == 0)).all()
+    # the scores' error is then tanh's and exp2's alone, below 2^-20 of at most cap each
+    ds = 2.0 ** -20 * (cap + 1.0) + (2.0 ** -22 * 70 if bias else 0.0)
+    u = 2.0 ** -8
+    A = torch.stack([(R.gather(vp, bt[0], 73, 0)[h // 4].abs()).max(0).values for h in range(8)])
+    bound = u * want.abs() + 2.01 * (u + ds) * A
+    got = tree_attention(q.to(device), kp.to(device), vp.to(device), bt.to(device),
+                         torch.tensor([70], dtype=torch.int32, device=device),
+                         _mask_tensor([1, 3, 5], device), sm_scale=scale, max_keys=73,
+                         **_args(kw, device)).cpu().double()
+    assert torch.isfinite(got).all()
+    assert ((got - want).abs() <= bound).all()
