@@ -599,3 +599,16 @@ def test_scales_far_above_the_cap(device, scale, cap, bias):
                          **_args(kw, device)).cpu().double()
     assert torch.isfinite(got).all()
     assert ((got - want).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("scale,cap", [(1e3, 1e-4), (1e4, 1e-6), (1e6, 1.0)])
+def test_zero_queries_at_scales_far_above_the_cap(device, scale, cap):
+    """Every product of the call is 0, the polynomial's range: scores of 0."""
+    q, kp, vp, bt = R.tree_case([70], 3, 8, 2, 64, BF)
+    for kw in (dict(cap=cap), dict(cap=cap, slopes=_slopes(8))):
+        want, tol = R.tree_want(q * 0, kp, vp, bt, [70], [1, 3, 5], scale=scale, **kw)
+        got = tree_attention((q * 0).to(device), kp.to(device), vp.to(device), bt.to(device),
+                             torch.tensor([70], dtype=torch.int32, device=device),
+                             _mask_tensor([1, 3, 5], device), sm_scale=scale, max_keys=73,
+                             **_args(kw, device)).cpu().double()
+        assert ((got - want).abs() <= tol).all()
