@@ -71,7 +71,7 @@ static Plan plan(long long tokens, long long longest, int B, int G, int Hkv, int
         tree ? blocks
              : std::max(tokens / TQ + std::min<long long>(B, tokens) / 2,
                         std::max<long long>(1, std::min<long long>(B, tokens)));
-    int tiles = std::max(1, (max_keys + kKT - 1) / kKT);
+    int tiles = (int)std::max(1LL, ((long long)max_keys + kKT - 1) / kKT);
     double mean = tiles;
     if (window > 0)
       mean = tiles = (int)std::min<long long>(

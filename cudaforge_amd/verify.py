@@ -222,7 +222,7 @@ def tree_attention_workspace_bytes(B: int, N: int, n_q_heads: int, n_kv_heads: i
     a bias, a window or fp16 tensors."""
     if scored or window:
         return int(_lib.load().cfa_tree_attention_scored_workspace_size(
-            B, N, n_q_heads, n_kv_heads, head_dim, max_keys, window, num_splits))
+            B, N, n_q_heads, n_kv_heads, head_dim, _int32(max_keys), _int32(window), num_splits))
     return int(_lib.load().cfa_tree_attention_workspace_size(B, N, n_q_heads, n_kv_heads,
                                                               head_dim, max_keys, num_splits))
 
@@ -250,6 +250,12 @@ def _check_slopes(alibi_slopes: Optional[torch.Tensor], Hq: int, dev) -> Optiona
     if tuple(alibi_slopes.shape) != (Hq,):
         raise ValueError(f"alibi_slopes must be [Hq] = [{Hq}]")
     return alibi_slopes.contiguous()
+
+
+def _int32(n: int) -> int:
+    """A bound as the entry points take it: past every position, the largest is the
+    same (a wider one would lose its upper bits on the way)."""
+    return min(int(n), 2 ** 31 - 1)
 
 
 def _aligned(q: torch.Tensor) -> torch.Tensor:
@@ -332,6 +338,7 @@ def tree_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
     scored = (soft_cap != 0.0 or alibi_slopes is not None or window != 0
               or dtype == torch.float16)
     if scored:
+        window, max_keys = _int32(window), _int32(max_keys)
         alibi_slopes = _check_slopes(alibi_slopes, Hq, dev)
         q = _aligned(q)
         out = _check_out(out, q)
@@ -351,7 +358,7 @@ def tree_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
                 q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), int(dtype == torch.float16),
                 block_tables.data_ptr(), block_tables.shape[1], ctx_lens.data_ptr(), nblk, nlayers,
                 int(layer), bs, tree_mask.data_ptr(), mstride, B, N, int(first_node), Hq, Hkv, D,
-                sm_scale, soft_cap, _ptr(alibi_slopes), int(window), int(max_keys),
+                sm_scale, soft_cap, _ptr(alibi_slopes), window, max_keys,
                 int(num_splits), out.data_ptr(), workspace.data_ptr(), workspace.numel(),
                 _stream_ptr(dev))
         else:
@@ -369,7 +376,8 @@ def prompt_attention_workspace_bytes(T: int, B: int, n_q_heads: int, n_kv_heads:
                                      head_dim: int, max_query: int, max_keys: int,
                                      window: int = 0, num_splits: int = 0) -> int:
     return int(_lib.load().cfa_prompt_attention_workspace_size(
-        T, B, n_q_heads, n_kv_heads, head_dim, max_query, max_keys, window, num_splits))
+        T, B, n_q_heads, n_kv_heads, head_dim, _int32(max_query), _int32(max_keys), _int32(window),
+        num_splits))
 
 
 def prompt_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
@@ -422,10 +430,9 @@ def prompt_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor
     out = _check_out(out, q)
     if sm_scale is None:
         sm_scale = D ** -0.5
-    if max_query is None:
-        max_query = max(T, 1)
-    if max_keys is None:
-        max_keys = max(block_tables.shape[1] * bs, 1)
+    window = _int32(window)
+    max_query = _int32(max(T, 1) if max_query is None else max_query)
+    max_keys = _int32(max(block_tables.shape[1] * bs, 1) if max_keys is None else max_keys)
     lib = _lib.load()
     with _on(dev):
         need = int(lib.cfa_prompt_attention_workspace_size(T, B, Hq, Hkv, D, max_query, max_keys,
@@ -435,7 +442,7 @@ def prompt_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor
             q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), int(dtype == torch.float16),
             block_tables.data_ptr(), block_tables.shape[1], ctx_lens.data_ptr(), nblk, nlayers,
             int(layer), bs, cu_seqlens.data_ptr(), T, B, Hq, Hkv, D, sm_scale, soft_cap,
-            _ptr(alibi_slopes), int(window), int(max_query), int(max_keys), int(num_splits),
+            _ptr(alibi_slopes), window, max_query, max_keys, int(num_splits),
             out.data_ptr(), workspace.data_ptr(), workspace.numel(), _stream_ptr(dev))
     _lib.check(rc, "cfa_prompt_attention")
     return out

@@ -116,3 +116,13 @@ def test_scales_past_fp32_are_refused():
             assert "sm_scale" in _lib.last_error()
         # (refused for something else, behind the scale's check)
         assert call(scale=2e38, keys=0) == _lib.CFA_ERR_ARG and "max_keys" in _lib.last_error()
+
+
+def test_bounds_past_32_bits():
+    far, most = 2 ** 32 + 5, 2 ** 31 - 1
+    for w, k in ((far, 1000), (0, far), (far, far)):
+        assert tree_attention_workspace_bytes(2, 15, 8, 2, 64, k, 4, scored=True, window=w) \
+            == tree_attention_workspace_bytes(2, 15, 8, 2, 64, min(k, most), 4, scored=True,
+                                              window=min(w, most)) > 0
+        assert prompt_attention_workspace_bytes(30, 2, 8, 2, 64, far, k, w, 4) \
+            == prompt_attention_workspace_bytes(30, 2, 8, 2, 64, most, min(k, most), min(w, most), 4) > 0

@@ -612,3 +612,22 @@ def test_zero_queries_at_scales_far_above_the_cap(device, scale, cap):
                              _mask_tensor([1, 3, 5], device), sm_scale=scale, max_keys=73,
                              **_args(kw, device)).cpu().double()
         assert ((got - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("far", [2 ** 31 - 1, 2 ** 31, 2 ** 32 + 5, 10 ** 15])
+def test_bounds_past_32_bits(device, far):
+    """A window or a guess beyond every position: as none."""
+    host = R.tree_case([300], 5, 8, 2, 64, BF)
+    q, kp, vp, bt = (x.to(device) for x in host)
+    lens, cu = (torch.tensor(x, dtype=torch.int32, device=device) for x in ([300], [0, 5]))
+    m = _mask_tensor([int(x) for x in T.ancestor_masks(T.chain_parents(5))], device)
+    kw = dict(num_splits=2, soft_cap=50.0)
+    assert torch.equal(tree_attention(q, kp, vp, bt, lens, m, max_keys=305, window=far, **kw),
+                       tree_attention(q, kp, vp, bt, lens, m, max_keys=305, **kw))
+    assert torch.equal(prompt_attention(q[0], kp, vp, bt, lens, cu, window=far, **kw),
+                       prompt_attention(q[0], kp, vp, bt, lens, cu, **kw))
+    want, tol = R.prompt_want(host[0][0], *host[1:], [300], [5], cap=50.0)
+    for splits in (0, 2):
+        got = prompt_attention(q[0], kp, vp, bt, lens, cu, max_query=far, max_keys=far, soft_cap=50.0,
+                               num_splits=splits)
+        assert ((got.cpu().double() - want).abs() <= tol).all()
