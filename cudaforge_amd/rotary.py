@@ -91,7 +91,7 @@ class Rotary:
         if kind not in takes:
             raise ValueError(f"scaling kind must be one of {[k for k in takes if k]}")
         optional = ("fast", "slow", "attention_factor") if kind == "yarn" else ()
-        missing = [k for k in takes[kind] if k not in sc]
+        missing = [k for k in takes[kind] if sc.get(k) is None]
         extra = [k for k in sc if k not in takes[kind] + optional]
         if missing or extra:
             raise ValueError(f"scaling {kind!r}: missing {missing}, not known {extra}")

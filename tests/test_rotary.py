@@ -129,3 +129,19 @@ def test_nothing_to_do_launches_nothing(change):
         ctypes.c_float(1e-6), None, None, None, a["nblk"], a["layers"], a["layer"], a["bs"], None,
         a["maxb"], None, None)
     assert rc == _lib.CFA_OK
+
+
+@pytest.mark.parametrize("scaling", [dict(kind="linear", factor=None), dict(kind="ntk", factor=None),
+                                     dict(kind="bands", factor=8.0, low=None, high=4.0, original=8192),
+                                     dict(kind="yarn", factor=None, original=4096)])
+def test_a_scaling_without_its_value_is_refused(scaling):
+    """None is no value: it is not taken for a factor of 1."""
+    with pytest.raises(ValueError, match="missing"):
+        Rotary(64, scaling=scaling)
+
+
+def test_optional_scaling_values_may_be_none():
+    a = Rotary(64, scaling=dict(kind="yarn", factor=4.0, original=4096, fast=None,
+                                attention_factor=None))
+    b = Rotary(64, scaling=dict(kind="yarn", factor=4.0, original=4096))
+    assert torch.equal(a.turns, b.turns) and a.factor == b.factor
