@@ -55,7 +55,7 @@ constexpr int kSumBits = 50;         // 8192 weights; a bin's count lies above t
 struct Args {
   const void *rows;
   long long stride;
-  int type, R, V, draws, slices;
+  int R, V, draws, slices;
   const float *temp, *top_p, *min_p;  // [R] or null: the scalar
   const int32_t *top_k;
   float temp0, top_p0, min_p0;
@@ -981,7 +981,6 @@ extern "C" int cfa_sample_rows(const void *rows, int64_t row_stride, int elem_ty
   Args a{};
   a.rows = rows;
   a.stride = row_stride;
-  a.type = elem_type;
   a.R = R;
   a.V = V;
   a.draws = draws;

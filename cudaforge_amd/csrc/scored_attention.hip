@@ -147,7 +147,6 @@ static int run(Args &a, const Plan &p, int D, int fp16, float sm_scale, float so
     return fail_arg("q, the pools and out must be 16-byte aligned");
   a.TQ = p.TQ;
   a.splits = p.splits;
-  a.blocks = (int)p.blocks;
   a.cap = soft_cap;
   a.scale = soft_cap > 0.0f ? sm_scale / soft_cap : sm_scale;
   if (soft_cap > 0.0f) {

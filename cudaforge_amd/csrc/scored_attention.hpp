@@ -83,7 +83,6 @@ struct Args {
   float2 *part_ml;        // [S, tokens, Hq] (exponent base in log2 units, sum)
   int T, B, N, q0, Nq;    // tokens in all; trees: nodes, first query node, queries
   int Hq, Hkv, G, TQ;     // TQ: tokens per block
-  int blocks;             // blocks launched (trees: B * ceil(Nq / TQ))
   int max_blocks, num_blocks, num_layers, layer, bs;
   int splits, window;
   int past;               // partials are stored past the caches

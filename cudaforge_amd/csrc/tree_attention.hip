@@ -77,13 +77,19 @@ struct Args {
   float scale_log2;        // sm_scale * log2(e)
 };
 
+// A wave's columns: Q^T pre-scaled by scale * log2(e), and their nodes.
+template <int D, int QT>
+struct TreeLane : Lane<D, QT> {
+  uint64_t anc[QT];  // ancestor-or-self masks
+};
+
 // VALU phase of tile t: mask (tiles reaching the tree), column maxima, the
 // rare rebase, and the probabilities P = exp2(S) in bf16.  S holds tile t's
 // scores relative to each column's exponent base b; the base only moves when
 // a column's maximum exceeds it by more than kRescaleSlack, which also
 // rescales O and l (they hold tiles < t, so this precedes tile t's PV).
 template <int D, int QT>
-__device__ __forceinline__ void valu_phase(const Lane<D, QT> &ln, int kbase, int ctx, Scores<QT> &S,
+__device__ __forceinline__ void valu_phase(const TreeLane<D, QT> &ln, int kbase, int ctx, Scores<QT> &S,
                                            Softmax<QT> &sm, f32x4 (&o)[QT][D / 16],
                                            f32x4 (&lacc)[QT], Probs<QT> &P) {
   if (kbase + kKT > ctx) {
@@ -172,7 +178,7 @@ __global__ __launch_bounds__(kNT) void tree_attn_kernel(Args a) {
 
   // query rows of this wave: r = (node - q0) * G + head-in-group; Q^T is
   // scaled by scale*log2(e) once here so that scores come out in log2 units
-  Lane<D, QT> ln;
+  TreeLane<D, QT> ln;
   ln.g = g;
   bool qvalid[QT];
   {

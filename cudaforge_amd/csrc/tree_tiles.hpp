@@ -235,7 +235,7 @@ __device__ __forceinline__ float column_max(float v) {
 
 // Per-wave state of the pipelined loop: 16-row query tiles qt of this wave,
 // scores of one 64-key tile s[qt][blk][T] (keys blk*32 + 8g + 4T + i) and its
-// bf16 probabilities p[qt][blk] (keys blk*32 + 8g + 0..7).
+// 16-bit probabilities p[qt][blk] (keys blk*32 + 8g + 0..7).
 template <int QT>
 struct Scores {
   f32x4 s[QT][2][2];
@@ -247,8 +247,7 @@ struct Probs {
 
 template <int D, int QT, class T = BF16>
 struct Lane {
-  typename Mfma<T>::frag qf[QT][D / 32];  // Q^T columns pre-scaled by scale*log2(e)
-  uint64_t anc[QT];       // ancestor-or-self masks of the wave's columns
+  typename Mfma<T>::frag qf[QT][D / 32];  // Q^T columns, scaled if the kernel wants it
   int koff[D / 32];        // K-tile LDS byte offsets of this lane's operand reads
   int vbase, vh;           // V-tile transposed-read offset and swizzle
   int g;                   // lane / 16
