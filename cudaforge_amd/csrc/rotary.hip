@@ -74,7 +74,7 @@ __device__ __forceinline__ uint4 load8(const void *p) {
   const u32x4 w = *reinterpret_cast<const at_element *>(p);
   return make_uint4(w.x, w.y, w.z, w.w);
 }
-// Past the caches: 8149 tokens 57 -> 52.4 us, and with the attention that reads them
+// Past the caches: 8149 tokens 54.2 -> 50.9 us, and with the attention that reads them
 // next 31.6 -> 29.7 (4 chunks of 256), 556 -> 558 (one of 8192).
 __device__ __forceinline__ void store8(uint16_t *p, const uint32_t (&w)[4]) {
   __builtin_nontemporal_store(u32x4{w[0], w[1], w[2], w[3]}, reinterpret_cast<at_element *>(p));

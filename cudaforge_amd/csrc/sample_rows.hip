@@ -27,10 +27,12 @@
 //     row, from cache) and selects among them by radix, to the exact token;
 //     then each draw's slice from the slices' kept masses, and the token by a
 //     scan of that slice.
-// Bound: the first launch by fp64 arithmetic (64 bf16 rows of 128256:
-// 15.5 us, 1.1 TB/s; 72 fp32 rows 18.6 us, 2 TB/s), the second by one CU's reading of
-// its row (40 to 85 GB/s) and its dependent phases (31 and 36 us; one row of 32000
-// 15.6), the probabilities by HBM (72 rows 12.8 us, 5.8 TB/s).
+// Bound: the first launch by vector arithmetic, the weights' in fp64 above all (64
+// bf16 rows of 128256: 16.4 us, 1.0 TB/s; 72 fp32 rows 19.3 us, 1.9 TB/s; the vector
+// units issue in 92 and 90% of the cycles of busy CUs, LDS is used in 33%), the second
+// by one CU's reading of its row (40 to 85 GB/s) and its dependent phases (31.6 and
+// 36.9 us, on 64 and 72 of 256 CUs, vector units 57 and 51%; one row of 32000 15.4),
+// the probabilities by HBM (72 rows 12.9 us, 5.7 TB/s).
 #include <hip/hip_runtime.h>
 
 #include "abi_internal.hpp"

@@ -14,8 +14,9 @@
 // The tiles, rings, transposed products and phases are those of
 // tree_attention.hip (tree_tiles.hpp): one work-group takes up to 256 query
 // rows (the G = Hq / Hkv heads of a KV head times 256 / G tokens; 128 or 64 rows
-// where those would leave CUs idle) over a split of the keys; its waves keep Q^T in registers while 64-key tiles of K and V
-// stream through LDS, and each lane owns one query column.  What differs:
+// where those would leave CUs idle) over a split of the keys; its waves keep Q^T in
+// registers while 64-key tiles of K and V stream through LDS, and each lane owns one
+// query column.  What differs:
 //  * Q stays as it is and the scale is applied to the products in fp32 (one
 //    fma a score, with the base): a pre-scaled Q would be rounded once more.
 //  * tanh.  While every |s / cap| of a wave's tile is below 1/2, tanh(t) / t is
@@ -23,12 +24,18 @@
 //    range, 5.4e-7): it keeps small scores exact under a large cap, where 1 -
 //    2 / (1 + e^2t) cancels, and with its coefficients in the products' units it
 //    is five fp32 operations, against two transcendental ones (16 cycles each)
-//    and three others.  Tiles beyond that take the exponential form.
+//    and three others.  Tiles beyond that take the exponential form (a prompt of
+//    8192, cap 50: 553 us with scores of deviation 2, 581 with 7, 596 with 12 and
+//    more, where every tile does; in fp16 648, 737, 763).
 //  * Capped scores without a bias lie in [-cap, cap], so bf16 probabilities
 //    need no running maximum while 2^(cap log2 e) times a sum of values stays
 //    in fp32's range (kFixedCap): P = exp2(s), no maxima, no rescaling.  Others
 //    keep the lazy base of tree_attention.hip.  P's rounding to the element
-//    type (the second product's operand) is the only one before the output's.
+//    type (the second product's operand) is the only one before the output's: the
+//    matrix instruction takes both operands in one type, and the row's sum is of
+//    the rounded values.  2-norm of the error against 64 bits in bf16: 0.0017 for
+//    the output's rounding alone, 0.0018 with P's under a base (the largest is then
+//    exact), 0.0022 without one.
 //  * Keys in front of the window's first are not read: a tile's transfers are
 //    clamped to the first visible position of its rows (their pages may be
 //    gone or reused), and whole tiles in front of it are skipped.
@@ -36,12 +43,15 @@
 //    and leave fp32 sums for a log-sum-exp merge.
 //
 // Bound: prompts by the matrix products and the scores' vector work beside them
-// (8192 tokens, 32 heads of 128 over 8: 494 us, 1113 TFLOP/s; capped at 50 567,
-// biased 546, both 714, a window of 1024 156; the matrix units busy 45% of the capped
-// one); single tokens by HBM (64 sequences to 4096 keys, capped: 125 us, 5.4 TB/s);
-// trees by both (16 of 63 nodes behind 4096, capped: 98 us with the merge, 690
-// TFLOP/s, 3 TB/s); small calls by latency (about 4.5 us in front of the first tile,
-// 0.8 to 1.6 a tile, 1.5 for the output, 4 for a merge).
+// (8192 tokens, 32 heads of 128 over 8: 485 us, 1134 TFLOP/s, matrix and vector units
+// each busy 54% of the cycles, in phases of two waves a SIMD; capped at 50 553, 46 and
+// 62%; biased 547; both 726, 34 and 61%, with 1.9 times the plain one's vector
+// instructions, and 847 where every tile takes the exponential form; a window of 1024
+// 156: four rounds of work-groups of 18 tiles at 1.6 us, and 6.8 each in front of the
+// first tile and for the output); single tokens by HBM (64 sequences to 4096 keys,
+// capped: 125 us, 5.4 TB/s); trees by both (16 of 63 nodes behind 4096, capped: 98 us
+// with the merge, 690 TFLOP/s, 3 TB/s); small calls by latency (about 4.5 us in front
+// of the first tile, 0.8 to 1.6 a tile, 1.5 for the output, 4 for a merge).
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -650,8 +660,9 @@ __global__ __launch_bounds__(kNT) void scored_attn_kernel(Args a) {
 // loads and stores pass the caches (16 trees of 63 nodes, two splits: the whole call
 // 102 -> 97 us).
 // REGS: splits whose loads are issued in one round, 4 for up to 4 splits, else 8 (16
-// trees of 63 nodes, two splits: 10.2 us with 2 or 4, 12.3 with 8, 17 with 16; one
-// token behind 8000, 32 splits: 14.3, 11.0, 9.6, 9.6).
+// trees of 63 nodes, two splits: in kernel traces 8.8 us with 4 and 10.9 with 8; by
+// itself, launched over and over, 10.2 with 2 or 4, 12.3 with 8, 17 with 16; one
+// token behind 8000, 32 splits: 14.3, 11.0, 9.6, 9.6 with 2, 4, 8 and 16).
 template <int D, class T, int REGS>
 __global__ __launch_bounds__(256) void scored_merge_kernel(Args a) {
   constexpr int kTPR = D / 4;

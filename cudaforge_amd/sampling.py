@@ -227,7 +227,9 @@ def sample_rows(rows: torch.Tensor, uniforms: Optional[torch.Tensor] = None, *,
     A row keeps its first tokens in the order of falling logits (equal ones:
     lower index first): rank < top_k (<= 0: off), softmax mass in front < top_p
     (1: off), probability >= min_p times the largest (0: off); temperature 0
-    keeps the largest alone.  uniforms fp32 [R, draws] in [0, 1) pick the first
+    keeps the largest alone.  The three are intersected: top_p is of the whole
+    row's mass, not of what top_k left, and keeps no fewer tokens than filters one
+    after the other, which renormalise in between.  uniforms fp32 [R, draws] in [0, 1) pick the first
     kept index whose kept mass exceeds u of the whole; without them they come
     from `generator` (`draws` a row, default 1).  -inf masks a token; a row of
     masked tokens alone gives -1.  Returns int32 [R, draws], and with

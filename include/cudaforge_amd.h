@@ -185,7 +185,9 @@ int cfa_sample(const float *rows, int64_t row_stride, int input_kind, int R, int
  * With w_i = exp((x_i - max) / T) and Z their sum, in the order of falling x
  * (equal values: lower index first) a row keeps its first tokens, those with
  * rank < top_k (<= 0: all), mass in front of them < top_p Z (>= 1: all) and w >=
- * min_p (<= 0: all), at least one.  A draw takes the first kept index, in the
+ * min_p (<= 0: all), at least one.  Z is the mass of the whole row, also where
+ * top_k takes off some (the three are intersected; samplers that apply top-p to
+ * what top-k left, renormalised, keep fewer).  A draw takes the first kept index, in the
  * order of indices, whose kept mass up to and with itself exceeds u times the
  * kept mass.  T <= 0 (and NaN) keeps the largest alone.  Unlike
  * CFA_SAMPLE_FILTERED, equal values at a border are not kept together.
@@ -511,8 +513,8 @@ int cfa_silu_mul(const void *gu, void *out, int M, int F, void *stream);
  *
  *   q [T, n_q_heads, head_dim], k, v [T, n_kv_heads, head_dim]: bf16, or fp16
  *     (fp16 = 1); element strides of tokens and heads are the caller's,
- *     head_dim (a multiple of 8, at most 256) is contiguous; 16-byte aligned
- *     heads take wide accesses
+ *     head_dim (a multiple of 8, at most 256) is contiguous; any element
+ *     alignment is taken alike
  *   y = x * rsqrt(mean(x^2) + eps) * w for q and k heads with q_norm / k_norm
  *     [head_dim] (NULL: y = x), of the element type or fp32 (norm_f32 = 1)
  *   the pairs of the first rotary_dim elements, (i, i + rotary_dim / 2) or with
