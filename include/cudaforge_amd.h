@@ -184,13 +184,15 @@ int cfa_sample(const float *rows, int64_t row_stride, int input_kind, int R, int
  *   uniforms    [R, draws] fp32 in [0, 1); draws <= 64, independent draws
  * With w_i = exp((x_i - max) / T) and Z their sum, in the order of falling x
  * (equal values: lower index first) a row keeps its first tokens, those with
- * rank < top_k (<= 0: all), mass in front of them < top_p Z (>= 1: all) and w >=
- * min_p (<= 0: all), at least one.  Z is the mass of the whole row, also where
- * top_k takes off some (the three are intersected; samplers that apply top-p to
- * what top-k left, renormalised, keep fewer).  A draw takes the first kept index, in the
- * order of indices, whose kept mass up to and with itself exceeds u times the
- * kept mass.  T <= 0 (and NaN) keeps the largest alone.  Unlike
- * CFA_SAMPLE_FILTERED, equal values at a border are not kept together.
+ * rank < top_k (<= 0: all), mass in front of them < top_p Z (>= 1: all) and w
+ * >= min_p (<= 0: all), at least one.  Z is the mass of the whole row, also
+ * where top_k takes off some (the three are intersected; samplers that apply
+ * top-p to what top-k left, renormalised, keep fewer).  min_p 1 keeps the
+ * values that equal the maximum, however near others are.  A draw takes the
+ * first kept index, in the order of indices, whose kept mass up to and with
+ * itself exceeds u times the kept mass.  T <= 0 (and NaN) keeps the largest
+ * alone.  Unlike CFA_SAMPLE_FILTERED, equal values at a border are not kept
+ * together.
  *   out_tokens  [R, draws] int32; -1 in a row whose every token is masked
  *   out_probs   [R, V] fp32 contiguous, or NULL: the kept tokens' weights over
  *               their sum, zeros elsewhere.  With draws = 0 only these
@@ -267,8 +269,9 @@ int cfa_tree_attention(const void *q, const void *k_pool, const void *v_pool,
  * sequence's queries see are not read; a NaN or infinity in the V of one between
  * them may reach all of that sequence's queries.  q, the pools and out must be
  * 16-byte aligned.
- * soft_cap is 0 or at least 1e-6.  The workspace size takes the query nodes (N
- * - first_node) for N; 0: none is needed. */
+ * soft_cap is 0 or at least 1e-6, and sm_scale / soft_cap in fp32's range.  The
+ * workspace size takes the query nodes (N - first_node) for N; 0: none is
+ * needed. */
 size_t cfa_tree_attention_scored_workspace_size(int B, int N, int n_q_heads, int n_kv_heads,
                                                 int head_dim, int max_keys, int window,
                                                 int num_splits);
