@@ -101,7 +101,7 @@ class KVPageCopyC(ctypes.Structure):
 
 
 # The ABI these signatures describe (CFA_ABI_VERSION of include/cudaforge_amd.h).
-ABI_VERSION = 201
+ABI_VERSION = 202
 
 # name -> (restype, argtypes); every symbol the header declares.
 SIGNATURES: dict[str, tuple] = {
@@ -152,6 +152,14 @@ SIGNATURES: dict[str, tuple] = {
         _i,
         [_p, _p, _p, _i, _p, _p, _i, _p, _i, _i, _i, _i, _i, _i, _i, _p, _p, _p],
     ),
+    "cfa_kv_commit_scaled": (
+        _i,
+        [_p, _p, _p, _p, _p, _i, _p, _p, _i, _p, _i, _i, _i, _i, _i, _i, _i, _p, _p, _p],
+    ),
+    "cfa_kv_gather": (
+        _i,
+        [_p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _p, _i, _p, _p, _i, _i, _p, _p, _p],
+    ),
     "cfa_w4a16_dequant": (_i, [_p, _p, _p, _i, _i, _i, _i, _p, _p]),
     "cfa_w4a16_dequant_t": (_i, [_p, _p, _p, _i, _i, _i, _i, _p, _p]),
     "cfa_w4a16_gemm": (_i, [_p, _p, _p, _i, _i, _i, _i, _i, _p, _p]),
@@ -174,6 +182,11 @@ SIGNATURES: dict[str, tuple] = {
         _i,
         [_p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _i, _p, _i, _i, _p, _i, _i, _i, _i, _p,
          _f, _i, _p, _p, _i, _f, _p, _p, _p, _i, _i, _i, _i, _p, _i, _p, _p],
+    ),
+    "cfa_qk_norm_rope_kv_e4m3": (
+        _i,
+        [_p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _i, _p, _i, _i, _p, _i, _i, _i, _i, _p,
+         _f, _i, _p, _p, _i, _f, _p, _p, _p, _p, _p, _i, _i, _i, _i, _p, _i, _p, _p],
     ),
     "cfa_silu_mul": (_i, [_p, _p, _i, _i, _p]),
     "cfa_gemm_bf16_skinny_workspace_size": (_sz, [_i, _i, _i, _i]),

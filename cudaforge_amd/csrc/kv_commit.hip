@@ -18,7 +18,9 @@
 // per (sequence, layer) checks the path once, one thread per entry.  Rows
 // with path[j] == j (the root, and any prefix of a chain) are already in
 // place and are neither read nor written; the others are compacted in path
-// order, so the batches hold only rows that move.
+// order, so the batches hold only rows that move.  In 8-bit pools each row's
+// scale byte (e4m3.hpp; scales[block][layer][kv_head][slot]) moves as one more
+// column, by one thread for each KV head of K and of V.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -34,6 +36,7 @@ constexpr int kMaxRowBytes = 512;  // head_dim * element size
 
 struct Args {
   uint8_t *kpool, *vpool;
+  uint8_t *kscale, *vscale;  // or null
   const int32_t *bt;
   const int32_t *ctx;
   const int32_t *paths;
@@ -53,8 +56,29 @@ __device__ __forceinline__ long long slot_base(const Args &a, int b, int pos) {
   return ((long long)blk * a.num_layers * a.Hkv * a.bs + pos % a.bs) * (long long)a.row_bytes;
 }
 
-constexpr int kBatch = 8;  // rows held in registers per thread at a time
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+constexpr int kBatch = 8;  // rows held in registers per thread at a time
+
+// One thread's column of the M rows that move, C at a time from byte offset off of
+// each row (`shrink`: from the row offsets' units to the column's).
+template <class C>
+__device__ __forceinline__ void move_column(uint8_t *pool, long long off, const long long *src,
+                                            const long long *dst, int M, int shrink) {
+  for (int j0 = 0; j0 < M; j0 += kBatch) {
+    // every load of a batch before any store of it; past the last move a
+    // batch repeats that move (the same bytes to the same place), so that
+    // loads and stores are unconditional and the batch stays in registers
+    // (a clang vector type: an array of HIP's uint4 struct is kept in
+    // scratch memory by the compiler)
+    C v[kBatch];
+#pragma unroll
+    for (int q = 0; q < kBatch; ++q)
+      v[q] = *reinterpret_cast<const C *>(pool + src[min(j0 + q, M - 1)] / shrink + off);
+#pragma unroll
+    for (int q = 0; q < kBatch; ++q)
+      *reinterpret_cast<C *>(pool + dst[min(j0 + q, M - 1)] / shrink + off) = v[q];
+  }
+}
 
 __global__ __launch_bounds__(kNT) void commit_kernel(Args a) {
   __shared__ long long src[kMaxPath], dst[kMaxPath];  // the rows that move, in path order
@@ -102,21 +126,13 @@ __global__ __launch_bounds__(kNT) void commit_kernel(Args a) {
     const int kv = col / (a.Hkv * cpr), h = (col / cpr) % a.Hkv, c = col % cpr;
     uint8_t *pool = kv ? a.vpool : a.kpool;
     const long long off = layer_off + h * head_stride + 16LL * c;
-    for (int j0 = 0; j0 < M; j0 += kBatch) {
-      // every load of a batch before any store of it; past the last move a
-      // batch repeats that move (the same bytes to the same place), so that
-      // loads and stores are unconditional and the batch stays in registers
-      // (a clang vector type: an array of HIP's uint4 struct is kept in
-      // scratch memory by the compiler)
-      u32x4 v[kBatch];
-#pragma unroll
-      for (int q = 0; q < kBatch; ++q)
-        v[q] = *reinterpret_cast<const u32x4 *>(pool + src[min(j0 + q, M - 1)] + off);
-#pragma unroll
-      for (int q = 0; q < kBatch; ++q)
-        *reinterpret_cast<u32x4 *>(pool + dst[min(j0 + q, M - 1)] + off) = v[q];
-    }
+    move_column<u32x4>(pool, off, src, dst, M, 1);
   }
+  if (a.kscale)
+    for (int col = threadIdx.x; col < 2 * a.Hkv; col += kNT)
+      move_column<uint8_t>(col < a.Hkv ? a.kscale : a.vscale,
+                           ((long long)layer * a.Hkv + col % a.Hkv) * a.bs, src, dst, M,
+                           a.row_bytes);
 }
 
 }  // namespace commit
@@ -124,12 +140,14 @@ __global__ __launch_bounds__(kNT) void commit_kernel(Args a) {
 
 using namespace cfa;
 
-extern "C" int cfa_kv_commit(void *k_pool, void *v_pool, const int32_t *block_tables,
-                             int max_blocks_per_seq, const int32_t *ctx_lens,
-                             const int32_t *paths, int path_stride, const int32_t *path_lens,
-                             int B, int num_blocks, int num_layers, int n_kv_heads,
-                             int block_size, int head_dim, int elem_bytes,
-                             int32_t *new_ctx_lens, int32_t *status, void *stream) {
+extern "C" int cfa_kv_commit_scaled(void *k_pool, void *v_pool, uint8_t *k_scales,
+                                    uint8_t *v_scales, const int32_t *block_tables,
+                                    int max_blocks_per_seq, const int32_t *ctx_lens,
+                                    const int32_t *paths, int path_stride,
+                                    const int32_t *path_lens, int B, int num_blocks,
+                                    int num_layers, int n_kv_heads, int block_size, int head_dim,
+                                    int elem_bytes, int32_t *new_ctx_lens, int32_t *status,
+                                    void *stream) {
   using namespace cfa::abi;
   clear_error();
   if (!k_pool || !v_pool || !block_tables || !ctx_lens || !paths || !path_lens)
@@ -142,10 +160,13 @@ extern "C" int cfa_kv_commit(void *k_pool, void *v_pool, const int32_t *block_ta
     return fail_arg("head_dim * elem_bytes must be a multiple of 16 and at most 512");
   if (path_stride < 1) return fail_arg("path_stride must be positive");
   if ((((uintptr_t)k_pool | (uintptr_t)v_pool) & 15) != 0) return fail_arg("pools must be 16-byte aligned");
+  if (!k_scales != !v_scales) return fail_arg("k_scales and v_scales go together");
   if (B > 65535) return fail_arg("B must be at most 65535");
   commit::Args a{};
   a.kpool = (uint8_t *)k_pool;
   a.vpool = (uint8_t *)v_pool;
+  a.kscale = k_scales;
+  a.vscale = v_scales;
   a.bt = block_tables;
   a.ctx = ctx_lens;
   a.paths = paths;
@@ -163,4 +184,16 @@ extern "C" int cfa_kv_commit(void *k_pool, void *v_pool, const int32_t *block_ta
   CFA_LAUNCH("kv_commit", commit::commit_kernel, dim3(num_layers, B), dim3(commit::kNT), 0,
              (hipStream_t)stream, a);
   return CFA_OK;
+}
+
+extern "C" int cfa_kv_commit(void *k_pool, void *v_pool, const int32_t *block_tables,
+                             int max_blocks_per_seq, const int32_t *ctx_lens,
+                             const int32_t *paths, int path_stride, const int32_t *path_lens,
+                             int B, int num_blocks, int num_layers, int n_kv_heads,
+                             int block_size, int head_dim, int elem_bytes,
+                             int32_t *new_ctx_lens, int32_t *status, void *stream) {
+  return cfa_kv_commit_scaled(k_pool, v_pool, nullptr, nullptr, block_tables, max_blocks_per_seq,
+                              ctx_lens, paths, path_stride, path_lens, B, num_blocks, num_layers,
+                              n_kv_heads, block_size, head_dim, elem_bytes, new_ctx_lens, status,
+                              stream);
 }

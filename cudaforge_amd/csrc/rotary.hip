@@ -7,7 +7,8 @@
 //   pair's frequency), as halves (i, i + R/2) or as neighbours (2i, 2i + 1):
 //   (a, b) -> factor * (a cos - b sin, b cos + a sin)
 // v is copied.  q goes to q_out [T, Hq, D], k and v to the sequence's slots
-// base[b] + j of pool[block][layer][kv_head][slot][D].
+// base[b] + j of pool[block][layer][kv_head][slot][D], as they are or as e4m3
+// codes with a scale a row (e4m3.hpp), quantised from the fp32 results.
 //
 // Angles.  At position 100000 an fp32 product p f is off by up to 0.004
 // radians, more than bf16 resolves.  Frequencies are therefore 64-bit
@@ -25,7 +26,9 @@
 #include <hip/hip_runtime.h>
 
 #include "abi_internal.hpp"
+#include "e4m3.hpp"
 #include "half_types.hpp"
+#include "packed_tokens.hpp"
 
 namespace cfa {
 namespace rotary {
@@ -45,10 +48,12 @@ struct Args {
   const void *q_w, *k_w;  // [D] or null
   int w_f32;
   float eps;
-  uint16_t *q_out, *kc, *vc;
+  uint16_t *q_out;
+  void *kc, *vc;
+  uint8_t *ks, *vs;  // e4m3: scales [blocks, layers, Hkv, bs]
   int num_blocks, max_blocks, bs;
   const int32_t *block_tables, *base;
-  long long blk_stride, layer_off, head_stride;
+  long long blk_stride, layer_off, head_stride;  // elements
   int chunks, rounds;  // waves a token; rounds of rows a wave
 };
 
@@ -63,6 +68,20 @@ __device__ __forceinline__ float group_sum(float v) {
   if constexpr (LPR >= 16) CFA_DPP(0x140);  // mirrored in 16 lanes: the other 8
 #undef CFA_DPP
   if constexpr (LPR >= 32) v += __shfl_xor(v, 16, 64);
+  return v;
+}
+
+// Largest over the LPR lanes of a head, every lane gets it.
+template <int LPR>
+__device__ __forceinline__ uint32_t group_max(uint32_t v) {
+#define CFA_DPP(ctrl) \
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, ctrl, 0xf, 0xf, true))
+  CFA_DPP(0xB1);  // the lanes of group_sum
+  CFA_DPP(0x4E);
+  if constexpr (LPR >= 8) CFA_DPP(0x141);
+  if constexpr (LPR >= 16) CFA_DPP(0x140);
+#undef CFA_DPP
+  if constexpr (LPR >= 32) v = max(v, (uint32_t)__shfl_xor((int)v, 16, 64));
   return v;
 }
 
@@ -126,27 +145,9 @@ __device__ __forceinline__ void angle(const Args &a, int p, uint64_t turns, floa
   sn = a.factor * __builtin_amdgcn_sinf(f);
 }
 
-// The sequence b and the place j in it of token t; false where t belongs to
-// none (in front of the first, or behind the last).
-__device__ __forceinline__ bool place(const Args &a, int t, int lane, int &b, int &j) {
-  if (!a.cu) {
-    b = t / a.n;
-    j = t - b * a.n;
-    return true;
-  }
-  b = 0;  // ends at or before t
-  for (int b0 = 0; b0 < a.B; b0 += 64) {
-    const bool ended = b0 + lane < a.B && a.cu[b0 + lane + 1] <= t;
-    b += __popcll(__ballot(ended));
-  }
-  if (b >= a.B) return false;
-  j = t - a.cu[b];
-  return j >= 0;
-}
-
 // One wave = one token and `rounds` times ITER * 64 / LPR consecutive rows of its
 // Hq q heads, Hkv k heads and Hkv v heads.
-template <class T, int LPR, int LAYOUT, int ITER>
+template <class T, int LPR, int LAYOUT, int ITER, bool E4M3>
 __global__ __launch_bounds__(kWaves * 64) void qk_norm_rope_kv_kernel(Args a) {
   constexpr int RPW = 64 / LPR;
   const int lane = threadIdx.x & 63, l = lane % LPR;
@@ -174,7 +175,7 @@ __global__ __launch_bounds__(kWaves * 64) void qk_norm_rope_kv_kernel(Args a) {
   };
   load(0);
   int b, j;
-  if (!place(a, t, lane, b, j)) return;
+  if (!place_token(a, t, lane, b, j)) return;
   // this lane's cosines and sines: c[i], s[i] of element e + i, the sine with
   // the sign that its partner's value takes
   float c[8], s[8], wq[8], wk[8];
@@ -233,6 +234,7 @@ __global__ __launch_bounds__(kWaves * 64) void qk_norm_rope_kv_kernel(Args a) {
   if (slot >= 0 && page < a.max_blocks) blk = a.block_tables[(long long)b * a.max_blocks + page];
   const bool mapped = blk >= 0 && blk < a.num_blocks;
   const long long at = blk * a.blk_stride + a.layer_off + (slot - page * a.bs) * a.D;
+  const long long at_scale = E4M3 ? at / a.D : 0;
 
   for (int round = 0; round < a.rounds; ++round) {
 #pragma unroll
@@ -273,11 +275,37 @@ __global__ __launch_bounds__(kWaves * 64) void qk_norm_rope_kv_kernel(Args a) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) y[i] = x[i ^ 1];
       }
-      if (row >= H || !mine) continue;
       // (elements behind the rotated ones are selected, not turned by 0: they
       // may be infinite)
+      auto turn = [&] {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = e + i < a.R ? x[i] * c[i] + y[i] * s[i] : x[i];
+        for (int i = 0; i < 8; ++i) x[i] = e + i < a.R ? x[i] * c[i] + y[i] * s[i] : x[i];
+      };
+      if constexpr (E4M3) {
+        // the whole group finds the row's scale
+        turn();
+        if (is_v) unpack8<T>(raw[it], x);
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = max(top, mine ? e4m3::magnitude(x[i]) : 0u);
+        const uint32_t byte = e4m3::scale_byte(group_max<LPR>(top));
+        if (row < H && mine && !is_q) {
+          if (!mapped) continue;
+          const float inv = e4m3::inverse_scale(byte);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[i] = e4m3::codable<T>(x[i]) * inv;
+          const long long head = is_v ? row - a.Hq - a.Hkv : row - a.Hq;
+          uint2 w;
+          w.x = e4m3::pack4(x[0], x[1], x[2], x[3]);
+          w.y = e4m3::pack4(x[4], x[5], x[6], x[7]);
+          *reinterpret_cast<uint2 *>((uint8_t *)(is_v ? a.vc : a.kc) + head * a.head_stride + at +
+                                     e) = w;
+          if (l == 0) (is_v ? a.vs : a.ks)[head * a.bs + at_scale] = (uint8_t)byte;
+          continue;
+        }
+      }
+      if (row >= H || !mine) continue;
+      if constexpr (!E4M3) turn();
       uint32_t w[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) w[i] = pack2<T>(x[2 * i], x[2 * i + 1]);
@@ -290,14 +318,14 @@ __global__ __launch_bounds__(kWaves * 64) void qk_norm_rope_kv_kernel(Args a) {
       if (is_q)
         store8(a.q_out + ((long long)t * a.Hq + row) * a.D + e, w);
       else if (mapped)
-        store8((is_v ? a.vc + (row - a.Hq - a.Hkv) * a.head_stride
-                          : a.kc + (row - a.Hq) * a.head_stride) + at + e, w);
+        store8((is_v ? (uint16_t *)a.vc + (row - a.Hq - a.Hkv) * a.head_stride
+                     : (uint16_t *)a.kc + (row - a.Hq) * a.head_stride) + at + e, w);
     }
     if (round + 1 < a.rounds) load(round + 1);
   }
 }
 
-template <class T, int LPR, int LAYOUT>
+template <class T, int LPR, int LAYOUT, bool E4M3>
 int launch(Args a, hipStream_t st) {
   constexpr int RPW = 64 / LPR;
   const int H = a.Hq + 2 * a.Hkv;
@@ -315,46 +343,47 @@ int launch(Args a, hipStream_t st) {
   // tokens 104 / 73 / 58.  With 2 / 6 / 8 / 12 rows in flight: 59.5 / 59.2 / 62 / 69.
   if (few >= 8192 * kIter) {
     const int all = (H + kIter * RPW - 1) / (kIter * RPW);
-    CFA_LAUNCH("qk_norm_rope_kv", (qk_norm_rope_kv_kernel<T, LPR, LAYOUT, kIter>),
+    CFA_LAUNCH("qk_norm_rope_kv", (qk_norm_rope_kv_kernel<T, LPR, LAYOUT, kIter, E4M3>),
                grid(kIter, all), dim3(kWaves * 64), 0, st, a);
   } else if (few >= 8192) {
-    CFA_LAUNCH("qk_norm_rope_kv", (qk_norm_rope_kv_kernel<T, LPR, LAYOUT, kIter>),
+    CFA_LAUNCH("qk_norm_rope_kv", (qk_norm_rope_kv_kernel<T, LPR, LAYOUT, kIter, E4M3>),
                grid(kIter, 1), dim3(kWaves * 64), 0, st, a);
   } else {
-    CFA_LAUNCH("qk_norm_rope_kv", (qk_norm_rope_kv_kernel<T, LPR, LAYOUT, 1>), grid(1, 1),
+    CFA_LAUNCH("qk_norm_rope_kv", (qk_norm_rope_kv_kernel<T, LPR, LAYOUT, 1, E4M3>), grid(1, 1),
                dim3(kWaves * 64), 0, st, a);
   }
   return CFA_OK;
 }
 
-template <class T, int LPR>
+template <class T, int LPR, bool E4M3>
 int launch_layout(const Args &a, int layout, hipStream_t st) {
   switch (layout) {
-    case kHalf: return launch<T, LPR, kHalf>(a, st);
-    case kHalfAny: return launch<T, LPR, kHalfAny>(a, st);
-    default: return launch<T, LPR, kNeighbours>(a, st);
+    case kHalf: return launch<T, LPR, kHalf, E4M3>(a, st);
+    case kHalfAny: return launch<T, LPR, kHalfAny, E4M3>(a, st);
+    default: return launch<T, LPR, kNeighbours, E4M3>(a, st);
   }
 }
 
-template <class T>
+template <class T, bool E4M3>
 int launch_type(const Args &a, int layout, hipStream_t st) {
-  if (a.D <= 32) return launch_layout<T, 4>(a, layout, st);
-  if (a.D <= 64) return launch_layout<T, 8>(a, layout, st);
-  if (a.D <= 128) return launch_layout<T, 16>(a, layout, st);
-  return launch_layout<T, 32>(a, layout, st);
+  if (a.D <= 32) return launch_layout<T, 4, E4M3>(a, layout, st);
+  if (a.D <= 64) return launch_layout<T, 8, E4M3>(a, layout, st);
+  if (a.D <= 128) return launch_layout<T, 16, E4M3>(a, layout, st);
+  return launch_layout<T, 32, E4M3>(a, layout, st);
 }
 
 }  // namespace rotary
 }  // namespace cfa
 
-extern "C" int cfa_qk_norm_rope_kv(
+extern "C" int cfa_qk_norm_rope_kv_e4m3(
     const void *q, int64_t q_stride_t, int64_t q_stride_h, const void *k, int64_t k_stride_t,
     int64_t k_stride_h, const void *v, int64_t v_stride_t, int64_t v_stride_h, int fp16,
     const int32_t *positions, int T, int B, const int32_t *cu_seqlens, int n_q_heads,
     int n_kv_heads, int head_dim, int rotary_dim, const uint64_t *turns, float factor,
     int interleaved, const void *q_norm, const void *k_norm, int norm_f32, float eps, void *q_out,
-    void *k_pool, void *v_pool, int num_blocks, int num_layers, int layer, int block_size,
-    const int32_t *block_tables, int max_blocks_per_seq, const int32_t *base_lens, void *stream) {
+    void *k_pool, void *v_pool, uint8_t *k_scales, uint8_t *v_scales, int num_blocks,
+    int num_layers, int layer, int block_size, const int32_t *block_tables, int max_blocks_per_seq,
+    const int32_t *base_lens, void *stream) {
   using namespace cfa::abi;
   using namespace cfa::rotary;
   clear_error();
@@ -362,6 +391,11 @@ extern "C" int cfa_qk_norm_rope_kv(
     return fail_arg("need T, B >= 0 and positive head counts");
   if (head_dim <= 0 || head_dim % 8 || head_dim > 256)
     return fail_arg("head_dim must be a multiple of 8, at most 256");
+  if (!k_scales != !v_scales) return fail_arg("k_scales and v_scales go together");
+  const bool e4m3 = k_scales != nullptr;
+  if (e4m3 && head_dim % 16) return fail_arg("e4m3 pools need head_dim to be a multiple of 16");
+  if (e4m3 && (((uintptr_t)k_pool | (uintptr_t)v_pool) & 15) != 0)
+    return fail_arg("e4m3 pools must be 16-byte aligned");
   if (rotary_dim < 0 || rotary_dim % 2 || rotary_dim > head_dim)
     return fail_arg("rotary_dim must be even, between 0 and head_dim");
   if (num_blocks <= 0 || num_layers <= 0 || layer < 0 || layer >= num_layers || block_size <= 0 ||
@@ -400,8 +434,10 @@ extern "C" int cfa_qk_norm_rope_kv(
   a.w_f32 = norm_f32;
   a.eps = eps;
   a.q_out = (uint16_t *)q_out;
-  a.kc = (uint16_t *)k_pool;
-  a.vc = (uint16_t *)v_pool;
+  a.kc = k_pool;
+  a.vc = v_pool;
+  a.ks = k_scales;
+  a.vs = v_scales;
   a.num_blocks = num_blocks;
   a.max_blocks = max_blocks_per_seq;
   a.bs = block_size;
@@ -412,6 +448,25 @@ extern "C" int cfa_qk_norm_rope_kv(
   a.layer_off = (long long)layer * n_kv_heads * a.head_stride;
   const int layout = interleaved ? kNeighbours : (rotary_dim % 16 == 0 ? kHalf : kHalfAny);
   hipStream_t st = (hipStream_t)stream;
-  return fp16 ? launch_type<cfa::FP16>(a, layout, st)
-              : launch_type<cfa::BF16>(a, layout, st);
+  if (e4m3)
+    return fp16 ? launch_type<cfa::FP16, true>(a, layout, st)
+                : launch_type<cfa::BF16, true>(a, layout, st);
+  return fp16 ? launch_type<cfa::FP16, false>(a, layout, st)
+              : launch_type<cfa::BF16, false>(a, layout, st);
+}
+
+extern "C" int cfa_qk_norm_rope_kv(
+    const void *q, int64_t q_stride_t, int64_t q_stride_h, const void *k, int64_t k_stride_t,
+    int64_t k_stride_h, const void *v, int64_t v_stride_t, int64_t v_stride_h, int fp16,
+    const int32_t *positions, int T, int B, const int32_t *cu_seqlens, int n_q_heads,
+    int n_kv_heads, int head_dim, int rotary_dim, const uint64_t *turns, float factor,
+    int interleaved, const void *q_norm, const void *k_norm, int norm_f32, float eps, void *q_out,
+    void *k_pool, void *v_pool, int num_blocks, int num_layers, int layer, int block_size,
+    const int32_t *block_tables, int max_blocks_per_seq, const int32_t *base_lens, void *stream) {
+  return cfa_qk_norm_rope_kv_e4m3(q, q_stride_t, q_stride_h, k, k_stride_t, k_stride_h, v,
+                                  v_stride_t, v_stride_h, fp16, positions, T, B, cu_seqlens,
+                                  n_q_heads, n_kv_heads, head_dim, rotary_dim, turns, factor,
+                                  interleaved, q_norm, k_norm, norm_f32, eps, q_out, k_pool,
+                                  v_pool, nullptr, nullptr, num_blocks, num_layers, layer,
+                                  block_size, block_tables, max_blocks_per_seq, base_lens, stream);
 }

@@ -115,7 +115,10 @@ class PagedKVCache:
     ``device=None`` picks the current HIP device; on a host without one the
     cache holds page tables only (no pools, host-side batch metadata).
     ``dtype`` overrides the pool element type chosen from
-    ``element_size_bytes`` (bf16 for 2 bytes).
+    ``element_size_bytes`` (bf16 for 2 bytes).  With ``torch.float8_e4m3fn``
+    (1 byte) ``key_scales`` and ``value_scales`` hold each row's scale (uint8
+    [total_gpu_blocks, num_layers, num_kv_heads, block_size]); forks, page copies
+    and ``commit_tree_paths`` carry them along.
     """
 
     def __init__(self, config: KVCacheConfig, allocator: Optional[Callable] = None, *,
@@ -134,6 +137,8 @@ class PagedKVCache:
         cap = c.max_supported_batch_size * c.max_blocks_per_sequence
         self.key_pool: Optional[torch.Tensor] = None
         self.value_pool: Optional[torch.Tensor] = None
+        self.key_scales: Optional[torch.Tensor] = None
+        self.value_scales: Optional[torch.Tensor] = None
         self._event = None
         if self.device is not None and self.device.type == "cuda":
             dt = dtype or _POOL_DTYPES.get(c.element_size_bytes)
@@ -142,6 +147,9 @@ class PagedKVCache:
             shape = (c.total_gpu_blocks, c.num_layers, c.num_kv_heads, c.block_size, c.head_dim)
             self.key_pool = self._pool(shape, dt, allocator)
             self.value_pool = self._pool(shape, dt, allocator)
+            if dt == torch.float8_e4m3fn:
+                self.key_scales = self._pool(shape[:4], torch.uint8, allocator)
+                self.value_scales = self._pool(shape[:4], torch.uint8, allocator)
             self._h_tables = torch.empty(cap, dtype=torch.int32, pin_memory=True)
             self._h_ctx = torch.empty(c.max_supported_batch_size, dtype=torch.int32,
                                       pin_memory=True)
@@ -316,8 +324,9 @@ class PagedKVCache:
         if self.key_pool is None:
             return
         for src, dst, n in self.pop_page_copies():
-            for pool in (self.key_pool, self.value_pool):
-                pool[dst, :, :, :n].copy_(pool[src, :, :, :n])
+            for pool in (self.key_pool, self.value_pool, self.key_scales, self.value_scales):
+                if pool is not None:
+                    pool[dst, :, :, :n].copy_(pool[src, :, :, :n])
 
     def block_info(self, block_id: int) -> tuple:
         """(reference count, tokens filled, is cached) of one page."""
@@ -346,7 +355,8 @@ class PagedKVCache:
         if self.key_pool is None:
             raise RuntimeError("this cache has no device pools")
         out = kv_commit(self.key_pool, self.value_pool, descriptor.block_tables, base_lens,
-                        paths, path_lens)
+                        paths, path_lens, k_scales=self.key_scales,
+                        v_scales=self.value_scales)
         new_lens = out.new_ctx_lens.cpu().tolist()
         status = out.status.cpu().tolist()
         for seq, n in zip(sequence_ids, new_lens):

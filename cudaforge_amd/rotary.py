@@ -17,7 +17,8 @@ import numpy as np
 import torch
 
 from . import _lib
-from .verify import _on, _ptr, _require_all, _require_cuda, _stream_ptr
+from .verify import (_cache_dtype, _check_scales, _on, _ptr, _require_all, _require_cuda,
+                     _stream_ptr)
 
 __all__ = ["Rotary", "qk_norm_rope_kv"]
 
@@ -155,7 +156,9 @@ def qk_norm_rope_kv(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions
                     block_tables: torch.Tensor, base_lens: torch.Tensor, *, layer: int = 0,
                     cu_seqlens: Optional[torch.Tensor] = None,
                     q_norm: Optional[torch.Tensor] = None, k_norm: Optional[torch.Tensor] = None,
-                    eps: float = 1e-6, q_out: Optional[torch.Tensor] = None) -> torch.Tensor:
+                    eps: float = 1e-6, q_out: Optional[torch.Tensor] = None,
+                    k_scales: Optional[torch.Tensor] = None,
+                    v_scales: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Norm the q and k heads, turn them by their positions, and write k and v
     into the pages (``cfa_qk_norm_rope_kv``).  Returns q_out [T, Hq, D].
 
@@ -172,6 +175,15 @@ def qk_norm_rope_kv(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions
     Tokens that belong to no sequence leave every output as it was, and so do
     k and v whose page is not mapped (-1, or behind the table).
     q_out must not overlap q, k or v.
+
+    With k_scales and v_scales (uint8 [num_blocks, num_layers, Hkv, block_size])
+    the pools are float8_e4m3fn (D a multiple of 16): each k and v row is
+    quantised from its fp32 values as it is written, code e4m3(x / 2^e), scale
+    byte e + 127, with the least e >= -126 that brings the row's largest finite
+    magnitude to 448 2^e or less.  What is not finite becomes NaN; from fp16, what
+    would round past that type's range stops at 61440.  ``verify.tree_attention``,
+    ``verify.prompt_attention``, ``verify.kv_commit`` and ``verify.kv_gather`` take
+    such pools with their scales.
     """
     if not isinstance(q, torch.Tensor) or q.dtype not in (torch.bfloat16, torch.float16):
         raise ValueError("q must be a bfloat16 or float16 tensor")
@@ -179,9 +191,10 @@ def qk_norm_rope_kv(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions
     if len(shape) != 3:
         raise ValueError("q must be [T, Hq, D]")
     T, Hq, D = shape
+    cache = _cache_dtype(k_scales, v_scales, dt)
     _require_all(dev, (("q", q, dt), ("k", k, dt), ("v", v, dt),
-                       ("positions", positions, torch.int32), ("k_pool", k_pool, dt),
-                       ("v_pool", v_pool, dt), ("block_tables", block_tables, torch.int32),
+                       ("positions", positions, torch.int32), ("k_pool", k_pool, cache),
+                       ("v_pool", v_pool, cache), ("block_tables", block_tables, torch.int32),
                        ("base_lens", base_lens, torch.int32)))
     _, q_st, q_sh = _heads3("q", q, T, D)
     Hkv, k_st, k_sh = _heads3("k", k, T, D)
@@ -197,6 +210,7 @@ def qk_norm_rope_kv(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions
     if k_pool.shape != pools:
         raise ValueError("k_pool and v_pool must have the same shape")
     nblk, nlayers, ph, bs, pd = pools
+    _check_scales(k_scales, v_scales, pools, dev)
     if ph != Hkv or pd != D:
         raise ValueError("the pools' heads and head_dim must be k's")
     tables, lens = block_tables.shape, base_lens.shape
@@ -247,13 +261,14 @@ def qk_norm_rope_kv(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions
     block_tables = block_tables.contiguous()
     base_lens = base_lens.contiguous()
     with _on(dev):
-        rc = _lib.load().cfa_qk_norm_rope_kv(
+        rc = _lib.load().cfa_qk_norm_rope_kv_e4m3(
             q.data_ptr(), q_st, q_sh, k.data_ptr(), k_st, k_sh, v.data_ptr(), v_st, v_sh,
             dt == torch.float16, positions.data_ptr(), T, B, _ptr(cu_seqlens), Hq, Hkv, D, rot,
             _ptr(turns), rotary.factor if rot else 1.0,
             rot > 0 and rotary.layout == "interleaved", _ptr(q_norm), _ptr(k_norm),
             norm is not None and norm.dtype == torch.float32, eps, q_out.data_ptr(),
-            k_pool.data_ptr(), v_pool.data_ptr(), nblk, nlayers, int(layer), bs,
+            k_pool.data_ptr(), v_pool.data_ptr(), _ptr(k_scales), _ptr(v_scales), nblk, nlayers,
+            int(layer), bs,
             block_tables.data_ptr(), tables[1], base_lens.data_ptr(), _stream_ptr(dev))
     _lib.check(rc, "cfa_qk_norm_rope_kv")
     return q_out

@@ -14,6 +14,7 @@ Reference semantics (paths inside Bahaa-Labs/CUDAForge):
   prompt_attention             dense causal attention of csrc/kernels/cuda/
                                flash_attn_v2.cu:45-195, over the paged layout
   kv_commit                    device half of append_tokens, paged_kv_cache.cpp:255-286
+  kv_gather                    rows of the paged layout, read back token by token
   tree_verify                  speculative.cpp:50-150 generalised to a draft tree
 """
 from __future__ import annotations
@@ -243,6 +244,23 @@ def _check_pools(k_pool: torch.Tensor, v_pool: torch.Tensor, D: int):
         raise ValueError("head_dim of q and of the pools differ")
 
 
+def _cache_dtype(k_scales, v_scales, dtype: torch.dtype) -> torch.dtype:
+    """The pools' type: e4m3 where there are scales, else `dtype`."""
+    if (k_scales is None) != (v_scales is None):
+        raise ValueError("k_scales and v_scales go together")
+    return dtype if k_scales is None else torch.float8_e4m3fn
+
+
+def _check_scales(k_scales, v_scales, pools, dev) -> None:
+    """The scales of e4m3 pools of that shape (None: 16-bit pools)."""
+    for name, s in (("k_scales", k_scales), ("v_scales", v_scales)):
+        if s is None:
+            continue
+        _require_cuda(name, s, torch.uint8, dev)
+        if s.shape != pools[:4] or not s.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous [blocks, layers, Hkv, block_size]")
+
+
 def _check_slopes(alibi_slopes: Optional[torch.Tensor], Hq: int, dev) -> Optional[torch.Tensor]:
     if alibi_slopes is None:
         return None
@@ -455,11 +473,13 @@ class KVCommitOutput:
 
 
 def kv_commit(k_pool: torch.Tensor, v_pool: torch.Tensor, block_tables: torch.Tensor,
-              ctx_lens: torch.Tensor, paths: torch.Tensor, path_lens: torch.Tensor
+              ctx_lens: torch.Tensor, paths: torch.Tensor, path_lens: torch.Tensor, *,
+              k_scales: Optional[torch.Tensor] = None, v_scales: Optional[torch.Tensor] = None
               ) -> KVCommitOutput:
     """Move each sequence's accepted tree nodes (paths [B, P] int32, node ids
     with the root 0 first, path_lens [B]) from slots ctx + node to ctx + j in
-    every layer and KV head of both pools (in place)."""
+    every layer and KV head of both pools (in place).  Of e4m3 pools the rows'
+    scales (uint8 [num_blocks, num_layers, Hkv, block_size]) move with them."""
     for name, pool in (("k_pool", k_pool), ("v_pool", v_pool)):
         if not isinstance(pool, torch.Tensor) or pool.device.type != "cuda":
             raise ValueError(f"{name} must be a HIP device tensor")
@@ -468,6 +488,11 @@ def kv_commit(k_pool: torch.Tensor, v_pool: torch.Tensor, block_tables: torch.Te
     if k_pool.shape != v_pool.shape or k_pool.dtype != v_pool.dtype:
         raise ValueError("k_pool and v_pool must match in shape and dtype")
     dev = k_pool.device
+    if v_pool.device != dev:
+        raise ValueError("k_pool and v_pool must be on the same device")
+    if _cache_dtype(k_scales, v_scales, k_pool.dtype) != k_pool.dtype:
+        raise ValueError("k_scales and v_scales go with float8_e4m3fn pools")
+    _check_scales(k_scales, v_scales, k_pool.shape, dev)
     nblk, nlayers, Hkv, bs, D = k_pool.shape
     _require_cuda("block_tables", block_tables, torch.int32, dev)
     B = block_tables.shape[0]
@@ -483,13 +508,97 @@ def kv_commit(k_pool: torch.Tensor, v_pool: torch.Tensor, block_tables: torch.Te
     out = KVCommitOutput(new_ctx_lens=torch.empty(B, dtype=torch.int32, device=dev),
                          status=torch.empty(B, dtype=torch.int32, device=dev))
     with torch.cuda.device(dev):
-        rc = _lib.load().cfa_kv_commit(
-            k_pool.data_ptr(), v_pool.data_ptr(), block_tables.data_ptr(), block_tables.shape[1],
-            ctx_lens.data_ptr(), paths.data_ptr(), paths.shape[1], path_lens.data_ptr(), B, nblk,
-            nlayers, Hkv, bs, D, k_pool.element_size(), out.new_ctx_lens.data_ptr(),
-            out.status.data_ptr(), _stream_ptr(dev))
+        rc = _lib.load().cfa_kv_commit_scaled(
+            k_pool.data_ptr(), v_pool.data_ptr(), _ptr(k_scales), _ptr(v_scales),
+            block_tables.data_ptr(), block_tables.shape[1], ctx_lens.data_ptr(), paths.data_ptr(),
+            paths.shape[1], path_lens.data_ptr(), B, nblk, nlayers, Hkv, bs, D,
+            k_pool.element_size(), out.new_ctx_lens.data_ptr(), out.status.data_ptr(),
+            _stream_ptr(dev))
     _lib.check(rc, "cfa_kv_commit")
     return out
+
+
+def kv_gather(k_pool: torch.Tensor, v_pool: torch.Tensor, block_tables: torch.Tensor,
+              starts: torch.Tensor, *, tokens: Optional[int] = None, layer: int = 0,
+              cu_seqlens: Optional[torch.Tensor] = None,
+              k_scales: Optional[torch.Tensor] = None, v_scales: Optional[torch.Tensor] = None,
+              dtype: Optional[torch.dtype] = None, k_out: Optional[torch.Tensor] = None,
+              v_out: Optional[torch.Tensor] = None):
+    """Read sequences' keys and values back out of their pages
+    (``cfa_kv_gather``).  Returns (k, v), each [T, Hkv, D].
+
+    Token j of sequence b is the row at slot starts[b] + j (starts [B] int32)
+    of `layer`, by block_tables [B, max_blocks] int32: without cu_seqlens the T
+    tokens are T / B per sequence, with it (int32 [B + 1], rising) token t is
+    number j = t - cu_seqlens[b].  T is k_out's, or `tokens`.  e4m3 pools
+    [num_blocks, num_layers, Hkv, block_size, D] with k_scales and v_scales
+    (uint8, their first four dimensions; ``rotary.qk_norm_rope_kv`` fills both)
+    give the values that the codes stand for, in `dtype` or the outputs' (bf16,
+    exact, or fp16, rounded once); bf16 and fp16 pools are copied.  D is a
+    multiple of 16, at most 256.
+
+    Tokens whose page is not mapped (-1, or behind the table) are zeros.  Rows
+    of no sequence keep what k_out and v_out had there (zeros without those).
+    """
+    if not isinstance(k_pool, torch.Tensor) or k_pool.device.type != "cuda":
+        raise ValueError("k_pool must be a HIP device tensor")
+    dev = k_pool.device
+    if (k_out is None) != (v_out is None):
+        raise ValueError("k_out and v_out go together")
+    if dtype is None:
+        if isinstance(k_out, torch.Tensor):
+            dtype = k_out.dtype
+        else:
+            dtype = torch.bfloat16 if k_scales is not None else k_pool.dtype
+    if dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError("the outputs must be bfloat16 or float16")
+    cache = _cache_dtype(k_scales, v_scales, dtype)
+    _require_all(dev, (("k_pool", k_pool, cache), ("v_pool", v_pool, cache),
+                       ("block_tables", block_tables, torch.int32),
+                       ("starts", starts, torch.int32)))
+    if k_pool.dim() != 5:
+        raise ValueError("k_pool must be [blocks, layers, Hkv, block_size, D]")
+    nblk, nlayers, Hkv, bs, D = k_pool.shape
+    _check_pools(k_pool, v_pool, D)
+    _check_scales(k_scales, v_scales, k_pool.shape, dev)
+    if starts.dim() != 1 or block_tables.dim() != 2 or block_tables.shape[0] != starts.shape[0]:
+        raise ValueError("starts must be [B] and block_tables [B, max_blocks]")
+    B = starts.shape[0]
+    if k_out is not None:
+        T = k_out.shape[0] if isinstance(k_out, torch.Tensor) and k_out.dim() else -1
+        if tokens not in (None, T):
+            raise ValueError("tokens differs from k_out's")
+        for name, t in (("k_out", k_out), ("v_out", v_out)):
+            _require_cuda(name, t, dtype, dev)
+            if tuple(t.shape) != (T, Hkv, D) or not t.is_contiguous() or t.data_ptr() % 16:
+                raise ValueError(f"{name} must be a contiguous, 16-byte aligned [T, Hkv, D]")
+        if abs(k_out.data_ptr() - v_out.data_ptr()) < 2 * T * Hkv * D:
+            raise ValueError("k_out and v_out must not overlap")
+    else:
+        if tokens is None:
+            raise ValueError("give tokens, or k_out and v_out")
+        T = int(tokens)
+        if T < 0:
+            raise ValueError("tokens must not be negative")
+    if cu_seqlens is not None:
+        _require_cuda("cu_seqlens", cu_seqlens, torch.int32, dev)
+        if tuple(cu_seqlens.shape) != (B + 1,):
+            raise ValueError("cu_seqlens must be [B + 1]")
+        cu_seqlens = cu_seqlens.contiguous()
+    elif T and (B == 0 or T % B):
+        raise ValueError("without cu_seqlens the tokens must be a multiple of the sequences")
+    if k_out is None:
+        new = torch.empty if cu_seqlens is None else torch.zeros
+        k_out, v_out = (new(T, Hkv, D, dtype=dtype, device=dev) for _ in range(2))
+    block_tables, starts = block_tables.contiguous(), starts.contiguous()
+    with _on(dev):
+        rc = _lib.load().cfa_kv_gather(
+            k_pool.data_ptr(), v_pool.data_ptr(), _ptr(k_scales), _ptr(v_scales),
+            dtype == torch.float16, nblk, nlayers, int(layer), Hkv, bs, D,
+            block_tables.data_ptr(), block_tables.shape[1], starts.data_ptr(), _ptr(cu_seqlens),
+            T, B, k_out.data_ptr(), v_out.data_ptr(), _stream_ptr(dev))
+    _lib.check(rc, "cfa_kv_gather")
+    return k_out, v_out
 
 
 @dataclass

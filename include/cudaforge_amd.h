@@ -60,7 +60,7 @@ const char *cfa_last_error(void);
  * [B, K+1].  Minor 1 of it adds cfa_qk_norm_rope_kv,
  * cfa_tree_attention_scored, cfa_prompt_attention and cfa_sample_rows.
  * Binding code checks the major before its first call. */
-#define CFA_ABI_VERSION 201
+#define CFA_ABI_VERSION 202
 int cfa_version(void);
 
 /* ---------------------------------------------------------------------------
@@ -383,6 +383,15 @@ int cfa_kv_commit(void *k_pool, void *v_pool, const int32_t *block_tables,
                   int path_stride, const int32_t *path_lens, int B, int num_blocks,
                   int num_layers, int n_kv_heads, int block_size, int head_dim, int elem_bytes,
                   int32_t *new_ctx_lens, int32_t *status, void *stream);
+/* The same for pools whose rows have a scale byte each (cfa_qk_norm_rope_kv_e4m3):
+ * k_scales, v_scales [num_blocks][num_layers][n_kv_heads][block_size] move with
+ * their rows.  NULL scales: cfa_kv_commit. */
+int cfa_kv_commit_scaled(void *k_pool, void *v_pool, uint8_t *k_scales, uint8_t *v_scales,
+                         const int32_t *block_tables, int max_blocks_per_seq,
+                         const int32_t *ctx_lens, const int32_t *paths, int path_stride,
+                         const int32_t *path_lens, int B, int num_blocks, int num_layers,
+                         int n_kv_heads, int block_size, int head_dim, int elem_bytes,
+                         int32_t *new_ctx_lens, int32_t *status, void *stream);
 
 /* ---------------------------------------------------------------------------
  * W4A16 weight dequantisation.
@@ -543,6 +552,40 @@ int cfa_qk_norm_rope_kv(const void *q, int64_t q_stride_t, int64_t q_stride_h, c
                         void *q_out, void *k_pool, void *v_pool, int num_blocks, int num_layers,
                         int layer, int block_size, const int32_t *block_tables,
                         int max_blocks_per_seq, const int32_t *base_lens, void *stream);
+
+/* The same into pools of e4m3 codes (8 bits: 4 of exponent, 3 of mantissa, no
+ * infinity): k_pool, v_pool of bytes in the same layout, 16-byte aligned, head_dim
+ * a multiple of 16; k_scales, v_scales [num_blocks][num_layers][n_kv_heads]
+ * [block_size] hold a byte for each row.  A row of fp32 results x is quantised
+ * with e = the least integer >= -126 that has max |x| <= 448 * 2^e (over its
+ * finite values): code e4m3(x * 2^-e), to nearest even, byte e + 127.  Values that
+ * are not finite become NaN codes; from fp16, those of at most 65504 that would
+ * round past it stop at 61440.  NULL scales: cfa_qk_norm_rope_kv. */
+int cfa_qk_norm_rope_kv_e4m3(const void *q, int64_t q_stride_t, int64_t q_stride_h, const void *k,
+                             int64_t k_stride_t, int64_t k_stride_h, const void *v,
+                             int64_t v_stride_t, int64_t v_stride_h, int fp16,
+                             const int32_t *positions, int T, int B, const int32_t *cu_seqlens,
+                             int n_q_heads, int n_kv_heads, int head_dim, int rotary_dim,
+                             const uint64_t *turns, float factor, int interleaved,
+                             const void *q_norm, const void *k_norm, int norm_f32, float eps,
+                             void *q_out, void *k_pool, void *v_pool, uint8_t *k_scales,
+                             uint8_t *v_scales, int num_blocks, int num_layers, int layer,
+                             int block_size, const int32_t *block_tables, int max_blocks_per_seq,
+                             const int32_t *base_lens, void *stream);
+
+/* Rows of the paged cache read back token by token: token j of sequence b, the
+ * row at slot starts[b] + j of `layer`, goes to k_out and v_out [T, n_kv_heads,
+ * head_dim] (bf16, or fp16 with fp16 = 1; contiguous).  cu_seqlens as for
+ * cfa_qk_norm_rope_kv.  With k_scales and v_scales the pools hold e4m3 codes and
+ * the outputs are code * 2^(byte - 127) (bytes 1 to 253; exact in bf16, rounded
+ * once in fp16); without, pools of the outputs' type are copied.  head_dim a
+ * multiple of 16, at most 256; pools and outputs 16-byte aligned.  Tokens whose
+ * page is not mapped are zeros; rows of no sequence are left as they are. */
+int cfa_kv_gather(const void *k_pool, const void *v_pool, const uint8_t *k_scales,
+                  const uint8_t *v_scales, int fp16, int num_blocks, int num_layers, int layer,
+                  int n_kv_heads, int block_size, int head_dim, const int32_t *block_tables,
+                  int max_blocks_per_seq, const int32_t *starts, const int32_t *cu_seqlens, int T,
+                  int B, void *k_out, void *v_out, void *stream);
 
 /* Few-row bf16 GEMM: c [M, N] = a [M, K] x w [K, N], all row-major bf16, fp32
  * accumulation on MFMA, 1 <= M <= 128, N % 64 == 0, K % 128 == 0, pointers
