@@ -124,6 +124,11 @@ SIGNATURES: dict[str, tuple] = {
     "cfa_sample_rows_workspace_size": (_sz, [_i, _i]),
     "cfa_sample_rows": (
         _i, [_p, _i64, _i, _i, _i, _i, _p, _f, _p, _i, _p, _f, _p, _f, _p, _p, _p, _p, _sz, _p]),
+    "cfa_adjust_logits": (
+        _i,
+        [_p, _i64, _i64, _i, _i, _i, _i, _p, _p, _p, _i, _p, _f, _p, _f, _p, _f, _p, _p, _i64, _p,
+         _p, _i64, _i, _p, _i, _i, _p, _p, _i64, _i64, _i, _p],
+    ),
     "cfa_tree_attention_workspace_size": (_sz, [_i, _i, _i, _i, _i, _i, _i]),
     "cfa_tree_attention": (
         _i,

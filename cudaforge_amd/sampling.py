@@ -24,6 +24,10 @@ renormalised), or greedy top-k; several independent draws per row.
 own temperature, top-k, top-p and min-p; ``filtered_probs`` gives the same
 rows' probabilities alone, for verification (``input_kind="probs"``).
 
+``adjust_logits`` (``cfa_adjust_logits``) goes in front of any of them, and of
+``verify.chain_verify`` and ``verify.tree_verify``: penalties of repeated tokens,
+biases and grammar masks, of single rows and of a draft tree's nodes.
+
 Every call runs on the HIP library; there is no CPU fallback.
 """
 from __future__ import annotations
@@ -34,7 +38,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from .verify import _KINDS, _on, _require_cuda, _stream_ptr, _workspace
+from .verify import _KINDS, _on, _ptr, _require_cuda, _stream_ptr, _workspace
 
 __all__ = [
     "SamplingParams",
@@ -46,6 +50,7 @@ __all__ = [
     "sample_rows",
     "sample_rows_workspace_bytes",
     "filtered_probs",
+    "adjust_logits",
 ]
 
 _SMODES = {"multinomial": _lib.CFA_SAMPLE_MULTINOMIAL, "filtered": _lib.CFA_SAMPLE_FILTERED,
@@ -286,6 +291,166 @@ def filtered_probs(rows: torch.Tensor, *, temperature=1.0, top_k=0, top_p=1.0, m
     ``input_kind="probs"`` of filtered distributions."""
     return sample_rows(rows, draws=0, temperature=temperature, top_k=top_k, top_p=top_p,
                        min_p=min_p, return_probs=True, workspace=workspace)[1]
+
+
+def _rows_strides(x: torch.Tensor):
+    """(B, N, V, stride of sequences, stride of rows) of [B, V] or [B, N, V]."""
+    if x.dim() == 2:
+        return x.shape[0], 1, x.shape[1], x.stride(0), x.stride(0)
+    return (*x.shape, x.stride(0), x.stride(1))
+
+
+def _span(x: torch.Tensor):
+    """First byte and the one behind the last that x covers."""
+    if x.numel() == 0:
+        return x.data_ptr(), x.data_ptr()
+    last = sum((n - 1) * st for n, st in zip(x.shape, x.stride()))
+    return x.data_ptr(), x.data_ptr() + (last + 1) * x.element_size()
+
+
+def adjust_logits(logits: torch.Tensor, *, history: Optional[torch.Tensor] = None,
+                  history_lens: Optional[torch.Tensor] = None,
+                  prompt_lens: Optional[torch.Tensor] = None, repetition=1.0, frequency=0.0,
+                  presence=0.0, node_tokens: Optional[torch.Tensor] = None,
+                  tree_mask: Optional[torch.Tensor] = None,
+                  bias_tokens: Optional[torch.Tensor] = None,
+                  bias_values: Optional[torch.Tensor] = None,
+                  allowed: Optional[torch.Tensor] = None,
+                  allowed_index: Optional[torch.Tensor] = None,
+                  out: Optional[torch.Tensor] = None,
+                  out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """Penalties of repeated tokens, biases and grammar masks on logits [B, V], or
+    [B, N, V] (N rows of each sequence: a draft tree's nodes, a chain's places);
+    fp32, bf16 or fp16.  Returns them in `out_dtype` (their own, or float32).
+
+    history [B, L] int32 holds each sequence's tokens, history_lens [B] int32 how
+    many of them count (default L), prompt_lens [B] int32 how many of those are its
+    prompt (default 0).  A token seen anywhere there has its logit divided (if
+    positive) or multiplied by `repetition`; one that stands c > 0 times behind the
+    prompt loses frequency * c + presence.  The three are numbers, or fp32 [B]
+    tensors.  With node_tokens [B, N] int32 and tree_mask (int64 [N] or [B, N], each
+    node's ancestor-or-self mask) a row also counts the tokens of its own path, as
+    generated ones; N is then at most 64.  (A chain is a tree of one path; a first
+    node whose token the history has already goes in as -1.)
+
+    bias_tokens int32 and bias_values fp32, [K] or [B, K], are added to their tokens'
+    logits; of the same token twice the last.  Ids outside the vocabulary, here, in
+    the history and in node_tokens, are passed over: -1 pads.  allowed int32 [M,
+    ceil(V / 32)] holds grammars' masks, token v in bit v % 32 of word v / 32, and
+    allowed_index int32 ([B] or [B, N]) the mask of each row (-1: none); without it
+    there is one for each row.  Masked tokens get -inf.
+
+    In fp32, rounded once.  out (default a new tensor) may be `logits` itself: what
+    nothing changes is then not touched.  Another tensor must not overlap them.
+    """
+    if not isinstance(logits, torch.Tensor) or logits.device.type != "cuda":
+        raise ValueError("logits must be a HIP device tensor")
+    if logits.dtype not in _ROW_TYPES:
+        raise ValueError("logits must be float32, bfloat16 or float16")
+    if logits.dim() not in (2, 3) or logits.shape[-1] == 0:
+        raise ValueError("logits must be [B, V] or [B, N, V] with V > 0")
+    dev = logits.device
+    inplace = out is logits
+    if logits.stride(-1) != 1 and not inplace:
+        logits = logits.contiguous()
+    B, N, V, sb, sn = _rows_strides(logits)
+
+    def ints(name, t, shape):
+        if t is None:
+            return None
+        _require_cuda(name, t, torch.int32, dev)
+        if tuple(t.shape) != shape:
+            raise ValueError(f"{name} must be {list(shape)}")
+        return t.contiguous()
+
+    if history is None and (history_lens is not None or prompt_lens is not None):
+        raise ValueError("history_lens and prompt_lens go with history")
+    if history is not None:
+        _require_cuda("history", history, torch.int32, dev)
+        if history.dim() != 2 or history.shape[0] != B:
+            raise ValueError(f"history must be [B, L] with B = {B}")
+        history = history.contiguous()
+    L = 0 if history is None else history.shape[1]
+    history_lens = ints("history_lens", history_lens, (B,))
+    prompt_lens = ints("prompt_lens", prompt_lens, (B,))
+    settings = [
+        _setting("repetition", repetition, B, torch.float32, dev,
+                 lambda v: 0.0 < v < float("inf"), "finite and positive"),
+        _setting("frequency", frequency, B, torch.float32, dev,
+                 lambda v: abs(v) < float("inf"), "finite"),
+        _setting("presence", presence, B, torch.float32, dev,
+                 lambda v: abs(v) < float("inf"), "finite")]
+    (r, r0, _), (f, f0, _), (p, p0, _) = settings
+    if (node_tokens is None) != (tree_mask is None):
+        raise ValueError("node_tokens and tree_mask go together")
+    mstride = 0
+    if node_tokens is not None:
+        if logits.dim() != 3 or N > 64:
+            raise ValueError("node_tokens go with logits [B, N, V] of at most 64 nodes")
+        node_tokens = ints("node_tokens", node_tokens, (B, N))
+        _require_cuda("tree_mask", tree_mask, torch.int64, dev)
+        if tuple(tree_mask.shape) == (B, N):
+            mstride = N
+        elif tuple(tree_mask.shape) != (N,):
+            raise ValueError("tree_mask must be [N] or [B, N]")
+        tree_mask = tree_mask.contiguous()
+    if (bias_tokens is None) != (bias_values is None):
+        raise ValueError("bias_tokens and bias_values go together")
+    K = bstride = 0
+    if bias_tokens is not None:
+        _require_cuda("bias_tokens", bias_tokens, torch.int32, dev)
+        _require_cuda("bias_values", bias_values, torch.float32, dev)
+        if bias_tokens.shape != bias_values.shape or bias_tokens.dim() not in (1, 2) or (
+                bias_tokens.dim() == 2 and bias_tokens.shape[0] != B):
+            raise ValueError("bias_tokens and bias_values must both be [K] or [B, K]")
+        K = bias_tokens.shape[-1]
+        bstride = K if bias_tokens.dim() == 2 else 0
+        bias_tokens, bias_values = bias_tokens.contiguous(), bias_values.contiguous()
+    words = masks = 0
+    if allowed is None and allowed_index is not None:
+        raise ValueError("allowed_index goes with allowed")
+    if allowed is not None:
+        _require_cuda("allowed", allowed, torch.int32, dev)
+        words = (V + 31) // 32
+        rows = tuple(logits.shape[:-1])
+        if allowed_index is not None:
+            allowed_index = ints("allowed_index", allowed_index, rows)
+            if allowed.dim() != 2 or allowed.shape[1] != words:
+                raise ValueError(f"allowed must be [M, ceil(V / 32)] = [M, {words}]")
+        elif tuple(allowed.shape) not in ((*rows, words), (B * N, words)):
+            raise ValueError("without allowed_index, allowed must have a mask for each row")
+        allowed = allowed.contiguous()
+        masks = allowed.numel() // words
+    if out is None:
+        out_dtype = logits.dtype if out_dtype is None else out_dtype
+        if out_dtype not in (logits.dtype, torch.float32):
+            raise ValueError("out_dtype must be float32 or the logits' dtype")
+        out = torch.empty(logits.shape, dtype=out_dtype, device=dev)
+    else:
+        if not isinstance(out, torch.Tensor) or out.dtype not in (logits.dtype, torch.float32) or (
+                out_dtype not in (None, out.dtype)):
+            raise ValueError("out must be float32 or of the logits' dtype (and of out_dtype)")
+        _require_cuda("out", out, out.dtype, dev)
+        if out.shape != logits.shape or out.stride(-1) != 1:
+            raise ValueError("out must have the logits' shape and a contiguous last dimension")
+        _, _, _, ob, on = _rows_strides(out)
+        if (N > 1 and on < V) or (B > 1 and ob < (N - 1) * on + V):
+            raise ValueError("out's rows must not overlap")
+        same = (out.data_ptr() == logits.data_ptr() and out.dtype == logits.dtype
+                and out.stride() == logits.stride())
+        (lo, hi), (olo, ohi) = _span(logits), _span(out)
+        if not same and lo < ohi and olo < hi:
+            raise ValueError("out must be the logits themselves or not overlap them")
+    _, _, _, ob, on = _rows_strides(out)
+    with _on(dev):
+        rc = _lib.load().cfa_adjust_logits(
+            logits.data_ptr(), sb, sn, _ROW_TYPES[logits.dtype], B, N, V, _ptr(history),
+            _ptr(history_lens), _ptr(prompt_lens), L, r, r0, f, f0, p, p0, _ptr(node_tokens),
+            _ptr(tree_mask), mstride, _ptr(bias_tokens), _ptr(bias_values), bstride, K,
+            _ptr(allowed), words, masks, _ptr(allowed_index), out.data_ptr(), ob, on,
+            out.dtype == torch.float32, _stream_ptr(dev))
+    _lib.check(rc, "cfa_adjust_logits")
+    return out
 
 
 class _Null:

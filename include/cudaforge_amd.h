@@ -208,6 +208,46 @@ int cfa_sample_rows(const void *rows, int64_t row_stride, int elem_type, int R, 
                     void *workspace, size_t workspace_bytes, void *stream);
 
 /* ---------------------------------------------------------------------------
+ * Logits in front of the sampler or the verification: penalties of repeated
+ * tokens, biases and grammar masks (no counterpart in the reference).
+ *
+ * logits: B sequences' N rows of V values (N = 1: a row each), fp32 (type 0), bf16
+ * (1) or fp16 (2), at element strides stride_b and stride_n.  For token v of row
+ * i of sequence b, in fp32, rounded once:
+ *   c = how often v stands in the generated tokens of history[b] and on the row's
+ *       path;  v counts as seen there and in the prompt
+ *   x = x > 0 ? x / repetition : x * repetition            (v seen)
+ *   x -= frequency * c + presence                          (c > 0)
+ *   x += bias_values[b][k]           (bias_tokens[b][k] = v; of several the last)
+ *   x = -inf                                       (the row's mask has no bit v)
+ *
+ *   history [B, L]: tokens; history_lens [B] (NULL: L) of them count, the first
+ *     prompt_lens [B] (NULL: 0) as the prompt.  Ids outside [0, V) are passed over
+ *     here, in node_tokens and in bias_tokens.  L = 0: none.
+ *   repetition, frequency, presence: fp32 [B], or NULL and the number for all
+ *     (repetition positive; 1, 0 and 0 leave the logits alone)
+ *   node_tokens [B, N], tree_mask ([N], or [B, N] at tree_mask_stride_b): draft
+ *     trees of at most 64 nodes; row i's path are the nodes of its mask, itself
+ *     among them (NULL: none)
+ *   bias_tokens, bias_values [K] a sequence at bias_stride_b (0: the same for all)
+ *   allowed [masks, words] bits, token v in bit v % 32 of word v / 32; row r = b * N
+ *     + i goes by mask allowed_index[r] (outside [0, masks): no mask), or by mask r
+ *     without allowed_index
+ *   out: the type of logits, or fp32 with out_f32 = 1; its own strides.  It may be
+ *     logits itself (same type and strides; what nothing changes is then neither
+ *     read nor written), and must not overlap them otherwise. */
+int cfa_adjust_logits(const void *logits, int64_t stride_b, int64_t stride_n, int type, int B,
+                      int N, int V, const int32_t *history, const int32_t *history_lens,
+                      const int32_t *prompt_lens, int L, const float *repetition,
+                      float repetition0, const float *frequency, float frequency0,
+                      const float *presence, float presence0, const int32_t *node_tokens,
+                      const uint64_t *tree_mask, int64_t tree_mask_stride_b,
+                      const int32_t *bias_tokens, const float *bias_values, int64_t bias_stride_b,
+                      int K, const int32_t *allowed, int words, int masks,
+                      const int32_t *allowed_index, void *out, int64_t out_stride_b,
+                      int64_t out_stride_n, int out_f32, void *stream);
+
+/* ---------------------------------------------------------------------------
  * Tree-masked verification attention over a paged KV cache (bf16, MFMA).
  *
  * No reference kernel exists (the reference's target forward recomputes the
