@@ -8,10 +8,14 @@
 namespace cfa {
 namespace scored {
 
-extern template int launch<64, BF16>(const Args &, bool, unsigned, hipStream_t);
-extern template int launch<128, BF16>(const Args &, bool, unsigned, hipStream_t);
-extern template int launch<64, FP16>(const Args &, bool, unsigned, hipStream_t);
-extern template int launch<128, FP16>(const Args &, bool, unsigned, hipStream_t);
+extern template int launch<64, BF16, false>(const Args &, bool, unsigned, hipStream_t);
+extern template int launch<128, BF16, false>(const Args &, bool, unsigned, hipStream_t);
+extern template int launch<64, FP16, false>(const Args &, bool, unsigned, hipStream_t);
+extern template int launch<128, FP16, false>(const Args &, bool, unsigned, hipStream_t);
+extern template int launch<64, BF16, true>(const Args &, bool, unsigned, hipStream_t);
+extern template int launch<128, BF16, true>(const Args &, bool, unsigned, hipStream_t);
+extern template int launch<64, FP16, true>(const Args &, bool, unsigned, hipStream_t);
+extern template int launch<128, FP16, true>(const Args &, bool, unsigned, hipStream_t);
 
 static size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 
@@ -48,7 +52,7 @@ struct Plan {
 // 8000: 208 without, 28 with 16.
 // `longest` bounds a sequence's queries; tokens is the number of all.
 static Plan plan(long long tokens, long long longest, int B, int G, int Hkv, int D, int max_keys,
-                 int window, int num_splits, bool tree) {
+                 int window, int sinks, bool e4m3, int num_splits, bool tree) {
   struct Rows {
     int rows;
     double first, tile, share;
@@ -75,11 +79,12 @@ static Plan plan(long long tokens, long long longest, int B, int G, int Hkv, int
     double mean = tiles;
     if (window > 0)
       mean = tiles = (int)std::min<long long>(
-          tiles, ((long long)window + (tree ? 64 : TQ) + kKT - 2) / kKT + 1);
+          tiles, ((long long)window + (tree ? 64 : TQ) + kKT - 2) / kKT + 1 +
+                     ((long long)sinks + kKT - 1) / kKT);
     else if (!tree)
       mean = std::max(1.0, tiles - 0.5 * (double)std::min<long long>(longest, max_keys) / kKT);
     const double cus = abi::device_cu_count(), items = (double)std::max(1LL, busy * Hkv);
-    const double bytes = items * mean * kKT * D * 4 / 6e6;
+    const double bytes = items * mean * kKT * D * (e4m3 ? 2 : 4) / 6e6;
     long long n = num_splits > 0 ? std::min(num_splits, tiles) : 1;
     while (true) {
       const long long per = (tiles + n - 1) / n;
@@ -108,7 +113,7 @@ static Plan plan(long long tokens, long long longest, int B, int G, int Hkv, int
   return p;
 }
 
-static int check_scores(float sm_scale, float soft_cap, int window) {
+static int check_scores(float sm_scale, float soft_cap, int window, int sinks) {
   using namespace cfa::abi;
   if (!std::isfinite(sm_scale)) return fail_arg("sm_scale must be finite");
   if (!(soft_cap == 0.0f || (soft_cap >= 1e-6f && std::isfinite(soft_cap))))
@@ -117,6 +122,7 @@ static int check_scores(float sm_scale, float soft_cap, int window) {
   if (!std::isfinite((soft_cap > 0.0f ? 2.0f * (sm_scale / soft_cap) : sm_scale) * 1.4426951f))
     return fail_arg("sm_scale is out of fp32's range (of soft_cap, where there is one)");
   if (window < 0) return fail_arg("window must not be negative (0: none)");
+  if (sinks < 0) return fail_arg("sinks must not be negative");
   return CFA_OK;
 }
 
@@ -179,11 +185,26 @@ static int run(Args &a, const Plan &p, int D, int fp16, float sm_scale, float so
   }
   a.past = (long long)p.splits * a.T * a.Hq * D * 4 <= 24LL << 20;
   hipStream_t st = (hipStream_t)stream;
-  if (D == 128)
-    return fp16 ? launch<128, FP16>(a, p.one, (unsigned)grid, st)
-                : launch<128, BF16>(a, p.one, (unsigned)grid, st);
-  return fp16 ? launch<64, FP16>(a, p.one, (unsigned)grid, st)
-              : launch<64, BF16>(a, p.one, (unsigned)grid, st);
+  const unsigned g = (unsigned)grid;
+#define CFA_TYPES(E4M3)                                                                      \
+  (D == 128 ? fp16 ? launch<128, FP16, E4M3>(a, p.one, g, st) : launch<128, BF16, E4M3>(a, p.one, g, st) \
+            : fp16 ? launch<64, FP16, E4M3>(a, p.one, g, st) : launch<64, BF16, E4M3>(a, p.one, g, st))
+  return a.kscale ? CFA_TYPES(true) : CFA_TYPES(false);
+#undef CFA_TYPES
+}
+
+// The pools, of q's type or of e4m3 codes with scales.
+static int set_pools(Args &a, const void *k_pool, const void *v_pool, const uint8_t *k_scales,
+                     const uint8_t *v_scales) {
+  using namespace cfa::abi;
+  if (!k_scales != !v_scales) return fail_arg("k_scales and v_scales go together");
+  if ((((uintptr_t)k_scales | (uintptr_t)v_scales) & 15) != 0)
+    return fail_arg("the scales must be 16-byte aligned");
+  a.kpool = (const uint16_t *)k_pool;
+  a.vpool = (const uint16_t *)v_pool;
+  a.kscale = k_scales;
+  a.vscale = v_scales;
+  return CFA_OK;
 }
 
 }  // namespace scored
@@ -191,24 +212,34 @@ static int run(Args &a, const Plan &p, int D, int fp16, float sm_scale, float so
 
 using namespace cfa::scored;
 
+extern "C" size_t cfa_tree_attention_cached_workspace_size(int B, int N, int n_q_heads,
+                                                           int n_kv_heads, int head_dim,
+                                                           int max_keys, int window, int sinks,
+                                                           int e4m3, int num_splits) {
+  cfa::abi::clear_error();
+  if (B <= 0 || N <= 0 || window < 0 || sinks < 0 ||
+      check_heads(n_q_heads, n_kv_heads, head_dim) != CFA_OK)
+    return 0;
+  const Plan p = plan((long long)B * N, N, B, n_q_heads / n_kv_heads, n_kv_heads, head_dim, max_keys,
+                      window, sinks, e4m3 != 0, num_splits, true);
+  return p.bytes((long long)B * N, n_q_heads, head_dim);
+}
+
 extern "C" size_t cfa_tree_attention_scored_workspace_size(int B, int N, int n_q_heads,
                                                            int n_kv_heads, int head_dim,
                                                            int max_keys, int window,
                                                            int num_splits) {
-  cfa::abi::clear_error();
-  if (B <= 0 || N <= 0 || window < 0 || check_heads(n_q_heads, n_kv_heads, head_dim) != CFA_OK)
-    return 0;
-  const Plan p = plan((long long)B * N, N, B, n_q_heads / n_kv_heads, n_kv_heads, head_dim, max_keys,
-                      window, num_splits, true);
-  return p.bytes((long long)B * N, n_q_heads, head_dim);
+  return cfa_tree_attention_cached_workspace_size(B, N, n_q_heads, n_kv_heads, head_dim, max_keys,
+                                                  window, 0, 0, num_splits);
 }
 
-extern "C" int cfa_tree_attention_scored(
-    const void *q, const void *k_pool, const void *v_pool, int fp16, const int32_t *block_tables,
-    int max_blocks_per_seq, const int32_t *ctx_lens, int num_blocks, int num_layers, int layer,
-    int block_size, const uint64_t *tree_mask, int64_t tree_mask_stride_b, int B, int N,
-    int first_node, int n_q_heads, int n_kv_heads, int head_dim, float sm_scale, float soft_cap,
-    const float *alibi_slopes, int window, int max_keys, int num_splits, void *out,
+extern "C" int cfa_tree_attention_cached(
+    const void *q, const void *k_pool, const void *v_pool, const uint8_t *k_scales,
+    const uint8_t *v_scales, int fp16, const int32_t *block_tables, int max_blocks_per_seq,
+    const int32_t *ctx_lens, int num_blocks, int num_layers, int layer, int block_size,
+    const uint64_t *tree_mask, int64_t tree_mask_stride_b, int B, int N, int first_node,
+    int n_q_heads, int n_kv_heads, int head_dim, float sm_scale, float soft_cap,
+    const float *alibi_slopes, int window, int sinks, int max_keys, int num_splits, void *out,
     void *workspace, size_t workspace_bytes, void *stream) {
   using namespace cfa::abi;
   clear_error();
@@ -218,15 +249,14 @@ extern "C" int cfa_tree_attention_scored(
   if (first_node < 0 || first_node >= N) return fail_arg("need 0 <= first_node < N");
   if (int rc = check_heads(n_q_heads, n_kv_heads, head_dim)) return rc;
   if (int rc = check_pool(num_blocks, num_layers, layer, block_size, max_blocks_per_seq)) return rc;
-  if (int rc = check_scores(sm_scale, soft_cap, window)) return rc;
+  if (int rc = check_scores(sm_scale, soft_cap, window, sinks)) return rc;
   if (max_keys < N) return fail_arg("max_keys must be at least N (context + tree tokens)");
   if ((long long)max_blocks_per_seq * block_size < max_keys)
     return fail_arg("max_blocks_per_seq * block_size must cover max_keys");
   if (num_splits < 0) return fail_arg("num_splits must not be negative");
   Args a{};
+  if (int rc = set_pools(a, k_pool, v_pool, k_scales, v_scales)) return rc;
   a.q = (const uint16_t *)q;
-  a.kpool = (const uint16_t *)k_pool;
-  a.vpool = (const uint16_t *)v_pool;
   a.bt = block_tables;
   a.ctx = ctx_lens;
   a.mask = tree_mask;
@@ -248,28 +278,54 @@ extern "C" int cfa_tree_attention_scored(
   a.layer = layer;
   a.bs = block_size;
   a.window = window;
-  const Plan p = plan(a.T, a.Nq, B, a.G, n_kv_heads, head_dim, max_keys, window, num_splits,
-                      true);
+  a.sinks = window > 0 ? sinks : 0;
+  const Plan p = plan(a.T, a.Nq, B, a.G, n_kv_heads, head_dim, max_keys, window, sinks,
+                      k_scales != nullptr, num_splits, true);
   return run(a, p, head_dim, fp16, sm_scale, soft_cap, workspace, workspace_bytes, stream);
+}
+
+extern "C" int cfa_tree_attention_scored(
+    const void *q, const void *k_pool, const void *v_pool, int fp16, const int32_t *block_tables,
+    int max_blocks_per_seq, const int32_t *ctx_lens, int num_blocks, int num_layers, int layer,
+    int block_size, const uint64_t *tree_mask, int64_t tree_mask_stride_b, int B, int N,
+    int first_node, int n_q_heads, int n_kv_heads, int head_dim, float sm_scale, float soft_cap,
+    const float *alibi_slopes, int window, int max_keys, int num_splits, void *out,
+    void *workspace, size_t workspace_bytes, void *stream) {
+  return cfa_tree_attention_cached(q, k_pool, v_pool, nullptr, nullptr, fp16, block_tables,
+                                   max_blocks_per_seq, ctx_lens, num_blocks, num_layers, layer,
+                                   block_size, tree_mask, tree_mask_stride_b, B, N, first_node,
+                                   n_q_heads, n_kv_heads, head_dim, sm_scale, soft_cap,
+                                   alibi_slopes, window, 0, max_keys, num_splits, out, workspace,
+                                   workspace_bytes, stream);
+}
+
+extern "C" size_t cfa_prompt_attention_cached_workspace_size(int T, int B, int n_q_heads,
+                                                             int n_kv_heads, int head_dim,
+                                                             int max_query, int max_keys,
+                                                             int window, int sinks, int e4m3,
+                                                             int num_splits) {
+  cfa::abi::clear_error();
+  if (B <= 0 || T <= 0 || max_query <= 0 || window < 0 || sinks < 0 ||
+      check_heads(n_q_heads, n_kv_heads, head_dim) != CFA_OK)
+    return 0;
+  const Plan p = plan(T, std::min(max_query, T), B, n_q_heads / n_kv_heads, n_kv_heads, head_dim,
+                      max_keys, window, sinks, e4m3 != 0, num_splits, false);
+  return p.bytes(T, n_q_heads, head_dim);
 }
 
 extern "C" size_t cfa_prompt_attention_workspace_size(int T, int B, int n_q_heads, int n_kv_heads,
                                                       int head_dim, int max_query, int max_keys,
                                                       int window, int num_splits) {
-  cfa::abi::clear_error();
-  if (B <= 0 || T <= 0 || max_query <= 0 || window < 0 ||
-      check_heads(n_q_heads, n_kv_heads, head_dim) != CFA_OK)
-    return 0;
-  const Plan p = plan(T, std::min(max_query, T), B, n_q_heads / n_kv_heads, n_kv_heads, head_dim,
-                      max_keys, window, num_splits, false);
-  return p.bytes(T, n_q_heads, head_dim);
+  return cfa_prompt_attention_cached_workspace_size(T, B, n_q_heads, n_kv_heads, head_dim,
+                                                    max_query, max_keys, window, 0, 0, num_splits);
 }
 
-extern "C" int cfa_prompt_attention(
-    const void *q, const void *k_pool, const void *v_pool, int fp16, const int32_t *block_tables,
-    int max_blocks_per_seq, const int32_t *ctx_lens, int num_blocks, int num_layers, int layer,
-    int block_size, const int32_t *cu_seqlens, int T, int B, int n_q_heads, int n_kv_heads,
-    int head_dim, float sm_scale, float soft_cap, const float *alibi_slopes, int window,
+extern "C" int cfa_prompt_attention_cached(
+    const void *q, const void *k_pool, const void *v_pool, const uint8_t *k_scales,
+    const uint8_t *v_scales, int fp16, const int32_t *block_tables, int max_blocks_per_seq,
+    const int32_t *ctx_lens, int num_blocks, int num_layers, int layer, int block_size,
+    const int32_t *cu_seqlens, int T, int B, int n_q_heads, int n_kv_heads, int head_dim,
+    float sm_scale, float soft_cap, const float *alibi_slopes, int window, int sinks,
     int max_query, int max_keys, int num_splits, void *out, void *workspace,
     size_t workspace_bytes, void *stream) {
   using namespace cfa::abi;
@@ -277,16 +333,15 @@ extern "C" int cfa_prompt_attention(
   if (T < 0 || B < 0) return fail_arg("need T, B >= 0");
   if (int rc = check_heads(n_q_heads, n_kv_heads, head_dim)) return rc;
   if (int rc = check_pool(num_blocks, num_layers, layer, block_size, max_blocks_per_seq)) return rc;
-  if (int rc = check_scores(sm_scale, soft_cap, window)) return rc;
+  if (int rc = check_scores(sm_scale, soft_cap, window, sinks)) return rc;
   if (max_query <= 0 || max_keys <= 0) return fail_arg("max_query and max_keys must be positive");
   if (num_splits < 0) return fail_arg("num_splits must not be negative");
+  Args a{};
+  if (int rc = set_pools(a, k_pool, v_pool, k_scales, v_scales)) return rc;
   if (T == 0 || B == 0) return CFA_OK;
   if (!q || !k_pool || !v_pool || !block_tables || !ctx_lens || !cu_seqlens || !out)
     return fail_arg("null pointer argument");
-  Args a{};
   a.q = (const uint16_t *)q;
-  a.kpool = (const uint16_t *)k_pool;
-  a.vpool = (const uint16_t *)v_pool;
   a.bt = block_tables;
   a.ctx = ctx_lens;
   a.cu = cu_seqlens;
@@ -303,7 +358,22 @@ extern "C" int cfa_prompt_attention(
   a.layer = layer;
   a.bs = block_size;
   a.window = window;
+  a.sinks = window > 0 ? sinks : 0;
   const Plan p = plan(T, std::min(max_query, T), B, a.G, n_kv_heads, head_dim, max_keys, window,
-                      num_splits, false);
+                      sinks, k_scales != nullptr, num_splits, false);
   return run(a, p, head_dim, fp16, sm_scale, soft_cap, workspace, workspace_bytes, stream);
+}
+
+extern "C" int cfa_prompt_attention(
+    const void *q, const void *k_pool, const void *v_pool, int fp16, const int32_t *block_tables,
+    int max_blocks_per_seq, const int32_t *ctx_lens, int num_blocks, int num_layers, int layer,
+    int block_size, const int32_t *cu_seqlens, int T, int B, int n_q_heads, int n_kv_heads,
+    int head_dim, float sm_scale, float soft_cap, const float *alibi_slopes, int window,
+    int max_query, int max_keys, int num_splits, void *out, void *workspace,
+    size_t workspace_bytes, void *stream) {
+  return cfa_prompt_attention_cached(q, k_pool, v_pool, nullptr, nullptr, fp16, block_tables,
+                                     max_blocks_per_seq, ctx_lens, num_blocks, num_layers, layer,
+                                     block_size, cu_seqlens, T, B, n_q_heads, n_kv_heads, head_dim,
+                                     sm_scale, soft_cap, alibi_slopes, window, 0, max_query,
+                                     max_keys, num_splits, out, workspace, workspace_bytes, stream);
 }

@@ -5,7 +5,7 @@
 //
 // For a query at position p and a key at position k that its mask leaves:
 //   s = scale q.k;  s = cap tanh(s / cap);  s -= slope_h (p - k)
-//   visible only while p - k < window
+//   visible only while p - k < window, or in the first `sinks` slots
 //   out = sum exp(s) v / sum exp(s)          (a row without keys: zeros)
 // A tree node's position is ctx + its depth, its visible keys the context and
 // its ancestors; token i of a prompt's chunk stands at ctx + i and sees every
@@ -39,6 +39,12 @@
 //  * Keys in front of the window's first are not read: a tile's transfers are
 //    clamped to the first visible position of its rows (their pages may be
 //    gone or reused), and whole tiles in front of it are skipped.
+//  * A cache of e4m3 codes (e4m3.hpp) is turned into 16 bits once a work-group: the
+//    codes of a tile come into LDS as they are, three tiles ahead and each wave's own
+//    eight keys of K and V by itself, and in its score phase a wave writes them,
+//    scaled, to rings of three K and three V tiles in the layout that the products
+//    read.  (Operands converted where they are read would cost every wave of the
+//    eight 128 conversions a tile instead of 16, beside the scores' vector work.)
 //  * Splits are cut on the device, from each block's own first and last tile,
 //    and leave fp32 sums for a log-sum-exp merge.
 //
@@ -59,6 +65,7 @@
 #include <type_traits>
 
 #include "abi_internal.hpp"
+#include "e4m3.hpp"
 #include "tree_tiles.hpp"
 
 namespace cfa {
@@ -76,12 +83,15 @@ constexpr float kT0 = 0.9999994557706551f, kT1 = -0.3332631793391637f, kT2 = 0.1
 // cap log2(e) up to which exp2 needs no base: sums of 2^24 keys times values
 // of 2^20 stay below 2^127, and 2^-80 is a normal bf16
 constexpr float kFixedCap = 80.0f;
+// rings of a cache of e4m3 codes: 16-bit K and V tiles, and tiles of codes
+constexpr int kCodeStages = 3;
 constexpr int kPeekSteps = 4;  // tiles of a split from which the last one is seen first
 
 struct Args {
   const uint16_t *q;      // [rows of tokens, Hq, D]
-  const uint16_t *kpool;  // [blocks, layers, Hkv, bs, D]
+  const uint16_t *kpool;  // [blocks, layers, Hkv, bs, D], of q's type or e4m3 codes
   const uint16_t *vpool;
+  const uint8_t *kscale, *vscale;  // e4m3: [blocks, layers, Hkv, bs], else null
   const int32_t *bt;      // [B, max_blocks]
   const int32_t *ctx;     // [B]
   const uint64_t *mask;   // trees: [N] or [B, N]; null: prompts
@@ -94,7 +104,7 @@ struct Args {
   int T, B, N, q0, Nq;    // tokens in all; trees: nodes, first query node, queries
   int Hq, Hkv, G, TQ;     // TQ: tokens per block
   int max_blocks, num_blocks, num_layers, layer, bs;
-  int splits, window;
+  int splits, window, sinks;  // sinks: 0 without a window
   int past;               // partials are stored past the caches
   float scale, cap;       // scale as given, or with a cap scale / cap
   // with a cap: its score in log2 units is x (k0 + k1 x^2 + k2 x^4 + k3 x^6) for
@@ -187,7 +197,7 @@ struct Row {
   float slope2;   // distance bias: slope * log2(e)
 };
 
-template <int D, int QT, class T, bool CAP, bool BIAS, bool FIXED>
+template <int D, int QT, class T, bool CAP, bool BIAS, bool FIXED, bool SINKS>
 __device__ __forceinline__ void raw_scores(const Lane<D, QT, T> &ln, const float (&base_of)[QT],
                                            const Args &a, float k0, float cap2, int kbase, int ctx,
                                            int least, int most_first, const Row *rows,
@@ -274,7 +284,13 @@ __device__ __forceinline__ void raw_scores(const Lane<D, QT, T> &ln, const float
         vis = n >= 64 ? ~0ull : (n <= 0 ? 0ull : ((1ull << n) - 1));
       }
       const int cut = min(r.first, tree ? ctx : r.first) - kbase;  // keys in front
+      uint64_t kept = 0;  // the first tokens
+      if constexpr (SINKS) {
+        const int n = a.sinks - kbase;
+        kept = n >= 64 ? vis : (n <= 0 ? 0ull : vis & ((1ull << n) - 1));
+      }
       if (cut > 0) vis = cut >= 64 ? 0ull : vis >> cut << cut;
+      if constexpr (SINKS) vis |= kept;
       vis >>= 8 * ln.g;
 #pragma unroll
       for (int blk = 0; blk < 2; ++blk)
@@ -346,17 +362,107 @@ __device__ __forceinline__ void score_phase(Scores<QT> &S, float (&b)[QT], f32x4
     }
 }
 
-template <int D, int QT, class T, bool CAP, bool BIAS, bool FIXED>
+// A wave's share of a tile of codes: its eight keys' K rows and V rows, 16 D bytes
+// at `codes`, and their scale bytes, 8 and 8 at `scales`.
+template <int D>
+struct CodeTransfers {
+  static constexpr int kLoads = (D == 128 ? 2 : 1) + 1;  // a tile, each wave
+  static constexpr int kWaveBytes = 16 * D;
+  // row (0 .. 7: K, 8 .. 15: V) and 16-code chunk of lane `lane` of transfer j
+  static __device__ __forceinline__ int row(int lane, int j) { return 8 * j + lane / (D / 16); }
+  static __device__ __forceinline__ int chunk(int lane) { return lane % (D / 16); }
+};
+
+// Four bytes a lane, HBM -> LDS (dma16's small sister; lanes that are off do nothing).
+__device__ __forceinline__ void dma4(const void *src, CFA_LDS void *lds) {
+  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dword %0, off" ::"v"(src), "s"(lds)
+               : "memory");
+}
+
+// Issue them for the tile at kbase.  koff: the row offset of the 16-key group that
+// holds the wave's keys.  A key that clamp_pos moves re-reads another's codes.
+template <int D>
+__device__ __forceinline__ void issue_codes(const Args &a, const long long *goff, int kbase, int from,
+                                            int sinks, int nkeys, uint8_t *codes, uint8_t *scales,
+                                            int wave, int lane) {
+  const long long off = uniform_i64(*goff);
+  const int group = kbase + 16 * (wave >> 1);
+  const int gstart = clamp_pos<true>(group, group, from, sinks, nkeys);
+#pragma unroll
+  for (int j = 0; j < CodeTransfers<D>::kLoads - 1; ++j) {
+    const int r = CodeTransfers<D>::row(lane, j);
+    const int pos = clamp_pos<true>(kbase + 8 * wave + (r & 7), group, from, sinks, nkeys);
+    const uint8_t *pool = (const uint8_t *)((D == 128 ? j == 0 : r < 8) ? a.kpool : a.vpool);
+    dma16(pool + off + ((pos - gstart) * D + CodeTransfers<D>::chunk(lane) * 16),
+          (CFA_LDS void *)(codes + j * 1024));
+  }
+  // (the group's bytes from its first slot on, whichever of its rows `off` points to)
+  if (lane < 4) {
+    const long long first = (off / D & ~15LL) + 8 * (wave & 1) + 4 * (lane & 1);
+    dma4((lane < 2 ? a.kscale : a.vscale) + first, (CFA_LDS void *)scales);
+  }
+}
+
+// Sixteen codes to 16-bit chunks c and c + 1 of a tile's row.
+template <class T>
+__device__ __forceinline__ void put_codes(const uint4 &w, float scale, uint8_t *row, int c, int swz) {
+  uint4 lo, hi;
+  lo.x = e4m3::unpack_pair<T, false>(w.x, scale);
+  lo.y = e4m3::unpack_pair<T, true>(w.x, scale);
+  lo.z = e4m3::unpack_pair<T, false>(w.y, scale);
+  lo.w = e4m3::unpack_pair<T, true>(w.y, scale);
+  hi.x = e4m3::unpack_pair<T, false>(w.z, scale);
+  hi.y = e4m3::unpack_pair<T, true>(w.z, scale);
+  hi.z = e4m3::unpack_pair<T, false>(w.w, scale);
+  hi.w = e4m3::unpack_pair<T, true>(w.w, scale);
+  *reinterpret_cast<uint4 *>(row + ((c ^ swz) << 4)) = lo;
+  *reinterpret_cast<uint4 *>(row + (((c + 1) ^ swz) << 4)) = hi;
+}
+
+// The wave's share of tile `kt` (first key kbase_k) into the K ring's tile kdst and
+// of tile `vt` into vdst, each from its own tile of codes; null: not that one.  Keys
+// that were re-read become (nearly) zeros: the byte of their slot may be anything.
+template <int D, class T>
+__device__ __forceinline__ void convert_codes(const uint8_t *kcodes, const uint8_t *kscales,
+                                              int kbase_k, uint8_t *kdst, const uint8_t *vcodes,
+                                              const uint8_t *vscales, int kbase_v, uint8_t *vdst,
+                                              int from, int sinks, int nkeys, int wave, int lane) {
+  constexpr int RB = Geo<D>::kRowBytes;
+#pragma unroll
+  for (int j = 0; j < CodeTransfers<D>::kLoads - 1; ++j) {
+    const int r = CodeTransfers<D>::row(lane, j), key = 8 * wave + (r & 7);
+    const bool is_k = D == 128 ? j == 0 : r < 8;
+    uint8_t *const dst = is_k ? kdst : vdst;
+    if (!dst) continue;
+    const uint8_t *codes = is_k ? kcodes : vcodes, *scales = is_k ? kscales : vscales;
+    const int group = (is_k ? kbase_k : kbase_v) + (key & ~15);
+    const int pos = (is_k ? kbase_k : kbase_v) + key;
+    const uint4 w = *reinterpret_cast<const uint4 *>(codes + j * 1024 + lane * 16);
+    const uint32_t byte = scales[r];
+    const float scale =
+        clamp_pos<true>(pos, group, from, sinks, nkeys) == pos ? e4m3::scale(byte) : 0.0f;
+    const int at = is_k ? k_row_of_key(key) : key;
+    put_codes<T>(w, scale, dst + at * RB, 2 * CodeTransfers<D>::chunk(lane),
+                 is_k ? k_swz<D>(at) : v_swz<D>(at));
+  }
+}
+
+template <int D, int QT, class T, bool CAP, bool BIAS, bool FIXED, bool E4M3, bool SINKS>
 __global__ __launch_bounds__(kNT) void scored_attn_kernel(Args a) {
   using Gm = Geo<D>;
   constexpr int kTileBytes = Gm::kTileBytes;
-  constexpr int kLoadsPerTile = Gm::kLoadsPerTile;
+  constexpr int kLoadsPerTile = E4M3 ? CodeTransfers<D>::kLoads : Gm::kLoadsPerTile;
+  constexpr int kKStages = E4M3 ? kCodeStages : tree::kKStages;
+  constexpr int kVStages = E4M3 ? kCodeStages : tree::kVStages;
+  constexpr int kWaveBytes = CodeTransfers<D>::kWaveBytes;
   __shared__ __align__(16) uint8_t kring[kKStages * kTileBytes];
   __shared__ __align__(16) uint8_t vring[kVStages * kTileBytes];
+  __shared__ __align__(16) uint8_t codes[E4M3 ? kCodeStages * kWaves * kWaveBytes : 16];
+  __shared__ __align__(16) uint8_t scales[E4M3 ? kCodeStages * kWaves * 16 : 16];
   // row offsets of the split's 16-key groups; a ring, refilled half a ring at a
   // time in longer splits (its size, and the rows', let two work-groups of one
   // query tile and head_dim 64 share a CU's LDS)
-  constexpr int kRing = D == 64 ? 512 : 1024;
+  constexpr int kRing = D == 64 || E4M3 ? 512 : 1024;
   __shared__ long long gtab[kRing];
   __shared__ long long gpeek[kKT / 16];
   // trees: how far node j's position lies from its slot, at 64 + j; 0 around them
@@ -403,7 +509,9 @@ __global__ __launch_bounds__(kNT) void scored_attn_kernel(Args a) {
     const int j = a.q0 + blk.i0;
     if (a.window > 0)  // nodes that lie `window` and more above are out of it
       for (int m = 0; m < a.N; ++m)
-        if (depth - __builtin_amdgcn_readlane(depth, m) >= a.window) mine &= ~(1ull << m);
+        if (depth - __builtin_amdgcn_readlane(depth, m) >= a.window &&
+            !(SINKS && ctx + m < a.sinks))
+          mine &= ~(1ull << m);
     const bool asks = lane >= j && lane < j + blk.nt;
     int d = asks ? depth : 64, behind = asks && mine ? 64 - __clzll((long long)mine) : 0;
 #pragma unroll
@@ -434,14 +542,29 @@ __global__ __launch_bounds__(kNT) void scored_attn_kernel(Args a) {
   }
   const int high = tree ? ctx + 63 : low + blk.nt - 1;  // no query stands behind it
   // the first position that any row sees, and the last first one
-  const int from = a.window > 0 ? min(max(low - a.window + 1, 0), tree ? ctx : nkeys - 1) : 0;
+  int from = a.window > 0 ? min(max(low - a.window + 1, 0), tree ? ctx : nkeys - 1) : 0;
   const int most_first = a.window > 0 ? max(high - a.window + 1, 0) : 0;
   // keys below it are visible to all (but the window)
   const int least = tree ? ctx : min(low + 1, nkeys);
+  int sinks = 0;  // the first tokens in front of `from`
+  if constexpr (SINKS) {
+    sinks = min(a.sinks, min(from, nkeys));
+    if (from >= nkeys) {  // they are all
+      nkeys = sinks;
+      from = 0;
+    }
+  }
+  // The tiles: by their place in the sequence, or with first tokens `ns` of these and
+  // then those from `from` on.
   const int tlo = from / kKT, thi = (nkeys + kKT - 1) / kKT;
-  const int tps = (thi - tlo + a.splits - 1) / a.splits;
-  const int t0 = tlo + split * tps, t1 = min(thi, t0 + tps);
-  const int steps = from < nkeys ? t1 - t0 : 0;
+  const int ns = SINKS ? min((sinks + kKT - 1) / kKT, tlo) : 0;
+  const int begin = SINKS ? 0 : tlo, end = SINKS ? ns + thi - tlo : thi;
+  const int tps = (end - begin + a.splits - 1) / a.splits;
+  const int t0 = begin + split * tps, t1 = min(end, t0 + tps);
+  const int steps = SINKS || from < nkeys ? t1 - t0 : 0;
+  // a tile's first key
+  const int skip = SINKS ? tlo - ns : 0;
+  auto key_of = [&](int i) { return (SINKS && i >= ns ? i + skip : i) * kKT; };
   constexpr float kLog2e = 1.4426950408889634f;
   const float cap2 = a.cap * kLog2e;
   // without a cap: score in log2 units = product * k0; with one: e^(2 s / cap)
@@ -475,14 +598,37 @@ __global__ __launch_bounds__(kNT) void scored_attn_kernel(Args a) {
 
   const DmaOffs<D> doff = dma_offsets<D>(wave, lane);
   auto issue_from = [&](const long long *tab, int u, uint8_t *kdst, uint8_t *vdst) {
-    const int kbase = (t0 + u) * kKT;
+    const int kbase = key_of(t0 + u);
     const long long *kt = tab + 2 * (wave >> 2) + (wave & 1);
     const long long *vt = tab + (wave >> 1);
-    if (kbase + kKT <= nkeys && kbase >= from)
+    if ((kbase + kKT <= nkeys && kbase >= from) || (SINKS && kbase + kKT <= sinks))
       issue_tile_full<D>(a, kt, vt, doff, kdst, vdst, wave);
     else
-      issue_tile<D, true>(a, kt, vt, kbase, nkeys, kdst, vdst, wave, lane, from);
+      issue_tile<D, true>(a, kt, vt, kbase, nkeys, kdst, vdst, wave, lane, from, sinks);
   };
+  // codes: this wave's parts of stage t % 3
+  auto codes_at = [&](int t) { return codes + ((t % kCodeStages) * kWaves + wave) * kWaveBytes; };
+  auto scales_at = [&](int t) { return scales + ((t % kCodeStages) * kWaves + wave) * 16; };
+  auto issue8_from = [&](const long long *tab, int u, int stage) {
+    issue_codes<D>(a, tab + (wave >> 1), key_of(t0 + u), from, sinks, nkeys, codes_at(stage),
+                   scales_at(stage), wave, lane);
+  };
+  auto issue8 = [&](int u) { issue8_from(gtab + u * (kKT / 16) % kRing, u, u); };
+  // K of tile ku and V of tile vu (-1: none) to 16 bits; the writes are done behind it
+  auto convert = [&](int ku, int vu) {
+    convert_codes<D, T>(codes_at(ku), scales_at(ku), key_of(t0 + ku),
+                        ku < steps ? kring + (ku % kKStages) * kTileBytes : nullptr, codes_at(vu),
+                        scales_at(vu), key_of(t0 + vu),
+                        vu >= 0 && vu < steps ? vring + (vu % kVStages) * kTileBytes : nullptr, from,
+                        sinks, nkeys, wave, lane);
+  };
+  // a wait for transfers that the same wave reads next
+  auto transfers_done = [&](bool but_one_tile) {
+    if (but_one_tile) wait_vmcnt<kLoadsPerTile>();
+    else wait_vmcnt<0>();
+    asm volatile("" ::: "memory");
+  };
+  auto writes_done = [&] { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); };
   auto issue = [&](int u, uint8_t *kdst, uint8_t *vdst) {
     issue_from(gtab + u * (kKT / 16) % kRing, u, kdst, vdst);
   };
@@ -491,8 +637,9 @@ __global__ __launch_bounds__(kNT) void scored_attn_kernel(Args a) {
   const int ng = steps * kPerTile;
   auto look_up = [&](int first, int n) {
     for (int i = first + tid; i < min(first + n, ng); i += kNT) {
-      gtab[i % kRing] =
-          group_row_offset<D, true>(a, btb, t0 * kPerTile + i, nkeys, h, from);
+      int gi = t0 * kPerTile + i;
+      if (SINKS && gi >= ns * kPerTile) gi += skip * kPerTile;
+      gtab[i % kRing] = group_row_offset<D, true>(a, btb, gi, nkeys, h, from, sinks);
     }
   };
   look_up(0, kRing);
@@ -500,8 +647,8 @@ __global__ __launch_bounds__(kNT) void scored_attn_kernel(Args a) {
   // bases before the first tile: from far to near, steep slopes would rescale
   // the outputs at every tile (the biased prompt of 8192 693 us against 546).
   const bool peek = BIAS && steps >= kPeekSteps;
-  if (BIAS && tid < kPerTile)
-    gpeek[tid] = group_row_offset<D, true>(a, btb, (t1 - 1) * kPerTile + tid, nkeys, h, from);
+  if (peek && tid < kPerTile)
+    gpeek[tid] = group_row_offset<D, true>(a, btb, key_of(t1 - 1) / 16 + tid, nkeys, h, from, sinks);
   wait_vmcnt<0>();
   __syncthreads();
 
@@ -520,20 +667,32 @@ __global__ __launch_bounds__(kNT) void scored_attn_kernel(Args a) {
   if (steps > 0) {
     // the phases and barriers of tree_attention.hip's loop
     // (the last K stage and V stage are free until the loop)
-    if (peek)
+    if (!E4M3 && peek)
       issue_from(gpeek, steps - 1, kring + (kKStages - 1) * kTileBytes,
                  vring + (kVStages - 1) * kTileBytes);
-    for (int u = 0; u < min(3, steps); ++u)
-      issue(u, kring + (u % kKStages) * kTileBytes, vring + (u % kVStages) * kTileBytes);
+    if constexpr (E4M3) {
+      if (peek) {  // through the stages of tile 2
+        issue8_from(gpeek, steps - 1, 2);
+        transfers_done(false);
+        convert_codes<D, T>(codes_at(2), scales_at(2), key_of(t1 - 1),
+                            kring + (kKStages - 1) * kTileBytes, nullptr, nullptr, 0, nullptr, from,
+                            sinks, nkeys, wave, lane);
+        writes_done();
+      }
+      for (int u = 0; u < min(3, steps); ++u) issue8(u);
+    } else {
+      for (int u = 0; u < min(3, steps); ++u)
+        issue(u, kring + (u % kKStages) * kTileBytes, vring + (u % kVStages) * kTileBytes);
+    }
     Scores<QT> S;
     const bool busy = wave * QT * 16 < rows;  // wave-uniform
     if constexpr (BIAS) {
       if (peek) {
-        wait_vmcnt<3 * kLoadsPerTile>();
+        if constexpr (!E4M3) wait_vmcnt<3 * kLoadsPerTile>();
         block_barrier();
         if (busy) {
           qk_tile(ln, kring + (kKStages - 1) * kTileBytes, zero, S);
-          raw_scores<D, QT, T, CAP, BIAS, FIXED>(ln, base, a, k0, cap2, (t1 - 1) * kKT, ctx, least,
+          raw_scores<D, QT, T, CAP, BIAS, FIXED, SINKS>(ln, base, a, k0, cap2, key_of(t1 - 1), ctx, least,
                                                  most_first, rows_at, smove + 64, S);
 #pragma unroll
           for (int qt = 0; qt < QT; ++qt) {
@@ -544,17 +703,25 @@ __global__ __launch_bounds__(kNT) void scored_attn_kernel(Args a) {
         block_barrier();
       }
     }
-    const int later = min(3, steps) - 1;
-    if (later >= 2) wait_vmcnt<2 * kLoadsPerTile>();
-    else if (later == 1) wait_vmcnt<kLoadsPerTile>();
-    else wait_vmcnt<0>();
+    if constexpr (E4M3) {
+      transfers_done(steps >= 3);
+      convert(0, 0);
+      convert(1, -1);
+      if (steps > 3) issue8(3);
+      writes_done();
+    } else {
+      const int later = min(3, steps) - 1;
+      if (later >= 2) wait_vmcnt<2 * kLoadsPerTile>();
+      else if (later == 1) wait_vmcnt<kLoadsPerTile>();
+      else wait_vmcnt<0>();
+    }
     block_barrier();
     const bool lag = wave >= kWaves / 2;
     if (lag) block_barrier();
     Probs<QT, T> P;
     if (busy) qk_tile(ln, kring, zero, S);
     for (int u = 0; u < steps; ++u) {
-      const int kbase = (t0 + u) * kKT;
+      const int kbase = key_of(t0 + u);
       const int ahead = u + 3;
       // (both halves' groups were in use until now: the one in front of this step
       // has no readers left, and its new entries have them half a ring on)
@@ -562,22 +729,35 @@ __global__ __launch_bounds__(kNT) void scored_attn_kernel(Args a) {
         look_up(u * kPerTile + kRing / 2, kRing / 2);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       }
-      if (!lag) {
+      if constexpr (E4M3) {
+        // A tile's K is written two steps before the products read it and its V one:
+        // between the two halves' phases the last reader of either ring's stage is
+        // then done, and both halves' writes are in front of the first.
         block_barrier();
+        transfers_done(u + 3 < steps);
+        convert(u + 2, u + 1);
+        if (u + 4 < steps) issue8(u + 4);
       } else {
-        if (u + 2 < steps) wait_vmcnt<kLoadsPerTile>();
-        else wait_vmcnt<0>();
-        block_barrier();
+        if (!lag) {
+          block_barrier();
+        } else {
+          if (u + 2 < steps) wait_vmcnt<kLoadsPerTile>();
+          else wait_vmcnt<0>();
+          block_barrier();
+        }
+        if (ahead < steps)
+          issue(ahead, kring + (ahead % kKStages) * kTileBytes,
+                vring + (ahead % kVStages) * kTileBytes);
       }
-      if (ahead < steps)
-        issue(ahead, kring + (ahead % kKStages) * kTileBytes,
-              vring + (ahead % kVStages) * kTileBytes);
       if (busy) {
-        raw_scores<D, QT, T, CAP, BIAS, FIXED>(ln, base, a, k0, cap2, kbase, ctx, least, most_first,
+        raw_scores<D, QT, T, CAP, BIAS, FIXED, SINKS>(ln, base, a, k0, cap2, kbase, ctx, least, most_first,
                                                rows_at, smove + 64, S);
         score_phase<D, QT, T, FIXED>(S, base, o, lacc, P);
       }
-      if (!lag) {
+      if constexpr (E4M3) {
+        writes_done();
+        block_barrier();
+      } else if (!lag) {
         if (ahead < steps) wait_vmcnt<2 * kLoadsPerTile>();
         else if (u + 2 < steps) wait_vmcnt<kLoadsPerTile>();
         else wait_vmcnt<0>();
@@ -607,7 +787,7 @@ __global__ __launch_bounds__(kNT) void scored_attn_kernel(Args a) {
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
       const int r0 = (wave * QT + qt) * 16;
-      uint8_t *const tile = kring + r0 * D * 2;
+      uint8_t *const tile = kring + (E4M3 ? wave * 16 : r0) * D * 2;
       const float ls = lacc[qt][0], inv = ls != 0.0f ? 1.0f / ls : 0.0f;
 #pragma unroll
       for (int dt = 0; dt < D / 16; ++dt) {
@@ -711,14 +891,22 @@ __global__ __launch_bounds__(256) void scored_merge_kernel(Args a) {
   __builtin_nontemporal_store(u32x2{w.x, w.y}, reinterpret_cast<u32x2 *>(a.out + row * D + e));
 }
 
-template <int D, int QT, class T>
+template <int D, int QT, class T, bool E4M3>
 int launch_scores(const Args &a, unsigned grid, hipStream_t st) {
   const bool cap = a.cap > 0.0f, bias = a.slopes != nullptr;
   const bool fixed = cap && !bias && std::is_same<T, BF16>::value &&
                      a.cap * 1.4426950408889634f <= kFixedCap;
-#define CFA_SCORED(C, B, F)                                                                  \
-  CFA_LAUNCH("scored_attn", (scored_attn_kernel<D, QT, T, C, B, F>), dim3(grid), dim3(kNT), 0, \
-             st, a)
+  // (the first tokens' tiles in a kernel of their own: with them in one, registers
+  // for the steps between tiles cost others the schedule of their operand reads)
+#define CFA_SCORED(C, B, F)                                                                    \
+  do {                                                                                         \
+    if (a.sinks > 0)                                                                           \
+      CFA_LAUNCH("scored_attn", (scored_attn_kernel<D, QT, T, C, B, F, E4M3, true>), dim3(grid), \
+                 dim3(kNT), 0, st, a);                                                         \
+    else                                                                                       \
+      CFA_LAUNCH("scored_attn", (scored_attn_kernel<D, QT, T, C, B, F, E4M3, false>), dim3(grid), \
+                 dim3(kNT), 0, st, a);                                                         \
+  } while (0)
   if (cap && bias) CFA_SCORED(true, true, false);
   else if (fixed) {
     if constexpr (std::is_same<T, BF16>::value) CFA_SCORED(true, false, true);
@@ -729,9 +917,10 @@ int launch_scores(const Args &a, unsigned grid, hipStream_t st) {
   return CFA_OK;
 }
 
-template <int D, class T>
+template <int D, class T, bool E4M3>
 int launch(const Args &a, bool one, unsigned grid, hipStream_t st) {
-  const int rc = one ? launch_scores<D, 1, T>(a, grid, st) : launch_scores<D, 2, T>(a, grid, st);
+  const int rc = one ? launch_scores<D, 1, T, E4M3>(a, grid, st)
+                     : launch_scores<D, 2, T, E4M3>(a, grid, st);
   if (rc != CFA_OK || a.splits == 1) return rc;
   const long long rows = (long long)a.T * a.Hq;
   const int per = 256 / (D / 4);

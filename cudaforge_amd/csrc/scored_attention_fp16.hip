@@ -3,7 +3,7 @@
 
 namespace cfa {
 namespace scored {
-template int launch<64, FP16>(const Args &, bool, unsigned, hipStream_t);
-template int launch<128, FP16>(const Args &, bool, unsigned, hipStream_t);
+template int launch<64, FP16, false>(const Args &, bool, unsigned, hipStream_t);
+template int launch<128, FP16, false>(const Args &, bool, unsigned, hipStream_t);
 }  // namespace scored
 }  // namespace cfa

@@ -79,6 +79,11 @@ __device__ __forceinline__ int k_key_of_row(int R) {
   return (R & ~31) + ((R >> 2) & 3) * 8 + ((R >> 4) & 1) * 4 + (R & 3);
 }
 
+// and the row of a key
+__device__ __forceinline__ int k_row_of_key(int key) {
+  return (key & ~31) | ((key >> 2) & 1) << 4 | ((key >> 3) & 3) << 2 | (key & 3);
+}
+
 // LDS swizzles (16-byte chunk c of a row sits at position c ^ swizzle):
 //   K-tile row R:  D = 128: R % 16;  D = 64: (R / 2) % 8.  A 16-row MFMA
 //     operand read then touches every bank once per 16 lanes.
@@ -96,11 +101,13 @@ __device__ __forceinline__ int v_swz(int key) {
 }
 
 // Key positions that a transfer reads lie below nkeys and, with kFrom, at
-// `from` or behind it; others re-read the nearest of those.
+// `from` or behind it or in front of `sinks` (sinks <= from < nkeys); others
+// re-read one of those: of the 16-key group at `group`, where it has any.
 template <bool kFrom>
-__device__ __forceinline__ int clamp_pos(int pos, int from, int nkeys) {
+__device__ __forceinline__ int clamp_pos(int pos, int group, int from, int sinks, int nkeys) {
   pos = min(pos, nkeys - 1);
-  return kFrom ? max(pos, from) : pos;
+  if (!kFrom || pos >= from || (uint32_t)pos < (uint32_t)sinks) return pos;
+  return group < sinks ? sinks - 1 : from;
 }
 
 // Pool element offset of the row holding position gstart = clamp_pos(16 gi),
@@ -109,8 +116,9 @@ __device__ __forceinline__ int clamp_pos(int pos, int from, int nkeys) {
 // a load outside the pool.
 template <int D, bool kFrom = false, class A>
 __device__ __forceinline__ long long group_row_offset(const A &a, const int32_t *btb, int gi,
-                                                      int nkeys, int h, int from = 0) {
-  const int gstart = clamp_pos<kFrom>(gi * 16, from, nkeys);
+                                                      int nkeys, int h, int from = 0,
+                                                      int sinks = 0) {
+  const int gstart = clamp_pos<kFrom>(gi * 16, gi * 16, from, sinks, nkeys);
   const int page = min(gstart / a.bs, a.max_blocks - 1);
   const int blk = min(max(btb[page], 0), a.num_blocks - 1);
   return (((long long)blk * a.num_layers + a.layer) * a.Hkv + h) * ((long long)a.bs * D) +
@@ -133,20 +141,20 @@ __device__ __forceinline__ long long uniform_i64(long long v) {
 template <int D, bool kFrom = false, class A>
 __device__ __forceinline__ void issue_tile(const A &a, const long long *kt, const long long *vt, int kbase,
                                            int nkeys, uint8_t *kdst, uint8_t *vdst, int wave,
-                                           int lane, int from = 0) {
+                                           int lane, int from = 0, int sinks = 0) {
   using Gm = Geo<D>;
   constexpr int RPL = Gm::kRowsPerLoad;
   const int sub = lane / Gm::kChunks, pc = lane % Gm::kChunks;
   {
     // K: the wave's rows hold keys of the tile's 16-group 2 (w / 4) + (w % 2)
     const int gi = kbase / 16 + 2 * (wave >> 2) + (wave & 1);
-    const int gstart = clamp_pos<kFrom>(gi * 16, from, nkeys);
+    const int gstart = clamp_pos<kFrom>(gi * 16, gi * 16, from, sinks, nkeys);
     const uint16_t *base = a.kpool + uniform_i64(*kt);
 #pragma unroll
     for (int j = 0; j < 8 / RPL; ++j) {
       const int R = 8 * wave + RPL * j + sub;
       const int c = pc ^ k_swz<D>(R);
-      const int pos = clamp_pos<kFrom>(kbase + k_key_of_row(R), from, nkeys);
+      const int pos = clamp_pos<kFrom>(kbase + k_key_of_row(R), gi * 16, from, sinks, nkeys);
       dma16(base + ((pos - gstart) * D + c * 8),
             (CFA_LDS void *)(kdst + (8 * wave + RPL * j) * Gm::kRowBytes));
     }
@@ -154,13 +162,13 @@ __device__ __forceinline__ void issue_tile(const A &a, const long long *kt, cons
   {
     // V: keys 8w..8w+7, in the tile's 16-group w / 2
     const int gi = kbase / 16 + (wave >> 1);
-    const int gstart = clamp_pos<kFrom>(gi * 16, from, nkeys);
+    const int gstart = clamp_pos<kFrom>(gi * 16, gi * 16, from, sinks, nkeys);
     const uint16_t *base = a.vpool + uniform_i64(*vt);
 #pragma unroll
     for (int j = 0; j < 8 / RPL; ++j) {
       const int key = 8 * wave + RPL * j + sub;
       const int c = pc ^ v_swz<D>(key);
-      const int pos = clamp_pos<kFrom>(kbase + key, from, nkeys);
+      const int pos = clamp_pos<kFrom>(kbase + key, gi * 16, from, sinks, nkeys);
       dma16(base + ((pos - gstart) * D + c * 8),
             (CFA_LDS void *)(vdst + (8 * wave + RPL * j) * Gm::kRowBytes));
     }

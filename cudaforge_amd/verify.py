@@ -218,12 +218,14 @@ def chain_verify(target: torch.Tensor, draft: Optional[torch.Tensor],
 
 def tree_attention_workspace_bytes(B: int, N: int, n_q_heads: int, n_kv_heads: int,
                                    head_dim: int, max_keys: int, num_splits: int = 0, *,
-                                   scored: bool = False, window: int = 0) -> int:
+                                   scored: bool = False, window: int = 0, sinks: int = 0,
+                                   e4m3: bool = False) -> int:
     """Workspace of ``tree_attention`` for N query nodes; `scored`: with a cap,
-    a bias, a window or fp16 tensors."""
-    if scored or window:
-        return int(_lib.load().cfa_tree_attention_scored_workspace_size(
-            B, N, n_q_heads, n_kv_heads, head_dim, _int32(max_keys), _int32(window), num_splits))
+    a bias, a window or fp16 tensors; `e4m3`: over pools with scales."""
+    if scored or window or e4m3:
+        return int(_lib.load().cfa_tree_attention_cached_workspace_size(
+            B, N, n_q_heads, n_kv_heads, head_dim, _int32(max_keys), _int32(window), _int32(sinks),
+            int(e4m3), num_splits))
     return int(_lib.load().cfa_tree_attention_workspace_size(B, N, n_q_heads, n_kv_heads,
                                                               head_dim, max_keys, num_splits))
 
@@ -299,7 +301,8 @@ def tree_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
                    num_splits: int = 0, out: Optional[torch.Tensor] = None,
                    workspace: Optional[torch.Tensor] = None, first_node: int = 0,
                    soft_cap: float = 0.0, alibi_slopes: Optional[torch.Tensor] = None,
-                   window: int = 0) -> torch.Tensor:
+                   window: int = 0, sinks: int = 0, k_scales: Optional[torch.Tensor] = None,
+                   v_scales: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Tree-masked attention of draft-tree nodes over a paged KV cache.
 
     q [B, Nq, Hq, D] bf16 (D = 128 or 64): the queries of tree nodes
@@ -313,13 +316,17 @@ def tree_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
 
     A tree of one node (tree_mask [1] holding 1) is plain decode.
 
-    Scores of other decoders (``cfa_tree_attention_scored``): soft_cap > 0
+    Scores of other decoders (``cfa_tree_attention_cached``): soft_cap > 0
     takes cap * tanh(s / cap) of each scaled score; alibi_slopes [Hq] fp32
     subtracts slope * distance, where a node stands at ctx_len + its depth (the
     bits of its mask less one); window > 0 hides keys at a distance of window
-    and more.  q and the pools may then be fp16, and Hq / Hkv * Nq may exceed
-    256; fp16 tensors take this path by themselves.  A query that sees no key
-    gets zeros.
+    and more, but those in a sequence's first `sinks` slots.  q and the pools may
+    then be fp16, and Hq / Hkv * Nq may exceed 256; fp16 tensors take this path by
+    themselves.  A query that sees no key gets zeros.
+
+    With k_scales and v_scales (uint8 [num_blocks, num_layers, Hkv, block_size])
+    the pools are float8_e4m3fn, as ``rotary.qk_norm_rope_kv`` writes them; q is
+    bf16 or fp16, and keys and values are taken in its type.
     """
     dtype = _half_dtype(q)
     _require_cuda("q", q, dtype)
@@ -331,11 +338,15 @@ def tree_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
         raise ValueError("first_node must be >= 0")
     N = first_node + Nq
     q = q.contiguous()
-    _require_all(dev, (("k_pool", k_pool, dtype), ("v_pool", v_pool, dtype),
+    cache = _cache_dtype(k_scales, v_scales, dtype)
+    _require_all(dev, (("k_pool", k_pool, cache), ("v_pool", v_pool, cache),
                        ("block_tables", block_tables, torch.int32),
                        ("ctx_lens", ctx_lens, torch.int32), ("tree_mask", tree_mask, torch.int64)))
     _check_pools(k_pool, v_pool, D)
     nblk, nlayers, Hkv, bs, _ = k_pool.shape
+    _check_scales(k_scales, v_scales, k_pool.shape, dev)
+    if sinks < 0:
+        raise ValueError("sinks must not be negative")
     if block_tables.dim() != 2 or block_tables.shape[0] != B:
         raise ValueError("block_tables must be [B, max_blocks]")
     block_tables = block_tables.contiguous()
@@ -353,10 +364,11 @@ def tree_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
         sm_scale = D ** -0.5
     if max_keys is None:
         max_keys = int(ctx_lens.max().item()) + N
+    e4m3 = k_scales is not None
     scored = (soft_cap != 0.0 or alibi_slopes is not None or window != 0
-              or dtype == torch.float16)
+              or dtype == torch.float16 or e4m3)
     if scored:
-        window, max_keys = _int32(window), _int32(max_keys)
+        window, sinks, max_keys = _int32(window), _int32(sinks), _int32(max_keys)
         alibi_slopes = _check_slopes(alibi_slopes, Hq, dev)
         q = _aligned(q)
         out = _check_out(out, q)
@@ -365,20 +377,20 @@ def tree_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
     lib = _lib.load()
     with _on(dev):
         if scored:
-            need = int(lib.cfa_tree_attention_scored_workspace_size(
-                B, Nq, Hq, Hkv, D, max_keys, window, num_splits))
+            need = int(lib.cfa_tree_attention_cached_workspace_size(
+                B, Nq, Hq, Hkv, D, max_keys, window, sinks, e4m3, num_splits))
         else:
             need = int(lib.cfa_tree_attention_workspace_size(B, Nq, Hq, Hkv, D, max_keys,
                                                              num_splits))
         workspace = _workspace(workspace, need, dev)
         if scored:
-            rc = lib.cfa_tree_attention_scored(
-                q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), int(dtype == torch.float16),
-                block_tables.data_ptr(), block_tables.shape[1], ctx_lens.data_ptr(), nblk, nlayers,
-                int(layer), bs, tree_mask.data_ptr(), mstride, B, N, int(first_node), Hq, Hkv, D,
-                sm_scale, soft_cap, _ptr(alibi_slopes), window, max_keys,
-                int(num_splits), out.data_ptr(), workspace.data_ptr(), workspace.numel(),
-                _stream_ptr(dev))
+            rc = lib.cfa_tree_attention_cached(
+                q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), _ptr(k_scales),
+                _ptr(v_scales), int(dtype == torch.float16), block_tables.data_ptr(),
+                block_tables.shape[1], ctx_lens.data_ptr(), nblk, nlayers, int(layer), bs,
+                tree_mask.data_ptr(), mstride, B, N, int(first_node), Hq, Hkv, D, sm_scale,
+                soft_cap, _ptr(alibi_slopes), window, sinks, max_keys, int(num_splits),
+                out.data_ptr(), workspace.data_ptr(), workspace.numel(), _stream_ptr(dev))
         else:
             rc = lib.cfa_tree_attention(
                 q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), block_tables.data_ptr(),
@@ -386,16 +398,17 @@ def tree_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
                 tree_mask.data_ptr(), mstride, B, N, int(first_node), Hq, Hkv, D,
                 sm_scale, int(max_keys), int(num_splits), out.data_ptr(),
                 workspace.data_ptr(), workspace.numel(), _stream_ptr(dev))
-    _lib.check(rc, "cfa_tree_attention_scored" if scored else "cfa_tree_attention")
+    _lib.check(rc, "cfa_tree_attention_cached" if scored else "cfa_tree_attention")
     return out
 
 
 def prompt_attention_workspace_bytes(T: int, B: int, n_q_heads: int, n_kv_heads: int,
                                      head_dim: int, max_query: int, max_keys: int,
-                                     window: int = 0, num_splits: int = 0) -> int:
-    return int(_lib.load().cfa_prompt_attention_workspace_size(
+                                     window: int = 0, num_splits: int = 0, *, sinks: int = 0,
+                                     e4m3: bool = False) -> int:
+    return int(_lib.load().cfa_prompt_attention_cached_workspace_size(
         T, B, n_q_heads, n_kv_heads, head_dim, _int32(max_query), _int32(max_keys), _int32(window),
-        num_splits))
+        _int32(sinks), int(e4m3), num_splits))
 
 
 def prompt_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
@@ -405,16 +418,19 @@ def prompt_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor
                      max_keys: Optional[int] = None, soft_cap: float = 0.0,
                      alibi_slopes: Optional[torch.Tensor] = None, window: int = 0,
                      num_splits: int = 0, out: Optional[torch.Tensor] = None,
-                     workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+                     workspace: Optional[torch.Tensor] = None, sinks: int = 0,
+                     k_scales: Optional[torch.Tensor] = None,
+                     v_scales: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Causal attention of prompt chunks over a paged KV cache
-    (``cfa_prompt_attention``).
+    (``cfa_prompt_attention_cached``).
 
     q [T, Hq, D] (bf16 or fp16, D = 128 or 64) holds B sequences' new tokens one
     after another: cu_seqlens int32 [B + 1] says where each begins.  ctx_lens
     [B] int32 are the tokens in front of each chunk (0 for a first one); the
     chunk's own K and V are in the pages already (``rotary.qk_norm_rope_kv``),
     and token i of it sees the slots up to ctx_len + i.  Pools, block_tables,
-    soft_cap, alibi_slopes and window are those of ``tree_attention``.
+    soft_cap, alibi_slopes, window, sinks, k_scales and v_scales are those of
+    ``tree_attention``.
     max_query and max_keys are guesses of the longest chunk and of the largest
     ctx_len + chunk (default T and the tables' capacity): they plan the call,
     and any positive values are right.  Rows of q behind the last sequence get
@@ -428,12 +444,16 @@ def prompt_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor
         raise ValueError("q must be [T, Hq, D]")
     T, Hq, D = q.shape
     q = q.contiguous()
-    _require_all(dev, (("k_pool", k_pool, dtype), ("v_pool", v_pool, dtype),
+    cache = _cache_dtype(k_scales, v_scales, dtype)
+    _require_all(dev, (("k_pool", k_pool, cache), ("v_pool", v_pool, cache),
                        ("ctx_lens", ctx_lens, torch.int32),
                        ("block_tables", block_tables, torch.int32),
                        ("cu_seqlens", cu_seqlens, torch.int32)))
     _check_pools(k_pool, v_pool, D)
     nblk, nlayers, Hkv, bs, _ = k_pool.shape
+    _check_scales(k_scales, v_scales, k_pool.shape, dev)
+    if sinks < 0:
+        raise ValueError("sinks must not be negative")
     if ctx_lens.dim() != 1:
         raise ValueError("ctx_lens must be [B]")
     B = ctx_lens.shape[0]
@@ -448,21 +468,23 @@ def prompt_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor
     out = _check_out(out, q)
     if sm_scale is None:
         sm_scale = D ** -0.5
-    window = _int32(window)
+    window, sinks = _int32(window), _int32(sinks)
     max_query = _int32(max(T, 1) if max_query is None else max_query)
     max_keys = _int32(max(block_tables.shape[1] * bs, 1) if max_keys is None else max_keys)
     lib = _lib.load()
     with _on(dev):
-        need = int(lib.cfa_prompt_attention_workspace_size(T, B, Hq, Hkv, D, max_query, max_keys,
-                                                           window, num_splits))
+        need = int(lib.cfa_prompt_attention_cached_workspace_size(
+            T, B, Hq, Hkv, D, max_query, max_keys, window, sinks, k_scales is not None,
+            num_splits))
         workspace = _workspace(workspace, need, dev)
-        rc = lib.cfa_prompt_attention(
-            q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), int(dtype == torch.float16),
+        rc = lib.cfa_prompt_attention_cached(
+            q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), _ptr(k_scales), _ptr(v_scales),
+            int(dtype == torch.float16),
             block_tables.data_ptr(), block_tables.shape[1], ctx_lens.data_ptr(), nblk, nlayers,
             int(layer), bs, cu_seqlens.data_ptr(), T, B, Hq, Hkv, D, sm_scale, soft_cap,
-            _ptr(alibi_slopes), window, max_query, max_keys, int(num_splits),
+            _ptr(alibi_slopes), window, sinks, max_query, max_keys, int(num_splits),
             out.data_ptr(), workspace.data_ptr(), workspace.numel(), _stream_ptr(dev))
-    _lib.check(rc, "cfa_prompt_attention")
+    _lib.check(rc, "cfa_prompt_attention_cached")
     return out
 
 

@@ -58,7 +58,9 @@ const char *cfa_last_error(void);
  * cfa_tree_verify takes (workspace, workspace_bytes) before its stream, and
  * python-mode cfa_chain_verify reads uniforms [B, K+2] (row stride K+2), not
  * [B, K+1].  Minor 1 of it adds cfa_qk_norm_rope_kv,
- * cfa_tree_attention_scored, cfa_prompt_attention and cfa_sample_rows.
+ * cfa_tree_attention_scored, cfa_prompt_attention and cfa_sample_rows; minor 2
+ * cfa_tree_attention_cached, cfa_prompt_attention_cached, cfa_qk_norm_rope_kv_e4m3,
+ * cfa_kv_gather, cfa_kv_commit_scaled and cfa_adjust_logits.
  * Binding code checks the major before its first call. */
 #define CFA_ABI_VERSION 202
 int cfa_version(void);
@@ -352,6 +354,44 @@ int cfa_prompt_attention(const void *q, const void *k_pool, const void *v_pool, 
                          const float *alibi_slopes, int window, int max_query, int max_keys,
                          int num_splits, void *out, void *workspace, size_t workspace_bytes,
                          void *stream);
+
+/* cfa_tree_attention_scored and cfa_prompt_attention over a cache of either kind,
+ * with first tokens that a window leaves visible.
+ *   k_scales, v_scales: NULL for pools of q's type; else the pools hold e4m3 codes
+ *     (cfa_qk_norm_rope_kv_e4m3) and these [num_blocks][num_layers][n_kv_heads]
+ *     [block_size] the rows' scale bytes (1 to 253), 16-byte aligned.  Keys and values
+ *     are code * 2^(byte - 127) in q's type: exact in bf16, rounded once in fp16
+ *     (which holds them from 2^-14 to 65504 exactly)
+ *   sinks: with a window, keys in a sequence's first `sinks` slots are visible at any
+ *     distance (to queries that their masks let see them; a tree's nodes count by
+ *     their slots).  Pages wholly between these and every query's window are not read.
+ * Everything else is as for those; both are calls of these with NULL scales and no
+ * sinks.  e4m3 of the workspace sizes: whether there are scales. */
+size_t cfa_tree_attention_cached_workspace_size(int B, int N, int n_q_heads, int n_kv_heads,
+                                                int head_dim, int max_keys, int window, int sinks,
+                                                int e4m3, int num_splits);
+int cfa_tree_attention_cached(const void *q, const void *k_pool, const void *v_pool,
+                              const uint8_t *k_scales, const uint8_t *v_scales, int fp16,
+                              const int32_t *block_tables, int max_blocks_per_seq,
+                              const int32_t *ctx_lens, int num_blocks, int num_layers, int layer,
+                              int block_size, const uint64_t *tree_mask, int64_t tree_mask_stride_b,
+                              int B, int N, int first_node, int n_q_heads, int n_kv_heads,
+                              int head_dim, float sm_scale, float soft_cap,
+                              const float *alibi_slopes, int window, int sinks, int max_keys,
+                              int num_splits, void *out, void *workspace, size_t workspace_bytes,
+                              void *stream);
+size_t cfa_prompt_attention_cached_workspace_size(int T, int B, int n_q_heads, int n_kv_heads,
+                                                  int head_dim, int max_query, int max_keys,
+                                                  int window, int sinks, int e4m3, int num_splits);
+int cfa_prompt_attention_cached(const void *q, const void *k_pool, const void *v_pool,
+                                const uint8_t *k_scales, const uint8_t *v_scales, int fp16,
+                                const int32_t *block_tables, int max_blocks_per_seq,
+                                const int32_t *ctx_lens, int num_blocks, int num_layers, int layer,
+                                int block_size, const int32_t *cu_seqlens, int T, int B,
+                                int n_q_heads, int n_kv_heads, int head_dim, float sm_scale,
+                                float soft_cap, const float *alibi_slopes, int window, int sinks,
+                                int max_query, int max_keys, int num_splits, void *out,
+                                void *workspace, size_t workspace_bytes, void *stream);
 
 /* ---------------------------------------------------------------------------
  * Tree verification: multi-candidate rejection sampling down a draft tree,
