@@ -1,6 +1,6 @@
 // scored_attention.hip -- the entry points of scored_attention.hpp: argument
 // checks, the plan of blocks and splits, and the workspace.
-#include "scored_attention.hpp"
+#include "few_rows_attention.hpp"
 
 #include <algorithm>
 #include <cmath>
@@ -17,12 +17,18 @@ extern template int launch<128, BF16, true>(const Args &, bool, unsigned, hipStr
 extern template int launch<64, FP16, true>(const Args &, bool, unsigned, hipStream_t);
 extern template int launch<128, FP16, true>(const Args &, bool, unsigned, hipStream_t);
 
+extern template int launch_few<64, BF16>(const Args &, bool, unsigned, hipStream_t);
+extern template int launch_few<128, BF16>(const Args &, bool, unsigned, hipStream_t);
+extern template int launch_few<64, FP16>(const Args &, bool, unsigned, hipStream_t);
+extern template int launch_few<128, FP16>(const Args &, bool, unsigned, hipStream_t);
+
 static size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 
 struct Plan {
   int TQ, splits;
   long long blocks;  // blocks to launch
   bool one;          // one 16-row query tile a wave
+  bool few;          // few_rows_attention.hpp
   size_t part_bytes(long long tokens, int Hq, int D) const {
     return align256((size_t)splits * tokens * Hq * D * 4);
   }
@@ -32,6 +38,56 @@ struct Plan {
                              align256((size_t)splits * tokens * Hq * sizeof(float2));
   }
 };
+
+// Tiles that a query's keys are in.
+static int tiles_of(int max_keys, int window, int sinks, int queries) {
+  const int tiles = (int)std::max(1LL, ((long long)max_keys + kKT - 1) / kKT);
+  if (window <= 0) return tiles;
+  return (int)std::min<long long>(tiles, ((long long)window + queries + kKT - 2) / kKT + 1 +
+                                             ((long long)sinks + kKT - 1) / kKT);
+}
+
+// Few rows over e4m3 codes (few_rows_attention.hpp): the splits of the least time, as
+// measured in us over 1 to 128 sequences of 100 to 32768 keys: a work-group's start and
+// end, each round of its four waves' tiles beside the bytes at 5.4 TB/s (as the larger
+// of the two, and a fifth more where they are the same), and a merge.  One token
+// of 32 heads of 128 over 8, splits 1 / 4 / 16 / 32: one sequence of 8192 keys 59 / 23 /
+// 14.1 / 14.2, 16 of 2048 25 / 21 / 38 / 63, 64 of 2048 51 / 71 / 167 / 310.
+static Plan plan_few(long long tokens, long long longest, int B, int G, int Hkv, int D,
+                     int max_keys, int window, int sinks, int num_splits, bool tree) {
+  Plan p{};
+  p.few = true;
+  p.one = std::max<long long>(longest, 1) * G <= 16;
+  p.TQ = (int)std::max<long long>(longest, 1);
+  p.blocks = tree ? B : tokens / p.TQ + B;
+  const int tiles = tiles_of(max_keys, window, sinks, tree ? 64 : p.TQ);
+  if (num_splits > 0) {
+    p.splits = std::min(num_splits, tiles);
+    return p;
+  }
+  const double first = (D == 64 ? 4.5 : 5.0) + (p.one ? 0.0 : 2.5);
+  const double round = (D == 64 ? 1.5 : 2.1) + (p.one ? 0.0 : 0.4);
+  const long long items = Hkv * std::max<long long>(1, tree ? B : std::min<long long>(B, tokens));
+  const long long slots = (long long)abi::device_cu_count() * few_groups(D, p.one ? 1 : 2);
+  const double bytes = (double)items * tiles * kKT * D * 2 / 5.4e6;
+  const long long rounds = (tiles + kFewWaves - 1) / kFewWaves;
+  const double merged = (double)tokens * Hkv * G * D * 8 / 5.2e6;  // a split's sums
+  double least = 0.0;
+  for (long long n = 1;;) {
+    const long long waves = (items * n + slots - 1) / slots, per = (rounds + n - 1) / n;
+    const double time = waves * first + std::pow(std::pow(waves * round * per, 4) +
+                                                     std::pow(bytes, 4), 0.25) +
+                        (n > 1 ? 2.5 + (0.12 + merged) * n : 0.0);
+    if (p.splits == 0 || time < least) {
+      p.splits = (int)n;
+      least = time;
+    }
+    // (the next number of splits that makes them shorter)
+    if (per == 1 || items * n > 4 * slots) break;
+    n = (rounds + per - 2) / (per - 1);
+  }
+  return p;
+}
 
 // Query rows of a block (256 in two tiles a wave, or 128 or 64 in one) and splits of
 // the keys, by the time that they would take.  In us, as measured over prompts of 128
@@ -62,6 +118,8 @@ static Plan plan(long long tokens, long long longest, int B, int G, int Hkv, int
       {{kMaxRows, 4.5, 1.4, 1.0}, {kMaxRows / 2, 3.0, 1.0, 1.4}, {kRowsOneTile, 2.5, 0.84, 2.0}}};
   const double merged = (double)tokens * Hkv * G * D * 8 / 5.2e6;  // a split's bytes
   Plan p{};
+  if (e4m3 && std::max<long long>(longest, 1) * G <= kFewTiles * 16)
+    return plan_few(tokens, longest, B, G, Hkv, D, max_keys, window, sinks, num_splits, tree);
   double least = 0.0;
   for (int i = 0; i < 3; ++i) {
     const Rows &c = kRows[D == 64][i];
@@ -75,13 +133,9 @@ static Plan plan(long long tokens, long long longest, int B, int G, int Hkv, int
         tree ? blocks
              : std::max(tokens / TQ + std::min<long long>(B, tokens) / 2,
                         std::max<long long>(1, std::min<long long>(B, tokens)));
-    int tiles = (int)std::max(1LL, ((long long)max_keys + kKT - 1) / kKT);
+    const int tiles = tiles_of(max_keys, window, sinks, tree ? 64 : TQ);
     double mean = tiles;
-    if (window > 0)
-      mean = tiles = (int)std::min<long long>(
-          tiles, ((long long)window + (tree ? 64 : TQ) + kKT - 2) / kKT + 1 +
-                     ((long long)sinks + kKT - 1) / kKT);
-    else if (!tree)
+    if (window <= 0 && !tree)
       mean = std::max(1.0, tiles - 0.5 * (double)std::min<long long>(longest, max_keys) / kKT);
     const double cus = abi::device_cu_count(), items = (double)std::max(1LL, busy * Hkv);
     const double bytes = items * mean * kKT * D * (e4m3 ? 2 : 4) / 6e6;
@@ -146,6 +200,17 @@ static int check_pool(int num_blocks, int num_layers, int layer, int block_size,
   return CFA_OK;
 }
 
+template <class T>
+static int launch_heads(const Args &a, const Plan &p, int D, unsigned grid, hipStream_t st) {
+  if (p.few)
+    return D == 128 ? launch_few<128, T>(a, p.one, grid, st) : launch_few<64, T>(a, p.one, grid, st);
+  if (a.kscale)
+    return D == 128 ? launch<128, T, true>(a, p.one, grid, st)
+                    : launch<64, T, true>(a, p.one, grid, st);
+  return D == 128 ? launch<128, T, false>(a, p.one, grid, st)
+                  : launch<64, T, false>(a, p.one, grid, st);
+}
+
 static int run(Args &a, const Plan &p, int D, int fp16, float sm_scale, float soft_cap,
                void *workspace, size_t workspace_bytes, void *stream) {
   using namespace cfa::abi;
@@ -186,11 +251,7 @@ static int run(Args &a, const Plan &p, int D, int fp16, float sm_scale, float so
   a.past = (long long)p.splits * a.T * a.Hq * D * 4 <= 24LL << 20;
   hipStream_t st = (hipStream_t)stream;
   const unsigned g = (unsigned)grid;
-#define CFA_TYPES(E4M3)                                                                      \
-  (D == 128 ? fp16 ? launch<128, FP16, E4M3>(a, p.one, g, st) : launch<128, BF16, E4M3>(a, p.one, g, st) \
-            : fp16 ? launch<64, FP16, E4M3>(a, p.one, g, st) : launch<64, BF16, E4M3>(a, p.one, g, st))
-  return a.kscale ? CFA_TYPES(true) : CFA_TYPES(false);
-#undef CFA_TYPES
+  return fp16 ? launch_heads<FP16>(a, p, D, g, st) : launch_heads<BF16>(a, p, D, g, st);
 }
 
 // The pools, of q's type or of e4m3 codes with scales.

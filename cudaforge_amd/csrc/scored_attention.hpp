@@ -447,34 +447,34 @@ __device__ __forceinline__ void convert_codes(const uint8_t *kcodes, const uint8
   }
 }
 
-template <int D, int QT, class T, bool CAP, bool BIAS, bool FIXED, bool E4M3, bool SINKS>
-__global__ __launch_bounds__(kNT) void scored_attn_kernel(Args a) {
-  using Gm = Geo<D>;
-  constexpr int kTileBytes = Gm::kTileBytes;
-  constexpr int kLoadsPerTile = E4M3 ? CodeTransfers<D>::kLoads : Gm::kLoadsPerTile;
-  constexpr int kKStages = E4M3 ? kCodeStages : tree::kKStages;
-  constexpr int kVStages = E4M3 ? kCodeStages : tree::kVStages;
-  constexpr int kWaveBytes = CodeTransfers<D>::kWaveBytes;
-  __shared__ __align__(16) uint8_t kring[kKStages * kTileBytes];
-  __shared__ __align__(16) uint8_t vring[kVStages * kTileBytes];
-  __shared__ __align__(16) uint8_t codes[E4M3 ? kCodeStages * kWaves * kWaveBytes : 16];
-  __shared__ __align__(16) uint8_t scales[E4M3 ? kCodeStages * kWaves * 16 : 16];
-  // row offsets of the split's 16-key groups; a ring, refilled half a ring at a
-  // time in longer splits (its size, and the rows', let two work-groups of one
-  // query tile and head_dim 64 share a CU's LDS)
-  constexpr int kRing = D == 64 || E4M3 ? 512 : 1024;
-  __shared__ long long gtab[kRing];
-  __shared__ long long gpeek[kKT / 16];
-  // trees: how far node j's position lies from its slot, at 64 + j; 0 around them
-  __shared__ float smove[192];
-  __shared__ Row srow[QT == 1 ? kMaxRows / 2 : kMaxRows];
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int col = lane & 15, g = lane >> 4;
-  const int split = blockIdx.x % a.splits, rest = blockIdx.x / a.splits;
-  const int h = rest % a.Hkv;
+// What a work-group's queries see: its block, the keys, and the tiles of its split.
+struct View {
   Block blk;
-  if (!__builtin_amdgcn_readfirstlane(find_block(a, rest / a.Hkv, lane, blk))) return;
+  int rows;  // query rows
+  int ctx, nkeys;
+  int from;   // the first position that any row sees, but `sinks` first tokens in front
+  int sinks;  // of it
+  int least, most_first;  // keys below `least` are visible to all, but those in front of
+                          // the window, which ends at most_first at the latest
+  int ns, skip;           // tiles of first tokens, and how many lie behind them
+  int t0, t1, steps;
+  // tile i's first key
+  template <bool SINKS>
+  __device__ __forceinline__ int key_of(int i) const {
+    return (SINKS && i >= ns ? i + skip : i) * kKT;
+  }
+};
+
+// Fills v, and for the QT query tiles from row `row0` on the lane's rows (but their
+// `first` and `slope2`) and which of them there are; with a bias and a tree, waves 0 to
+// 2 fill smove.  False: no queries here.
+template <int QT, bool BIAS, bool SINKS>
+__device__ __forceinline__ bool look_round(const Args &a, int block, int split, int row0, int wave,
+                                           int lane, View &v, Row (&row)[QT], bool (&qvalid)[QT],
+                                           float *smove) {
+  const int col = lane & 15;
+  Block blk;
+  if (!__builtin_amdgcn_readfirstlane(find_block(a, block, lane, blk))) return false;
   // (the same in every lane; told to the compiler, since everything that steers
   // the loop and its transfers follows from them)
   blk.b = __builtin_amdgcn_readfirstlane(blk.b);
@@ -492,11 +492,6 @@ __global__ __launch_bounds__(kNT) void scored_attn_kernel(Args a) {
   const int ctx = min(max(blk.ctx, 0), tree ? max(cap_keys - last, 0) : 0x7fffffff - last);
   int nkeys = min(ctx + last, cap_keys);  // trees: cut behind the last visible node
 
-  Lane<D, QT, T> ln;
-  float base[QT];  // exponent bases
-  Row row[QT];
-  bool qvalid[QT];
-  ln.g = g;
   int low;  // the first query's position (trees: the shallowest's)
   if (tree) {
     const uint64_t nodes = a.N >= 64 ? ~0ull : ((1ull << a.N) - 1);
@@ -523,7 +518,7 @@ __global__ __launch_bounds__(kNT) void scored_attn_kernel(Args a) {
     nkeys = ctx + __builtin_amdgcn_readfirstlane(behind);
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
-      const int r = (wave * QT + qt) * 16 + col;
+      const int r = row0 + qt * 16 + col;
       qvalid[qt] = r < rows;
       const int node = j + (qvalid[qt] ? r / a.G : 0);
       const uint64_t anc = __shfl((unsigned long long)mine, node, 64);
@@ -534,7 +529,7 @@ __global__ __launch_bounds__(kNT) void scored_attn_kernel(Args a) {
     low = ctx + blk.i0;
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
-      const int r = (wave * QT + qt) * 16 + col;
+      const int r = row0 + qt * 16 + col;
       qvalid[qt] = r < rows;
       row[qt].pos = low + (qvalid[qt] ? r / a.G : 0);
       row[qt].anc = min(row[qt].pos + 1, nkeys);
@@ -562,9 +557,63 @@ __global__ __launch_bounds__(kNT) void scored_attn_kernel(Args a) {
   const int tps = (end - begin + a.splits - 1) / a.splits;
   const int t0 = begin + split * tps, t1 = min(end, t0 + tps);
   const int steps = SINKS || from < nkeys ? t1 - t0 : 0;
-  // a tile's first key
-  const int skip = SINKS ? tlo - ns : 0;
-  auto key_of = [&](int i) { return (SINKS && i >= ns ? i + skip : i) * kKT; };
+  v.blk = blk;
+  v.rows = rows;
+  v.ctx = ctx;
+  v.nkeys = nkeys;
+  v.from = from;
+  v.sinks = sinks;
+  v.least = least;
+  v.most_first = most_first;
+  v.ns = ns;
+  v.skip = SINKS ? tlo - ns : 0;
+  v.t0 = t0;
+  v.t1 = t1;
+  v.steps = steps;
+  return true;
+}
+
+template <int D, int QT, class T, bool CAP, bool BIAS, bool FIXED, bool E4M3, bool SINKS>
+__global__ __launch_bounds__(kNT) void scored_attn_kernel(Args a) {
+  using Gm = Geo<D>;
+  constexpr int kTileBytes = Gm::kTileBytes;
+  constexpr int kLoadsPerTile = E4M3 ? CodeTransfers<D>::kLoads : Gm::kLoadsPerTile;
+  constexpr int kKStages = E4M3 ? kCodeStages : tree::kKStages;
+  constexpr int kVStages = E4M3 ? kCodeStages : tree::kVStages;
+  constexpr int kWaveBytes = CodeTransfers<D>::kWaveBytes;
+  __shared__ __align__(16) uint8_t kring[kKStages * kTileBytes];
+  __shared__ __align__(16) uint8_t vring[kVStages * kTileBytes];
+  __shared__ __align__(16) uint8_t codes[E4M3 ? kCodeStages * kWaves * kWaveBytes : 16];
+  __shared__ __align__(16) uint8_t scales[E4M3 ? kCodeStages * kWaves * 16 : 16];
+  // row offsets of the split's 16-key groups; a ring, refilled half a ring at a
+  // time in longer splits (its size, and the rows', let two work-groups of one
+  // query tile and head_dim 64 share a CU's LDS)
+  constexpr int kRing = D == 64 || E4M3 ? 512 : 1024;
+  __shared__ long long gtab[kRing];
+  __shared__ long long gpeek[kKT / 16];
+  // trees: how far node j's position lies from its slot, at 64 + j; 0 around them
+  __shared__ float smove[192];
+  __shared__ Row srow[QT == 1 ? kMaxRows / 2 : kMaxRows];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane & 15, g = lane >> 4;
+  const int split = blockIdx.x % a.splits, rest = blockIdx.x / a.splits;
+  const int h = rest % a.Hkv;
+  Lane<D, QT, T> ln;
+  float base[QT];  // exponent bases
+  Row row[QT];
+  bool qvalid[QT];
+  ln.g = g;
+  View view;
+  if (!look_round<QT, BIAS, SINKS>(a, rest / a.Hkv, split, wave * QT * 16, wave, lane, view, row,
+                                   qvalid, smove))
+    return;
+  const Block &blk = view.blk;
+  const int b = blk.b, rows = view.rows, ctx = view.ctx, nkeys = view.nkeys;
+  const int from = view.from, sinks = view.sinks, least = view.least;
+  const int most_first = view.most_first, ns = view.ns, skip = view.skip;
+  const int t0 = view.t0, t1 = view.t1, steps = view.steps;
+  auto key_of = [&](int i) { return view.key_of<SINKS>(i); };
   constexpr float kLog2e = 1.4426950408889634f;
   const float cap2 = a.cap * kLog2e;
   // without a cap: score in log2 units = product * k0; with one: e^(2 s / cap)
@@ -647,7 +696,7 @@ __global__ __launch_bounds__(kNT) void scored_attn_kernel(Args a) {
   // bases before the first tile: from far to near, steep slopes would rescale
   // the outputs at every tile (the biased prompt of 8192 693 us against 546).
   const bool peek = BIAS && steps >= kPeekSteps;
-  if (peek && tid < kPerTile)
+  if (BIAS && tid < kPerTile)
     gpeek[tid] = group_row_offset<D, true>(a, btb, key_of(t1 - 1) / 16 + tid, nkeys, h, from, sinks);
   wait_vmcnt<0>();
   __syncthreads();
@@ -917,11 +966,9 @@ int launch_scores(const Args &a, unsigned grid, hipStream_t st) {
   return CFA_OK;
 }
 
-template <int D, class T, bool E4M3>
-int launch(const Args &a, bool one, unsigned grid, hipStream_t st) {
-  const int rc = one ? launch_scores<D, 1, T, E4M3>(a, grid, st)
-                     : launch_scores<D, 2, T, E4M3>(a, grid, st);
-  if (rc != CFA_OK || a.splits == 1) return rc;
+template <int D, class T>
+int launch_merge(const Args &a, hipStream_t st) {
+  if (a.splits == 1) return CFA_OK;
   const long long rows = (long long)a.T * a.Hq;
   const int per = 256 / (D / 4);
   const dim3 merges((unsigned)((rows + per - 1) / per));
@@ -930,6 +977,13 @@ int launch(const Args &a, bool one, unsigned grid, hipStream_t st) {
   else
     CFA_LAUNCH("scored_merge", (scored_merge_kernel<D, T, 8>), merges, dim3(256), 0, st, a);
   return CFA_OK;
+}
+
+template <int D, class T, bool E4M3>
+int launch(const Args &a, bool one, unsigned grid, hipStream_t st) {
+  const int rc = one ? launch_scores<D, 1, T, E4M3>(a, grid, st)
+                     : launch_scores<D, 2, T, E4M3>(a, grid, st);
+  return rc != CFA_OK ? rc : launch_merge<D, T>(a, st);
 }
 
 }  // namespace scored
