@@ -39,12 +39,16 @@
 //  * Keys in front of the window's first are not read: a tile's transfers are
 //    clamped to the first visible position of its rows (their pages may be
 //    gone or reused), and whole tiles in front of it are skipped.
-//  * A cache of e4m3 codes (e4m3.hpp) is turned into 16 bits once a work-group: the
-//    codes of a tile come into LDS as they are, three tiles ahead and each wave's own
-//    eight keys of K and V by itself, and in its score phase a wave writes them,
-//    scaled, to rings of three K and three V tiles in the layout that the products
-//    read.  (Operands converted where they are read would cost every wave of the
-//    eight 128 conversions a tile instead of 16, beside the scores' vector work.)
+//  * A cache of e4m3 codes (e4m3.hpp) is turned into 16 bits once a work-group.  Each
+//    wave takes eight keys of K and V of every tile into registers, a step ahead, and in
+//    its score phase writes them, scaled, to rings of three K and three V tiles in the
+//    layout that the products read.  (Operands converted where they are read would
+//    cost every wave of the eight 128 conversions a tile instead of 16; codes that come
+//    through LDS are written and read there once more, beside the operands' reads which
+//    are all that it gives: the prompt of 8192 600 us against 550.)  The row sums are
+//    then added up from the probabilities in fp32: the registers that the matrix unit
+//    would sum in are the ones that the codes need, and without them the compiler drops
+//    the schedule of the operand reads (660 us).
 //  * Splits are cut on the device, from each block's own first and last tile,
 //    and leave fp32 sums for a log-sum-exp merge.
 //
@@ -83,8 +87,7 @@ constexpr float kT0 = 0.9999994557706551f, kT1 = -0.3332631793391637f, kT2 = 0.1
 // cap log2(e) up to which exp2 needs no base: sums of 2^24 keys times values
 // of 2^20 stay below 2^127, and 2^-80 is a normal bf16
 constexpr float kFixedCap = 80.0f;
-// rings of a cache of e4m3 codes: 16-bit K and V tiles, and tiles of codes
-constexpr int kCodeStages = 3;
+constexpr int kCodeStages = 3;  // rings of K and V tiles that were e4m3 codes
 constexpr int kPeekSteps = 4;  // tiles of a split from which the last one is seen first
 
 struct Args {
@@ -318,16 +321,19 @@ __device__ __forceinline__ float score_max(const Scores<QT> &S, int qt) {
 
 // Scores of one tile to probabilities; the columns' lazy bases b (log2 units; 0:
 // none yet, where the sum is 0 too) where FIXED does not hold.
-template <int D, int QT, class T, bool FIXED>
+template <int D, int QT, class T, bool FIXED, bool LANES>
 __device__ __forceinline__ void score_phase(Scores<QT> &S, float (&b)[QT], f32x4 (&o)[QT][D / 16],
-                                            f32x4 (&lacc)[QT], Probs<QT, T> &P) {
+                                            f32x4 (&lacc)[QT], float (&sum)[QT], bool (&set)[QT],
+                                            Probs<QT, T> &P) {
   if constexpr (!FIXED) {
     float mx[QT];
     bool any = false;
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
       mx[qt] = score_max(S, qt);
-      const bool unset = b[qt] == 0.0f && lacc[qt][0] == 0.0f && mx[qt] > -INFINITY;
+      const bool unset =
+          (LANES ? !set[qt] : b[qt] == 0.0f && lacc[qt][0] == 0.0f) && mx[qt] > -INFINITY;
+      if constexpr (LANES) set[qt] = set[qt] || mx[qt] > -INFINITY;
       mx[qt] = mx[qt] > kRescaleSlack || unset ? mx[qt] : 0.0f;  // what the base moves by
       any |= mx[qt] != 0.0f;
     }
@@ -337,7 +343,8 @@ __device__ __forceinline__ void score_phase(Scores<QT> &S, float (&b)[QT], f32x4
         // (a base falls only while the sums are still 0)
         const float alpha = __builtin_amdgcn_exp2f(-fmaxf(mx[qt], 0.0f));
         b[qt] += mx[qt];
-        lacc[qt] *= alpha;
+        if constexpr (LANES) sum[qt] *= alpha;
+        else lacc[qt] *= alpha;
 #pragma unroll
         for (int dt = 0; dt < D / 16; ++dt) o[qt][dt] *= alpha;
 #pragma unroll
@@ -354,96 +361,66 @@ __device__ __forceinline__ void score_phase(Scores<QT> &S, float (&b)[QT], f32x4
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          P.p[qt][blk][t * 4 + i] =
-              (typename T::elem)__builtin_amdgcn_exp2f(S.s[qt][blk][t][i]);
+        for (int i = 0; i < 4; ++i) {
+          const float p = __builtin_amdgcn_exp2f(S.s[qt][blk][t][i]);
+          if constexpr (LANES) sum[qt] += p;
+          P.p[qt][blk][t * 4 + i] = (typename T::elem)p;
+        }
       // keep the exponentials in this phase (see tree_attention.hip)
       asm volatile("" ::"v"(P.p[qt][blk]));
     }
 }
 
-// A wave's share of a tile of codes: its eight keys' K rows and V rows, 16 D bytes
-// at `codes`, and their scale bytes, 8 and 8 at `scales`.
+// A wave's share of a tile of codes, 16 a lane: its eight keys' K rows and V rows of D
+// codes, one load of a lane each at head_dim 128 and one for both (the lower lanes K) at
+// 64, and the rows' scale bytes.
 template <int D>
-struct CodeTransfers {
-  static constexpr int kLoads = (D == 128 ? 2 : 1) + 1;  // a tile, each wave
-  static constexpr int kWaveBytes = 16 * D;
-  // row (0 .. 7: K, 8 .. 15: V) and 16-code chunk of lane `lane` of transfer j
-  static __device__ __forceinline__ int row(int lane, int j) { return 8 * j + lane / (D / 16); }
+struct Codes {
+  static constexpr int kLoads = D == 128 ? 2 : 1;
+  uint4 w[kLoads];
+  uint32_t byte[kLoads];
+  // key (in the wave's eight) and 16-code chunk of a lane; whether its load j is K's
+  static __device__ __forceinline__ int key(int lane) { return lane / (D / 16) & 7; }
   static __device__ __forceinline__ int chunk(int lane) { return lane % (D / 16); }
+  static __device__ __forceinline__ bool is_k(int lane, int j) {
+    return D == 128 ? j == 0 : lane < 32;
+  }
 };
 
-// Four bytes a lane, HBM -> LDS (dma16's small sister; lanes that are off do nothing).
-__device__ __forceinline__ void dma4(const void *src, CFA_LDS void *lds) {
-  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dword %0, off" ::"v"(src), "s"(lds)
-               : "memory");
-}
-
-// Issue them for the tile at kbase.  koff: the row offset of the 16-key group that
-// holds the wave's keys.  A key that clamp_pos moves re-reads another's codes.
+// Where in a 16-bit K or V tile a lane puts the first of the two 16-byte chunks of its
+// load j; the second lies at that ^ 16.  Lanes with bit 2 begin with their second half:
+// the eight lanes of a pass then meet all 32 banks once (a row's even chunks alone,
+// every second bank twice).
 template <int D>
-__device__ __forceinline__ void issue_codes(const Args &a, const long long *goff, int kbase, int from,
-                                            int sinks, int nkeys, uint8_t *codes, uint8_t *scales,
-                                            int wave, int lane) {
-  const long long off = uniform_i64(*goff);
-  const int group = kbase + 16 * (wave >> 1);
-  const int gstart = clamp_pos<true>(group, group, from, sinks, nkeys);
-#pragma unroll
-  for (int j = 0; j < CodeTransfers<D>::kLoads - 1; ++j) {
-    const int r = CodeTransfers<D>::row(lane, j);
-    const int pos = clamp_pos<true>(kbase + 8 * wave + (r & 7), group, from, sinks, nkeys);
-    const uint8_t *pool = (const uint8_t *)((D == 128 ? j == 0 : r < 8) ? a.kpool : a.vpool);
-    dma16(pool + off + ((pos - gstart) * D + CodeTransfers<D>::chunk(lane) * 16),
-          (CFA_LDS void *)(codes + j * 1024));
-  }
-  // (the group's bytes from its first slot on, whichever of its rows `off` points to)
-  if (lane < 4) {
-    const long long first = (off / D & ~15LL) + 8 * (wave & 1) + 4 * (lane & 1);
-    dma4((lane < 2 ? a.kscale : a.vscale) + first, (CFA_LDS void *)scales);
-  }
+__device__ __forceinline__ int codes_place(int wave, int lane, int j) {
+  const int key = 8 * wave + Codes<D>::key(lane);
+  const bool is_k = Codes<D>::is_k(lane, j);
+  const int row = is_k ? k_row_of_key(key) : key, swz = is_k ? k_swz<D>(row) : v_swz<D>(row);
+  return row * Geo<D>::kRowBytes +
+         (((2 * Codes<D>::chunk(lane) + (lane >> 2 & 1)) ^ swz) << 4);
 }
 
-// Sixteen codes to 16-bit chunks c and c + 1 of a tile's row.
-template <class T>
-__device__ __forceinline__ void put_codes(const uint4 &w, float scale, uint8_t *row, int c, int swz) {
-  uint4 lo, hi;
-  lo.x = e4m3::unpack_pair<T, false>(w.x, scale);
-  lo.y = e4m3::unpack_pair<T, true>(w.x, scale);
-  lo.z = e4m3::unpack_pair<T, false>(w.y, scale);
-  lo.w = e4m3::unpack_pair<T, true>(w.y, scale);
-  hi.x = e4m3::unpack_pair<T, false>(w.z, scale);
-  hi.y = e4m3::unpack_pair<T, true>(w.z, scale);
-  hi.z = e4m3::unpack_pair<T, false>(w.w, scale);
-  hi.w = e4m3::unpack_pair<T, true>(w.w, scale);
-  *reinterpret_cast<uint4 *>(row + ((c ^ swz) << 4)) = lo;
-  *reinterpret_cast<uint4 *>(row + (((c + 1) ^ swz) << 4)) = hi;
-}
-
-// The wave's share of tile `kt` (first key kbase_k) into the K ring's tile kdst and
-// of tile `vt` into vdst, each from its own tile of codes; null: not that one.  Keys
-// that were re-read become (nearly) zeros: the byte of their slot may be anything.
-template <int D, class T>
-__device__ __forceinline__ void convert_codes(const uint8_t *kcodes, const uint8_t *kscales,
-                                              int kbase_k, uint8_t *kdst, const uint8_t *vcodes,
-                                              const uint8_t *vscales, int kbase_v, uint8_t *vdst,
-                                              int from, int sinks, int nkeys, int wave, int lane) {
-  constexpr int RB = Geo<D>::kRowBytes;
+// The lane's codes to 16 bits, K's into kdst and (with V) V's into vdst.
+template <int D, class T, bool V>
+__device__ __forceinline__ void put_codes(const Codes<D> &c, const int (&place)[Codes<D>::kLoads],
+                                          uint8_t *kdst, uint8_t *vdst, int lane) {
+  const bool turned = lane & 4;
 #pragma unroll
-  for (int j = 0; j < CodeTransfers<D>::kLoads - 1; ++j) {
-    const int r = CodeTransfers<D>::row(lane, j), key = 8 * wave + (r & 7);
-    const bool is_k = D == 128 ? j == 0 : r < 8;
+  for (int j = 0; j < Codes<D>::kLoads; ++j) {
+    const bool is_k = Codes<D>::is_k(lane, j);
+    if (!V && !is_k) continue;
     uint8_t *const dst = is_k ? kdst : vdst;
-    if (!dst) continue;
-    const uint8_t *codes = is_k ? kcodes : vcodes, *scales = is_k ? kscales : vscales;
-    const int group = (is_k ? kbase_k : kbase_v) + (key & ~15);
-    const int pos = (is_k ? kbase_k : kbase_v) + key;
-    const uint4 w = *reinterpret_cast<const uint4 *>(codes + j * 1024 + lane * 16);
-    const uint32_t byte = scales[r];
-    const float scale =
-        clamp_pos<true>(pos, group, from, sinks, nkeys) == pos ? e4m3::scale(byte) : 0.0f;
-    const int at = is_k ? k_row_of_key(key) : key;
-    put_codes<T>(w, scale, dst + at * RB, 2 * CodeTransfers<D>::chunk(lane),
-                 is_k ? k_swz<D>(at) : v_swz<D>(at));
+    const uint4 w = c.w[j];
+    const float s = e4m3::scale(c.byte[j]);
+    const uint32_t w0 = turned ? w.z : w.x, w1 = turned ? w.w : w.y;
+    const uint32_t w2 = turned ? w.x : w.z, w3 = turned ? w.y : w.w;
+    const uint4 first = make_uint4(e4m3::unpack_pair<T, false>(w0, s), e4m3::unpack_pair<T, true>(w0, s),
+                                   e4m3::unpack_pair<T, false>(w1, s), e4m3::unpack_pair<T, true>(w1, s));
+    const uint4 second = make_uint4(
+        e4m3::unpack_pair<T, false>(w2, s), e4m3::unpack_pair<T, true>(w2, s),
+        e4m3::unpack_pair<T, false>(w3, s), e4m3::unpack_pair<T, true>(w3, s));
+    *reinterpret_cast<uint4 *>(dst + place[j]) = first;
+    *reinterpret_cast<uint4 *>(dst + (place[j] ^ 16)) = second;
   }
 }
 
@@ -577,14 +554,11 @@ template <int D, int QT, class T, bool CAP, bool BIAS, bool FIXED, bool E4M3, bo
 __global__ __launch_bounds__(kNT) void scored_attn_kernel(Args a) {
   using Gm = Geo<D>;
   constexpr int kTileBytes = Gm::kTileBytes;
-  constexpr int kLoadsPerTile = E4M3 ? CodeTransfers<D>::kLoads : Gm::kLoadsPerTile;
+  constexpr int kLoadsPerTile = Gm::kLoadsPerTile;
   constexpr int kKStages = E4M3 ? kCodeStages : tree::kKStages;
   constexpr int kVStages = E4M3 ? kCodeStages : tree::kVStages;
-  constexpr int kWaveBytes = CodeTransfers<D>::kWaveBytes;
   __shared__ __align__(16) uint8_t kring[kKStages * kTileBytes];
   __shared__ __align__(16) uint8_t vring[kVStages * kTileBytes];
-  __shared__ __align__(16) uint8_t codes[E4M3 ? kCodeStages * kWaves * kWaveBytes : 16];
-  __shared__ __align__(16) uint8_t scales[E4M3 ? kCodeStages * kWaves * 16 : 16];
   // row offsets of the split's 16-key groups; a ring, refilled half a ring at a
   // time in longer splits (its size, and the rows', let two work-groups of one
   // query tile and head_dim 64 share a CU's LDS)
@@ -655,27 +629,42 @@ __global__ __launch_bounds__(kNT) void scored_attn_kernel(Args a) {
     else
       issue_tile<D, true>(a, kt, vt, kbase, nkeys, kdst, vdst, wave, lane, from, sinks);
   };
-  // codes: this wave's parts of stage t % 3
-  auto codes_at = [&](int t) { return codes + ((t % kCodeStages) * kWaves + wave) * kWaveBytes; };
-  auto scales_at = [&](int t) { return scales + ((t % kCodeStages) * kWaves + wave) * 16; };
-  auto issue8_from = [&](const long long *tab, int u, int stage) {
-    issue_codes<D>(a, tab + (wave >> 1), key_of(t0 + u), from, sinks, nkeys, codes_at(stage),
-                   scales_at(stage), wave, lane);
+  // e4m3 codes: the lane's of K of the tile at kbase_k (group offsets at ktab) and of V of
+  // another (null: none)
+  int place[Codes<D>::kLoads];
+#pragma unroll
+  for (int j = 0; j < Codes<D>::kLoads; ++j) place[j] = codes_place<D>(wave, lane, j);
+  struct Rows {  // of a tile: its group's row offset (uniform), the lane's row in that
+    long long off;
+    int in;
   };
-  auto issue8 = [&](int u) { issue8_from(gtab + u * (kKT / 16) % kRing, u, u); };
-  // K of tile ku and V of tile vu (-1: none) to 16 bits; the writes are done behind it
-  auto convert = [&](int ku, int vu) {
-    convert_codes<D, T>(codes_at(ku), scales_at(ku), key_of(t0 + ku),
-                        ku < steps ? kring + (ku % kKStages) * kTileBytes : nullptr, codes_at(vu),
-                        scales_at(vu), key_of(t0 + vu),
-                        vu >= 0 && vu < steps ? vring + (vu % kVStages) * kTileBytes : nullptr, from,
-                        sinks, nkeys, wave, lane);
+  auto rows_of = [&](long long off, int kbase) {
+    Rows r;
+    r.off = uniform_i64(off);
+    const int key = 8 * wave + Codes<D>::key(lane);
+    r.in = key & 15;
+    if (!((kbase + kKT <= nkeys && kbase >= from) || (SINKS && kbase + kKT <= sinks))) {
+      const int group = kbase + (key & ~15);
+      r.in = clamp_pos<true>(kbase + key, group, from, sinks, nkeys) -
+             clamp_pos<true>(group, group, from, sinks, nkeys);
+    }
+    return r;
   };
-  // a wait for transfers that the same wave reads next
-  auto transfers_done = [&](bool but_one_tile) {
-    if (but_one_tile) wait_vmcnt<kLoadsPerTile>();
-    else wait_vmcnt<0>();
-    asm volatile("" ::: "memory");
+  auto load = [&](const Rows &k, const Rows &v, Codes<D> &c) {
+#pragma unroll
+    for (int j = 0; j < Codes<D>::kLoads; ++j) {
+      const bool is_k = Codes<D>::is_k(lane, j);
+      const long long off = is_k ? k.off : v.off;
+      const int in = is_k ? k.in : v.in;
+      const uint8_t *pool = (const uint8_t *)(is_k ? a.kpool : a.vpool) + off;
+      c.w[j] = *reinterpret_cast<const uint4 *>(pool + (uint32_t)(in * D + Codes<D>::chunk(lane) * 16));
+      c.byte[j] = ((is_k ? a.kscale : a.vscale) + off / D)[(uint32_t)in];
+    }
+  };
+  auto tile_off = [&](int u) { return gtab[u * (kKT / 16) % kRing + (wave >> 1)]; };
+  auto put = [&](int ku, int vu, const Codes<D> &c) {
+    put_codes<D, T, true>(c, place, kring + (ku % kKStages) * kTileBytes,
+                          vring + (vu % kVStages) * kTileBytes, lane);
   };
   auto writes_done = [&] { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); };
   auto issue = [&](int u, uint8_t *kdst, uint8_t *vdst) {
@@ -705,9 +694,12 @@ __global__ __launch_bounds__(kNT) void scored_attn_kernel(Args a) {
   f32x4 lacc[QT];
   const Row *const rows_at = srow + wave * QT * 16 + col;
   float zero[QT];
+  float sum[QT];   // e4m3: the lane's part of a row's sum, and whether its base is set
+  bool set[QT];
 #pragma unroll
   for (int qt = 0; qt < QT; ++qt) {
-    zero[qt] = 0.0f;
+    zero[qt] = sum[qt] = 0.0f;
+    set[qt] = false;
     lacc[qt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int dt = 0; dt < D / 16; ++dt) o[qt][dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -719,16 +711,29 @@ __global__ __launch_bounds__(kNT) void scored_attn_kernel(Args a) {
     if (!E4M3 && peek)
       issue_from(gpeek, steps - 1, kring + (kKStages - 1) * kTileBytes,
                  vring + (kVStages - 1) * kTileBytes);
+    // Tiles past the last are the last once more: nothing reads them, and with every load
+    // and store unconditional the compiler's waits are exact.
+    Codes<D> coming;
+    Rows krows;         // of the K that is coming
+    long long off = 0;  // of the next tile
+    auto tile = [&](int u) { return min(u, steps - 1); };
     if constexpr (E4M3) {
-      if (peek) {  // through the stages of tile 2
-        issue8_from(gpeek, steps - 1, 2);
-        transfers_done(false);
-        convert_codes<D, T>(codes_at(2), scales_at(2), key_of(t1 - 1),
-                            kring + (kKStages - 1) * kTileBytes, nullptr, nullptr, 0, nullptr, from,
-                            sinks, nkeys, wave, lane);
+      Codes<D> first, second;
+      if (peek) {
+        const Rows r = rows_of(gpeek[wave >> 1], key_of(t1 - 1));
+        load(r, r, coming);
+        put_codes<D, T, false>(coming, place, kring + (kKStages - 1) * kTileBytes, nullptr, lane);
         writes_done();
       }
-      for (int u = 0; u < min(3, steps); ++u) issue8(u);
+      const Rows r0 = rows_of(tile_off(0), key_of(t0));
+      const Rows r1 = rows_of(tile_off(tile(1)), key_of(t0 + tile(1)));
+      krows = rows_of(tile_off(tile(2)), key_of(t0 + tile(2)));
+      off = tile_off(tile(3));
+      load(r0, r0, first);
+      load(r1, r1, second);
+      load(krows, r1, coming);
+      put(0, 0, first);
+      put_codes<D, T, false>(second, place, kring + kTileBytes, nullptr, lane);
     } else {
       for (int u = 0; u < min(3, steps); ++u)
         issue(u, kring + (u % kKStages) * kTileBytes, vring + (u % kVStages) * kTileBytes);
@@ -747,16 +752,13 @@ __global__ __launch_bounds__(kNT) void scored_attn_kernel(Args a) {
           for (int qt = 0; qt < QT; ++qt) {
             const float m = score_max(S, qt);
             base[qt] = m > -INFINITY ? m : 0.0f;
+            set[qt] = m > -INFINITY;
           }
         }
         block_barrier();
       }
     }
     if constexpr (E4M3) {
-      transfers_done(steps >= 3);
-      convert(0, 0);
-      convert(1, -1);
-      if (steps > 3) issue8(3);
       writes_done();
     } else {
       const int later = min(3, steps) - 1;
@@ -783,9 +785,11 @@ __global__ __launch_bounds__(kNT) void scored_attn_kernel(Args a) {
         // between the two halves' phases the last reader of either ring's stage is
         // then done, and both halves' writes are in front of the first.
         block_barrier();
-        transfers_done(u + 3 < steps);
-        convert(u + 2, u + 1);
-        if (u + 4 < steps) issue8(u + 4);
+        const Rows vrows = krows;
+        krows = rows_of(off, key_of(t0 + tile(u + 3)));
+        put(u + 2, u + 1, coming);
+        load(krows, vrows, coming);
+        off = tile_off(tile(u + 4));
       } else {
         if (!lag) {
           block_barrier();
@@ -801,7 +805,7 @@ __global__ __launch_bounds__(kNT) void scored_attn_kernel(Args a) {
       if (busy) {
         raw_scores<D, QT, T, CAP, BIAS, FIXED, SINKS>(ln, base, a, k0, cap2, kbase, ctx, least, most_first,
                                                rows_at, smove + 64, S);
-        score_phase<D, QT, T, FIXED>(S, base, o, lacc, P);
+        score_phase<D, QT, T, FIXED, E4M3>(S, base, o, lacc, sum, set, P);
       }
       if constexpr (E4M3) {
         writes_done();
@@ -817,11 +821,18 @@ __global__ __launch_bounds__(kNT) void scored_attn_kernel(Args a) {
       __builtin_amdgcn_s_setprio(1);
       if (busy)
         // (one query tile has half the products per operand read)
-        mfma_phase<D, QT, T, QT == 1 ? 4 : 2>(ln, kring + ((u + 1) % kKStages) * kTileBytes,
+        mfma_phase<D, QT, T, QT == 1 ? 4 : 2, !E4M3, E4M3 ? 6 : 8>(ln, kring + ((u + 1) % kKStages) * kTileBytes,
                    vring + (u % kVStages) * kTileBytes, zero, P, S, o, lacc);
       __builtin_amdgcn_s_setprio(0);
     }
     if (!lag) block_barrier();
+  }
+  if constexpr (E4M3) {
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+      sum[qt] += __shfl_xor(sum[qt], 16, 64);
+      lacc[qt][0] = sum[qt] + __shfl_xor(sum[qt], 32, 64);
+    }
   }
 
   // Results pass the caches, since what these hold dirty at a kernel's end delays the
@@ -858,7 +869,7 @@ __global__ __launch_bounds__(kNT) void scored_attn_kernel(Args a) {
     }
     return;
   }
-  auto put = [&](f32x4 *at, f32x4 v) {
+  auto put_sums = [&](f32x4 *at, f32x4 v) {
     // (the empty asm keep the compiler from joining the two into a plain store)
     if (a.past) {
       asm volatile("");
@@ -878,7 +889,7 @@ __global__ __launch_bounds__(kNT) void scored_attn_kernel(Args a) {
     float *pp = a.part_o + prow * D;
 #pragma unroll
     for (int dt = 0; dt < D / 16; ++dt)
-      put(reinterpret_cast<f32x4 *>(pp + dt * 16 + 4 * g), o[qt][dt]);
+      put_sums(reinterpret_cast<f32x4 *>(pp + dt * 16 + 4 * g), o[qt][dt]);
     if (g == 0) a.part_ml[prow] = make_float2(ls != 0.0f ? base[qt] : -INFINITY, ls);
   }
 }

@@ -295,14 +295,14 @@ struct Softmax {
   bool valid[QT];
 };
 
-// MFMA phase of tile t: O^T += V_t^T P^T and l += 1^T P^T, then
+// MFMA phase of tile t: O^T += V_t^T P^T and (SUMS) l += 1^T P^T, then
 // S = K_{t+1} Q^T - b (tile t+1's scores; for the last tile the stage read is
 // stale and the result unused).  The QK products run k-slice outermost so
 // that eight independent accumulation chains interleave: a dependent MFMA
 // issued right behind its predecessor stalls the matrix pipe.  Lane (g, col)
 // reads V rows blk*32 + 8g + 0..7 at d = dt*16 + col through two transposed
 // 4x16 reads.
-template <int D, int QT, class E = BF16, int READS = 2>
+template <int D, int QT, class E = BF16, int READS = 2, bool SUMS = true, int AHEAD = 8>
 __device__ __forceinline__ void mfma_phase(const Lane<D, QT, E> &ln, const uint8_t *Knext, const uint8_t *Vs,
                                            const float *b, const Probs<QT, E> &P, Scores<QT> &S,
                                            f32x4 (&o)[QT][D / 16], f32x4 (&lacc)[QT]) {
@@ -315,11 +315,13 @@ __device__ __forceinline__ void mfma_phase(const Lane<D, QT, E> &ln, const uint8
   for (int qt = 0; qt < QT; ++qt) negb[qt] = f32x4{-b[qt], -b[qt], -b[qt], -b[qt]};
   // the column sums first: they read no LDS, so they cover the latency of
   // the phase's first operand reads (about 1.5%)
+  if constexpr (SUMS) {
 #pragma unroll
-  for (int blk = 0; blk < 2; ++blk)
+    for (int blk = 0; blk < 2; ++blk)
 #pragma unroll
-    for (int qt = 0; qt < QT; ++qt)
-      lacc[qt] = Mfma<E>::run(ones, P.p[qt][blk], lacc[qt]);
+      for (int qt = 0; qt < QT; ++qt)
+        lacc[qt] = Mfma<E>::run(ones, P.p[qt][blk], lacc[qt]);
+  }
 #pragma unroll
   for (int blk = 0; blk < 2; ++blk) {
 #pragma unroll
@@ -347,11 +349,11 @@ __device__ __forceinline__ void mfma_phase(const Lane<D, QT, E> &ln, const uint8
               Mfma<E>::run(kf, ln.qf[qt][kk], kk == 0 ? negb[qt] : S.s[qt][blk][T]);
       }
 #if CFA_TA_SGB
-  // software pipeline of the operand reads: four fragments ahead, then READS
-  // reads after every pair of MFMAs
-  __builtin_amdgcn_sched_group_barrier(0x0100, 8, 0);
+  // software pipeline of the operand reads: AHEAD of them (four fragments) first, then
+  // READS reads after every pair of MFMAs
+  __builtin_amdgcn_sched_group_barrier(0x0100, AHEAD, 0);
 #pragma unroll
-  for (int j = 0; j < Geo<D, QT>::kMfma / 2; ++j) {
+  for (int j = 0; j < (Geo<D, QT>::kMfma - (SUMS ? 0 : 2 * QT)) / 2; ++j) {
     __builtin_amdgcn_sched_group_barrier(0x0008, 2, 0);
     __builtin_amdgcn_sched_group_barrier(0x0100, READS, 0);
   }
