@@ -622,8 +622,9 @@ __global__ __launch_bounds__(kNT) void scored_attn_kernel(Args a) {
   const DmaOffs<D> doff = dma_offsets<D>(wave, lane);
   auto issue_from = [&](const long long *tab, int u, uint8_t *kdst, uint8_t *vdst) {
     const int kbase = key_of(t0 + u);
-    const long long *kt = tab + 2 * (wave >> 2) + (wave & 1);
-    const long long *vt = tab + (wave >> 1);
+    // (read here, in front of the branch)
+    const long long koff = tab[2 * (wave >> 2) + (wave & 1)], voff = tab[wave >> 1];
+    const long long *kt = &koff, *vt = &voff;
     if ((kbase + kKT <= nkeys && kbase >= from) || (SINKS && kbase + kKT <= sinks))
       issue_tile_full<D>(a, kt, vt, doff, kdst, vdst, wave);
     else

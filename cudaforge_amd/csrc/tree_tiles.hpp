@@ -106,8 +106,9 @@ __device__ __forceinline__ int v_swz(int key) {
 template <bool kFrom>
 __device__ __forceinline__ int clamp_pos(int pos, int group, int from, int sinks, int nkeys) {
   pos = min(pos, nkeys - 1);
-  if (!kFrom || pos >= from || (uint32_t)pos < (uint32_t)sinks) return pos;
-  return group < sinks ? sinks - 1 : from;
+  if (!kFrom || (uint32_t)pos < (uint32_t)sinks) return pos;
+  // (without first tokens one instruction)
+  return (uint32_t)group < (uint32_t)sinks && pos < from ? sinks - 1 : max(pos, from);
 }
 
 // Pool element offset of the row holding position gstart = clamp_pos(16 gi),
