@@ -145,6 +145,27 @@ __device__ __forceinline__ void angle(const Args &a, int p, uint64_t turns, floa
   sn = a.factor * __builtin_amdgcn_sinf(f);
 }
 
+// The same to about a rounding, for what becomes codes: an e4m3 code moves a whole step of
+// 2^-3 where its value crosses a boundary, so errors of the arithmetic are kept below the
+// values' own roundings.  The turn less its nearest quarter is exact in integers; over
+// [-1/8, 1/8] turns sin(2 pi f) / f and cos(2 pi f) are polynomials in f^2, fitted for the
+// least relative error (2^-28 and 2^-34).
+__device__ __forceinline__ void fine_angle(const Args &a, int p, uint64_t turns, float &cs,
+                                           float &sn) {
+  const uint32_t turn = (uint32_t)((turns * (uint64_t)(int64_t)p) >> 32);
+  const uint32_t quarter = (turn + 0x20000000u) >> 30;
+  const float f = (float)(int32_t)(turn - (quarter << 30)) * 0x1p-32f;
+  const float z = f * f;
+  const float sine =
+      f * (0x1.921fb6p+2f + z * (-0x1.4abbbap+5f + z * (0x1.465e92p+6f + z * -0x1.2d9302p+6f)));
+  const float cosine =
+      1.0f + z * (-0x1.3bd3ccp+4f + z * (0x1.03c1dap+6f + z * (-0x1.55c4eap+6f + z * 0x1.d99f54p+5f)));
+  const float along = a.factor * (quarter & 1 ? sine : cosine);
+  const float across = a.factor * (quarter & 1 ? cosine : sine);
+  cs = (quarter + 1) & 2 ? -along : along;
+  sn = quarter & 2 ? -across : across;
+}
+
 // One wave = one token and `rounds` times ITER * 64 / LPR consecutive rows of its
 // Hq q heads, Hkv k heads and Hkv v heads.
 template <class T, int LPR, int LAYOUT, int ITER, bool E4M3>
@@ -179,28 +200,41 @@ __global__ __launch_bounds__(kWaves * 64) void qk_norm_rope_kv_kernel(Args a) {
   // this lane's cosines and sines: c[i], s[i] of element e + i, the sine with
   // the sign that its partner's value takes
   float c[8], s[8], wq[8], wk[8];
+  uint32_t fine[8];  // what fine_angle's differ by, as bf16 pairs (2^-31 of the value)
   const int half = a.R / 2;
   const int p = a.pos[t];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     c[i] = 1.0f;
     s[i] = 0.0f;
+    fine[i] = 0;
   }
+  // element e + i (and its pair's second, of neighbours) at a pair's frequency
+  auto angles = [&](uint64_t turns, int i, bool front) {
+    float cs, sn, csf, snf;
+    angle(a, p, turns, cs, sn);
+    c[i] = cs;
+    s[i] = front ? -sn : sn;
+    if constexpr (LAYOUT == kNeighbours) {
+      c[i + 1] = cs;
+      s[i + 1] = sn;
+    }
+    if constexpr (E4M3) {
+      fine_angle(a, p, turns, csf, snf);
+      fine[i] = pack2<BF16>(csf - cs, front ? sn - snf : snf - sn);
+      if constexpr (LAYOUT == kNeighbours) fine[i + 1] = pack2<BF16>(csf - cs, snf - sn);
+    }
+  };
   if constexpr (LAYOUT == kNeighbours) {
     if (e + 8 <= a.R) {
       uint64_t f[4];
       turns_at<4>(a, e / 2, f);
 #pragma unroll
-      for (int i = 0; i < 8; i += 2) angle(a, p, f[i / 2], c[i], s[i + 1]);
+      for (int i = 0; i < 8; i += 2) angles(f[i / 2], i, true);
     } else {
 #pragma unroll
       for (int i = 0; i < 8; i += 2)
-        if (e + i < a.R) angle(a, p, a.turns[(e + i) / 2], c[i], s[i + 1]);
-    }
-#pragma unroll
-    for (int i = 0; i < 8; i += 2) {
-      c[i + 1] = c[i];
-      s[i] = -s[i + 1];
+        if (e + i < a.R) angles(a.turns[(e + i) / 2], i, true);
     }
   } else if constexpr (LAYOUT == kHalf) {
     if (e < a.R) {  // a lane's eight lie in one half
@@ -208,18 +242,14 @@ __global__ __launch_bounds__(kWaves * 64) void qk_norm_rope_kv_kernel(Args a) {
       uint64_t f[8];
       turns_at<8>(a, first ? e : e - half, f);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        angle(a, p, f[i], c[i], s[i]);
-        s[i] = first ? -s[i] : s[i];
-      }
+      for (int i = 0; i < 8; ++i) angles(f[i], i, first);
     }
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       if (e + i < a.R) {
         const bool first = e + i < half;
-        angle(a, p, a.turns[first ? e + i : e + i - half], c[i], s[i]);
-        if (first) s[i] = -s[i];
+        angles(a.turns[first ? e + i : e + i - half], i, first);
       }
     }
   }
@@ -277,35 +307,47 @@ __global__ __launch_bounds__(kWaves * 64) void qk_norm_rope_kv_kernel(Args a) {
       }
       // (elements behind the rotated ones are selected, not turned by 0: they
       // may be infinite)
-      auto turn = [&] {
+      auto turn = [&](const float(&c)[8], const float(&s)[8]) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] = e + i < a.R ? x[i] * c[i] + y[i] * s[i] : x[i];
       };
+      // (the wave's q rows alone need no scale; theirs are the 16-bit caches' bits)
+      const int last = row0 - lane / LPR + (round * ITER + it) * RPW + RPW - 1;
+      const bool codes = E4M3 && __builtin_amdgcn_readfirstlane(last) >= a.Hq;
       if constexpr (E4M3) {
-        // the whole group finds the row's scale
-        turn();
-        if (is_v) unpack8<T>(raw[it], x);
-        uint32_t top = 0;
+        if (codes) {
+          float cr[8], sr[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) top = max(top, mine ? e4m3::magnitude(x[i]) : 0u);
-        const uint32_t byte = e4m3::scale_byte(group_max<LPR>(top));
-        if (row < H && mine && !is_q) {
-          if (!mapped) continue;
-          const float inv = e4m3::inverse_scale(byte);
+          for (int i = 0; i < 8; ++i) {
+            unpack2<BF16>(is_q ? 0u : fine[i], cr[i], sr[i]);
+            cr[i] += c[i];
+            sr[i] += s[i];
+          }
+          turn(cr, sr);
+          // the whole group finds the row's scale
+          if (is_v) unpack8<T>(raw[it], x);
+          uint32_t top = 0;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) x[i] = e4m3::codable<T>(x[i]) * inv;
-          const long long head = is_v ? row - a.Hq - a.Hkv : row - a.Hq;
-          uint2 w;
-          w.x = e4m3::pack4(x[0], x[1], x[2], x[3]);
-          w.y = e4m3::pack4(x[4], x[5], x[6], x[7]);
-          *reinterpret_cast<uint2 *>((uint8_t *)(is_v ? a.vc : a.kc) + head * a.head_stride + at +
-                                     e) = w;
-          if (l == 0) (is_v ? a.vs : a.ks)[head * a.bs + at_scale] = (uint8_t)byte;
-          continue;
+          for (int i = 0; i < 8; ++i) top = max(top, mine ? e4m3::magnitude(x[i]) : 0u);
+          const uint32_t byte = e4m3::scale_byte(group_max<LPR>(top));
+          if (row < H && mine && !is_q) {
+            if (!mapped) continue;
+            const float inv = e4m3::inverse_scale(byte);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = e4m3::codable<T>(x[i]) * inv;
+            const long long head = is_v ? row - a.Hq - a.Hkv : row - a.Hq;
+            uint2 w;
+            w.x = e4m3::pack4(x[0], x[1], x[2], x[3]);
+            w.y = e4m3::pack4(x[4], x[5], x[6], x[7]);
+            *reinterpret_cast<uint2 *>((uint8_t *)(is_v ? a.vc : a.kc) + head * a.head_stride +
+                                       at + e) = w;
+            if (l == 0) (is_v ? a.vs : a.ks)[head * a.bs + at_scale] = (uint8_t)byte;
+            continue;
+          }
         }
       }
       if (row >= H || !mine) continue;
-      if constexpr (!E4M3) turn();
+      if (!codes) turn(c, s);
       uint32_t w[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) w[i] = pack2<T>(x[2 * i], x[2 * i + 1]);
