@@ -22,8 +22,12 @@
 // pair is one exchange between two of its lanes.  A wave keeps one token, so
 // that its angles and the norms' weights are formed once for its heads.  8149
 // tokens of 48 heads of 128: 51 us, 3.9 TB/s (pages scattered, 256 bytes a row); 504
-// tokens 7 us, 8 tokens 5.
+// tokens 7 us, 8 tokens 5.  Into e4m3 pages (184 MB): 68 us for the 8149, 6 for 8, with
+// keys in 64 bits.  In fp32 56 to 60, but then 12 to 26 of 8.4 million codes were other
+// than their exact values', against 0 or 1.
 #include <hip/hip_runtime.h>
+
+#include <type_traits>
 
 #include "abi_internal.hpp"
 #include "e4m3.hpp"
@@ -54,7 +58,8 @@ struct Args {
   int num_blocks, max_blocks, bs;
   const int32_t *block_tables, *base;
   long long blk_stride, layer_off, head_stride;  // elements
-  int chunks, rounds;  // waves a token; rounds of rows a wave
+  int chunks, rounds;        // waves a token; rounds of rows a wave
+  int kv_chunks, kv_rounds;  // e4m3: the same of its k and v rows, `chunks` of its q rows
 };
 
 // Sum over the LPR lanes of a head, every lane gets it.
@@ -68,6 +73,13 @@ __device__ __forceinline__ float group_sum(float v) {
   if constexpr (LPR >= 16) CFA_DPP(0x140);  // mirrored in 16 lanes: the other 8
 #undef CFA_DPP
   if constexpr (LPR >= 32) v += __shfl_xor(v, 16, 64);
+  return v;
+}
+
+template <int LPR>
+__device__ __forceinline__ double group_sum(double v) {
+#pragma unroll
+  for (int d = 1; d < LPR; d *= 2) v += __shfl_xor(v, d, 64);
   return v;
 }
 
@@ -145,39 +157,70 @@ __device__ __forceinline__ void angle(const Args &a, int p, uint64_t turns, floa
   sn = a.factor * __builtin_amdgcn_sinf(f);
 }
 
-// The same to about a rounding, for what becomes codes: an e4m3 code moves a whole step of
-// 2^-3 where its value crosses a boundary, so errors of the arithmetic are kept below the
-// values' own roundings.  The turn less its nearest quarter is exact in integers; over
-// [-1/8, 1/8] turns sin(2 pi f) / f and cos(2 pi f) are polynomials in f^2, fitted for the
-// least relative error (2^-28 and 2^-34).
-__device__ __forceinline__ void fine_angle(const Args &a, int p, uint64_t turns, float &cs,
-                                           float &sn) {
+// The same to 2^-30, for what becomes codes: there a rounding on the way in can move the
+// result by a whole step of 2^-3, so keys are formed in 64 bits and rounded once.  The turn less its nearest quarter is
+// exact in integers; over [-1/8, 1/8] turns sin(2 pi f) / f and cos(2 pi f) are
+// polynomials in f^2, fitted for the least relative error (2^-37 and 2^-34).
+__device__ __forceinline__ void fine_angle(const Args &a, int p, uint64_t turns, double &cs,
+                                           double &sn) {
   const uint32_t turn = (uint32_t)((turns * (uint64_t)(int64_t)p) >> 32);
   const uint32_t quarter = (turn + 0x20000000u) >> 30;
-  const float f = (float)(int32_t)(turn - (quarter << 30)) * 0x1p-32f;
-  const float z = f * f;
-  const float sine =
-      f * (0x1.921fb6p+2f + z * (-0x1.4abbbap+5f + z * (0x1.465e92p+6f + z * -0x1.2d9302p+6f)));
-  const float cosine =
-      1.0f + z * (-0x1.3bd3ccp+4f + z * (0x1.03c1dap+6f + z * (-0x1.55c4eap+6f + z * 0x1.d99f54p+5f)));
-  const float along = a.factor * (quarter & 1 ? sine : cosine);
-  const float across = a.factor * (quarter & 1 ? cosine : sine);
+  const double f = (double)(int32_t)(turn - (quarter << 30)) * 0x1p-32;
+  const double z = f * f;
+  const double sine =
+      f * (6.283185307151002 +
+           z * (-41.341702150556394 +
+                z * (81.60520380748551 + z * (-76.69777415285763 + z * 41.46989043587605))));
+  const double cosine =
+      0.9999999999439374 +
+      z * (-19.739208633036213 +
+           z * (64.9393107446243 + z * (-85.44229797458063 + z * 59.202796144154824)));
+  const double along = (double)a.factor * (quarter & 1 ? sine : cosine);
+  const double across = (double)a.factor * (quarter & 1 ? cosine : sine);
   cs = (quarter + 1) & 2 ? -along : along;
   sn = quarter & 2 ? -across : across;
 }
 
+// 1 / sqrt(mean) in 64 bits: the fp32 root and a step of Newton's (none where that is 0
+// or infinite).
+__device__ __forceinline__ double fine_rsqrt(double mean) {
+  const float r = rsqrtf((float)mean);
+  if (!(r > 0.0f && r < INFINITY)) return r;
+  return r + 0.5 * r * (1.0 - mean * r * r);
+}
+
+// v as fp32, rounded to odd: toward zero, with the last bit set where bits were lost, so
+// that the code's rounding behind it is v's own (no second rounding to a tie).
+__device__ __forceinline__ float round_to_odd(double v) {
+  const float f = (float)v;
+  const double d = f;
+  uint32_t w = __float_as_uint(f);
+  w -= __builtin_fabs(d) > __builtin_fabs(v) ? 1u : 0u;
+  w |= d != v ? 1u : 0u;
+  return __uint_as_float(w);
+}
+
 // One wave = one token and `rounds` times ITER * 64 / LPR consecutive rows of its
-// Hq q heads, Hkv k heads and Hkv v heads.
+// Hq q heads, Hkv k heads and Hkv v heads.  With e4m3 pools q rows, in the 16-bit caches'
+// arithmetic (and bits) whatever the cache, and k and v rows are different waves', which
+// then hold one kind of angles and weights each: four waves a SIMD, where both take 142
+// registers (three waves; without the bound 131: 90 us against 81 with kv_gather's).
 template <class T, int LPR, int LAYOUT, int ITER, bool E4M3>
-__global__ __launch_bounds__(kWaves * 64) void qk_norm_rope_kv_kernel(Args a) {
+__global__ __launch_bounds__(kWaves * 64, E4M3 && LAYOUT != kHalfAny ? 4 : 1) void
+qk_norm_rope_kv_kernel(Args a) {
   constexpr int RPW = 64 / LPR;
   const int lane = threadIdx.x & 63, l = lane % LPR;
   const long long item = (long long)blockIdx.x * kWaves + (threadIdx.x >> 6);
-  const int t = (int)(item / a.chunks), chunk = (int)(item % a.chunks);
+  const int all = a.chunks + (E4M3 ? a.kv_chunks : 0);
+  const int t = (int)(item / all), chunk = (int)(item % all);
   if (t >= a.T) return;
-  const int e = 8 * l, H = a.Hq + 2 * a.Hkv;
+  const int e = 8 * l;
+  const bool kv = E4M3 && __builtin_amdgcn_readfirstlane(chunk) >= a.chunks;
+  const int rounds = kv ? a.kv_rounds : a.rounds;
+  const int H = E4M3 && !kv ? a.Hq : a.Hq + 2 * a.Hkv;  // the wave's rows end here
   const bool mine = e < a.D;
-  const int row0 = chunk * a.rounds * ITER * RPW + lane / LPR;
+  const int row0 = (kv ? a.Hq + (chunk - a.chunks) * rounds * ITER * RPW
+                       : chunk * rounds * ITER * RPW) + lane / LPR;
 
   uint4 raw[ITER];
   auto load = [&](int round) {
@@ -197,66 +240,8 @@ __global__ __launch_bounds__(kWaves * 64) void qk_norm_rope_kv_kernel(Args a) {
   load(0);
   int b, j;
   if (!place_token(a, t, lane, b, j)) return;
-  // this lane's cosines and sines: c[i], s[i] of element e + i, the sine with
-  // the sign that its partner's value takes
-  float c[8], s[8], wq[8], wk[8];
-  uint32_t fine[8];  // what fine_angle's differ by, as bf16 pairs (2^-31 of the value)
   const int half = a.R / 2;
   const int p = a.pos[t];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    c[i] = 1.0f;
-    s[i] = 0.0f;
-    fine[i] = 0;
-  }
-  // element e + i (and its pair's second, of neighbours) at a pair's frequency
-  auto angles = [&](uint64_t turns, int i, bool front) {
-    float cs, sn, csf, snf;
-    angle(a, p, turns, cs, sn);
-    c[i] = cs;
-    s[i] = front ? -sn : sn;
-    if constexpr (LAYOUT == kNeighbours) {
-      c[i + 1] = cs;
-      s[i + 1] = sn;
-    }
-    if constexpr (E4M3) {
-      fine_angle(a, p, turns, csf, snf);
-      fine[i] = pack2<BF16>(csf - cs, front ? sn - snf : snf - sn);
-      if constexpr (LAYOUT == kNeighbours) fine[i + 1] = pack2<BF16>(csf - cs, snf - sn);
-    }
-  };
-  if constexpr (LAYOUT == kNeighbours) {
-    if (e + 8 <= a.R) {
-      uint64_t f[4];
-      turns_at<4>(a, e / 2, f);
-#pragma unroll
-      for (int i = 0; i < 8; i += 2) angles(f[i / 2], i, true);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; i += 2)
-        if (e + i < a.R) angles(a.turns[(e + i) / 2], i, true);
-    }
-  } else if constexpr (LAYOUT == kHalf) {
-    if (e < a.R) {  // a lane's eight lie in one half
-      const bool first = e < half;
-      uint64_t f[8];
-      turns_at<8>(a, first ? e : e - half, f);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) angles(f[i], i, first);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if (e + i < a.R) {
-        const bool first = e + i < half;
-        angles(a.turns[first ? e + i : e + i - half], i, first);
-      }
-    }
-  }
-  if (mine) {
-    weights8<T>(a.q_w, a.w_f32, e, wq);
-    weights8<T>(a.k_w, a.w_f32, e, wk);
-  }
   // the page of this token's slot
   const long long slot = (long long)a.base[b] + j;
   const long long page = slot / a.bs;
@@ -264,107 +249,180 @@ __global__ __launch_bounds__(kWaves * 64) void qk_norm_rope_kv_kernel(Args a) {
   if (slot >= 0 && page < a.max_blocks) blk = a.block_tables[(long long)b * a.max_blocks + page];
   const bool mapped = blk >= 0 && blk < a.num_blocks;
   const long long at = blk * a.blk_stride + a.layer_off + (slot - page * a.bs) * a.D;
-  const long long at_scale = E4M3 ? at / a.D : 0;
-
-  for (int round = 0; round < a.rounds; ++round) {
+  // of the partners' p
+  auto exchange = [&](const float(&p)[8], float(&y)[8]) {
+    if constexpr (LAYOUT == kHalf) {
+      // R / 2 is a multiple of 8: the partner's elements are one lane's
+      const int to = e < half ? lane + half / 8 : (e < a.R ? lane - half / 8 : lane);
 #pragma unroll
-    for (int it = 0; it < ITER; ++it) {
-      const int row = row0 + (round * ITER + it) * RPW;
-      const bool is_q = row < a.Hq, is_v = row >= a.Hq + a.Hkv;
-      float x[8], y[8];
-      unpack8<T>(raw[it], x);
-      float ss = 0.0f;
+      for (int i = 0; i < 8; ++i) y[i] = __shfl(p[i], to, 64);
+    } else if constexpr (LAYOUT == kHalfAny) {
+      // element by element: partner e + i +- R / 2, in lane (e + i +- R / 2) / 8
 #pragma unroll
-      for (int i = 0; i < 8; ++i) ss += x[i] * x[i];
-      ss = group_sum<LPR>(ss);
-      const bool norm = (is_q ? a.q_w : a.k_w) != nullptr;
-      const float inv = norm ? rsqrtf(ss / (float)a.D + a.eps) : 1.0f;
+      for (int i = 0; i < 8; ++i) {
+        const int el = e + i;
+        const int pe = el < half ? el + half : (el < a.R ? el - half : el);
+        const int from = lane - l + pe / 8;
+        float v = 0.0f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] *= inv * (is_q ? wq[i] : wk[i]);
-      if constexpr (LAYOUT == kHalf) {
-        // R / 2 is a multiple of 8: the partner's elements are one lane's
-        const int to = e < half ? lane + half / 8 : (e < a.R ? lane - half / 8 : lane);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = __shfl(x[i], to, 64);
-      } else if constexpr (LAYOUT == kHalfAny) {
-        // element by element: partner e + i +- R / 2, in lane (e + i +- R / 2) / 8
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int el = e + i;
-          const int pe = el < half ? el + half : (el < a.R ? el - half : el);
-          const int from = lane - l + pe / 8;
-          float v = 0.0f;
-#pragma unroll
-          for (int m = 0; m < 8; ++m) {
-            const float got = __shfl(x[m], from, 64);
-            if (pe % 8 == m) v = got;
-          }
-          y[i] = v;
+        for (int m = 0; m < 8; ++m) {
+          const float got = __shfl(p[m], from, 64);
+          if (pe % 8 == m) v = got;
         }
+        y[i] = v;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = p[i ^ 1];
+    }
+  };
+
+  auto pass = [&](auto codes) {
+    constexpr bool CODES = decltype(codes)::value;
+    // this lane's cosines and sines: c[i], s[i] of element e + i, the sine with
+    // the sign that its partner's value takes
+    float c[8], s[8], wq[8], wk[8];
+    uint32_t fine[8];  // what fine_angle's differ by, as bf16 pairs (2^-31 of the value)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      c[i] = 1.0f;
+      s[i] = 0.0f;
+      fine[i] = 0;
+    }
+    // element e + i (and its pair's second, of neighbours) at a pair's frequency
+    auto angles = [&](uint64_t turns, int i, bool front) {
+      float cs, sn;
+      angle(a, p, turns, cs, sn);
+      c[i] = cs;
+      s[i] = front ? -sn : sn;
+      if constexpr (LAYOUT == kNeighbours) {
+        c[i + 1] = cs;
+        s[i + 1] = sn;
+      }
+      if constexpr (CODES) {
+        double csf, snf;
+        fine_angle(a, p, turns, csf, snf);
+        const float dc = (float)(csf - cs), ds = (float)(snf - sn);
+        fine[i] = pack2<BF16>(dc, front ? -ds : ds);
+        if constexpr (LAYOUT == kNeighbours) fine[i + 1] = pack2<BF16>(dc, ds);
+      }
+    };
+    if constexpr (LAYOUT == kNeighbours) {
+      if (e + 8 <= a.R) {
+        uint64_t f[4];
+        turns_at<4>(a, e / 2, f);
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) angles(f[i / 2], i, true);
       } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = x[i ^ 1];
+        for (int i = 0; i < 8; i += 2)
+          if (e + i < a.R) angles(a.turns[(e + i) / 2], i, true);
       }
-      // (elements behind the rotated ones are selected, not turned by 0: they
-      // may be infinite)
-      auto turn = [&](const float(&c)[8], const float(&s)[8]) {
+    } else if constexpr (LAYOUT == kHalf) {
+      if (e < a.R) {  // a lane's eight lie in one half
+        const bool first = e < half;
+        uint64_t f[8];
+        turns_at<8>(a, first ? e : e - half, f);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = e + i < a.R ? x[i] * c[i] + y[i] * s[i] : x[i];
-      };
-      // (the wave's q rows alone need no scale; theirs are the 16-bit caches' bits)
-      const int last = row0 - lane / LPR + (round * ITER + it) * RPW + RPW - 1;
-      const bool codes = E4M3 && __builtin_amdgcn_readfirstlane(last) >= a.Hq;
-      if constexpr (E4M3) {
-        if (codes) {
-          float cr[8], sr[8];
+        for (int i = 0; i < 8; ++i) angles(f[i], i, first);
+      }
+    } else {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            unpack2<BF16>(is_q ? 0u : fine[i], cr[i], sr[i]);
-            cr[i] += c[i];
-            sr[i] += s[i];
+      for (int i = 0; i < 8; ++i) {
+        if (e + i < a.R) {
+          const bool first = e + i < half;
+          angles(a.turns[first ? e + i : e + i - half], i, first);
+        }
+      }
+    }
+    if (mine) {
+      if constexpr (!CODES) weights8<T>(a.q_w, a.w_f32, e, wq);
+      if constexpr (CODES || !E4M3) weights8<T>(a.k_w, a.w_f32, e, wk);
+    }
+
+    for (int round = 0; round < rounds; ++round) {
+#pragma unroll
+      for (int it = 0; it < ITER; ++it) {
+        const int row = row0 + (round * ITER + it) * RPW;
+        const bool is_q = row < a.Hq, is_v = row >= a.Hq + a.Hkv;
+        float x[8], y[8];
+        unpack8<T>(raw[it], x);
+        // (elements behind the rotated ones are selected, not turned by 0: they may be
+        // infinite)
+        if constexpr (CODES) {
+          if (__builtin_amdgcn_readfirstlane(row - lane / LPR) < a.Hq + a.Hkv) {  // keys
+            double ss = 0.0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) ss += (double)(x[i] * x[i]);
+            const double inv =
+                a.k_w ? fine_rsqrt(group_sum<LPR>(ss) / a.D + (double)a.eps) : 1.0;
+            // (16-bit values by 16-bit weights: the products are exact)
+            float z[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) z[i] = x[i] * wk[i];
+            exchange(z, y);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              float dc, ds;
+              unpack2<BF16>(fine[i], dc, ds);
+              const double turned =
+                  (double)z[i] * ((double)c[i] + dc) + (double)y[i] * ((double)s[i] + ds);
+              const float key = round_to_odd((e + i < a.R ? turned : (double)z[i]) * inv);
+              x[i] = is_v ? x[i] : key;
+            }
           }
-          turn(cr, sr);
           // the whole group finds the row's scale
-          if (is_v) unpack8<T>(raw[it], x);
           uint32_t top = 0;
 #pragma unroll
           for (int i = 0; i < 8; ++i) top = max(top, mine ? e4m3::magnitude(x[i]) : 0u);
           const uint32_t byte = e4m3::scale_byte(group_max<LPR>(top));
-          if (row < H && mine && !is_q) {
-            if (!mapped) continue;
-            const float inv = e4m3::inverse_scale(byte);
+          if (row >= H || !mine || !mapped) continue;
+          const float inv = e4m3::inverse_scale(byte);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = e4m3::codable<T>(x[i]) * inv;
-            const long long head = is_v ? row - a.Hq - a.Hkv : row - a.Hq;
-            uint2 w;
-            w.x = e4m3::pack4(x[0], x[1], x[2], x[3]);
-            w.y = e4m3::pack4(x[4], x[5], x[6], x[7]);
-            *reinterpret_cast<uint2 *>((uint8_t *)(is_v ? a.vc : a.kc) + head * a.head_stride +
-                                       at + e) = w;
-            if (l == 0) (is_v ? a.vs : a.ks)[head * a.bs + at_scale] = (uint8_t)byte;
-            continue;
+          for (int i = 0; i < 8; ++i) x[i] = e4m3::codable<T>(x[i]) * inv;
+          const long long head = is_v ? row - a.Hq - a.Hkv : row - a.Hq;
+          uint2 w;
+          w.x = e4m3::pack4(x[0], x[1], x[2], x[3]);
+          w.y = e4m3::pack4(x[4], x[5], x[6], x[7]);
+          *reinterpret_cast<uint2 *>((uint8_t *)(is_v ? a.vc : a.kc) + head * a.head_stride + at +
+                                     e) = w;
+          if (l == 0) (is_v ? a.vs : a.ks)[head * a.bs + at / a.D] = (uint8_t)byte;
+        } else {
+          float ss = 0.0f;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) ss += x[i] * x[i];
+          ss = group_sum<LPR>(ss);
+          const bool norm = (E4M3 || is_q ? a.q_w : a.k_w) != nullptr;
+          const float inv = norm ? rsqrtf(ss / (float)a.D + a.eps) : 1.0f;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[i] *= inv * (E4M3 || is_q ? wq[i] : wk[i]);
+          exchange(x, y);
+          if (row >= H || !mine) continue;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[i] = e + i < a.R ? x[i] * c[i] + y[i] * s[i] : x[i];
+          uint32_t w[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) w[i] = pack2<T>(x[2 * i], x[2 * i + 1]);
+          if (!E4M3 && is_v) {  // as it is
+            w[0] = raw[it].x;
+            w[1] = raw[it].y;
+            w[2] = raw[it].z;
+            w[3] = raw[it].w;
           }
+          if (E4M3 || is_q)
+            store8(a.q_out + ((long long)t * a.Hq + row) * a.D + e, w);
+          else if (mapped)
+            store8((is_v ? (uint16_t *)a.vc + (row - a.Hq - a.Hkv) * a.head_stride
+                         : (uint16_t *)a.kc + (row - a.Hq) * a.head_stride) + at + e, w);
         }
       }
-      if (row >= H || !mine) continue;
-      if (!codes) turn(c, s);
-      uint32_t w[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] = pack2<T>(x[2 * i], x[2 * i + 1]);
-      if (is_v) {  // as it is
-        w[0] = raw[it].x;
-        w[1] = raw[it].y;
-        w[2] = raw[it].z;
-        w[3] = raw[it].w;
-      }
-      if (is_q)
-        store8(a.q_out + ((long long)t * a.Hq + row) * a.D + e, w);
-      else if (mapped)
-        store8((is_v ? (uint16_t *)a.vc + (row - a.Hq - a.Hkv) * a.head_stride
-                     : (uint16_t *)a.kc + (row - a.Hq) * a.head_stride) + at + e, w);
+      if (round + 1 < rounds) load(round + 1);
     }
-    if (round + 1 < a.rounds) load(round + 1);
-  }
+  };
+  if (kv)
+    pass(std::integral_constant<bool, E4M3>{});
+  else
+    pass(std::false_type{});
 }
 
 template <class T, int LPR, int LAYOUT, bool E4M3>
@@ -372,10 +430,14 @@ int launch(Args a, hipStream_t st) {
   constexpr int RPW = 64 / LPR;
   const int H = a.Hq + 2 * a.Hkv;
   const long long few = (long long)a.T * ((H + RPW - 1) / RPW);
-  auto grid = [&](int iter, int rounds) {
-    a.rounds = rounds;
-    a.chunks = (H + iter * rounds * RPW - 1) / (iter * rounds * RPW);
-    return dim3((unsigned)(((long long)a.T * a.chunks + kWaves - 1) / kWaves));
+  const int rows = E4M3 ? a.Hq : H;
+  auto up = [](int n, int per) { return (n + per - 1) / per; };
+  auto grid = [&](int iter, bool all) {
+    a.rounds = all ? up(rows, iter * RPW) : 1;
+    a.chunks = up(rows, iter * a.rounds * RPW);
+    a.kv_rounds = E4M3 ? (all ? up(2 * a.Hkv, iter * RPW) : 1) : 0;
+    a.kv_chunks = E4M3 ? up(2 * a.Hkv, iter * a.kv_rounds * RPW) : 0;
+    return dim3((unsigned)(((long long)a.T * (a.chunks + a.kv_chunks) + kWaves - 1) / kWaves));
   };
   // `few`: waves of one row a lane group.  A token's heads all in one wave where
   // that leaves 8192 waves of kIter rows' work (angles and weights are then formed
@@ -384,14 +446,13 @@ int launch(Args a, hipStream_t st) {
   // tokens 10.1 / 10.6 / 14, 2000 tokens 22 / 19.6 / 20.5, 3200 tokens 36 / 27 / 24, 8149
   // tokens 104 / 73 / 58.  With 2 / 6 / 8 / 12 rows in flight: 59.5 / 59.2 / 62 / 69.
   if (few >= 8192 * kIter) {
-    const int all = (H + kIter * RPW - 1) / (kIter * RPW);
     CFA_LAUNCH("qk_norm_rope_kv", (qk_norm_rope_kv_kernel<T, LPR, LAYOUT, kIter, E4M3>),
-               grid(kIter, all), dim3(kWaves * 64), 0, st, a);
+               grid(kIter, true), dim3(kWaves * 64), 0, st, a);
   } else if (few >= 8192) {
     CFA_LAUNCH("qk_norm_rope_kv", (qk_norm_rope_kv_kernel<T, LPR, LAYOUT, kIter, E4M3>),
-               grid(kIter, 1), dim3(kWaves * 64), 0, st, a);
+               grid(kIter, false), dim3(kWaves * 64), 0, st, a);
   } else {
-    CFA_LAUNCH("qk_norm_rope_kv", (qk_norm_rope_kv_kernel<T, LPR, LAYOUT, 1, E4M3>), grid(1, 1),
+    CFA_LAUNCH("qk_norm_rope_kv", (qk_norm_rope_kv_kernel<T, LPR, LAYOUT, 1, E4M3>), grid(1, false),
                dim3(kWaves * 64), 0, st, a);
   }
   return CFA_OK;
