@@ -16,6 +16,10 @@
 //      p' = p 2^e, while the row's sum is of p itself.
 //   The next tile's K and V are asked for as soon as the present tile's products with
 //   Q have read its K.
+// Measured, 32 heads of 128 over 8: 64 single tokens behind 1024 to 4096 keys 74 us, 4.6
+// TB/s of codes (132 with the tiles that a work-group shares, which are turned into 16
+// bits first); one token behind 1000 keys of its window 8.5, of which about 5 pass in
+// front of the first tile, and 2.4 for the merge.
 // In bf16 p' has fp32's range.  In fp16 it is kept to the largest scale that the wave
 // has met (p' = p 2^(e - E) <= p, and the sums are multiples of 2^E), so that it is as
 // exact as p where it counts.

@@ -5,7 +5,9 @@
 // Token j of sequence b is the row at slot start[b] + j of
 // pool[block][layer][kv_head][slot][D]; out = code 2^(byte - 127), exact in bf16.
 //
-// Bound: HBM.  A row's D codes are read and 2 D bytes written once; 16 codes a lane.
+// Bound: HBM.  A row's D codes are read and 2 D bytes written once; 16 codes a lane, a
+// wave a token, whose page is looked up once for its heads.  8 sequences of 4096 tokens,
+// 8 heads of 128 (202 MB): 45 us, 4.5 TB/s; one of 8149 tokens 12, 93 tokens 3.4.
 #include <hip/hip_runtime.h>
 
 #include "abi_internal.hpp"
