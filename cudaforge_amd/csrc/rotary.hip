@@ -201,23 +201,175 @@ __device__ __forceinline__ float round_to_odd(double v) {
 }
 
 // One wave = one token and `rounds` times ITER * 64 / LPR consecutive rows of its
-// Hq q heads, Hkv k heads and Hkv v heads.  With e4m3 pools q rows, in the 16-bit caches'
-// arithmetic (and bits) whatever the cache, and k and v rows are different waves', which
-// then hold one kind of angles and weights each: four waves a SIMD, where both take 142
-// registers (three waves; without the bound 131: 90 us against 81 with kv_gather's).
-template <class T, int LPR, int LAYOUT, int ITER, bool E4M3>
-__global__ __launch_bounds__(kWaves * 64, E4M3 && LAYOUT != kHalfAny ? 4 : 1) void
-qk_norm_rope_kv_kernel(Args a) {
+// Hq q heads, Hkv k heads and Hkv v heads.
+template <class T, int LPR, int LAYOUT, int ITER>
+__global__ __launch_bounds__(kWaves * 64) void qk_norm_rope_kv_kernel(Args a) {
   constexpr int RPW = 64 / LPR;
   const int lane = threadIdx.x & 63, l = lane % LPR;
   const long long item = (long long)blockIdx.x * kWaves + (threadIdx.x >> 6);
-  const int all = a.chunks + (E4M3 ? a.kv_chunks : 0);
+  const int t = (int)(item / a.chunks), chunk = (int)(item % a.chunks);
+  if (t >= a.T) return;
+  const int e = 8 * l, H = a.Hq + 2 * a.Hkv;
+  const bool mine = e < a.D;
+  const int row0 = chunk * a.rounds * ITER * RPW + lane / LPR;
+
+  uint4 raw[ITER];
+  auto load = [&](int round) {
+#pragma unroll
+    for (int it = 0; it < ITER; ++it) {
+      const int row = row0 + (round * ITER + it) * RPW;
+      raw[it] = make_uint4(0, 0, 0, 0);
+      if (row < H && mine) {
+        const uint16_t *src =
+            row < a.Hq ? a.q + t * a.q_st + row * a.q_sh
+                       : row < a.Hq + a.Hkv ? a.k + t * a.k_st + (row - a.Hq) * a.k_sh
+                                            : a.v + t * a.v_st + (row - a.Hq - a.Hkv) * a.v_sh;
+        raw[it] = load8(src + e);
+      }
+    }
+  };
+  load(0);
+  int b, j;
+  if (!place_token(a, t, lane, b, j)) return;
+  // this lane's cosines and sines: c[i], s[i] of element e + i, the sine with
+  // the sign that its partner's value takes
+  float c[8], s[8], wq[8], wk[8];
+  const int half = a.R / 2;
+  const int p = a.pos[t];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    c[i] = 1.0f;
+    s[i] = 0.0f;
+  }
+  if constexpr (LAYOUT == kNeighbours) {
+    if (e + 8 <= a.R) {
+      uint64_t f[4];
+      turns_at<4>(a, e / 2, f);
+#pragma unroll
+      for (int i = 0; i < 8; i += 2) angle(a, p, f[i / 2], c[i], s[i + 1]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; i += 2)
+        if (e + i < a.R) angle(a, p, a.turns[(e + i) / 2], c[i], s[i + 1]);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+      c[i + 1] = c[i];
+      s[i] = -s[i + 1];
+    }
+  } else if constexpr (LAYOUT == kHalf) {
+    if (e < a.R) {  // a lane's eight lie in one half
+      const bool first = e < half;
+      uint64_t f[8];
+      turns_at<8>(a, first ? e : e - half, f);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        angle(a, p, f[i], c[i], s[i]);
+        s[i] = first ? -s[i] : s[i];
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (e + i < a.R) {
+        const bool first = e + i < half;
+        angle(a, p, a.turns[first ? e + i : e + i - half], c[i], s[i]);
+        if (first) s[i] = -s[i];
+      }
+    }
+  }
+  if (mine) {
+    weights8<T>(a.q_w, a.w_f32, e, wq);
+    weights8<T>(a.k_w, a.w_f32, e, wk);
+  }
+  // the page of this token's slot
+  const long long slot = (long long)a.base[b] + j;
+  const long long page = slot / a.bs;
+  int blk = -1;
+  if (slot >= 0 && page < a.max_blocks) blk = a.block_tables[(long long)b * a.max_blocks + page];
+  const bool mapped = blk >= 0 && blk < a.num_blocks;
+  const long long at = blk * a.blk_stride + a.layer_off + (slot - page * a.bs) * a.D;
+
+  for (int round = 0; round < a.rounds; ++round) {
+#pragma unroll
+    for (int it = 0; it < ITER; ++it) {
+      const int row = row0 + (round * ITER + it) * RPW;
+      const bool is_q = row < a.Hq, is_v = row >= a.Hq + a.Hkv;
+      float x[8], y[8];
+      unpack8<T>(raw[it], x);
+      float ss = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) ss += x[i] * x[i];
+      ss = group_sum<LPR>(ss);
+      const bool norm = (is_q ? a.q_w : a.k_w) != nullptr;
+      const float inv = norm ? rsqrtf(ss / (float)a.D + a.eps) : 1.0f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] *= inv * (is_q ? wq[i] : wk[i]);
+      if constexpr (LAYOUT == kHalf) {
+        // R / 2 is a multiple of 8: the partner's elements are one lane's
+        const int to = e < half ? lane + half / 8 : (e < a.R ? lane - half / 8 : lane);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = __shfl(x[i], to, 64);
+      } else if constexpr (LAYOUT == kHalfAny) {
+        // element by element: partner e + i +- R / 2, in lane (e + i +- R / 2) / 8
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int el = e + i;
+          const int pe = el < half ? el + half : (el < a.R ? el - half : el);
+          const int from = lane - l + pe / 8;
+          float v = 0.0f;
+#pragma unroll
+          for (int m = 0; m < 8; ++m) {
+            const float got = __shfl(x[m], from, 64);
+            if (pe % 8 == m) v = got;
+          }
+          y[i] = v;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = x[i ^ 1];
+      }
+      if (row >= H || !mine) continue;
+      // (elements behind the rotated ones are selected, not turned by 0: they
+      // may be infinite)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = e + i < a.R ? x[i] * c[i] + y[i] * s[i] : x[i];
+      uint32_t w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = pack2<T>(x[2 * i], x[2 * i + 1]);
+      if (is_v) {  // as it is
+        w[0] = raw[it].x;
+        w[1] = raw[it].y;
+        w[2] = raw[it].z;
+        w[3] = raw[it].w;
+      }
+      if (is_q)
+        store8(a.q_out + ((long long)t * a.Hq + row) * a.D + e, w);
+      else if (mapped)
+        store8((is_v ? (uint16_t *)a.vc + (row - a.Hq - a.Hkv) * a.head_stride
+                          : (uint16_t *)a.kc + (row - a.Hq) * a.head_stride) + at + e, w);
+    }
+    if (round + 1 < a.rounds) load(round + 1);
+  }
+}
+
+// The same into e4m3 pools.  q rows, in the arithmetic above (and its bits), and k and v
+// rows are different waves', which
+// then hold one kind of angles and weights each: four waves a SIMD, where both take 142
+// registers (three waves; without the bound 131: 90 us against 81 with kv_gather's).
+template <class T, int LPR, int LAYOUT, int ITER>
+__global__ __launch_bounds__(kWaves * 64, LAYOUT != kHalfAny ? 4 : 1) void
+qk_norm_rope_kv_e4m3_kernel(Args a) {
+  constexpr int RPW = 64 / LPR;
+  const int lane = threadIdx.x & 63, l = lane % LPR;
+  const long long item = (long long)blockIdx.x * kWaves + (threadIdx.x >> 6);
+  const int all = a.chunks + a.kv_chunks;
   const int t = (int)(item / all), chunk = (int)(item % all);
   if (t >= a.T) return;
   const int e = 8 * l;
-  const bool kv = E4M3 && __builtin_amdgcn_readfirstlane(chunk) >= a.chunks;
+  const bool kv = __builtin_amdgcn_readfirstlane(chunk) >= a.chunks;
   const int rounds = kv ? a.kv_rounds : a.rounds;
-  const int H = E4M3 && !kv ? a.Hq : a.Hq + 2 * a.Hkv;  // the wave's rows end here
+  const int H = !kv ? a.Hq : a.Hq + 2 * a.Hkv;  // the wave's rows end here
   const bool mine = e < a.D;
   const int row0 = (kv ? a.Hq + (chunk - a.chunks) * rounds * ITER * RPW
                        : chunk * rounds * ITER * RPW) + lane / LPR;
@@ -281,7 +433,7 @@ qk_norm_rope_kv_kernel(Args a) {
     constexpr bool CODES = decltype(codes)::value;
     // this lane's cosines and sines: c[i], s[i] of element e + i, the sine with
     // the sign that its partner's value takes
-    float c[8], s[8], wq[8], wk[8];
+    float c[8], s[8], w8[8];  // w8: the norm's weights
     uint32_t fine[8];  // what fine_angle's differ by, as bf16 pairs (2^-31 of the value)
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -336,15 +488,14 @@ qk_norm_rope_kv_kernel(Args a) {
       }
     }
     if (mine) {
-      if constexpr (!CODES) weights8<T>(a.q_w, a.w_f32, e, wq);
-      if constexpr (CODES || !E4M3) weights8<T>(a.k_w, a.w_f32, e, wk);
+      weights8<T>(CODES ? a.k_w : a.q_w, a.w_f32, e, w8);
     }
 
     for (int round = 0; round < rounds; ++round) {
 #pragma unroll
       for (int it = 0; it < ITER; ++it) {
         const int row = row0 + (round * ITER + it) * RPW;
-        const bool is_q = row < a.Hq, is_v = row >= a.Hq + a.Hkv;
+        const bool is_v = row >= a.Hq + a.Hkv;
         float x[8], y[8];
         unpack8<T>(raw[it], x);
         // (elements behind the rotated ones are selected, not turned by 0: they may be
@@ -359,7 +510,7 @@ qk_norm_rope_kv_kernel(Args a) {
             // (16-bit values by 16-bit weights: the products are exact)
             float z[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) z[i] = x[i] * wk[i];
+            for (int i = 0; i < 8; ++i) z[i] = x[i] * w8[i];
             exchange(z, y);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
@@ -392,10 +543,9 @@ qk_norm_rope_kv_kernel(Args a) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) ss += x[i] * x[i];
           ss = group_sum<LPR>(ss);
-          const bool norm = (E4M3 || is_q ? a.q_w : a.k_w) != nullptr;
-          const float inv = norm ? rsqrtf(ss / (float)a.D + a.eps) : 1.0f;
+          const float inv = a.q_w ? rsqrtf(ss / (float)a.D + a.eps) : 1.0f;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) x[i] *= inv * (E4M3 || is_q ? wq[i] : wk[i]);
+          for (int i = 0; i < 8; ++i) x[i] *= inv * w8[i];
           exchange(x, y);
           if (row >= H || !mine) continue;
 #pragma unroll
@@ -403,24 +553,14 @@ qk_norm_rope_kv_kernel(Args a) {
           uint32_t w[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) w[i] = pack2<T>(x[2 * i], x[2 * i + 1]);
-          if (!E4M3 && is_v) {  // as it is
-            w[0] = raw[it].x;
-            w[1] = raw[it].y;
-            w[2] = raw[it].z;
-            w[3] = raw[it].w;
-          }
-          if (E4M3 || is_q)
-            store8(a.q_out + ((long long)t * a.Hq + row) * a.D + e, w);
-          else if (mapped)
-            store8((is_v ? (uint16_t *)a.vc + (row - a.Hq - a.Hkv) * a.head_stride
-                         : (uint16_t *)a.kc + (row - a.Hq) * a.head_stride) + at + e, w);
+          store8(a.q_out + ((long long)t * a.Hq + row) * a.D + e, w);
         }
       }
       if (round + 1 < rounds) load(round + 1);
     }
   };
   if (kv)
-    pass(std::integral_constant<bool, E4M3>{});
+    pass(std::true_type{});
   else
     pass(std::false_type{});
 }
@@ -445,15 +585,21 @@ int launch(Args a, hipStream_t st) {
   // us, 48 heads of 128, one row a group / kIter rows / all heads in a wave: 504
   // tokens 10.1 / 10.6 / 14, 2000 tokens 22 / 19.6 / 20.5, 3200 tokens 36 / 27 / 24, 8149
   // tokens 104 / 73 / 58.  With 2 / 6 / 8 / 12 rows in flight: 59.5 / 59.2 / 62 / 69.
-  if (few >= 8192 * kIter) {
-    CFA_LAUNCH("qk_norm_rope_kv", (qk_norm_rope_kv_kernel<T, LPR, LAYOUT, kIter, E4M3>),
-               grid(kIter, true), dim3(kWaves * 64), 0, st, a);
-  } else if (few >= 8192) {
-    CFA_LAUNCH("qk_norm_rope_kv", (qk_norm_rope_kv_kernel<T, LPR, LAYOUT, kIter, E4M3>),
-               grid(kIter, false), dim3(kWaves * 64), 0, st, a);
+  const bool all = few >= 8192 * kIter;
+  if constexpr (E4M3) {
+    if (few >= 8192)
+      CFA_LAUNCH("qk_norm_rope_kv", (qk_norm_rope_kv_e4m3_kernel<T, LPR, LAYOUT, kIter>),
+                 grid(kIter, all), dim3(kWaves * 64), 0, st, a);
+    else
+      CFA_LAUNCH("qk_norm_rope_kv", (qk_norm_rope_kv_e4m3_kernel<T, LPR, LAYOUT, 1>),
+                 grid(1, false), dim3(kWaves * 64), 0, st, a);
   } else {
-    CFA_LAUNCH("qk_norm_rope_kv", (qk_norm_rope_kv_kernel<T, LPR, LAYOUT, 1, E4M3>), grid(1, false),
-               dim3(kWaves * 64), 0, st, a);
+    if (few >= 8192)
+      CFA_LAUNCH("qk_norm_rope_kv", (qk_norm_rope_kv_kernel<T, LPR, LAYOUT, kIter>),
+                 grid(kIter, all), dim3(kWaves * 64), 0, st, a);
+    else
+      CFA_LAUNCH("qk_norm_rope_kv", (qk_norm_rope_kv_kernel<T, LPR, LAYOUT, 1>),
+                 grid(1, false), dim3(kWaves * 64), 0, st, a);
   }
   return CFA_OK;
 }
