@@ -354,9 +354,9 @@ __global__ __launch_bounds__(kWaves * 64) void qk_norm_rope_kv_kernel(Args a) {
 }
 
 // The same into e4m3 pools.  q rows, in the arithmetic above (and its bits), and k and v
-// rows are different waves', which
-// then hold one kind of angles and weights each: four waves a SIMD, where both take 142
-// registers (three waves; without the bound 131: 90 us against 81 with kv_gather's).
+// rows are different waves', which then hold one kind of angles and weights each: four
+// waves a SIMD, where both kinds take 142 registers and leave three.  (8149 tokens with
+// the read behind them: 81 us; without the bound on registers 131 of them, and 90.)
 template <class T, int LPR, int LAYOUT, int ITER>
 __global__ __launch_bounds__(kWaves * 64, LAYOUT != kHalfAny ? 4 : 1) void
 qk_norm_rope_kv_e4m3_kernel(Args a) {
