@@ -172,7 +172,8 @@ __global__ __launch_bounds__(kFewNT, few_groups(D, QT)) void few_rows_kernel(Arg
   uint32_t top_byte = 1;  // fp16: the largest V scale so far
   const Row *const rows_at = srow + col;
 
-  int i = view.t1 - 1 - wave;
+  // (a split without keys has no tile, also where the window's first tile is numbered)
+  int i = (view.steps > 0 ? view.t1 : view.t0) - 1 - wave;
   int stage = 0, n = 0;
   long long offs = 0;
   int next_block = 0;
