@@ -20,9 +20,12 @@
 // TB/s of codes (132 with the tiles that a work-group shares, which are turned into 16
 // bits first); one token behind 1000 keys of its window 8.5, of which about 5 pass in
 // front of the first tile, and 2.4 for the merge.
-// In bf16 p' has fp32's range.  In fp16 it is kept to the largest scale that the wave
-// has met (p' = p 2^(e - E) <= p, and the sums are multiples of 2^E), so that it is as
-// exact as p where it counts.
+// p' needs fp32's range: the scales of a tile's keys lie 2^30 and more apart, and the
+// largest may be that of a key that a row does not see.  V's codes are therefore taken as
+// bf16, exactly, whatever q's type, and p' as bf16 too; for fp16 q in two parts, the
+// rounded value and the rest, which keep 16 bits of it (bf16 q of 8 nodes over 4096 keys,
+// 16 sequences: 37 us with one part, 41 with two; fp16 39 with p' in fp16 relative to the
+// largest scale met, which lost the small values beside a large one).
 #pragma once
 
 #include "scored_attention.hpp"
@@ -43,6 +46,7 @@ __global__ __launch_bounds__(kFewNT, few_groups(D, QT)) void few_rows_kernel(Arg
   constexpr int kTileBytes = kKT * D;  // of codes
   constexpr int kHalves = D / 64;      // 16-code loads of a lane for one key
   constexpr int kRowsPerLoad = 1024 / D;
+  constexpr int kParts = std::is_same<T, BF16>::value ? 1 : 2;  // of a probability
   constexpr int kMerge = QT * 16 * (D + 4);  // floats of a wave's sums
   constexpr int kStageBytes = kFewWaves * 2 * kTileBytes;
   constexpr int kMergeBytes = kFewWaves * kMerge * 4;
@@ -169,7 +173,6 @@ __global__ __launch_bounds__(kFewNT, few_groups(D, QT)) void few_rows_kernel(Arg
 #pragma unroll
     for (int dt = 0; dt < D / 16; ++dt) o[qt][dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   }
-  uint32_t top_byte = 1;  // fp16: the largest V scale so far
   const Row *const rows_at = srow + col;
 
   // (a split without keys has no tile, also where the window's first tile is numbered)
@@ -261,47 +264,25 @@ __global__ __launch_bounds__(kFewNT, few_groups(D, QT)) void few_rows_kernel(Arg
           for (int t = 0; t < 2; ++t) S.s[qt][b][t] -= by[qt];
       }
     }
-    if constexpr (!std::is_same<T, BF16>::value) {
-      uint32_t most = 0;
+    // O^T += V^T P^T, 32 keys at a time
+    const uint8_t *const vs = vlds + stage * kTileBytes;
 #pragma unroll
-      for (int b = 0; b < 2; ++b)
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int k = 0; k < 4; ++k) most = max(most, (vb[b][t] >> (8 * k)) & 255u);
-      most = max(most, (uint32_t)__shfl_xor((int)most, 16, 64));
-      most = __builtin_amdgcn_readfirstlane(max(most, (uint32_t)__shfl_xor((int)most, 32, 64)));
-      if (most > top_byte) {
-        const float alpha = e4m3::scale(max((int)top_byte - (int)most + 127, 0));
-        top_byte = most;
-#pragma unroll
-        for (int qt = 0; qt < QT; ++qt)
-#pragma unroll
-          for (int dt = 0; dt < D / 16; ++dt) o[qt][dt] *= alpha;
-      }
-    }
-    Probs<QT, T> P;
-#pragma unroll
-    for (int b = 0; b < 2; ++b)
+    for (int b = 0; b < 2; ++b) {
+      typename Mfma<BF16>::frag p[QT], rest[QT];
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          uint32_t byte = (vb[b][t] >> (8 * k)) & 255u;
-          if constexpr (!std::is_same<T, BF16>::value)
-            byte = (uint32_t)max((int)byte - (int)top_byte + 127, 0);
-          const float f = e4m3::scale(byte);
+          const float f = e4m3::scale((vb[b][t] >> (8 * k)) & 255u);
 #pragma unroll
           for (int qt = 0; qt < QT; ++qt) {
-            const float p = __builtin_amdgcn_exp2f(S.s[qt][b][t][k]);
-            sum[qt] += p;
-            P.p[qt][b][t * 4 + k] = (typename T::elem)(p * f);
+            const float x = __builtin_amdgcn_exp2f(S.s[qt][b][t][k]);
+            sum[qt] += x;
+            const __bf16 high = (__bf16)(x * f);
+            p[qt][t * 4 + k] = high;
+            if constexpr (kParts == 2) rest[qt][t * 4 + k] = (__bf16)(x * f - (float)high);
           }
         }
-    // O^T += V^T P^T
-    const uint8_t *const vs = vlds + stage * kTileBytes;
-#pragma unroll
-    for (int b = 0; b < 2; ++b)
 #pragma unroll
       for (int dt = 0; dt < D / 16; ++dt) {
         const int key = b * 32 + 8 * g + (col >> 1);
@@ -309,12 +290,16 @@ __global__ __launch_bounds__(kFewNT, few_groups(D, QT)) void few_rows_kernel(Arg
         const i32x2 w = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
             (CFA_LDS i32x2 *)(vs + key * D + ((dt ^ swz) << 4) + (col & 1) * 8));
         const uint4 v = make_uint4(
-            e4m3::unpack_pair<T, false>(w.x, 1.0f), e4m3::unpack_pair<T, true>(w.x, 1.0f),
-            e4m3::unpack_pair<T, false>(w.y, 1.0f), e4m3::unpack_pair<T, true>(w.y, 1.0f));
-        const auto vf = __builtin_bit_cast(typename Mfma<T>::frag, v);
+            e4m3::unpack_pair<BF16, false>(w.x, 1.0f), e4m3::unpack_pair<BF16, true>(w.x, 1.0f),
+            e4m3::unpack_pair<BF16, false>(w.y, 1.0f), e4m3::unpack_pair<BF16, true>(w.y, 1.0f));
+        const auto vf = __builtin_bit_cast(typename Mfma<BF16>::frag, v);
 #pragma unroll
-        for (int qt = 0; qt < QT; ++qt) o[qt][dt] = Mfma<T>::run(vf, P.p[qt][b], o[qt][dt]);
+        for (int qt = 0; qt < QT; ++qt) {
+          o[qt][dt] = Mfma<BF16>::run(vf, p[qt], o[qt][dt]);
+          if constexpr (kParts == 2) o[qt][dt] = Mfma<BF16>::run(vf, rest[qt], o[qt][dt]);
+        }
       }
+    }
   }
 
   // The waves' sums: a row's is over the four lanes of its column.
@@ -329,15 +314,13 @@ __global__ __launch_bounds__(kFewNT, few_groups(D, QT)) void few_rows_kernel(Arg
   }
   __syncthreads();  // every wave is done with its V
   float *const merge = reinterpret_cast<float *>(lds);
-  const float unit =
-      std::is_same<T, BF16>::value ? 1.0f : e4m3::scale(top_byte);  // what o counts in
 #pragma unroll
   for (int qt = 0; qt < QT; ++qt) {
     const int r = qt * 16 + col;
     float m = sbase[0][r];
 #pragma unroll
     for (int w = 1; w < kFewWaves; ++w) m = fmaxf(m, sbase[w][r]);
-    const float mine = sum[qt] != 0.0f ? __builtin_amdgcn_exp2f(base[qt] - m) * unit : 0.0f;
+    const float mine = sum[qt] != 0.0f ? __builtin_amdgcn_exp2f(base[qt] - m) : 0.0f;
 #pragma unroll
     for (int dt = 0; dt < D / 16; ++dt)
       *reinterpret_cast<f32x4 *>(merge + (wave * QT * 16 + r) * (D + 4) + dt * 16 + 4 * g) =
