@@ -8,7 +8,7 @@
 //   (a, b) -> factor * (a cos - b sin, b cos + a sin)
 // v is copied.  q goes to q_out [T, Hq, D], k and v to the sequence's slots
 // base[b] + j of pool[block][layer][kv_head][slot][D], as they are or as e4m3
-// codes with a scale a row (e4m3.hpp), quantised from the fp32 results.
+// codes with a scale a row (e4m3.hpp): v's elements, and k's results in 64 bits.
 //
 // Angles.  At position 100000 an fp32 product p f is off by up to 0.004
 // radians, more than bf16 resolves.  Frequencies are therefore 64-bit
@@ -22,9 +22,9 @@
 // pair is one exchange between two of its lanes.  A wave keeps one token, so
 // that its angles and the norms' weights are formed once for its heads.  8149
 // tokens of 48 heads of 128: 51 us, 3.9 TB/s (pages scattered, 256 bytes a row); 504
-// tokens 7 us, 8 tokens 5.  Into e4m3 pages (184 MB): 68 us for the 8149, 6 for 8, with
+// tokens 7 us, 8 tokens 5.  Into e4m3 pages (184 MB): 61 us for the 8149, 6 for 8, with
 // keys in 64 bits.  In fp32 56 to 60, but then 12 to 26 of 8.4 million codes were other
-// than their exact values', against 0 or 1.
+// than their exact values', against none.
 #include <hip/hip_runtime.h>
 
 #include <type_traits>
@@ -136,6 +136,14 @@ __device__ __forceinline__ void weights8(const void *w, int f32, int e, float (&
   }
 }
 
+// One of them.
+template <class T>
+__device__ __forceinline__ float weight(const void *w, int f32, int e) {
+  if (!w) return 1.0f;
+  if (f32) return reinterpret_cast<const float *>(w)[e];
+  return (float)reinterpret_cast<const typename T::elem *>(w)[e];
+}
+
 // N frequencies from number i on.
 template <int N>
 __device__ __forceinline__ void turns_at(const Args &a, int i, uint64_t (&t)[N]) {
@@ -181,11 +189,11 @@ __device__ __forceinline__ void fine_angle(const Args &a, int p, uint64_t turns,
   sn = quarter & 2 ? -across : across;
 }
 
-// 1 / sqrt(mean) in 64 bits: the fp32 root and a step of Newton's (none where that is 0
-// or infinite).
+// 1 / sqrt(mean) in 64 bits: the instruction's (some 2^-23) and a step of Newton's (none
+// where that is 0 or infinite).
 __device__ __forceinline__ double fine_rsqrt(double mean) {
-  const float r = rsqrtf((float)mean);
-  if (!(r > 0.0f && r < INFINITY)) return r;
+  const double r = __builtin_amdgcn_rsq(mean);
+  if (!(r > 0.0 && r < INFINITY)) return r;
   return r + 0.5 * r * (1.0 - mean * r * r);
 }
 
@@ -355,8 +363,9 @@ __global__ __launch_bounds__(kWaves * 64) void qk_norm_rope_kv_kernel(Args a) {
 
 // The same into e4m3 pools.  q rows, in the arithmetic above (and its bits), and k and v
 // rows are different waves', which then hold one kind of angles and weights each: four
-// waves a SIMD, where both kinds take 142 registers and leave three.  (8149 tokens with
-// the read behind them: 81 us; without the bound on registers 131 of them, and 90.)
+// waves a SIMD, where both kinds took 142 registers and left three.  (8149 tokens: 61 us;
+// without the bound on registers 130 of them, and 71.)  Partners exchange the elements as
+// they are read, exact in fp32, and what multiplies them is formed in 64 bits once a wave.
 template <class T, int LPR, int LAYOUT, int ITER>
 __global__ __launch_bounds__(kWaves * 64, LAYOUT != kHalfAny ? 4 : 1) void
 qk_norm_rope_kv_e4m3_kernel(Args a) {
@@ -402,6 +411,7 @@ qk_norm_rope_kv_e4m3_kernel(Args a) {
   const bool mapped = blk >= 0 && blk < a.num_blocks;
   const long long at = blk * a.blk_stride + a.layer_off + (slot - page * a.bs) * a.D;
   // of the partners' p
+  __shared__ __align__(16) float swap[LAYOUT == kHalfAny ? kWaves * 64 * 8 : 1];
   auto exchange = [&](const float(&p)[8], float(&y)[8]) {
     if constexpr (LAYOUT == kHalf) {
       // R / 2 is a multiple of 8: the partner's elements are one lane's
@@ -409,66 +419,39 @@ qk_norm_rope_kv_e4m3_kernel(Args a) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) y[i] = __shfl(p[i], to, 64);
     } else if constexpr (LAYOUT == kHalfAny) {
-      // element by element: partner e + i +- R / 2, in lane (e + i +- R / 2) / 8
+      // element by element, through the wave's LDS (in order within a wave)
+      float *const own = swap + (threadIdx.x & ~63) * 8;
+      float4 *const mine8 = reinterpret_cast<float4 *>(own + lane * 8);
+      mine8[0] = make_float4(p[0], p[1], p[2], p[3]);
+      mine8[1] = make_float4(p[4], p[5], p[6], p[7]);
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const int el = e + i;
-        const int pe = el < half ? el + half : (el < a.R ? el - half : el);
-        const int from = lane - l + pe / 8;
-        float v = 0.0f;
-#pragma unroll
-        for (int m = 0; m < 8; ++m) {
-          const float got = __shfl(p[m], from, 64);
-          if (pe % 8 == m) v = got;
-        }
-        y[i] = v;
+        y[i] = own[(lane - l) * 8 + (el < half ? el + half : (el < a.R ? el - half : el))];
       }
+      __builtin_amdgcn_wave_barrier();
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i) y[i] = p[i ^ 1];
     }
   };
 
-  auto pass = [&](auto codes) {
-    constexpr bool CODES = decltype(codes)::value;
-    // this lane's cosines and sines: c[i], s[i] of element e + i, the sine with
-    // the sign that its partner's value takes
-    float c[8], s[8], w8[8];  // w8: the norm's weights
-    uint32_t fine[8];  // what fine_angle's differ by, as bf16 pairs (2^-31 of the value)
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      c[i] = 1.0f;
-      s[i] = 0.0f;
-      fine[i] = 0;
-    }
-    // element e + i (and its pair's second, of neighbours) at a pair's frequency
-    auto angles = [&](uint64_t turns, int i, bool front) {
-      float cs, sn;
-      angle(a, p, turns, cs, sn);
-      c[i] = cs;
-      s[i] = front ? -sn : sn;
-      if constexpr (LAYOUT == kNeighbours) {
-        c[i + 1] = cs;
-        s[i + 1] = sn;
-      }
-      if constexpr (CODES) {
-        double csf, snf;
-        fine_angle(a, p, turns, csf, snf);
-        const float dc = (float)(csf - cs), ds = (float)(snf - sn);
-        fine[i] = pack2<BF16>(dc, front ? -ds : ds);
-        if constexpr (LAYOUT == kNeighbours) fine[i + 1] = pack2<BF16>(dc, ds);
-      }
-    };
+  // turn(frequency, i, whether it is the pair's first) for each of the lane's elements
+  // e + i that turn (neighbours: for the pairs' first ones)
+  auto angles = [&](auto turn) {
     if constexpr (LAYOUT == kNeighbours) {
       if (e + 8 <= a.R) {
         uint64_t f[4];
         turns_at<4>(a, e / 2, f);
 #pragma unroll
-        for (int i = 0; i < 8; i += 2) angles(f[i / 2], i, true);
+        for (int i = 0; i < 8; i += 2) turn(f[i / 2], i, true);
       } else {
 #pragma unroll
         for (int i = 0; i < 8; i += 2)
-          if (e + i < a.R) angles(a.turns[(e + i) / 2], i, true);
+          if (e + i < a.R) turn(a.turns[(e + i) / 2], i, true);
       }
     } else if constexpr (LAYOUT == kHalf) {
       if (e < a.R) {  // a lane's eight lie in one half
@@ -476,21 +459,51 @@ qk_norm_rope_kv_e4m3_kernel(Args a) {
         uint64_t f[8];
         turns_at<8>(a, first ? e : e - half, f);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) angles(f[i], i, first);
+        for (int i = 0; i < 8; ++i) turn(f[i], i, first);
       }
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         if (e + i < a.R) {
           const bool first = e + i < half;
-          angles(a.turns[first ? e + i : e + i - half], i, first);
+          turn(a.turns[first ? e + i : e + i - half], i, first);
         }
       }
     }
-    if (mine) {
-      weights8<T>(CODES ? a.k_w : a.q_w, a.w_f32, e, w8);
-    }
+  };
 
+  if (kv) {
+    // element e + i of a key is x ca[i] + y cb[i], y its partner in the pair: the norm's
+    // weights times the cosine, and the partner's times the sine with its sign
+    double ca[8], cb[8];
+    {
+      float w[8], wp[8];
+      weights8<T>(a.k_w, a.w_f32, mine ? e : 0, w);
+      if constexpr (LAYOUT == kHalf) {
+        weights8<T>(a.k_w, a.w_f32, e < half ? e + half : e < a.R ? e - half : 0, wp);
+      } else if constexpr (LAYOUT == kNeighbours) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) wp[i] = w[i ^ 1];
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        ca[i] = w[i];
+        cb[i] = 0.0;
+      }
+      auto turn = [&](uint64_t turns, int i, bool front) {
+        double cs, sn;
+        fine_angle(a, p, turns, cs, sn);
+        ca[i] = w[i] * cs;
+        if constexpr (LAYOUT == kHalfAny)
+          wp[i] = weight<T>(a.k_w, a.w_f32, front ? e + i + half : e + i - half);
+        cb[i] = wp[i] * (front ? -sn : sn);
+        if constexpr (LAYOUT == kNeighbours) {
+          ca[i + 1] = w[i + 1] * cs;
+          cb[i + 1] = wp[i + 1] * sn;
+        }
+      };
+      angles(turn);
+    }
     for (int round = 0; round < rounds; ++round) {
 #pragma unroll
       for (int it = 0; it < ITER; ++it) {
@@ -498,71 +511,86 @@ qk_norm_rope_kv_e4m3_kernel(Args a) {
         const bool is_v = row >= a.Hq + a.Hkv;
         float x[8], y[8];
         unpack8<T>(raw[it], x);
-        // (elements behind the rotated ones are selected, not turned by 0: they may be
-        // infinite)
-        if constexpr (CODES) {
-          if (__builtin_amdgcn_readfirstlane(row - lane / LPR) < a.Hq + a.Hkv) {  // keys
-            double ss = 0.0;
+        if (__builtin_amdgcn_readfirstlane(row - lane / LPR) < a.Hq + a.Hkv) {  // keys
+          double ss = 0.0;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) ss += (double)(x[i] * x[i]);
-            const double inv =
-                a.k_w ? fine_rsqrt(group_sum<LPR>(ss) / a.D + (double)a.eps) : 1.0;
-            // (16-bit values by 16-bit weights: the products are exact)
-            float z[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) z[i] = x[i] * w8[i];
-            exchange(z, y);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              float dc, ds;
-              unpack2<BF16>(fine[i], dc, ds);
-              const double turned =
-                  (double)z[i] * ((double)c[i] + dc) + (double)y[i] * ((double)s[i] + ds);
-              const float key = round_to_odd((e + i < a.R ? turned : (double)z[i]) * inv);
-              x[i] = is_v ? x[i] : key;
-            }
-          }
-          // the whole group finds the row's scale
-          uint32_t top = 0;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) top = max(top, mine ? e4m3::magnitude(x[i]) : 0u);
-          const uint32_t byte = e4m3::scale_byte(group_max<LPR>(top));
-          if (row >= H || !mine || !mapped) continue;
-          const float inv = e4m3::inverse_scale(byte);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) x[i] = e4m3::codable<T>(x[i]) * inv;
-          const long long head = is_v ? row - a.Hq - a.Hkv : row - a.Hq;
-          uint2 w;
-          w.x = e4m3::pack4(x[0], x[1], x[2], x[3]);
-          w.y = e4m3::pack4(x[4], x[5], x[6], x[7]);
-          *reinterpret_cast<uint2 *>((uint8_t *)(is_v ? a.vc : a.kc) + head * a.head_stride + at +
-                                     e) = w;
-          if (l == 0) (is_v ? a.vs : a.ks)[head * a.bs + at / a.D] = (uint8_t)byte;
-        } else {
-          float ss = 0.0f;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) ss += x[i] * x[i];
-          ss = group_sum<LPR>(ss);
-          const float inv = a.q_w ? rsqrtf(ss / (float)a.D + a.eps) : 1.0f;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) x[i] *= inv * w8[i];
+          for (int i = 0; i < 8; ++i) ss += (double)x[i] * x[i];
+          const double inv = a.k_w ? fine_rsqrt(group_sum<LPR>(ss) / a.D + (double)a.eps) : 1.0;
           exchange(x, y);
-          if (row >= H || !mine) continue;
+          // (elements behind the rotated ones are selected, not turned by 0: they may be
+          // infinite)
 #pragma unroll
-          for (int i = 0; i < 8; ++i) x[i] = e + i < a.R ? x[i] * c[i] + y[i] * s[i] : x[i];
-          uint32_t w[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) w[i] = pack2<T>(x[2 * i], x[2 * i + 1]);
-          store8(a.q_out + ((long long)t * a.Hq + row) * a.D + e, w);
+          for (int i = 0; i < 8; ++i) {
+            const double own = (double)x[i] * ca[i];
+            const double key = (e + i < a.R ? own + (double)y[i] * cb[i] : own) * inv;
+            x[i] = is_v ? x[i] : round_to_odd(key);
+          }
         }
+        // the whole group finds the row's scale
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = max(top, mine ? e4m3::magnitude(x[i]) : 0u);
+        const uint32_t byte = e4m3::scale_byte(group_max<LPR>(top));
+        if (row >= H || !mine || !mapped) continue;
+        const float inv = e4m3::inverse_scale(byte);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = e4m3::codable<T>(x[i]) * inv;
+        const long long head = is_v ? row - a.Hq - a.Hkv : row - a.Hq;
+        uint2 w;
+        w.x = e4m3::pack4(x[0], x[1], x[2], x[3]);
+        w.y = e4m3::pack4(x[4], x[5], x[6], x[7]);
+        *reinterpret_cast<uint2 *>((uint8_t *)(is_v ? a.vc : a.kc) + head * a.head_stride + at +
+                                   e) = w;
+        if (l == 0) (is_v ? a.vs : a.ks)[head * a.bs + at / a.D] = (uint8_t)byte;
       }
       if (round + 1 < rounds) load(round + 1);
     }
-  };
-  if (kv)
-    pass(std::true_type{});
-  else
-    pass(std::false_type{});
+    return;
+  }
+
+  // this lane's cosines and sines: c[i], s[i] of element e + i, the sine with
+  // the sign that its partner's value takes
+  float c[8], s[8], w8[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    c[i] = 1.0f;
+    s[i] = 0.0f;
+  }
+  angles([&](uint64_t turns, int i, bool front) {
+    float cs, sn;
+    angle(a, p, turns, cs, sn);
+    c[i] = cs;
+    s[i] = front ? -sn : sn;
+    if constexpr (LAYOUT == kNeighbours) {
+      c[i + 1] = cs;
+      s[i + 1] = sn;
+    }
+  });
+  if (mine) weights8<T>(a.q_w, a.w_f32, e, w8);
+  for (int round = 0; round < rounds; ++round) {
+#pragma unroll
+    for (int it = 0; it < ITER; ++it) {
+      const int row = row0 + (round * ITER + it) * RPW;
+      float x[8], y[8];
+      unpack8<T>(raw[it], x);
+      float ss = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) ss += x[i] * x[i];
+      ss = group_sum<LPR>(ss);
+      const float inv = a.q_w ? rsqrtf(ss / (float)a.D + a.eps) : 1.0f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] *= inv * w8[i];
+      exchange(x, y);
+      if (row >= H || !mine) continue;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = e + i < a.R ? x[i] * c[i] + y[i] * s[i] : x[i];
+      uint32_t w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = pack2<T>(x[2 * i], x[2 * i + 1]);
+      store8(a.q_out + ((long long)t * a.Hq + row) * a.D + e, w);
+    }
+    if (round + 1 < rounds) load(round + 1);
+  }
 }
 
 template <class T, int LPR, int LAYOUT, bool E4M3>
