@@ -165,15 +165,16 @@ __device__ __forceinline__ void angle(const Args &a, int p, uint64_t turns, floa
   sn = a.factor * __builtin_amdgcn_sinf(f);
 }
 
-// The same to 2^-30, for what becomes codes: there a rounding on the way in can move the
-// result by a whole step of 2^-3, so keys are formed in 64 bits and rounded once.  The turn less its nearest quarter is
-// exact in integers; over [-1/8, 1/8] turns sin(2 pi f) / f and cos(2 pi f) are
-// polynomials in f^2, fitted for the least relative error (2^-37 and 2^-34).
+// The same in 64 bits, for what becomes codes: there a rounding on the way in can move
+// the result by a whole step of 2^-3, so keys are formed in 64 bits and rounded once.
+// The turn less its nearest quarter is exact in integers; over [-1/8, 1/8] turns
+// sin(2 pi f) / f and cos(2 pi f) are polynomials in f^2, fitted for the least relative
+// error (2^-37 and 2^-34).
 __device__ __forceinline__ void fine_angle(const Args &a, int p, uint64_t turns, double &cs,
                                            double &sn) {
-  const uint32_t turn = (uint32_t)((turns * (uint64_t)(int64_t)p) >> 32);
-  const uint32_t quarter = (turn + 0x20000000u) >> 30;
-  const double f = (double)(int32_t)(turn - (quarter << 30)) * 0x1p-32;
+  const uint64_t turn = turns * (uint64_t)(int64_t)p;
+  const uint32_t quarter = (uint32_t)((turn + (1ull << 61)) >> 62);
+  const double f = (double)(int64_t)(turn - ((uint64_t)quarter << 62)) * 0x1p-64;
   const double z = f * f;
   const double sine =
       f * (6.283185307151002 +

@@ -56,9 +56,10 @@ def _write(x, w, pos, rotary, Hkv, dtype, eps=1e-6):
 
 def _check_codes(got, e, want, mag):
     """Within half a code's step of the exact value, but for what the arithmetic in 64 bits
-    is off by: the angle's upper 32 bits (2^-32 of a turn), less than 2^-28 (|a| + |b|) in
-    all.  The largest of a row sets its scale: 448 2^e is not below it."""
-    tol = 2.0 ** -28 * mag
+    is off by: the polynomials of sine and cosine (2^-34 and 2^-37 of theirs), the root's
+    one step of Newton's (2^-43) and some roundings of 2^-53, less than 2^-32 (|a| + |b|)
+    in all.  The largest of a row sets its scale: 448 2^e is not below it."""
+    tol = 2.0 ** -32 * mag
     top, at = want.abs().max(-1)
     off = tol.gather(-1, at[..., None])[..., 0]
     least = [torch.where(m > E.TOP * torch.exp2(_exponent(m) - 8), _exponent(m) - 7,
