@@ -13,7 +13,7 @@
 //   V  through the wave's own LDS, codes as they are (half the LDS bytes of 16-bit
 //      tiles); a transposed read gives a lane eight keys of one element, and since
 //      each key has a scale of its own, the scale goes to the key's probability:
-//      p' = p 2^e, while the row's sum is of p itself.
+//      p' = p 2^e, rounded to bf16; the row's sum is of what p' was rounded to, over 2^e.
 //   The next tile's K and V are asked for as soon as the present tile's products with
 //   Q have read its K.
 // Measured, 32 heads of 128 over 8: 64 single tokens behind 1024 to 4096 keys 74 us, 4.6
@@ -23,7 +23,7 @@
 // p' needs fp32's range: the scales of a tile's keys lie 2^30 and more apart, and the
 // largest may be that of a key that a row does not see.  V's codes are therefore taken as
 // bf16, exactly, whatever q's type, and p' as bf16 too; for fp16 q in two parts, the
-// rounded value and the rest, which keep 16 bits of it (bf16 q of 8 nodes over 4096 keys,
+// rounded value and the rest, which keep 16 bits of it, and then the sum is of p (bf16 q of 8 nodes over 4096 keys,
 // 16 sequences: 37 us with one part, 41 with two; fp16 39 with p' in fp16 relative to the
 // largest scale met, which lost the small values beside a large one).
 #pragma once
@@ -268,21 +268,36 @@ __global__ __launch_bounds__(kFewNT, few_groups(D, QT)) void few_rows_kernel(Arg
     const uint8_t *const vs = vlds + stage * kTileBytes;
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
-      typename Mfma<BF16>::frag p[QT], rest[QT];
+      u32x4 p[QT], rest[QT];
+      float part[QT] = {};
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float f = e4m3::scale((vb[b][t] >> (8 * k)) & 255u);
+        for (int k = 0; k < 4; k += 2) {
+          // two keys' scales as a bf16 pair, and one over them
+          const uint32_t pair =
+              __builtin_amdgcn_perm(0u, vb[b][t], k == 0 ? 0x0c010c00u : 0x0c030c02u) << 7;
+          const uint32_t back = 0x7f007f00u - pair;
+          float f0, f1;
+          unpack2<BF16>(pair, f0, f1);
 #pragma unroll
           for (int qt = 0; qt < QT; ++qt) {
-            const float x = __builtin_amdgcn_exp2f(S.s[qt][b][t][k]);
-            sum[qt] += x;
-            const __bf16 high = (__bf16)(x * f);
-            p[qt][t * 4 + k] = high;
-            if constexpr (kParts == 2) rest[qt][t * 4 + k] = (__bf16)(x * f - (float)high);
+            const float x0 = __builtin_amdgcn_exp2f(S.s[qt][b][t][k]);
+            const float x1 = __builtin_amdgcn_exp2f(S.s[qt][b][t][k + 1]);
+            const uint32_t high = pack2<BF16>(x0 * f0, x1 * f1);
+            p[qt][t * 2 + k / 2] = high;
+            if constexpr (kParts == 2) {
+              float h0, h1;
+              unpack2<BF16>(high, h0, h1);
+              rest[qt][t * 2 + k / 2] = pack2<BF16>(x0 * f0 - h0, x1 * f1 - h1);
+              sum[qt] += x0 + x1;
+            } else {  // of the rounded ones
+              part[qt] = dot2(BF16{}, high, back, part[qt]);
+            }
           }
         }
+#pragma unroll
+      for (int qt = 0; qt < QT; ++qt) sum[qt] += part[qt];
 #pragma unroll
       for (int dt = 0; dt < D / 16; ++dt) {
         const int key = b * 32 + 8 * g + (col >> 1);
@@ -292,11 +307,13 @@ __global__ __launch_bounds__(kFewNT, few_groups(D, QT)) void few_rows_kernel(Arg
         const uint4 v = make_uint4(
             e4m3::unpack_pair<BF16, false>(w.x, 1.0f), e4m3::unpack_pair<BF16, true>(w.x, 1.0f),
             e4m3::unpack_pair<BF16, false>(w.y, 1.0f), e4m3::unpack_pair<BF16, true>(w.y, 1.0f));
-        const auto vf = __builtin_bit_cast(typename Mfma<BF16>::frag, v);
+        typedef Mfma<BF16>::frag frag;
+        const auto vf = __builtin_bit_cast(frag, v);
 #pragma unroll
         for (int qt = 0; qt < QT; ++qt) {
-          o[qt][dt] = Mfma<BF16>::run(vf, p[qt], o[qt][dt]);
-          if constexpr (kParts == 2) o[qt][dt] = Mfma<BF16>::run(vf, rest[qt], o[qt][dt]);
+          o[qt][dt] = Mfma<BF16>::run(vf, __builtin_bit_cast(frag, p[qt]), o[qt][dt]);
+          if constexpr (kParts == 2)
+            o[qt][dt] = Mfma<BF16>::run(vf, __builtin_bit_cast(frag, rest[qt]), o[qt][dt]);
         }
       }
     }

@@ -45,11 +45,13 @@
 //    layout that the products read.  (Operands converted where they are read would
 //    cost every wave of the eight 128 conversions a tile instead of 16; codes that come
 //    through LDS are written and read there once more, beside the operands' reads which
-//    are all that it gives: the prompt of 8192 600 us against 550.)  The row sums are
-//    then added up from the probabilities in fp32: the registers that the matrix unit
-//    would sum in are the ones that the codes need, and without them the compiler drops
-//    the schedule of the operand reads (660 us).  The prompt of 8192 takes 545 to 565 us
-//    (16 bits: 485), 16 trees of 63 nodes 91 with the merge.  Up to 32 query rows go
+//    are all that it gives: the prompt of 8192 600 us against 550.)  The row sums, of
+//    the rounded probabilities here too, are then pairwise products with ones: the
+//    registers that the matrix unit would sum in are the ones that the codes need, and
+//    without them the compiler drops the schedule of the operand reads (660 us).  The
+//    prompt of 8192 takes 530 to 560 us (16 bits: 485), 16 trees of 63 nodes 86 with the
+//    merge (of 64-wide heads 443 and 81; with sums of the unrounded ones 534 and 87, 443
+//    and 80).  Up to 32 query rows go
 //    by few_rows_attention.hpp, where the codes stay codes.
 //  * Splits are cut on the device, from each block's own first and last tile,
 //    and leave fp32 sums for a log-sum-exp merge.
@@ -365,11 +367,18 @@ __device__ __forceinline__ void score_phase(Scores<QT> &S, float (&b)[QT], f32x4
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const float p = __builtin_amdgcn_exp2f(S.s[qt][blk][t][i]);
-          if constexpr (LANES) sum[qt] += p;
           P.p[qt][blk][t * 4 + i] = (typename T::elem)p;
         }
       // keep the exponentials in this phase (see tree_attention.hip)
       asm volatile("" ::"v"(P.p[qt][blk]));
+      if constexpr (LANES) {  // the sum of the rounded ones
+        const uint32_t ones = std::is_same<T, BF16>::value ? 0x3f803f80u : 0x3c003c00u;
+        const auto w = __builtin_bit_cast(u32x4, P.p[qt][blk]);
+        float part = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) part = dot2(T{}, w[i], ones, part);
+        sum[qt] += part;
+      }
     }
 }
 

@@ -70,6 +70,18 @@ struct Mfma<FP16> {
   }
 };
 
+// a.x b.x + a.y b.y + c of pairs in fp32 (off by 2^-22 of the largest, and toward zero:
+// for short sums).
+__device__ __forceinline__ float dot2(BF16, uint32_t a, uint32_t b, float c) {
+  typedef __bf16 pair __attribute__((ext_vector_type(2)));
+  return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(pair, a), __builtin_bit_cast(pair, b), c,
+                                         false);
+}
+__device__ __forceinline__ float dot2(FP16, uint32_t a, uint32_t b, float c) {
+  typedef _Float16 pair __attribute__((ext_vector_type(2)));
+  return __builtin_amdgcn_fdot2(__builtin_bit_cast(pair, a), __builtin_bit_cast(pair, b), c, false);
+}
+
 __device__ __forceinline__ uint4 ld_g16(const uint16_t *p) {
   return *reinterpret_cast<const uint4 *>(p);
 }

@@ -134,3 +134,27 @@ def test_values_below_one_of_no_weight(device, spread, dtype):
     got = prompt_attention(q[0].to(device), dev[0], dev[2], bt.to(device), _int([ctx], device),
                            _int([0, 2], device), **args)
     _near(got, want, A, dtype)
+
+
+@pytest.mark.parametrize("N", [1, 3, 8, 30, 63])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("splits", [1, 3])
+def test_values_that_are_all_alike(device, N, D, dtype, splits):
+    """Each element of V the same in every row, coded under different scales: what the
+    probabilities are rounded to is in the row's sum too, so that they cancel but for fp32
+    roundings (2^-24 each, of less than 2^10 of them), far less than half a step."""
+    g = torch.Generator().manual_seed(N)
+    pools, bt = C.case([500], N, 2, D, dtype, e4m3=True)
+    codes, scales = pools[1]
+    value = torch.randint(8, 16, (D,), generator=g).float() / 8        # 1 to 2, exact
+    up = torch.randint(-3, 7, scales.shape, generator=g)               # 2^up is in the code
+    codes.copy_((value * torch.exp2(up.float())[..., None]).to(torch.float8_e4m3fn))
+    scales.copy_((127 - up).to(torch.uint8))
+    q = (4.0 * torch.randn(1, N, 8, D, generator=g)).to(dtype)
+    mask = torch.arange(N)
+    mask = (1 << mask) | ((1 << mask) - 1)                             # a chain
+    dev = [t.to(device) for p in pools for t in p]
+    got = tree_attention(q.to(device), dev[0], dev[2], bt.to(device), _int([500], device),
+                         mask.to(device), k_scales=dev[1], v_scales=dev[3], num_splits=splits)
+    assert torch.equal(got.cpu(), value.to(dtype).expand_as(q))
