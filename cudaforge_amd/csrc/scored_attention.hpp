@@ -323,6 +323,9 @@ __device__ __forceinline__ float score_max(const Scores<QT> &S, int qt) {
   return column_max(v);
 }
 
+// The next instruction begins on a fetch's 32 bytes.
+__device__ __forceinline__ void fetch_line() { asm volatile(".p2align 5"); }
+
 // Scores of one tile to probabilities; the columns' lazy bases b (log2 units; 0:
 // none yet, where the sum is 0 too) where FIXED does not hold.
 template <int D, int QT, class T, bool FIXED, bool LANES>
@@ -570,6 +573,13 @@ __global__ __launch_bounds__(kNT) void scored_attn_kernel(Args a) {
   constexpr int kVStages = E4M3 ? kCodeStages : tree::kVStages;
   __shared__ __align__(16) uint8_t kring[kKStages * kTileBytes];
   __shared__ __align__(16) uint8_t vring[kVStages * kTileBytes];
+  // Both phases' code on fetch lines: where it lies otherwise follows from the length of
+  // all code in front of the loop, and the same loop takes up to 5% more at some places
+  // (64-wide heads, the biased prompt of 8192, moved by 4 bytes at a time: 476 to 498 us).
+  // Aligned / as it came, us of that prompt: biased 481 / 498, biased and capped 644 /
+  // 650, plain 390 / 405, with a window 125 / 128; left as they came are capped ones (fp16
+  // 578 / 562), codes (456 / 448) and 128-wide heads (532 to 712, within 1% either way).
+  constexpr bool kAligned = D == 64 && !E4M3 && (BIAS || !CAP);
   // row offsets of the split's 16-key groups; a ring, refilled half a ring at a
   // time in longer splits (its size, and the rows', let two work-groups of one
   // query tile and head_dim 64 share a CU's LDS)
@@ -815,6 +825,7 @@ __global__ __launch_bounds__(kNT) void scored_attn_kernel(Args a) {
                 vring + (ahead % kVStages) * kTileBytes);
       }
       if (busy) {
+        if constexpr (kAligned) fetch_line();
         raw_scores<D, QT, T, CAP, BIAS, FIXED, SINKS>(ln, base, a, k0, cap2, kbase, ctx, least, most_first,
                                                rows_at, smove + 64, S);
         score_phase<D, QT, T, FIXED, E4M3>(S, base, o, lacc, sum, set, P);
@@ -831,10 +842,12 @@ __global__ __launch_bounds__(kNT) void scored_attn_kernel(Args a) {
         block_barrier();
       }
       __builtin_amdgcn_s_setprio(1);
-      if (busy)
+      if (busy) {
+        if constexpr (kAligned) fetch_line();
         // (one query tile has half the products per operand read)
         mfma_phase<D, QT, T, QT == 1 ? 4 : 2, !E4M3, E4M3 ? 6 : 8>(ln, kring + ((u + 1) % kKStages) * kTileBytes,
                    vring + (u % kVStages) * kTileBytes, zero, P, S, o, lacc);
+      }
       __builtin_amdgcn_s_setprio(0);
     }
     if (!lag) block_barrier();
