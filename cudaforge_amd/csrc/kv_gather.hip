@@ -108,7 +108,8 @@ extern "C" int cfa_kv_gather(const void *k_pool, const void *v_pool, const uint8
   if (!cu_seqlens && T % B) return fail_arg("without cu_seqlens T must be a multiple of B");
   if ((((uintptr_t)k_pool | (uintptr_t)v_pool | (uintptr_t)k_out | (uintptr_t)v_out) & 15) != 0)
     return fail_arg("the pools and outputs must be 16-byte aligned");
-  if (T >= 1 << 26) return fail_arg("too many tokens for one call (2^26 and more)");
+  // (a launch has less than 2^32 threads)
+  if ((T + 3LL) / 4 >= 1 << 24) return fail_arg("too many tokens for one call (about 2^26)");
   cfa::gather::Args a{};
   a.kpool = (const uint8_t *)k_pool;
   a.vpool = (const uint8_t *)v_pool;

@@ -601,12 +601,12 @@ int launch(Args a, hipStream_t st) {
   const long long few = (long long)a.T * ((H + RPW - 1) / RPW);
   const int rows = E4M3 ? a.Hq : H;
   auto up = [](int n, int per) { return (n + per - 1) / per; };
-  auto grid = [&](int iter, bool all) {
+  auto groups = [&](int iter, bool all) {
     a.rounds = all ? up(rows, iter * RPW) : 1;
     a.chunks = up(rows, iter * a.rounds * RPW);
     a.kv_rounds = E4M3 ? (all ? up(2 * a.Hkv, iter * RPW) : 1) : 0;
     a.kv_chunks = E4M3 ? up(2 * a.Hkv, iter * a.kv_rounds * RPW) : 0;
-    return dim3((unsigned)(((long long)a.T * (a.chunks + a.kv_chunks) + kWaves - 1) / kWaves));
+    return ((long long)a.T * (a.chunks + a.kv_chunks) + kWaves - 1) / kWaves;
   };
   // `few`: waves of one row a lane group.  A token's heads all in one wave where
   // that leaves 8192 waves of kIter rows' work (angles and weights are then formed
@@ -614,21 +614,25 @@ int launch(Args a, hipStream_t st) {
   // us, 48 heads of 128, one row a group / kIter rows / all heads in a wave: 504
   // tokens 10.1 / 10.6 / 14, 2000 tokens 22 / 19.6 / 20.5, 3200 tokens 36 / 27 / 24, 8149
   // tokens 104 / 73 / 58.  With 2 / 6 / 8 / 12 rows in flight: 59.5 / 59.2 / 62 / 69.
-  const bool all = few >= 8192 * kIter;
+  const bool many = few >= 8192, all = few >= 8192 * kIter;
+  const long long n = many ? groups(kIter, all) : groups(1, false);
+  if (n * kWaves * 64 >= 1LL << 32)  // a launch's threads
+    return abi::fail_arg("too many tokens and heads for one call");
+  const dim3 grid((unsigned)n);
   if constexpr (E4M3) {
-    if (few >= 8192)
+    if (many)
       CFA_LAUNCH("qk_norm_rope_kv", (qk_norm_rope_kv_e4m3_kernel<T, LPR, LAYOUT, kIter>),
-                 grid(kIter, all), dim3(kWaves * 64), 0, st, a);
+                 grid, dim3(kWaves * 64), 0, st, a);
     else
       CFA_LAUNCH("qk_norm_rope_kv", (qk_norm_rope_kv_e4m3_kernel<T, LPR, LAYOUT, 1>),
-                 grid(1, false), dim3(kWaves * 64), 0, st, a);
+                 grid, dim3(kWaves * 64), 0, st, a);
   } else {
-    if (few >= 8192)
+    if (many)
       CFA_LAUNCH("qk_norm_rope_kv", (qk_norm_rope_kv_kernel<T, LPR, LAYOUT, kIter>),
-                 grid(kIter, all), dim3(kWaves * 64), 0, st, a);
+                 grid, dim3(kWaves * 64), 0, st, a);
     else
       CFA_LAUNCH("qk_norm_rope_kv", (qk_norm_rope_kv_kernel<T, LPR, LAYOUT, 1>),
-                 grid(1, false), dim3(kWaves * 64), 0, st, a);
+                 grid, dim3(kWaves * 64), 0, st, a);
   }
   return CFA_OK;
 }

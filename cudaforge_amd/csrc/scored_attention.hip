@@ -240,7 +240,7 @@ static int run(Args &a, const Plan &p, int D, int fp16, float sm_scale, float so
   const long long grid = (long long)p.splits * a.Hkv * p.blocks;
   if (grid * kNT >= (1LL << 32)) return fail_arg("too many queries for one call");
   if (p.splits > 1) {
-    if ((long long)a.T * a.Hq * (D / 4) >= (1LL << 32))  // the merge's threads
+    if (((long long)a.T * a.Hq * (D / 4) + 255) / 256 >= (1LL << 24))  // the merge's threads
       return fail_arg("too many queries for one call");
     if (!workspace || workspace_bytes < p.bytes(a.T, a.Hq, D))
       return fail_arg("workspace too small (see the entry point's _workspace_size)");
