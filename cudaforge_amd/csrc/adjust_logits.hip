@@ -26,6 +26,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <cmath>
 
 #include "abi_internal.hpp"
 #include "half_types.hpp"
@@ -348,7 +349,10 @@ extern "C" int cfa_adjust_logits(
   if (type < 0 || type > 2) return fail_arg("type must be 0 (fp32), 1 (bf16) or 2 (fp16)");
   if (node_tokens && N > kMaxNodes) return fail_arg("at most 64 tree nodes");
   if (!node_tokens != !tree_mask) return fail_arg("node_tokens and tree_mask go together");
-  if (!repetition && !(repetition0 > 0.0f)) return fail_arg("repetition must be positive");
+  if (!repetition && !(repetition0 > 0.0f && std::isfinite(repetition0)))
+    return fail_arg("repetition must be positive and finite");
+  if ((!frequency && !std::isfinite(frequency0)) || (!presence && !std::isfinite(presence0)))
+    return fail_arg("frequency and presence must be finite");
   if (allowed && ((long long)words * 32 < V || masks < 0))
     return fail_arg("allowed needs a bit for every token");
   if (B == 0 || N == 0) return CFA_OK;

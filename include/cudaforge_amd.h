@@ -227,7 +227,7 @@ int cfa_sample_rows(const void *rows, int64_t row_stride, int elem_type, int R, 
  *     prompt_lens [B] (NULL: 0) as the prompt.  Ids outside [0, V) are passed over
  *     here, in node_tokens and in bias_tokens.  L = 0: none.
  *   repetition, frequency, presence: fp32 [B], or NULL and the number for all
- *     (repetition positive; 1, 0 and 0 leave the logits alone)
+ *     (finite, repetition positive; 1, 0 and 0 leave the logits alone)
  *   node_tokens [B, N], tree_mask ([N], or [B, N] at tree_mask_stride_b): draft
  *     trees of at most 64 nodes; row i's path are the nodes of its mask, itself
  *     among them (NULL: none)

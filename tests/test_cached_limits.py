@@ -1,5 +1,5 @@
-"""CPU tier: calls whose grids would have 2^32 threads, which no launch takes, are refused
-(none reaches a device)."""
+"""CPU tier: refusals at the ends of ranges (none reaches a device): grids of 2^32 threads,
+which no launch takes, and numbers that are not fp32 values."""
 import ctypes
 
 import pytest
@@ -34,3 +34,13 @@ def test_merge(T):
         256, 256, 256, None, None, 0, 256, 1 << 20, 256, 8, 1, 0, 16, 256, T, 1, 1, 1, 128, f(0.1),
         f(0.0), None, 0, 0, T, 128, 2, 256, 256, need, None)
     assert rc == _lib.CFA_ERR_ARG and "too many" in _lib.last_error()
+
+
+@pytest.mark.parametrize("r,fr,p", [(float("inf"), 0, 0), (1e39, 0, 0), (1e-50, 0, 0), (1, 1e39, 0),
+                                    (1, float("nan"), 0), (1, 0, -1e39), (1, 0, float("inf"))])
+def test_penalties(r, fr, p):
+    rc = _lib.load().cfa_adjust_logits(256, 100, 100, 1, 2, 1, 100, 256, None, None, 5, None, f(r),
+                                       None, f(fr), None, f(p), None, None, 0, None, None, 0, 0,
+                                       None, 0, 0, None, 256, 100, 100, 0, None)
+    assert rc == _lib.CFA_ERR_ARG
+    assert "finite" in _lib.last_error()
