@@ -21,8 +21,11 @@
 // keep it to sixteen of a vocabulary of 128256).  us a call, bf16: 64 rows of 128256
 // alone 7.3, behind 2000 tokens each 11.3, and with biases and masks 13.5; 504 nodes of
 // 8 trees to fp32 (388 MB) 71, behind 2000 tokens 88 (4.4 TB/s; a copy of the same
-// tensors takes 67), behind 8000 108.  With the penalties in the streaming loop,
-// instead of behind it for the listed tokens, the rows took 17.3 and the trees 90.
+// tensors takes 67), behind 8000 108 (145 if they are all different).  Each group counts
+// all of its sequence's history, so that long ones cost: behind 30000 and 100000 such
+// tokens one row 19 and 49, 64 rows 44 and 111, the trees 218 and 427.  With the
+// penalties in the streaming loop, instead of behind it for the listed tokens, the rows
+// took 17.3 and the trees 90.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

@@ -23,9 +23,10 @@
 // p' needs fp32's range: the scales of a tile's keys lie 2^30 and more apart, and the
 // largest may be that of a key that a row does not see.  V's codes are therefore taken as
 // bf16, exactly, whatever q's type, and p' as bf16 too; for fp16 q in two parts, the
-// rounded value and the rest, which keep 16 bits of it, and then the sum is of p (bf16 q of 8 nodes over 4096 keys,
-// 16 sequences: 37 us with one part, 41 with two; fp16 39 with p' in fp16 relative to the
-// largest scale met, which lost the small values beside a large one).
+// rounded value and the rest, which keep 16 bits of it, and then the sum is of p (16 trees
+// of 8 nodes over 4096 keys, bf16 q: 37 us with one part, 41 with two; fp16 40, and 39
+// with p' in fp16 relative to the largest scale met, which lost the small values beside a
+// large one).
 #pragma once
 
 #include "scored_attention.hpp"

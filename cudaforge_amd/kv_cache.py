@@ -56,6 +56,7 @@ class KVCacheConfig:
 
     @property
     def bytes_per_block(self) -> int:
+        """Of one pool (an 8-bit cache's scales, 1 / head_dim as many, are apart)."""
         return self.num_layers * self.layer_block_bytes
 
     def _c(self) -> _lib.KVCacheConfigC:

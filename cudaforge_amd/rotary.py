@@ -166,7 +166,7 @@ def qk_norm_rope_kv(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions
     projection (any strides of tokens and heads; elements contiguous; D a
     multiple of 8, at most 256); positions [T] int32; `rotary` None: no
     rotation.  q_norm / k_norm [D]: RMSNorm weights of each head, of q's dtype
-    or fp32 (None: no norm).  All in fp32, rounded once.
+    or fp32 (None: no norm).  In fp32, rounded once.
 
     Token t of sequence b goes to slot base_lens[b] + j of `layer` in k_pool /
     v_pool [num_blocks, num_layers, Hkv, block_size, D] by block_tables [B,
@@ -178,10 +178,12 @@ def qk_norm_rope_kv(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions
 
     With k_scales and v_scales (uint8 [num_blocks, num_layers, Hkv, block_size])
     the pools are float8_e4m3fn (D a multiple of 16): each k and v row is
-    quantised from its fp32 values as it is written, code e4m3(x / 2^e), scale
-    byte e + 127, with the least e >= -126 that brings the row's largest finite
-    magnitude to 448 2^e or less.  What is not finite becomes NaN; from fp16, what
-    would round past that type's range stops at 61440.  ``verify.tree_attention``,
+    quantised as it is written, keys from values formed in 64 bits, code
+    e4m3(x / 2^e), scale byte e + 127, with the least e >= -126 that brings the
+    row's largest finite magnitude to 448 2^e or less.  What is not finite becomes
+    NaN; from fp16, values of at most 65504 that would round past it stop at 61440
+    (larger ones, finite in 64 bits, are coded as they are and read back in fp16 as
+    infinity).  ``verify.tree_attention``,
     ``verify.prompt_attention``, ``verify.kv_commit`` and ``verify.kv_gather`` take
     such pools with their scales.
     """

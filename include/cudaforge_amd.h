@@ -636,9 +636,9 @@ int cfa_qk_norm_rope_kv(const void *q, int64_t q_stride_t, int64_t q_stride_h, c
 /* The same into pools of e4m3 codes (8 bits: 4 of exponent, 3 of mantissa, no
  * infinity): k_pool, v_pool of bytes in the same layout, 16-byte aligned, head_dim
  * a multiple of 16; k_scales, v_scales [num_blocks][num_layers][n_kv_heads]
- * [block_size] hold a byte for each row.  A row of fp32 results x is quantised
- * with e = the least integer >= -126 that has max |x| <= 448 * 2^e (over its
- * finite values): code e4m3(x * 2^-e), to nearest even, byte e + 127.  Values that
+ * [block_size] hold a byte for each row.  A row of results x (keys formed in 64
+ * bits, whatever the norm's type; q is as above) is quantised with e = the least
+ * integer >= -126 that has max |x| <= 448 * 2^e (over its finite values): code e4m3(x * 2^-e), to nearest even, byte e + 127.  Values that
  * are not finite become NaN codes; from fp16, those of at most 65504 that would
  * round past it stop at 61440.  NULL scales: cfa_qk_norm_rope_kv. */
 int cfa_qk_norm_rope_kv_e4m3(const void *q, int64_t q_stride_t, int64_t q_stride_h, const void *k,
