@@ -27,8 +27,6 @@
 // than their exact values', against none.
 #include <hip/hip_runtime.h>
 
-#include <type_traits>
-
 #include "abi_internal.hpp"
 #include "e4m3.hpp"
 #include "half_types.hpp"

@@ -638,9 +638,10 @@ int cfa_qk_norm_rope_kv(const void *q, int64_t q_stride_t, int64_t q_stride_h, c
  * a multiple of 16; k_scales, v_scales [num_blocks][num_layers][n_kv_heads]
  * [block_size] hold a byte for each row.  A row of results x (keys formed in 64
  * bits, whatever the norm's type; q is as above) is quantised with e = the least
- * integer >= -126 that has max |x| <= 448 * 2^e (over its finite values): code e4m3(x * 2^-e), to nearest even, byte e + 127.  Values that
- * are not finite become NaN codes; from fp16, those of at most 65504 that would
- * round past it stop at 61440.  NULL scales: cfa_qk_norm_rope_kv. */
+ * integer >= -126 that has max |x| <= 448 * 2^e (over its finite values): code
+ * e4m3(x * 2^-e), to nearest even, byte e + 127.  Values that are not finite become
+ * NaN codes; from fp16, those of at most 65504 that would round past it stop at
+ * 61440.  NULL scales: cfa_qk_norm_rope_kv. */
 int cfa_qk_norm_rope_kv_e4m3(const void *q, int64_t q_stride_t, int64_t q_stride_h, const void *k,
                              int64_t k_stride_t, int64_t k_stride_h, const void *v,
                              int64_t v_stride_t, int64_t v_stride_h, int fp16,
